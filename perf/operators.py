@@ -1,0 +1,441 @@
+"""The timed work of the operators around a routed-experts layer, as a program that trains
+or serves one calls them:
+
+- "norm": the norm of the tokens before the layer, with the residual stream's addition where
+  there is one, forward (`norm.normed`) and backward (`norm.normed_backward`: the gradient to
+  the tokens, and the gain's and bias's over all of them);
+- "route": the router's backward (`router.route_backward`): from the gradient of the picks'
+  weights to the tokens', the router kernel's and its bias's;
+- "int8": an experts' product with operands in 8-bit integers, a scale for each row of the
+  tokens and each column of the kernels (`grouped_int8.quantized`, `grouped_int8.rows`).
+
+Where `own` is false, `run` computes them in plain form, by elementary torch operations in
+float32 (float64 next to a rounding border), rounded once at the end.
+"""
+
+import math
+
+import torch
+
+own = False
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+
+
+def _norm(**kw):
+    return {"kind": "norm", "direction": "forward", "norm": "rmsnorm", "dtype": "bfloat16",
+            "bias": False, "residual": False, **kw}
+
+
+def _route(**kw):
+    return {"kind": "route", "router": "softmax", "groups": 1, "top_groups": 1, "scaling": 1.0,
+            "normalize": True, "balance": False, "add": False, **kw}
+
+
+def _int8(**kw):
+    return {"kind": "int8", **kw}
+
+
+QWEN3 = {"d": 2048, "experts": 128, "k": 8}  # Qwen3-30B-A3B's layer
+DEEPSEEK = {"d": 7168, "experts": 256, "k": 8}  # DeepSeek-V3's
+QWEN3_UP = 2 * 768  # its experts' up kernels' columns, (up, gate) pairs
+
+
+def listed():
+    return [
+        # a decode step of one sequence: one token, the widest rows, launch and latency
+        _norm(name="norm one token", tokens=1, d=7168, residual=True),
+        # a training or prompt batch's norm with the residual stream's addition
+        _norm(name="norm batch", tokens=16384, d=2048, residual=True),
+        # a float32 layer's layernorm with its bias, an odd batch of odd rows
+        _norm(name="norm odd float32", tokens=3001, d=1443, norm="layernorm", dtype="float32",
+              bias=True),
+        # the backward of a layernorm with its bias beside a residual stream (gpt-oss-120b's width)
+        _norm(name="norm backward", tokens=8192, d=2880, direction="backward", norm="layernorm",
+              bias=True, residual=True),
+        # the widest rows' backward, a whole batch
+        _norm(name="norm backward wide", tokens=16384, d=7168, direction="backward"),
+        # a small float32 layer's backward, odd in both dimensions
+        _norm(name="norm backward odd", tokens=1001, d=1027, direction="backward",
+              norm="layernorm", dtype="float32", bias=True),
+        # a short batch's router backward
+        _route(name="route backward 500", tokens=500, **QWEN3),
+        # a training batch's, added to the gradient that came back through the experts
+        _route(name="route backward batch", tokens=16384, add=True, **QWEN3),
+        # sigmoid scores, grouped picks, a balance loss's gradient on the scores
+        _route(name="route backward grouped", tokens=8192, router="sigmoid", groups=8,
+               top_groups=4, scaling=2.5, balance=True, **DEEPSEEK),
+        # a decode step's up product: a row or two with each expert that is picked
+        _int8(name="int8 decode 8", tokens=8, n=QWEN3_UP, **QWEN3),
+        # a larger decode batch, or a short odd prompt: a dozen rows an expert
+        _int8(name="int8 decode 201", tokens=201, n=QWEN3_UP, **QWEN3),
+        # a long prompt's
+        _int8(name="int8 prompt", tokens=16384, n=QWEN3_UP, **QWEN3),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    """An integer of [lo, hi], spread evenly over its logarithm."""
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["norm", "norm", "route", "int8"])
+    if kind == "norm":
+        d = _log_int(rng, 64, 8192)
+        if rng.random() < 0.6:
+            d = max(64, d // 8 * 8)
+        dtype = rng.choice(["bfloat16", "bfloat16", "float32"])
+        most = min(32768, 117_000_000 // d // (2 if dtype == "float32" else 1))
+        kind_of = rng.choice(["rmsnorm", "layernorm"])
+        return _norm(tokens=_log_int(rng, 1, most), d=d, norm=kind_of, dtype=dtype,
+                     direction=rng.choice(["forward", "backward"]),
+                     bias=kind_of == "layernorm" and rng.random() < 0.7,
+                     residual=rng.random() < 0.5)
+    experts = rng.choice([8, 16, 32, 60, 64, 96, 128, 160, 256])
+    k = rng.choice([1, 2, 4, 6, 8])
+    if kind == "route":
+        d = 16 * _log_int(rng, 8, 448)
+        grouped = experts % 8 == 0 and experts >= 64 and rng.random() < 0.4
+        return _route(tokens=_log_int(rng, 1, min(32768, 58_000_000 // d)), d=d, experts=experts,
+                      k=k, router="sigmoid" if grouped else rng.choice(["softmax", "sigmoid"]),
+                      groups=8 if grouped else 1, top_groups=4 if grouped else 1,
+                      scaling=2.5 if grouped else 1.0, normalize=k > 1 or rng.random() < 0.5,
+                      balance=rng.random() < 0.3, add=rng.random() < 0.5)
+    d, n = _log_int(rng, 96, 7168), 4 * _log_int(rng, 32, 1024)
+    while experts * d * n > 4.0e8:
+        experts = max(8, experts // 2)
+        if experts == 8:
+            n = max(128, n // 2 // 4 * 4)
+    k = min(k, experts)
+    most = int(min(16384, 131072 // k, 4.1e11 / (k * d * n)))
+    return _int8(tokens=_log_int(rng, 1, max(1, most)), d=d, experts=experts, k=k, n=n)
+
+
+# --- inputs ------------------------------------------------------------------------------
+
+
+def _dtype(case):
+    return F32 if case.get("dtype") == "float32" else BF16
+
+
+def _randn(gen, *shape):
+    return torch.randn(*shape, generator=gen, device="cuda")
+
+
+def _tokens(gen, t, d):
+    """N(0, 1) with a thousandth of the values 100 times as large, as a layer's tokens are."""
+    z = _randn(gen, t, d)
+    at = torch.randint(t * d, (max(1, t * d // 1000),), generator=gen, device="cuda")
+    z.view(-1)[at] *= 100
+    return z
+
+
+def _scores(logits, router):
+    return torch.softmax(logits, -1) if router == "softmax" else torch.sigmoid(logits)
+
+
+def _picked(scores, groups, keep, k):
+    """Each token's k experts, the best first, from the `keep` best of `groups` groups (a group
+    by the sum of its two best)."""
+    choice = scores
+    if groups > 1:
+        g = choice.view(choice.shape[0], groups, -1)
+        best = torch.topk(torch.topk(g, 2, -1).values.sum(-1), keep, -1).indices
+        kept = torch.zeros(g.shape[:2], dtype=torch.bool, device=g.device).scatter_(1, best, True)
+        choice = torch.where(kept[..., None], g, -torch.inf).view(choice.shape)
+    return torch.topk(choice, k, -1).indices
+
+
+def _inputs(case, seed):
+    """The case's inputs, by name."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    t, d, dt = case["tokens"], case["d"], _dtype(case)
+    if case["kind"] == "norm":
+        x = {"x": (_tokens(gen, t, d) + 0.5 * _randn(gen, d)).to(dt),
+             "scale": (1 + 0.1 * _randn(gen, d)).to(dt),
+             "bias": (0.1 * _randn(gen, d)).to(dt) if case["bias"] else None,
+             "residual": None, "dy": None, "d_summed": None, "stats": None}
+        if case["direction"] == "forward":
+            x["residual"] = _randn(gen, t, d).to(dt) if case["residual"] else None
+            return x
+        x["dy"] = (0.01 * _randn(gen, t, d)).to(dt)
+        x["d_summed"] = (0.01 * _randn(gen, t, d)).to(dt) if case["residual"] else None
+        # what the forward kept: each row's mean (0 for an rmsnorm) and 1 / root mean square
+        v = x["x"].double()
+        mean = v.mean(-1) if case["norm"] == "layernorm" else torch.zeros_like(v[:, 0])
+        rstd = ((v - mean[:, None]).square().mean(-1) + EPS).rsqrt()
+        x["stats"] = torch.stack([mean, rstd], -1).float()
+        return x
+    e, k = case["experts"], case["k"]
+    if case["kind"] == "route":
+        x = {"x": _tokens(gen, t, d).to(BF16), "kernel": (0.02 * _randn(gen, d, e)).to(BF16)}
+        x["logits"] = x["x"].float() @ x["kernel"].float()
+        s = _scores(x["logits"], case["router"])
+        x["idx"] = _picked(s, case["groups"], case["top_groups"], k).int().contiguous()
+        x["d_weights"] = (0.01 * _randn(gen, t, k)).to(BF16)
+        # a balance loss's gradient: each expert's share of the picks on every token's score
+        share = torch.bincount(x["idx"].view(-1).long(), minlength=e).float() / (t * k)
+        x["d_scores"] = (1e-3 * e * share).expand(t, e).contiguous() if case["balance"] else None
+        x["dz"] = (0.01 * _randn(gen, t, d)).to(BF16) if case["add"] else None
+        return x
+    x = {"z": _tokens(gen, t, d).to(BF16)}
+    # each token's picks, drawn with the experts' own offsets; sorted by expert, stably
+    picks = torch.topk(_randn(gen, t, e) + 0.5 * _randn(gen, e), k, -1).indices.view(-1)
+    x["order"] = torch.sort(picks, stable=True).indices.int()
+    x["sizes"] = torch.bincount(picks, minlength=e).int()
+    x["kernels"] = torch.empty(e, d, case["n"], dtype=BF16, device="cuda")
+    for part in x["kernels"]:  # a kernel at a time: they are large
+        part.copy_(0.02 * _randn(gen, d, case["n"]))
+    return x
+
+
+EPS = 1e-6
+
+
+def prepare(case, seed):
+    x = _inputs(case, seed)
+    if case["kind"] != "int8":
+        return {"case": case, **x}
+    # A program that multiplies in 8 bits keeps its kernels quantized, and the sort of the
+    # picks gives the groups' sizes and their tiles.
+    m = x["order"].numel()
+    kernels, ends = x.pop("kernels"), torch.cumsum(x["sizes"].long(), 0)
+    state = {"case": case, **x, "filled": ends[-1:].int()}
+    if own:
+        from bux_amd import grouped_int8, grouped_mxfp8
+        state["quantized"] = grouped_int8.quantized_kernels(kernels)
+        state["tiles"] = grouped_mxfp8.tiles_of(x["sizes"], grouped_mxfp8.whole(m), m)
+        return state
+    codes, state["kernel_scales"] = _to_int8(kernels.transpose(1, 2))
+    state["kernel_codes"] = codes.to(torch.int8)  # (experts, n, d)
+    # the rows of each expert in a slot of the most rows that one has
+    start = ends - x["sizes"].long()
+    expert = torch.repeat_interleave(torch.arange(case["experts"], device="cuda"), x["sizes"].long())
+    state["most"] = max(1, int(x["sizes"].max()))
+    state["slot"] = expert * state["most"] + torch.arange(m, device="cuda") - start[expert]
+    return state
+
+
+# --- the operators in plain form -----------------------------------------------------------
+
+
+def _plain_norm(x, s):
+    v = x.float()
+    mean = v.mean(-1, keepdim=True) if s["case"]["norm"] == "layernorm" else 0.0
+    u = v - mean
+    y = u * torch.rsqrt(u.square().mean(-1, keepdim=True) + EPS) * s["scale"].float()
+    if s["bias"] is not None:
+        y = y + s["bias"].float()
+    return y.to(x.dtype)
+
+
+def _plain_norm_backward(s):
+    x, dt = s["x"].float(), s["x"].dtype
+    dy, scale = s["dy"].float(), s["scale"].float()
+    mean, rstd = s["stats"][:, :1], s["stats"][:, 1:]
+    n = (x - mean) * rstd
+    dn = dy * scale
+    dx = dn - n * (dn * n).mean(-1, keepdim=True)
+    if s["case"]["norm"] == "layernorm":
+        dx = dx - dn.mean(-1, keepdim=True)
+    dx = dx * rstd
+    if s["d_summed"] is not None:
+        dx = dx + s["d_summed"].float()
+    return {"x": dx.to(dt), "scale": (dy * n).sum(0),
+            "bias": dy.sum(0) if s["bias"] is not None else None}
+
+
+def _plain_route_backward(s):
+    case, at = s["case"], s["idx"].long()
+    score = _scores(s["logits"], case["router"])
+    dw = s["d_weights"].float() * case["scaling"]
+    if case["normalize"]:
+        w = score.gather(1, at)
+        total = w.sum(-1, keepdim=True)
+        dw = (dw - (dw * w).sum(-1, keepdim=True) / total) / total
+    ds = torch.zeros_like(score).scatter_(1, at, dw)
+    if s["d_scores"] is not None:
+        ds = ds + s["d_scores"]
+    if case["router"] == "softmax":
+        dl = score * (ds - (ds * score).sum(-1, keepdim=True))
+    else:
+        dl = ds * score * (1 - score)
+    dx = dl @ s["kernel"].float().T
+    if s["dz"] is not None:
+        dx = dx + s["dz"].float()
+    return {"x": dx.to(BF16), "kernel": (s["x"].float().T @ dl).to(BF16), "bias": dl.sum(0)}
+
+
+def _to_int8(x):
+    """Rows x in 8-bit integers: the nearest to 127 x / max |x| (the even one at a tie, which
+    float64 tells), and each row's scale, max |x| / 127. Codes as float32."""
+    top = x.abs().amax(-1).float()
+    codes = torch.empty(x.shape, dtype=F32, device=x.device)
+    if x.dim() == 2:
+        codes.copy_(torch.round(x.double() * 127 / top.double().clamp_min(1e-300)[..., None]))
+    else:
+        for part, row, most in zip(codes, x, top):  # a kernel at a time: they are large
+            part.copy_(torch.round(row.double() * 127 / most.double().clamp_min(1e-300)[..., None]))
+    return codes, top / 127
+
+
+def _plain_int8(s):
+    case, e, most = s["case"], s["case"]["experts"], s["most"]
+    codes, scales = _to_int8(s["z"])
+    token = s["order"].long() // case["k"]
+    rows = torch.zeros(e * most, case["d"], dtype=F32, device="cuda")
+    rows[s["slot"]] = codes[token]
+    y = torch.bmm(rows.view(e, most, -1), s["kernel_codes"].float().transpose(1, 2).contiguous())
+    y = (y * s["kernel_scales"][:, None, :]).view(e * most, -1)[s["slot"]]
+    return {"y": (y * scales[token][:, None]).to(BF16)}
+
+
+def _plain(s):
+    case = s["case"]
+    if case["kind"] == "norm":
+        if case["direction"] == "backward":
+            return _plain_norm_backward(s)
+        if s["residual"] is None:
+            return {"out": _plain_norm(s["x"], s)}
+        summed = (s["x"].float() + s["residual"].float()).to(s["x"].dtype)
+        return {"out": _plain_norm(summed, s), "summed": summed}
+    return _plain_route_backward(s) if case["kind"] == "route" else _plain_int8(s)
+
+
+# --- the framework's -------------------------------------------------------------------------
+
+
+def _call(s):
+    from bux_amd import grouped_int8, moe, norm, router
+    case = s["case"]
+    if case["kind"] == "norm":
+        settings = moe.ExpertNorm(case["norm"], EPS, bias=case["bias"])
+        if case["direction"] == "backward":
+            g = norm.normed_backward(s["dy"], s["x"], s["stats"], settings, s["scale"],
+                                     d_summed=s["d_summed"])
+            return {"x": g.x, "scale": g.scale, "bias": g.bias}
+        r = norm.normed(s["x"], settings, s["scale"], s["bias"], residual=s["residual"])
+        if s["residual"] is None:
+            return {"out": r.out}
+        return {"out": r.out, "summed": r.summed}
+    if case["kind"] == "route":
+        g = router.route_backward(
+            s["x"], s["kernel"], s["idx"], s["logits"], s["d_weights"], router=case["router"],
+            normalize_top_k=case["normalize"], routed_scaling_factor=case["scaling"],
+            d_scores=s["d_scores"], dz=s["dz"])
+        return {"x": g.x, "kernel": g.kernel, "bias": g.bias}
+    m, tiles = s["order"].numel(), s["tiles"]
+    a = grouped_int8.quantized(s["z"], s["filled"], s["order"], case["k"], tiles.m)
+    return {"y": grouped_int8.rows(a, s["quantized"], s["sizes"], BF16, height=m, tiles=tiles)}
+
+
+def run(state):
+    if own:
+        return _call(state)
+    return _plain(state)
+
+
+# --- what a pass cannot do without --------------------------------------------------------
+
+
+def work(case):
+    t, d = case["tokens"], case["d"]
+    size = 4 if case.get("dtype") == "float32" else 2
+    if case["kind"] == "norm":
+        params = d * size * (2 if case["bias"] else 1)
+        if case["direction"] == "forward":
+            return {"bytes": t * d * size * (4 if case["residual"] else 2) + params,
+                    "flops": 8 * t * d}
+        return {"bytes": t * d * size * (4 if case["residual"] else 3) + t * 8 + params
+                + d * 4 * (2 if case["bias"] else 1), "flops": 16 * t * d}
+    e, k = case["experts"], case["k"]
+    if case["kind"] == "route":
+        read = t * d * 2 + d * e * 2 + t * e * 4 + t * k * 6
+        read += t * e * 4 * case["balance"] + t * d * 2 * case["add"]
+        return {"bytes": read + t * d * 2 + d * e * 2 + e * 4, "flops": 4 * t * d * e}
+    m, n = t * k, case["n"]
+    # the kernels of the experts that even picks reach
+    live = e * (1 - (1 - k / e) ** t)
+    return {"bytes": int(t * d * 2 + live * (d * n + 4 * n) + m * 4 + m * n * 2),
+            "flops": 2 * m * d * n}
+
+
+# --- in 64 bits ------------------------------------------------------------------------------
+
+
+def _exact_norm(case, x):
+    v, centred = x["x"].to(F64), case["norm"] == "layernorm"
+    out = {}
+    if x["residual"] is not None:
+        kept = x["x"].float().add(x["residual"].float()).to(x["x"].dtype)  # held in the rows' type
+        v = kept.to(F64)
+        out["summed"] = v
+    if centred:
+        v = v - v.sum(-1, keepdim=True) / case["d"]
+    r = 1 / torch.sqrt(v.pow(2).sum(-1, keepdim=True) / case["d"] + EPS)
+    gain = x["scale"].to(F64)
+    if case["direction"] == "forward":
+        out["out"] = v * r * gain + (0 if x["bias"] is None else x["bias"].to(F64))
+        return out
+    g = x["dy"].to(F64)
+    h = g * gain
+    # the normalization's Jacobian applied to h: r (h - mean h - v r^2 mean(h v))
+    dx = r * (h - v * r.pow(2) * (h * v).sum(-1, keepdim=True) / case["d"])
+    if centred:
+        dx = dx - r * h.sum(-1, keepdim=True) / case["d"]
+    if x["d_summed"] is not None:
+        dx = dx + x["d_summed"].to(F64)
+    return {"x": dx, "scale": torch.einsum("td,td->d", g, v * r),
+            "bias": None if x["bias"] is None else g.sum(0)}
+
+
+def _exact_route(case, x):
+    z = x["logits"].to(F64)
+    top = z.max(-1, keepdim=True).values
+    p = torch.exp(z - top)
+    p = p / p.sum(-1, keepdim=True) if case["router"] == "softmax" else 1 / (1 + torch.exp(-z))
+    picked = torch.zeros_like(p)
+    picked.scatter_(1, x["idx"].long(), 1.0)
+    up = torch.zeros_like(p)
+    up.scatter_(1, x["idx"].long(), x["d_weights"].to(F64) * case["scaling"])
+    if case["normalize"]:
+        # w = p picked / sum(p picked)
+        total = (p * picked).sum(-1, keepdim=True)
+        up = picked * (up / total - (up * p).sum(-1, keepdim=True) / total.pow(2))
+    if x["d_scores"] is not None:
+        up = up + x["d_scores"].to(F64)
+    if case["router"] == "softmax":
+        dl = p * up - p * (p * up).sum(-1, keepdim=True)
+    else:
+        dl = up * (p - p * p)
+    dx = torch.mm(dl, x["kernel"].to(F64).t().contiguous())
+    if x["dz"] is not None:
+        dx += x["dz"].to(F64)
+    return {"x": dx, "kernel": torch.mm(x["x"].to(F64).t().contiguous(), dl), "bias": dl.sum(0)}
+
+
+def _exact_int8(case, x):
+    def codes(v):
+        v = v.to(F64)
+        top = v.abs().max(-1, keepdim=True).values
+        return torch.round(torch.where(top > 0, v * 127 / top, 0.0)), top / 127
+
+    q, s = codes(x["z"])
+    token = x["order"].long() // case["k"]
+    y = torch.empty(token.numel(), case["n"], dtype=F64, device="cuda")
+    at = 0
+    for kernel, size in zip(x["kernels"], x["sizes"].tolist()):
+        if size:
+            rows = token[at:at + size]
+            w, ws = codes(kernel.t())
+            y[at:at + size] = torch.mm(q[rows], w.t().contiguous()) * s[rows] * ws.t()
+        at += size
+    return {"y": y}
+
+
+def exact(case, seed):
+    x = _inputs(case, seed)
+    if case["kind"] == "norm":
+        return _exact_norm(case, x)
+    return _exact_route(case, x) if case["kind"] == "route" else _exact_int8(case, x)
