@@ -307,9 +307,9 @@ def _plain(s):
 
 
 def _call(s):
-    from bux_amd import grouped_int8, moe, norm, router
     case = s["case"]
     if case["kind"] == "norm":
+        from bux_amd import moe, norm
         settings = moe.ExpertNorm(case["norm"], EPS, bias=case["bias"])
         if case["direction"] == "backward":
             g = norm.normed_backward(s["dy"], s["x"], s["stats"], settings, s["scale"],
@@ -320,11 +320,13 @@ def _call(s):
             return {"out": r.out}
         return {"out": r.out, "summed": r.summed}
     if case["kind"] == "route":
+        from bux_amd import router
         g = router.route_backward(
             s["x"], s["kernel"], s["idx"], s["logits"], s["d_weights"], router=case["router"],
             normalize_top_k=case["normalize"], routed_scaling_factor=case["scaling"],
             d_scores=s["d_scores"], dz=s["dz"])
         return {"x": g.x, "kernel": g.kernel, "bias": g.bias}
+    from bux_amd import grouped_int8
     m, tiles = s["order"].numel(), s["tiles"]
     a = grouped_int8.quantized(s["z"], s["filled"], s["order"], case["k"], tiles.m)
     return {"y": grouped_int8.rows(a, s["quantized"], s["sizes"], BF16, height=m, tiles=tiles)}
