@@ -116,6 +116,13 @@ SIGNATURES = {
     "bux_expert_norm_backward_f32": (
         _int, [_p, _p, _i32, _i64, _p, _i64, _i64, _p, _p, _i32, _norm, _p, _p, _p, _p, _p, _p, _p,
                _p, _size, _p]),
+    "bux_norm_forward": (_int, [_p, _p, _i64, _i64, _norm, _p, _p, _p, _p, _p, _p]),
+    "bux_norm_forward_f32": (_int, [_p, _p, _i64, _i64, _norm, _p, _p, _p, _p, _p, _p]),
+    "bux_norm_backward_workspace_size": (_size, [_i64, _i64]),
+    "bux_norm_backward": (
+        _int, [_p, _p, _p, _p, _i64, _i64, _norm, _p, _p, _p, _p, _p, _size, _p]),
+    "bux_norm_backward_f32": (
+        _int, [_p, _p, _p, _p, _i64, _i64, _norm, _p, _p, _p, _p, _p, _size, _p]),
     "bux_glu_forward": (_int, [_p, _p, _p, _i64, _i64, _ffn, _p, _p]),
     "bux_glu_backward": (_int, [_p, _p, _p, _p, _i64, _i64, _ffn, _p, _p, _p]),
     "bux_glu_forward_f32": (_int, [_p, _p, _p, _i64, _i64, _ffn, _p, _p]),

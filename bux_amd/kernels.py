@@ -8,6 +8,7 @@ on a gfx950 GPU (MI355X), unless ``BUX_KERNELS=off``. There is no other
 implementation to fall back to: an op called where they do not run raises.
 """
 
+import contextlib
 import functools
 import os
 
@@ -73,6 +74,16 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def stream() -> int:
     """Return the current HIP stream's handle, on which every op enqueues its kernels."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+_CURRENT = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """A context in which `t`'s GPU is the current one: for the op's buffers, its stream and
+    its launches."""
+    index = t.get_device()
+    return _CURRENT if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

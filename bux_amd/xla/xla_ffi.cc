@@ -640,6 +640,60 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxExpertNormBackward, ExpertNormBackward,
                                   .Attr<int64_t>("index_div") BUX_NORM_ATTRS.Ret<In>()
                                   .Ret<In>().Ret<In>().Ret<In>().Ret<In>());
 
+// --- the tokens' norm -------------------------------------------------------------------
+// x [m, d]; residual (with summed), scale, bias, stats and d_summed may be empty.
+
+template <typename T>
+static ffi::Error token_norm_as(hipStream_t s, In x, In residual, In scale, In bias,
+                                const bux_norm& norm, Out summed, Out out, Out stats) {
+  if constexpr (sizeof(T) == 4)
+    return status(bux_norm_forward_f32(at<const T>(x), at<const T>(residual), dim(x, 0), dim(x, 1),
+                                       &norm, at<const T>(scale), at<const T>(bias), at<T>(summed),
+                                       at<T>(out), at<float>(stats), s));
+  else
+    return status(bux_norm_forward(at<const T>(x), at<const T>(residual), dim(x, 0), dim(x, 1),
+                                   &norm, at<const T>(scale), at<const T>(bias), at<T>(summed),
+                                   at<T>(out), at<float>(stats), s));
+}
+template <typename T>
+static ffi::Error token_norm_grad_as(hipStream_t s, In dy, In x, In stats, In d_summed, In scale,
+                                     const bux_norm& norm, Out dx, Out d_scale, Out d_bias,
+                                     Out ws) {
+  if constexpr (sizeof(T) == 4)
+    return status(bux_norm_backward_f32(
+        at<const T>(dy), at<const T>(x), at<const float>(stats), at<const T>(d_summed), dim(x, 0),
+        dim(x, 1), &norm, at<const T>(scale), at<T>(dx), at<float>(d_scale), at<float>(d_bias),
+        at<void>(ws), ws->size_bytes(), s));
+  else
+    return status(bux_norm_backward(
+        at<const T>(dy), at<const T>(x), at<const float>(stats), at<const T>(d_summed), dim(x, 0),
+        dim(x, 1), &norm, at<const T>(scale), at<T>(dx), at<float>(d_scale), at<float>(d_bias),
+        at<void>(ws), ws->size_bytes(), s));
+}
+
+static ffi::Error NormForward(hipStream_t s, In x, In residual, In scale, In bias,
+                              BUX_NORM_PARAMS, Out summed, Out out, Out stats) {
+  const bux_norm norm = BUX_NORM;
+  return f32(x) ? token_norm_as<float>(s, x, residual, scale, bias, norm, summed, out, stats)
+                : token_norm_as<uint16_t>(s, x, residual, scale, bias, norm, summed, out, stats);
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxNormForward, NormForward,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
+                                  .Arg<In>() BUX_NORM_ATTRS.Ret<In>().Ret<In>().Ret<In>());
+
+static ffi::Error NormBackward(hipStream_t s, In dy, In x, In stats, In d_summed, In scale,
+                               BUX_NORM_PARAMS, Out dx, Out d_scale, Out d_bias, Out ws) {
+  const bux_norm norm = BUX_NORM;
+  return f32(x) ? token_norm_grad_as<float>(s, dy, x, stats, d_summed, scale, norm, dx, d_scale,
+                                            d_bias, ws)
+                : token_norm_grad_as<uint16_t>(s, dy, x, stats, d_summed, scale, norm, dx, d_scale,
+                                               d_bias, ws);
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxNormBackward, NormBackward,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
+                                  .Arg<In>().Arg<In>() BUX_NORM_ATTRS.Ret<In>().Ret<In>()
+                                  .Ret<In>().Ret<In>());
+
 // --- the router ----------------------------------------------------------------------
 // x [t, d], kernel [d, n_logits]; bias and choice_bias may be empty, as may the sinks,
 // scores and logits results.

@@ -503,6 +503,44 @@ int bux_expert_norm_backward_f32(const float* dy, const int32_t* index, int32_t 
                                  size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * The tokens' norm before a layer, with the residual stream's addition.
+ *
+ * The model's Norm (src/bux/architecture/layers/norm.py:14-78) of m rows of d columns (8 to
+ * 12288, any such d), settings `bux_norm`'s, in float32 inside with one rounding at the end
+ * (bux_expert_norm_forward rounds at every step):
+ *   u = x + residual, rounded to the rows' type and stored in `summed`; without a residual
+ *     (NULL, with `summed` NULL too) u = x;
+ *   v = u, or with scale_input u g;  g = scale, or 1 + scale if zero_centered, 1 if not affine;
+ *   c = v - mean(v) (BUX_LAYERNORM) or v;  r = 1 / sqrt(mean(c^2) + eps);
+ *   out = c r g + bias (without scale_input), c r + bias (with it).
+ * scale and bias [d], NULL where the norm has none; stats float32 [m, 2]: each row's mean (0
+ * for an rmsnorm) and r, for the backward; NULL to skip. Rows follow one another without a
+ * gap; any alignment of an element.
+ * bux_norm_backward: given dy [m, d], u (x, or `summed`), the stats and d_summed [m, d] (the
+ * gradient that reaches u past the norm; NULL for none), dx [m, d] = the norm's gradient plus
+ * d_summed, in float32 with one rounding (the gradient to x and to the residual alike); and
+ * d_scale, d_bias float32 [d], their sums over the rows in a fixed order (written; NULL where
+ * the norm has none). workspace: bux_norm_backward_workspace_size(m, d) bytes, at most 8 m d and
+ * at most 8192 d; it never falls as m or d grows.
+ */
+int bux_norm_forward(const uint16_t* x, const uint16_t* residual, int64_t m, int64_t d,
+                     const bux_norm* norm, const uint16_t* scale, const uint16_t* bias,
+                     uint16_t* summed, uint16_t* out, float* stats, void* stream);
+size_t bux_norm_backward_workspace_size(int64_t m, int64_t d);
+int bux_norm_backward(const uint16_t* dy, const uint16_t* x, const float* stats,
+                      const uint16_t* d_summed, int64_t m, int64_t d, const bux_norm* norm,
+                      const uint16_t* scale, uint16_t* dx, float* d_scale, float* d_bias,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* The same for float32 rows, parameters and gradients. */
+int bux_norm_forward_f32(const float* x, const float* residual, int64_t m, int64_t d,
+                         const bux_norm* norm, const float* scale, const float* bias,
+                         float* summed, float* out, float* stats, void* stream);
+int bux_norm_backward_f32(const float* dy, const float* x, const float* stats,
+                          const float* d_summed, int64_t m, int64_t d, const bux_norm* norm,
+                          const float* scale, float* dx, float* d_scale, float* d_bias,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------
  * a-8 with a-4. The activation and its gradient, quantized as they are computed.
  *
  * The reference fuses the activation and the weight into its up GEMM's epilogue on

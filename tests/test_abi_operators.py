@@ -1,0 +1,72 @@
+"""The C-ABI of the operators around the experts without a GPU: the host-side checks turn bad
+shapes, settings and workspaces into error codes and messages before any kernel launch."""
+
+import ctypes
+import os
+
+import pytest
+
+from bux_amd import _lib
+
+P = ctypes.c_void_p(16)  # never dereferenced: the checks fail first
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_lib.PATH):
+        pytest.fail(f"{_lib.PATH} is not built: run python -m bux_amd.build")
+    return _lib.load()
+
+
+def _msg(lib) -> str:
+    return lib.bux_last_error().decode()
+
+
+def _norm(kind=0, affine=1, bias=1, eps=1e-6):
+    return ctypes.byref(_lib.NormStruct(kind, affine, 0, 0, bias, eps))
+
+
+@pytest.mark.parametrize("twin", ["", "_f32"])
+def test_the_tokens_norm_rejects_bad_arguments(lib, twin):
+    forward = getattr(lib, "bux_norm_forward" + twin)
+    backward = getattr(lib, "bux_norm_backward" + twin)
+
+    def fwd(m=4, d=64, norm=_norm(), residual=None, scale=P, bias=P, summed=None, x=P, out=P):
+        return forward(x, residual, m, d, norm, scale, bias, summed, out, P, None)
+
+    def bwd(m=4, d=64, norm=_norm(), dy=P, scale=P, d_scale=P, d_bias=P, ws=P, nbytes=1 << 20,
+            stats=P):
+        return backward(dy, P, stats, None, m, d, norm, scale, P, d_scale, d_bias, ws, nbytes, None)
+
+    for call in (fwd, bwd):
+        for bad in ({"d": 7}, {"d": 12289}, {"m": -1}, {"m": 1 << 31}):
+            assert call(**bad) == 1 and "bad shape" in _msg(lib), bad
+        assert call(norm=None) == 1 and "NULL norm" in _msg(lib)
+        assert call(norm=_norm(kind=2)) == 1 and "kind 2" in _msg(lib)
+        assert call(norm=_norm(eps=-1.0)) == 1 and "eps" in _msg(lib)
+        assert call(norm=_norm(eps=float("nan"))) == 1 and "eps" in _msg(lib)
+        assert call(scale=None) == 1 and "scale" in _msg(lib)
+    assert fwd(bias=None) == 1 and "bias" in _msg(lib)
+    assert fwd(residual=P) == 1 and "summed" in _msg(lib)
+    assert fwd(summed=P) == 1 and "summed" in _msg(lib)
+    assert fwd(x=None) == 1 and "NULL buffer" in _msg(lib)
+    assert fwd(out=None) == 1 and "NULL buffer" in _msg(lib)
+    assert fwd(m=0, x=None, out=None) == 0
+    assert bwd(d_scale=None) == 1 and "d_scale" in _msg(lib)
+    assert bwd(d_bias=None) == 1 and "d_bias" in _msg(lib)
+    assert bwd(dy=None) == 1 and "NULL buffer" in _msg(lib)
+    assert bwd(stats=None) == 1 and "NULL buffer" in _msg(lib)
+    assert bwd(nbytes=2 * 4 * 64 * 4 - 1) == 2 and "workspace" in _msg(lib)
+    assert bwd(ws=None) == 2 and "workspace" in _msg(lib)
+
+
+def test_the_tokens_norms_workspace_never_falls_as_rows_grow(lib):
+    size = lib.bux_norm_backward_workspace_size
+    for d in (8, 1537, 2048, 12288):
+        sizes = [size(m, d) for m in [*range(0, 1100), 4096, 70000, 1 << 30]]
+        assert sizes == sorted(sizes) and sizes[0] == 0
+        assert all(s <= 8 * m * d for m, s in enumerate(sizes[:1100]))
+        assert sizes[-1] <= 8192 * d
+    for m in (1, 513, 70000):
+        sizes = [size(m, d) for d in range(8, 12289)]
+        assert sizes == sorted(sizes)
