@@ -152,6 +152,10 @@ SIGNATURES = {
     "bux_route": (
         _int, [_p, _p, _p, _i64, _i64, _i32, _f32, _int, _i32, _p, _i32, _i32, _i32, _int, _f32,
                _p, _p, _p, _p, _p, _p, _size, _p]),
+    "bux_route_backward_workspace_size": (_size, [_i64, _i64, _i32]),
+    "bux_route_backward": (
+        _int, [_p, _p, _i64, _i64, _i32, _f32, _int, _i32, _p, _i32, _int, _f32, _p, _p, _p, _p, _p,
+               _p, _p, _p, _p, _p, _size, _p]),
 }
 
 # Constants of include/bux_amd.h.

@@ -389,6 +389,10 @@ int settings_of(const char* name, int64_t m, int64_t d, const bux_norm* norm, co
   BUX_CHECK(m >= 0 && m < (1LL << 31) && d >= VEC && d <= MAX_WIDTH,
             "%s: bad shape m=%lld d=%lld (d of %d to %lld)", name, (long long)m, (long long)d, VEC,
             (long long)MAX_WIDTH);
+  // a launch holds fewer than 2^32 threads, and a row takes 64 of them at least
+  BUX_CHECK(m * ceil_div(d, 64 * VEC * MAX_CHUNKS) < (1LL << 25),
+            "%s: m=%lld rows of d=%lld are more than a launch holds", name, (long long)m,
+            (long long)d);
   BUX_CHECK(norm != nullptr, "%s: NULL norm", name);
   BUX_CHECK(norm->kind == BUX_LAYERNORM || norm->kind == BUX_RMSNORM,
             "%s: kind %d is neither BUX_LAYERNORM nor BUX_RMSNORM", name, norm->kind);

@@ -8,6 +8,10 @@ fields are ``MoEConfig``'s (src/bux/config.py:236-275): ``router``,
 ``router_logit_scale``, ``normalize_top_k``, ``routed_scaling_factor``,
 ``num_groups``, ``top_k_groups``; the kernel's columns past the scored experts are the
 shared experts' sinks (``shared_expert_sink``, moe.py:143-153).
+
+`route_backward` is its transpose for training (``bux_route_backward``): from the gradients
+that the experts' backward gives the picks' weights, and those of losses on the scores and
+logits, to the tokens, the router's kernel and its bias.
 """
 
 from typing import NamedTuple
@@ -15,7 +19,7 @@ from typing import NamedTuple
 import torch
 
 from bux_amd import _lib
-from bux_amd.kernels import lib, ptr, require, stream, workspace
+from bux_amd.kernels import lib, on_device, ptr, require, stream, workspace
 
 ROUTERS = {"softmax": _lib.ROUTER_SOFTMAX, "sigmoid": _lib.ROUTER_SIGMOID,
            "sqrtsoftplus": _lib.ROUTER_SQRTSOFTPLUS}
@@ -79,3 +83,73 @@ def route(x: torch.Tensor, kernel: torch.Tensor, *, top_k: int, scored: int | No
 
     return Routed(shaped(idx, top_k), shaped(weights, top_k), shaped(sinks, n - scored),
                   shaped(scores, scored), shaped(logits, n))
+
+
+class RouteGrads(NamedTuple):
+    """What `route_backward` returns."""
+
+    x: torch.Tensor  # bfloat16, x's shape: to the tokens (plus dz)
+    kernel: torch.Tensor  # bfloat16 (d, n): to the router's kernel
+    bias: torch.Tensor  # float32 (n,): to the router's own bias
+
+
+def route_backward(x: torch.Tensor, kernel: torch.Tensor, idx: torch.Tensor, logits: torch.Tensor,
+                   d_weights: torch.Tensor, *, scored: int | None = None, router: str = "softmax",
+                   router_logit_scale: float = 1.0, normalize_top_k: bool = True,
+                   routed_scaling_factor: float = 1.0, d_sinks: torch.Tensor | None = None,
+                   d_scores: torch.Tensor | None = None, d_logits: torch.Tensor | None = None,
+                   dz: torch.Tensor | None = None) -> RouteGrads:
+    """The gradients of `route` (of the same x, kernel and settings) given those of its picks'
+    weights, `d_weights` (..., k) bfloat16: idx and logits as `route` returned them
+    (``with_logits``).
+
+    d_sinks: the sinks' weights' gradient (..., n - scored) bfloat16. d_scores: float32 (...,
+    scored), the gradient of a loss on the scores (a balance loss). d_logits: float32 (..., n),
+    of one on the logits (a z-loss). dz: bfloat16 of x's shape, the gradient that reached the
+    tokens through the experts (`moe.experts_backward`'s "z"), added before x's gradient is
+    rounded. The roundings to bfloat16 in the forward pass gradients as they are; the aux-free
+    `router_bias` has none. The sums' order is fixed."""
+    require(x, kernel, idx, logits, d_weights, d_sinks, d_scores, d_logits, dz)
+    if x.dtype != torch.bfloat16 or kernel.dtype != torch.bfloat16:
+        raise TypeError("x and kernel are bfloat16")
+    if router not in ROUTERS:
+        raise ValueError(f"router {router!r}: one of {sorted(ROUTERS)}")
+    lead, d = x.shape[:-1], x.shape[-1]
+    if kernel.dim() != 2 or kernel.shape[0] != d:
+        raise ValueError(f"kernel {tuple(kernel.shape)} for width {d}")
+    n = kernel.shape[1]
+    scored = n if scored is None else scored
+    if not 1 <= scored <= n:
+        raise ValueError(f"scored={scored} outside [1, {n}]")
+    if idx.dim() != x.dim():
+        raise ValueError(f"idx {tuple(idx.shape)} for tokens {tuple(x.shape)}")
+    k = idx.shape[-1]
+    for name, v, dtype, width in (
+            ("idx", idx, torch.int32, k), ("logits", logits, torch.float32, n),
+            ("d_weights", d_weights, torch.bfloat16, k),
+            ("d_sinks", d_sinks, torch.bfloat16, n - scored),
+            ("d_scores", d_scores, torch.float32, scored),
+            ("d_logits", d_logits, torch.float32, n), ("dz", dz, torch.bfloat16, d)):
+        if v is None:
+            continue
+        if v.dtype != dtype or v.shape != (*lead, width) or v.device != x.device:
+            raise ValueError(f"{name}: {dtype} {(*lead, width)} on {x.device}, not {v.dtype} "
+                             f"{tuple(v.shape)} on {v.device}")
+    if kernel.device != x.device:
+        raise ValueError(f"kernel on {kernel.device} beside tokens on {x.device}")
+    t = x.numel() // d if d else 0
+    dev = x.device
+    with on_device(x):
+        dx = torch.empty_like(x)
+        d_kernel = torch.empty_like(kernel)
+        d_bias = torch.empty(n, dtype=torch.float32, device=dev)
+        ws = workspace(lib().bux_route_backward_workspace_size(t, d, n), dev)
+        rc = lib().bux_route_backward(
+            ptr(x), ptr(kernel), t, d, n, router_logit_scale, ROUTERS[router], scored, ptr(idx), k,
+            int(normalize_top_k), routed_scaling_factor, ptr(logits), ptr(d_weights), ptr(d_sinks),
+            ptr(d_scores), ptr(d_logits), ptr(dz), ptr(dx), ptr(d_kernel), ptr(d_bias), ptr(ws),
+            ws.numel(), stream())
+    if rc == 1:  # BUX_E_ARGUMENT
+        raise ValueError(lib().bux_last_error().decode())
+    _lib.check(rc)
+    return RouteGrads(dx, d_kernel, d_bias)

@@ -718,6 +718,29 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxRoute, Route,
                                   .Attr<int64_t>("normalize").Attr<float>("scaling")
                                   .Ret<In>().Ret<In>().Ret<In>().Ret<In>().Ret<In>().Ret<In>());
 
+// x [t, d], kernel [d, n_logits]; d_sinks, d_scores, d_logits and dz may be empty, as may the
+// bias's gradient.
+static ffi::Error RouteBackward(hipStream_t s, In x, In kernel, In idx, In logits, In d_weights,
+                                In d_sinks, In d_scores, In d_logits, In dz, float logit_scale,
+                                int64_t router, int64_t scored, int64_t normalize, float scaling,
+                                Out dx, Out d_kernel, Out d_bias, Out ws) {
+  return status(bux_route_backward(
+      at<const uint16_t>(x), at<const uint16_t>(kernel), dim(x, 0), dim(x, 1),
+      static_cast<int32_t>(dim(kernel, 1)), logit_scale, static_cast<int>(router),
+      static_cast<int32_t>(scored), at<const int32_t>(idx), static_cast<int32_t>(dim(idx, 1)),
+      static_cast<int>(normalize), scaling, at<const float>(logits),
+      at<const uint16_t>(d_weights), at<const uint16_t>(d_sinks), at<const float>(d_scores),
+      at<const float>(d_logits), at<const uint16_t>(dz), at<uint16_t>(dx), at<uint16_t>(d_kernel),
+      at<float>(d_bias), at<void>(ws), ws->size_bytes(), s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxRouteBackward, RouteBackward,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
+                                  .Arg<In>().Arg<In>().Arg<In>().Arg<In>().Arg<In>().Arg<In>()
+                                  .Attr<float>("logit_scale").Attr<int64_t>("router")
+                                  .Attr<int64_t>("scored").Attr<int64_t>("normalize")
+                                  .Attr<float>("scaling").Ret<In>().Ret<In>().Ret<In>()
+                                  .Ret<In>());
+
 // --- the MXFP8 wire rows ----------------------------------------------------------------
 
 // packed [m, d + d/32]; index may be empty.

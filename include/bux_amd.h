@@ -675,6 +675,30 @@ int bux_route(const uint16_t* x, const uint16_t* kernel, const float* bias, int6
               float scaling, int32_t* idx, uint16_t* weights, uint16_t* sinks, float* scores,
               float* logits, void* workspace, size_t workspace_bytes, void* stream);
 
+/* bux_route_backward: the router's transpose (of bux_route, moe.py:249-270): given the
+ * gradients of the picks' weights, and of the sinks' (d_sinks), of the scores (d_scores, before
+ * the choice bias: a balance loss's) and of the logits (d_logits: a z-loss's), each NULL for
+ * none but the first:
+ *   dx [t, d] = dz + G kernel^T, d_kernel [d, n_logits] = x^T G, d_bias [n_logits] = the sum of
+ *   G over the tokens; G [t, n_logits] the gradient of x @ kernel + bias.
+ * logits float32 [t, n_logits] and idx [t, k] as bux_route wrote them (idx outside [0, scored)
+ * takes no part; one made twice counts twice); d_weights bfloat16 [t, k]; d_sinks bfloat16
+ * [t, n_logits - scored]; d_scores float32 [t, scored]; d_logits float32 [t, n_logits]; dz
+ * bfloat16 [t, d], the gradient that reached the tokens on other ways (NULL for none), added
+ * before the one rounding. dx, d_kernel bfloat16; d_bias float32, NULL to skip. The forward's
+ * roundings to bfloat16 pass gradients as they are; the choice bias has none. float32 sums, in
+ * a fixed order; G enters its products in two bfloat16 parts (2^-17 of each). The limits of
+ * bux_route, without groups. workspace: bux_route_backward_workspace_size(t, d, n_logits)
+ * bytes: G, and d_kernel's partial sums. */
+size_t bux_route_backward_workspace_size(int64_t t, int64_t d, int32_t n_logits);
+int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int64_t t, int64_t d,
+                       int32_t n_logits, float logit_scale, int router, int32_t scored,
+                       const int32_t* idx, int32_t k, int normalize, float scaling,
+                       const float* logits, const uint16_t* d_weights, const uint16_t* d_sinks,
+                       const float* d_scores, const float* d_logits, const uint16_t* dz,
+                       uint16_t* dx, uint16_t* d_kernel, float* d_bias, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------------
  * MXFP8 rows of bytes: what an expert-parallel dispatch in MXFP8 sends a token.
  *

@@ -70,3 +70,23 @@ def test_the_tokens_norms_workspace_never_falls_as_rows_grow(lib):
     for m in (1, 513, 70000):
         sizes = [size(m, d) for d in range(8, 12289)]
         assert sizes == sorted(sizes)
+
+
+def test_the_routers_backward_rejects_bad_arguments(lib):
+    def call(t=8, d=64, n=32, router=0, scored=30, k=2, kernel=P, d_kernel=P, x=P, d_sinks=P,
+             ws=P, nbytes=1 << 24):
+        return lib.bux_route_backward(x, kernel, t, d, n, 1.0, router, scored, P, k, 1, 1.0, P, P,
+                                      d_sinks, None, None, None, P, d_kernel, P, ws, nbytes, None)
+
+    for bad, word in (({"t": -1}, "t=-1"), ({"d": 40}, "d=40"), ({"d": 0}, "d=0"),
+                      ({"n": 0}, "n_logits=0"), ({"n": 1025}, "n_logits=1025"),
+                      ({"scored": 0}, "scored=0"), ({"scored": 33}, "scored=33"),
+                      ({"router": 3}, "router=3"), ({"k": 0}, "k=0"), ({"k": 17}, "k=17"),
+                      ({"scored": 1, "k": 2}, "k=2"), ({"scored": 32}, "d_sinks"),
+                      ({"kernel": None}, "NULL"), ({"d_kernel": None}, "NULL"), ({"x": None}, "NULL"),
+                      ({"t": 1 << 30, "d": 4096}, "launch")):
+        assert call(**bad) == 1 and word in _msg(lib), (bad, _msg(lib))
+    need = lib.bux_route_backward_workspace_size(8, 64, 32)
+    assert need >= 8 * 32 * 4 + 64 * 32 * 4
+    assert call(nbytes=need - 1) == 2 and "workspace" in _msg(lib)
+    assert call(ws=None) == 2 and "workspace" in _msg(lib)
