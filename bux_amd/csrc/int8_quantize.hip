@@ -1,0 +1,414 @@
+// 8-bit integers with a scale a row: rows of tokens (by pick too), the activation's rows as
+// they are computed, and the columns of the experts' kernels.
+//
+//   s = max |x| / 127,  q = the integer nearest 127 x / max |x|, the even one at a tie
+//
+// q is that of the exact quotient. In bfloat16, 127 / max |x| goes in two float32 parts, hi and
+// lo, and x hi + (x lo) is the quotient rounded once (to 2^-29 of it): a quotient that is no tie
+// lies 2^-17 from one at least (two products of 8-bit mantissas, over one), twice the rounding
+// there, and a tie is a float32. In float32 the quotient's nearest integer n comes in float64
+// and 127 x - n max |x|, exact there, moves it by one where it exceeds half of max |x|. A row of
+// zeros has scale 0 and codes 0; one that holds an infinity or a NaN has that as its scale and
+// codes of 0, so that its products are NaN.
+//
+// The codes are in the GEMM's tiled layout, [K / 64][rows][64] with K padded to whole 128s.
+// Bound by HBM: a wave takes a row, in registers where it has at most 512 C columns (else read
+// twice, the second time from L2); a workgroup's 4 rows write 256 bytes of each K chunk in one run.
+
+#include <type_traits>
+
+#include "glu.h"
+
+namespace bux {
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int64_t MAX_K = 131072;  // 127^2 K stays below 2^31
+
+template <typename T>
+struct Part {
+  T at[8];
+};
+
+// The larger magnitude's bits of a part's 8 values: as unsigned integers, with infinities above
+// every finite value and NaN above those.
+__device__ __forceinline__ uint32_t top_of(const Part<uint16_t>& p) {
+  const uint4 w = __builtin_bit_cast(uint4, p);
+  uint32_t m = max_abs_pair(max_abs_pair(max_abs_pair(max_abs_pair(0u, w.x), w.y), w.z), w.w);
+  return larger_half(m) << 16;  // as a float32's bits
+}
+__device__ __forceinline__ uint32_t top_of(const Part<float>& p) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = __float_as_uint(p.at[j]) & 0x7fffffffu;
+    m = b > m ? b : m;
+  }
+  return m;
+}
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const uint32_t u = __shfl_xor(v, o);
+    v = u > v ? u : v;
+  }
+  return v;
+}
+
+// How a row whose largest magnitude is `top` turns into codes.
+template <typename T>
+struct Coder {
+  float scale;
+  float pre, hi, lo;    // bfloat16: the quotient is x pre hi + x pre lo
+  double most, inverse;  // float32
+  __device__ __forceinline__ explicit Coder(uint32_t top) {
+    const float a = __uint_as_float(top);
+    scale = a / 127.0f;
+    const bool live = top > 0 && top < 0x7f800000u;
+    if constexpr (std::is_same<T, uint16_t>::value) {
+      // tiny rows first times 2^64, so that 127 / a stays finite; in others 1
+      pre = live ? (a < 0x1p-100f ? 0x1p64f : 1.0f) : 0.0f;
+      const float b = a * pre;
+      hi = live ? 127.0f / b : 0.0f;
+      lo = live ? __builtin_fmaf(-hi, b, 127.0f) / b : 0.0f;
+    } else {
+      most = live ? a : 0.0;
+      inverse = live ? 127.0 / static_cast<double>(a) : 0.0;
+    }
+  }
+  // The code of x in the low byte; 0 for every x of a row of zeros, infinities or NaN.
+  __device__ __forceinline__ uint32_t code(float x) const {
+    if constexpr (std::is_same<T, uint16_t>::value) {
+#pragma clang fp contract(off)
+      if (hi == 0.0f) return 0;
+      const float v = x * pre;
+      const float q = __builtin_fmaf(v, hi, v * lo);
+      // adding 1.5 2^23 rounds to the nearest integer, the even one at a tie
+      return __float_as_uint(q + 12582912.0f);
+    } else {
+      if (most == 0.0) return 0;
+      const double v = x;
+      double n = __builtin_rint(v * inverse);
+      const double r = __builtin_fma(-n, most, 127.0 * v);  // exact
+      if (2.0 * r > most) n += 1.0;
+      else if (2.0 * r < -most) n -= 1.0;
+      else if (__builtin_fabs(2.0 * r) == most) n = 2.0 * __builtin_rint(0.5 * (n + r / most));
+      return static_cast<uint32_t>(static_cast<int32_t>(n));
+    }
+  }
+  __device__ __forceinline__ uint2 codes(const Part<T>& p) const {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      w[j / 4] |= (code(Elem<T>::value(p.at[j])) & 0xffu) << (8 * (j % 4));
+    return make_uint2(w[0], w[1]);
+  }
+};
+
+// --- rows ------------------------------------------------------------------------------
+
+// Where a row's values come from: x[row], or x[index[row] / index_div] (a row of 0 where that
+// lies outside x's `sources` rows). VECTOR: 16-byte loads (columns a multiple of 8).
+template <typename T, bool VECTOR>
+struct Rows {
+  const T* x;
+  const int32_t* index;
+  int32_t index_div;
+  int64_t sources, cols;
+  struct Row {
+    const T* at;  // NULL: a row of 0
+  };
+  __device__ __forceinline__ Row row(int64_t i) const {
+    if (index == nullptr) return Row{x + i * cols};
+    const int32_t pick = index[i];
+    const int64_t src = pick < 0 ? -1 : pick / index_div;
+    return Row{src >= 0 && src < sources ? x + src * cols : nullptr};
+  }
+  __device__ __forceinline__ Part<T> load(const Row& r, int64_t c) const {
+    Part<T> p{};
+    if (r.at == nullptr || c >= cols) return p;
+    if constexpr (VECTOR) {
+      struct __attribute__((packed, aligned(sizeof(T)))) Any {
+        Part<T> p;
+      };
+      p = reinterpret_cast<const Any*>(r.at + c)->p;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < cols) p.at[j] = r.at[c + j];
+    }
+    return p;
+  }
+};
+
+// The activation's rows, each value rounded to the layer's type as bux_glu_forward rounds it.
+template <typename K, typename T>
+struct Units {
+  const T* projected;
+  const T* weights;
+  int64_t cols;  // f, a multiple of 4
+  Act act;
+  struct Row {
+    const T* at;
+    float w;
+  };
+  __device__ __forceinline__ Row row(int64_t i) const {
+    return Row{projected + i * cols * (K::gated ? 2 : 1), Elem<T>::value(weights[i])};
+  }
+  __device__ __forceinline__ Part<T> load(const Row& r, int64_t c) const {
+    constexpr bool F32 = std::is_same<T, float>::value;
+    struct __attribute__((packed, aligned(sizeof(T)))) Eight {
+      Part<T> p;
+    };
+    struct __attribute__((packed, aligned(sizeof(T)))) Four {
+      T at[4];
+    };
+    Part<T> p{};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int64_t u = c + 4 * half;
+      if (u >= cols) continue;
+      float v[8];
+      if constexpr (K::gated) {
+        const Part<T> in = reinterpret_cast<const Eight*>(r.at + 2 * u)->p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = Elem<T>::value(in.at[j]);
+      } else {
+        const Four in = *reinterpret_cast<const Four*>(r.at + u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] = Elem<T>::value(in.at[j]);
+          v[2 * j + 1] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        p.at[4 * half + j] = Elem<T>::make(glu_unit<K, F32>(act, v[2 * j], v[2 * j + 1], r.w));
+    }
+    return p;
+  }
+};
+
+// A wave a row of the copy's `height`: rows from `rows` or *filled on are 0. C: the row's parts
+// a lane keeps, or 0 to read them twice.
+template <typename T, int C, typename Source>
+__global__ __launch_bounds__(THREADS) void rows_kernel(Source from, int64_t rows, int64_t height,
+                                                       const int32_t* __restrict__ filled,
+                                                       int64_t cols, int64_t k,
+                                                       uint8_t* __restrict__ values,
+                                                       float* __restrict__ scales) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * (THREADS / 64) +
+                    __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (i >= height) return;
+  const int64_t live = filled && *filled < rows ? *filled : rows;
+  uint8_t* const out = values + i * 64;
+  auto put = [&](int64_t c, uint2 codes) {
+    if (c < k) *reinterpret_cast<uint2*>(out + (c >> 6) * (height * 64) + (c & 63)) = codes;
+  };
+  if (i >= live) {
+    for (int64_t c = 8 * lane; c < k; c += 512) put(c, make_uint2(0, 0));
+    if (lane == 0) scales[i] = 0.0f;
+    return;
+  }
+  const typename Source::Row row = from.row(i);
+  if constexpr (C > 0) {
+    Part<T> p[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) p[j] = from.load(row, 512 * j + 8 * lane);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const uint32_t t = top_of(p[j]);
+      top = t > top ? t : top;
+    }
+    const Coder<T> coder(wave_top(top));
+#pragma unroll
+    for (int j = 0; j < C; ++j) put(512 * j + 8 * lane, coder.codes(p[j]));
+    if (lane == 0) scales[i] = coder.scale;
+  } else {
+    uint32_t top = 0;
+    for (int64_t c = 8 * lane; c < cols; c += 512) {
+      const uint32_t t = top_of(from.load(row, c));
+      top = t > top ? t : top;
+    }
+    const Coder<T> coder(wave_top(top));
+    for (int64_t c = 8 * lane; c < k; c += 512) put(c, coder.codes(from.load(row, c)));
+    if (lane == 0) scales[i] = coder.scale;
+  }
+}
+
+template <typename T, int C, typename Source>
+int launch_rows(const char* kernel, const Source& from, int64_t rows, int64_t height,
+                const int32_t* filled, int64_t cols, uint8_t* values, float* scales,
+                hipStream_t s) {
+  const int64_t k = ceil_div(cols, 128) * 128;
+  hipLaunchKernelGGL((rows_kernel<T, C, Source>),
+                     dim3(static_cast<unsigned>(ceil_div(height, THREADS / 64))), dim3(THREADS), 0,
+                     s, from, rows, height, filled, cols, k, values, scales);
+  return launched(kernel);
+}
+
+// --- the kernels' columns ------------------------------------------------------------------
+
+// A workgroup 64 columns of a group's (k, n) matrix: each wave every 4th row of it, a lane a
+// column; then 64 rows at a time through LDS, so that a lane writes 16 bytes of a column.
+constexpr int PITCH = 80;  // bytes of a column's 64 codes in LDS, 16-byte aligned
+template <typename T>
+__global__ __launch_bounds__(THREADS) void columns_kernel(const T* __restrict__ w, int64_t cols,
+                                                          int64_t n, int64_t k,
+                                                          uint8_t* __restrict__ values,
+                                                          float* __restrict__ scales) {
+  __shared__ uint32_t tops[THREADS / 64][64];
+  __shared__ __align__(16) uint8_t tile[64 * PITCH];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t col_blocks = (n + 63) / 64;
+  const int64_t g = blockIdx.x / col_blocks, c = (blockIdx.x % col_blocks) * 64 + lane;
+  const T* const from = w + g * cols * n + (c < n ? c : n - 1);
+  uint32_t top = 0;
+#pragma unroll 8
+  for (int64_t r = wave; r < cols; r += 4) {
+    const uint32_t b = __float_as_uint(Elem<T>::value(from[r * n])) & 0x7fffffffu;
+    top = b > top ? b : top;
+  }
+  tops[wave][lane] = top;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < THREADS / 64; ++j) top = tops[j][lane] > top ? tops[j][lane] : top;
+  const Coder<T> coder(top);
+  if (wave == 0 && c < n) scales[g * n + c] = coder.scale;
+  uint8_t* const out = values + g * n * k;
+  const int64_t c0 = c - lane;
+  for (int64_t r0 = 0; r0 < k; r0 += 64) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // this wave's 16 of the 64 rows, 4 a word
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t r = r0 + wave * 16 + q * 4 + j;
+        const float x = r < cols ? Elem<T>::value(from[r * n]) : 0.0f;
+        word |= (coder.code(x) & 0xffu) << (8 * j);
+      }
+      *reinterpret_cast<uint32_t*>(tile + lane * PITCH + wave * 16 + q * 4) = word;
+    }
+    __syncthreads();
+    const int column = threadIdx.x >> 2, piece = threadIdx.x & 3;
+    if (c0 + column < n)
+      *reinterpret_cast<uint4*>(out + (r0 >> 6) * (n * 64) + (c0 + column) * 64 + piece * 16) =
+          *reinterpret_cast<const uint4*>(tile + column * PITCH + piece * 16);
+    __syncthreads();
+  }
+}
+
+int check_copy(const char* name, int64_t rows, int64_t cols, int64_t height) {
+  BUX_CHECK(rows >= 0 && height >= rows && height < (1LL << 26),
+            "%s: bad shape rows=%lld height=%lld (at least the rows, below 2^26)", name,
+            (long long)rows, (long long)height);
+  BUX_CHECK(cols > 0 && cols <= MAX_K, "%s: cols=%lld outside [1, %lld]", name, (long long)cols,
+            (long long)MAX_K);
+  return BUX_OK;
+}
+
+template <typename T>
+int quantize(const char* name, const T* x, const int32_t* index, int32_t index_div,
+             int64_t sources, int64_t rows, int64_t cols, int64_t height, const int32_t* filled,
+             uint8_t* values, float* scales, void* stream) {
+  if (int rc = check_copy(name, rows, cols, height)) return rc;
+  BUX_CHECK(index == nullptr || (index_div >= 1 && sources >= 0), "%s: index_div=%d sources=%lld",
+            name, index_div, (long long)sources);
+  if (height == 0) return BUX_OK;
+  BUX_CHECK(values && scales && (rows == 0 || x || (index && sources == 0)), "%s: NULL buffer",
+            name);
+  auto go = [&](auto c, auto vector) {
+    const Rows<T, decltype(vector)::value> from{x, index, index_div, sources, cols};
+    return launch_rows<T, decltype(c)::value>("int8 rows_kernel", from, rows, height, filled, cols,
+                                              values, scales, as_stream(stream));
+  };
+  if (cols % 8 != 0) return go(std::integral_constant<int, 0>{}, std::false_type{});
+  if (cols <= 1024) return go(std::integral_constant<int, 2>{}, std::true_type{});
+  if (cols <= 2048) return go(std::integral_constant<int, 4>{}, std::true_type{});
+  if (cols <= 4096) return go(std::integral_constant<int, 8>{}, std::true_type{});
+  if (cols <= 8192) return go(std::integral_constant<int, 16>{}, std::true_type{});
+  return go(std::integral_constant<int, 0>{}, std::true_type{});
+}
+
+template <typename T>
+int quantize_units(const char* name, const T* projected, const T* weights, const int32_t* filled,
+                   int64_t m, int64_t f, const bux_ffn* ffn, int64_t height, uint8_t* values,
+                   float* scales, void* stream) {
+  if (int rc = check_copy(name, m, f, height)) return rc;
+  BUX_CHECK(f % 4 == 0, "%s: f=%lld is not a multiple of 4", name, (long long)f);
+  Act act;
+  if (int rc = act_of(name, ffn, &act)) return rc;
+  if (height == 0) return BUX_OK;
+  BUX_CHECK(values && scales && (m == 0 || (projected && weights)), "%s: NULL buffer", name);
+  return with_kind(act, [&](auto kind) {
+    const Units<decltype(kind), T> from{projected, weights, f, act};
+    auto go = [&](auto c) {
+      return launch_rows<T, decltype(c)::value>("int8 units rows_kernel", from, m, height, filled,
+                                                f, values, scales, as_stream(stream));
+    };
+    if (f <= 1024) return go(std::integral_constant<int, 2>{});
+    if (f <= 4096) return go(std::integral_constant<int, 8>{});
+    return go(std::integral_constant<int, 0>{});
+  });
+}
+
+template <typename T>
+int quantize_columns(const char* name, const T* w, int64_t groups, int64_t k, int64_t n,
+                     uint8_t* values, float* scales, void* stream) {
+  BUX_CHECK(groups >= 0 && n > 0 && k > 0 && k <= MAX_K && groups * ceil_div(n, 64) < (1LL << 24),
+            "%s: bad shape groups=%lld k=%lld n=%lld (k up to %lld)", name, (long long)groups,
+            (long long)k, (long long)n, (long long)MAX_K);
+  if (groups == 0) return BUX_OK;
+  BUX_CHECK(w && values && scales, "%s: NULL buffer", name);
+  hipLaunchKernelGGL((columns_kernel<T>), dim3(static_cast<unsigned>(groups * ceil_div(n, 64))),
+                     dim3(THREADS), 0, as_stream(stream), w, k, n, ceil_div(k, 128) * 128, values,
+                     scales);
+  return launched("int8 columns_kernel");
+}
+
+}  // namespace
+}  // namespace bux
+
+extern "C" int bux_int8_quantize(const uint16_t* x, const int32_t* index, int32_t index_div,
+                                 int64_t sources, int64_t rows, int64_t cols, int64_t height,
+                                 const int32_t* filled, uint8_t* values, float* scales,
+                                 void* stream) {
+  bux::clear_error();
+  return bux::quantize("bux_int8_quantize", x, index, index_div, sources, rows, cols, height,
+                       filled, values, scales, stream);
+}
+extern "C" int bux_int8_quantize_f32(const float* x, const int32_t* index, int32_t index_div,
+                                     int64_t sources, int64_t rows, int64_t cols, int64_t height,
+                                     const int32_t* filled, uint8_t* values, float* scales,
+                                     void* stream) {
+  bux::clear_error();
+  return bux::quantize("bux_int8_quantize_f32", x, index, index_div, sources, rows, cols, height,
+                       filled, values, scales, stream);
+}
+extern "C" int bux_int8_glu(const uint16_t* projected, const uint16_t* weights,
+                            const int32_t* filled, int64_t m, int64_t f, const bux_ffn* ffn,
+                            int64_t height, uint8_t* values, float* scales, void* stream) {
+  bux::clear_error();
+  return bux::quantize_units("bux_int8_glu", projected, weights, filled, m, f, ffn, height, values,
+                             scales, stream);
+}
+extern "C" int bux_int8_glu_f32(const float* projected, const float* weights,
+                                const int32_t* filled, int64_t m, int64_t f, const bux_ffn* ffn,
+                                int64_t height, uint8_t* values, float* scales, void* stream) {
+  bux::clear_error();
+  return bux::quantize_units("bux_int8_glu_f32", projected, weights, filled, m, f, ffn, height,
+                             values, scales, stream);
+}
+extern "C" int bux_int8_quantize_columns(const uint16_t* w, int64_t groups, int64_t k, int64_t n,
+                                         uint8_t* values, float* scales, void* stream) {
+  bux::clear_error();
+  return bux::quantize_columns("bux_int8_quantize_columns", w, groups, k, n, values, scales, stream);
+}
+extern "C" int bux_int8_quantize_columns_f32(const float* w, int64_t groups, int64_t k, int64_t n,
+                                             uint8_t* values, float* scales, void* stream) {
+  bux::clear_error();
+  return bux::quantize_columns("bux_int8_quantize_columns_f32", w, groups, k, n, values, scales,
+                               stream);
+}

@@ -25,9 +25,9 @@ from typing import NamedTuple
 
 import torch
 
-from bux_amd import _lib, grouped, grouped_mxfp8
+from bux_amd import _lib, grouped, grouped_int8, grouped_mxfp8
 from bux_amd.grouped_mxfp8 import Tiled
-from bux_amd.kernels import lib, ptr, require, stream, workspace
+from bux_amd.kernels import lib, on_device, ptr, require, stream, workspace
 from bux_amd.spans import span
 
 
@@ -229,6 +229,31 @@ def weighted_units_quantized(ffn: Ffn, projected: torch.Tensor, weights: torch.T
         ptr(projected), ptr(weights), ptr(filled), m, f, ctypes.byref(st), height, ptr(h),
         *_ptrs(row), *_ptrs(col), stream()))
     return row, col, h
+
+
+def weighted_units_int8(ffn: Ffn, projected: torch.Tensor, weights: torch.Tensor,
+                        filled: torch.Tensor | None = None, height: int | None = None
+                        ) -> grouped_int8.Int8:
+    """Return `weighted_units` in 8-bit integers with a scale a row, computed and quantized in
+    one pass: what ``grouped_int8.quantized`` gives of it, bit for bit. `height` (by default m)
+    rows of the copy; rows from `filled` on are 0."""
+    require(projected, weights, filled)
+    m, f, gated = _gating(projected)
+    f32 = _f32(projected, weights)
+    if weights.numel() != m:
+        raise ValueError(f"weighted_units_int8: {weights.numel()} weights for {m} rows")
+    height = m if height is None else height
+    dev = projected.device
+    with on_device(projected):
+        out = grouped_int8.Int8(
+            torch.empty(grouped_mxfp8.whole(f, grouped_mxfp8.K_ALIGN) // 64, height, 64,
+                        dtype=torch.int8, device=dev),
+            torch.empty(height, dtype=torch.float32, device=dev))
+        st = ffn.struct(gated)
+        quantize = lib().bux_int8_glu_f32 if f32 else lib().bux_int8_glu
+        _lib.check(quantize(ptr(projected), ptr(weights), ptr(filled), m, f, ctypes.byref(st),
+                            height, ptr(out.values), ptr(out.scales), stream()))
+    return out
 
 
 def weighted_units_backward_quantized(
@@ -819,3 +844,78 @@ def experts_backward(saved: Saved, dy: torch.Tensor, up: torch.Tensor, down: tor
         if norm is not None:
             grads["dv"] = dy_rows
     return grads
+
+
+# --- Serving in 8-bit integers -------------------------------------------------------------
+
+
+class Int8Weights(NamedTuple):
+    """The experts' kernels in 8-bit integers, a scale each output column: what `experts_int8`
+    keeps of them."""
+
+    up: grouped_int8.Int8  # each W_up^T: f p rows of K = d
+    down: grouped_int8.Int8  # each W_down^T: d rows of K = f
+    up_shape: tuple  # (E, d, f, p)
+    down_shape: tuple  # (E, f, d)
+
+
+def in_int8(up: torch.Tensor, down: torch.Tensor) -> Int8Weights:
+    """Return the experts' kernels (E, d, f, p) and (E, f, d), bfloat16 or float32, in 8-bit
+    integers for `experts_int8`: once, as a serving program loads them."""
+    if up.dim() != 4 or down.dim() != 3 or up.shape[3] not in (1, 2):
+        raise ValueError(f"in_int8: kernels (E, d, f, p) and (E, f, d), not {tuple(up.shape)} and "
+                         f"{tuple(down.shape)}")
+    e, d, f, p = up.shape
+    if tuple(down.shape) != (e, f, d):
+        raise ValueError(f"in_int8: kernels {tuple(up.shape)} and {tuple(down.shape)}")
+    if d % 8 != 0 or f % 4 != 0:
+        raise ValueError(f"in_int8: d={d} is a multiple of 8, f={f} of 4")
+    return Int8Weights(grouped_int8.quantized_kernels(up.reshape(e, d, f * p)),
+                       grouped_int8.quantized_kernels(down), tuple(up.shape), tuple(down.shape))
+
+
+def experts_int8(
+    z: torch.Tensor, idx: torch.Tensor, weights: torch.Tensor, quantized: Int8Weights,
+    ffn: Ffn = Ffn(), up_bias: torch.Tensor | None = None, down_bias: torch.Tensor | None = None,
+    norm: ExpertNorm | None = None, norm_scale: torch.Tensor | None = None,
+    norm_bias: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Return the routed experts' output (t, d) in z's dtype with both products in 8-bit
+    integers: `experts_forward` for serving (it has no backward). The tokens z (t, d), bfloat16
+    or float32, are quantized with a scale a row as they are gathered by expert, the activation
+    with a scale a row as it is computed; the products' sums are exact, each rounded once to z's
+    dtype. idx (t, k) int32, weights (t, k), the biases and the norm as `experts_forward`'s."""
+    t, k = idx.shape
+    e, d, f, p = quantized.up_shape
+    m = t * k
+    dt = _layer_dtype("experts_int8", z)
+    if z.dim() != 2 or tuple(z.shape) != (t, d):
+        raise ValueError(f"experts_int8: tokens {tuple(z.shape)} for picks {tuple(idx.shape)} and "
+                         f"kernels {quantized.up_shape}")
+    if weights.numel() != m:
+        raise ValueError(f"experts_int8: {weights.numel()} weights for {m} picks")
+    weights, = _cast(dt, weights)
+    up_bias, down_bias, norm_scale, norm_bias = _cast(dt, up_bias, down_bias, norm_scale, norm_bias)
+    height = grouped_mxfp8.whole(m)
+    with span("permute"):
+        s, row_weights, tiles = sort_for_layer(idx, e, weights, height)
+    with span("quantize x"):
+        x = grouped_int8.quantized(z, s.filled, s.order, k, height)
+    with span("up fprop"):
+        projected = grouped_int8.rows(
+            x, quantized.up, s.sizes, dt, height=m, tiles=tiles,
+            bias=None if up_bias is None else up_bias.reshape(e, f * p))
+    act_weights = row_weights if norm is None else torch.ones_like(row_weights)
+    with span("activation + quantize h"):
+        h = weighted_units_int8(ffn, projected.view(m, f, p), act_weights, s.filled, height)
+    with span("down fprop"):
+        y = grouped_int8.rows(h, quantized.down, s.sizes, dt, height=m, tiles=tiles)
+    if norm is not None:
+        with span("expert norm"):
+            y = expert_norm_forward(y, s.offsets, norm, norm_scale, norm_bias, row_weights,
+                                    None if down_bias is None else down_bias.reshape(e, d))
+    with span("combine"):
+        if down_bias is None or norm is not None:
+            return sum_by_token(y, s.inverse.view(t, k))
+        return sum_by_token_biased(y, s.inverse.view(t, k), down_bias.reshape(e, d), s.offsets,
+                                   row_weights)

@@ -694,6 +694,71 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxNormBackward, NormBackward,
                                   .Arg<In>().Arg<In>() BUX_NORM_ATTRS.Ret<In>().Ret<In>()
                                   .Ret<In>().Ret<In>());
 
+// --- the experts' products in 8-bit integers -----------------------------------------------
+// values [K/64, height, 64] (a stack: [groups, K/64, n, 64]), scales [height] ([groups, n]);
+// index, filled and bias may be empty.
+
+static ffi::Error Int8Quantize(hipStream_t s, In x, In index, In filled, int64_t index_div,
+                               int64_t rows, Out values, Out scales) {
+  const int64_t height = dim(values, 1), cols = dim(x, 1), sources = dim(x, 0);
+  const int32_t div = static_cast<int32_t>(index_div);
+  if (f32(x))
+    return status(bux_int8_quantize_f32(at<const float>(x), at<const int32_t>(index), div, sources,
+                                        rows, cols, height, at<const int32_t>(filled),
+                                        at<uint8_t>(values), at<float>(scales), s));
+  return status(bux_int8_quantize(at<const uint16_t>(x), at<const int32_t>(index), div, sources,
+                                  rows, cols, height, at<const int32_t>(filled),
+                                  at<uint8_t>(values), at<float>(scales), s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8Quantize, Int8Quantize,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
+                                  .Attr<int64_t>("index_div").Attr<int64_t>("rows").Ret<In>()
+                                  .Ret<In>());
+
+// projected [m, f, p] (p = 2 gated, 1 plain), weights [m].
+static ffi::Error Int8Glu(hipStream_t s, In projected, In weights, In filled, BUX_FFN_PARAMS,
+                          Out values, Out scales) {
+  const bux_ffn ffn = BUX_FFN;
+  const int64_t m = dim(projected, 0), f = dim(projected, 1), height = dim(values, 1);
+  if (f32(projected))
+    return status(bux_int8_glu_f32(at<const float>(projected), at<const float>(weights),
+                                   at<const int32_t>(filled), m, f, &ffn, height,
+                                   at<uint8_t>(values), at<float>(scales), s));
+  return status(bux_int8_glu(at<const uint16_t>(projected), at<const uint16_t>(weights),
+                             at<const int32_t>(filled), m, f, &ffn, height, at<uint8_t>(values),
+                             at<float>(scales), s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8Glu, Int8Glu,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
+                                  BUX_FFN_ATTRS.Ret<In>().Ret<In>());
+
+// w [groups, k, n].
+static ffi::Error Int8QuantizeColumns(hipStream_t s, In w, Out values, Out scales) {
+  if (f32(w))
+    return status(bux_int8_quantize_columns_f32(at<const float>(w), dim(w, 0), dim(w, 1), dim(w, 2),
+                                                at<uint8_t>(values), at<float>(scales), s));
+  return status(bux_int8_quantize_columns(at<const uint16_t>(w), dim(w, 0), dim(w, 1), dim(w, 2),
+                                          at<uint8_t>(values), at<float>(scales), s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8QuantizeColumns, Int8QuantizeColumns,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Ret<In>().Ret<In>());
+
+static ffi::Error Int8GroupedRowsListed(hipStream_t s, In a_values, In a_scales, In b_values,
+                                        In b_scales, In list, In bias, Out y) {
+  if (bias.size_bytes() &&
+      (bias.element_type() != y->element_type() ||
+       static_cast<int64_t>(bias.element_count()) != dim(b_scales, 0) * dim(b_scales, 1)))
+    return mismatch("BuxInt8GroupedRowsListed: bias is [groups, n] of the product's dtype");
+  return status(bux_int8_grouped_rows_listed(
+      at<const uint8_t>(a_values), at<const float>(a_scales), at<const uint8_t>(b_values),
+      at<const float>(b_scales), at<void>(list), list.size_bytes(),
+      static_cast<int32_t>(dim(b_values, 0)), dim(a_values, 1), dim(b_values, 2),
+      dim(a_values, 0) * 64, dim(y, 0), dtype_of(y), at<const void>(bias), at<void>(y), s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8GroupedRowsListed, Int8GroupedRowsListed,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
+                                  .Arg<In>().Arg<In>().Arg<In>().Ret<In>());
+
 // --- the router ----------------------------------------------------------------------
 // x [t, d], kernel [d, n_logits]; bias and choice_bias may be empty, as may the sinks,
 // scores and logits results.

@@ -644,6 +644,52 @@ int bux_mx_grouped_dglu(const uint8_t* a_values, const uint8_t* a_scales, const 
                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * The experts' products in 8-bit integers, for serving: no counterpart in the reference, beside
+ * its MXFP8 ones (a-4, a-6).
+ *
+ * A row x in 8-bit integers: codes q = the integer nearest 127 x / max |x| (the even one at a
+ * tie), and a float32 scale max |x| / 127. A row of zeros has scale 0 and codes 0; one that
+ * holds an infinity or a NaN has that as its scale and codes of 0, so that its products are NaN.
+ * Codes are int8 in the tiled layout, [K / 64][rows][64] with K whole 128s (codes 0 past the
+ * columns); scales float32 [rows]. Columns up to 131072.
+ *
+ * bux_int8_quantize: rows of x, as bux_mx_quantize takes them (index, index_div, sources, filled
+ *   likewise; height any, >= rows): values [K/64][height][64], scales [height]; rows from `rows`
+ *   or *filled on are 0. Any cols.
+ * bux_int8_glu: rows of the activation of projected and the weights, as bux_glu_forward computes
+ *   and rounds them (bux_glu_forward, then bux_int8_quantize, bit for bit), in one pass. f a
+ *   multiple of 4.
+ * bux_int8_quantize_columns: the columns of `groups` matrices w (k, n): for each, n rows of k:
+ *   values [groups][K/64][n][64], scales [groups][n].
+ * bux_int8_grouped_rows_listed: bux_mx_grouped_rows_listed for these: y[i][c] = (sum_k a[i][k]
+ *   b[g(i)][c][k]) (a_scales[i] b_scales[g(i)][c]) + bias[g(i)][c], the sums exact (32-bit
+ *   integers), the rest float32, one rounding to out_dtype; bias [groups, n] of out_dtype, or
+ *   NULL; rows from sum(sizes) to height 0. The list (bux_mx_grouped_tiles, or
+ *   bux_moe_permute_layer's) is checked as there. n a multiple of 4, m and n up to 33,554,176.
+ */
+int bux_int8_quantize(const uint16_t* x, const int32_t* index, int32_t index_div, int64_t sources,
+                      int64_t rows, int64_t cols, int64_t height, const int32_t* filled,
+                      uint8_t* values, float* scales, void* stream);
+int bux_int8_quantize_f32(const float* x, const int32_t* index, int32_t index_div, int64_t sources,
+                          int64_t rows, int64_t cols, int64_t height, const int32_t* filled,
+                          uint8_t* values, float* scales, void* stream);
+int bux_int8_glu(const uint16_t* projected, const uint16_t* weights, const int32_t* filled,
+                 int64_t m, int64_t f, const bux_ffn* ffn, int64_t height, uint8_t* values,
+                 float* scales, void* stream);
+int bux_int8_glu_f32(const float* projected, const float* weights, const int32_t* filled,
+                     int64_t m, int64_t f, const bux_ffn* ffn, int64_t height, uint8_t* values,
+                     float* scales, void* stream);
+int bux_int8_quantize_columns(const uint16_t* w, int64_t groups, int64_t k, int64_t n,
+                              uint8_t* values, float* scales, void* stream);
+int bux_int8_quantize_columns_f32(const float* w, int64_t groups, int64_t k, int64_t n,
+                                  uint8_t* values, float* scales, void* stream);
+int bux_int8_grouped_rows_listed(const uint8_t* a_values, const float* a_scales,
+                                 const uint8_t* b_values, const float* b_scales, void* list,
+                                 size_t list_bytes, int32_t groups, int64_t m, int64_t n,
+                                 int64_t k, int64_t height, int out_dtype, const void* bias,
+                                 void* y, void* stream);
+
+/* ---------------------------------------------------------------------------------
  * The router (the path's feed: its picks are a-1's idx, its weights a-8's).
  *
  * Replaces MoE._route (src/bux/architecture/experts/moe.py:236-273) off training, with

@@ -90,3 +90,48 @@ def test_the_routers_backward_rejects_bad_arguments(lib):
     assert need >= 8 * 32 * 4 + 64 * 32 * 4
     assert call(nbytes=need - 1) == 2 and "workspace" in _msg(lib)
     assert call(ws=None) == 2 and "workspace" in _msg(lib)
+
+
+@pytest.mark.parametrize("twin", ["", "_f32"])
+def test_the_int8_quantizers_reject_bad_arguments(lib, twin):
+    quantize = getattr(lib, "bux_int8_quantize" + twin)
+    glu = getattr(lib, "bux_int8_glu" + twin)
+    columns = getattr(lib, "bux_int8_quantize_columns" + twin)
+
+    def rows(rows=8, cols=64, height=8, index=None, div=1, sources=8, x=P, values=P):
+        return quantize(x, index, div, sources, rows, cols, height, None, values, P, None)
+
+    for bad, word in (({"rows": -1}, "rows=-1"), ({"height": 7}, "height=7"),
+                      ({"height": 1 << 26}, "height"), ({"cols": 0}, "cols=0"),
+                      ({"cols": 131073}, "cols=131073"), ({"index": P, "div": 0}, "index_div=0"),
+                      ({"index": P, "sources": -1}, "sources=-1"), ({"x": None}, "NULL"),
+                      ({"values": None}, "NULL")):
+        assert rows(**bad) == 1 and word in _msg(lib), (bad, _msg(lib))
+    assert rows(rows=0, height=0, x=None, values=None) == 0
+
+    def units(m=8, f=64, height=8, act=0, projected=P):
+        ffn = _lib.FfnStruct(act, 1, 0, 0.0, 0, 0.0, 0.0)
+        return glu(projected, P, None, m, f, ctypes.byref(ffn), height, P, P, None)
+
+    for bad, word in (({"f": 66}, "f=66"), ({"f": 0}, "cols=0"), ({"height": 4}, "height=4"),
+                      ({"act": 10}, "activation 10"), ({"projected": None}, "NULL")):
+        assert units(**bad) == 1 and word in _msg(lib), (bad, _msg(lib))
+    for g, k, n, w in ((-1, 64, 64, P), (1, 0, 64, P), (1, 64, 0, P), (1, 131073, 64, P),
+                       (1, 64, 64, None)):
+        assert columns(w, g, k, n, P, P, None) == 1, (g, k, n)
+
+
+def test_the_int8_products_reject_bad_arguments(lib):
+    def call(groups=4, m=128, n=64, k=128, height=128, out=0, a=P, y=P, llist=P, nbytes=1 << 20):
+        return lib.bux_int8_grouped_rows_listed(a, P, P, P, llist, nbytes, groups, m, n, k, height,
+                                                out, None, y, None)
+
+    for bad, word in (({"groups": 0}, "groups=0"), ({"groups": 4097}, "groups=4097"),
+                      ({"k": 64}, "k=64"), ({"k": 0}, "k=0"), ({"k": 131200}, "k=131200"),
+                      ({"n": 66}, "n=66"), ({"n": 0}, "n=0"), ({"m": -1}, "m=-1"),
+                      ({"m": 33_554_177, "nbytes": 1 << 40}, "33554176"), ({"out": 2}, "out_dtype"),
+                      ({"a": None}, "NULL"), ({"y": None}, "NULL")):
+        assert call(**bad) == 1 and word in _msg(lib), (bad, _msg(lib))
+    need = lib.bux_mx_grouped_rows_workspace_size(4, 128, 128)
+    assert call(nbytes=need - 1) == 2 and "list" in _msg(lib)
+    assert call(llist=None) == 2 and "list" in _msg(lib)
