@@ -13,6 +13,7 @@
 // the 16 bytes of K 16 (l / 32) .. + 15; accumulators as the float MFMAs'.
 
 #include "epilogue.h"
+#include "int8_direct.h"
 #include "tiles.h"
 
 namespace bux {
@@ -382,9 +383,12 @@ extern "C" int bux_int8_grouped_rows_listed(const uint8_t* a_values, const float
   if (list == nullptr || list_bytes < need)
     return fail(BUX_E_WORKSPACE, "%s: list of %zu bytes, %zu needed", name, list_bytes, need);
   if (height == 0) return BUX_OK;
+  hipStream_t s = as_stream(stream);
+  if (int8_rows_direct(m, groups))
+    return launch_int8_direct(a_values, a_scales, b_values, b_scales, list, slots, groups, m, n, k,
+                              height, out_dtype, bias, y, s);
   const Operand A{a_values, a_scales, static_cast<int32_t>(k), static_cast<int32_t>(m)};
   const Operand B{b_values, b_scales, static_cast<int32_t>(k), static_cast<int32_t>(n)};
-  hipStream_t s = as_stream(stream);
   return out_dtype == BUX_BF16 ? launch_rows<uint16_t>(A, B, groups, n, height, list, slots, bias, y, s)
                                : launch_rows<float>(A, B, groups, n, height, list, slots, bias, y, s);
 }

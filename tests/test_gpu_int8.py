@@ -7,6 +7,8 @@ these compare bit for bit. The products of real values lie within what the round
 codes allows, half a code of either operand.
 """
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -236,6 +238,69 @@ def test_products(lib, case, biased, dtype):
         want = _product(ac, a.scales.cpu(), bc, b.scales.cpu(), sizes, height, dtype,
                         None if bias is None else bias.cpu())
         assert torch.equal(y.cpu(), want), (height, (y.cpu() != want).nonzero()[:5])
+
+
+# few rows a group, some groups with many: sizes, rows of a past them, k, n
+FEW = [
+    ([1, 0, 2, 0, 1, 1], 0, 2048, 132),
+    ([0] * 12 + [200] + [0] * 12, 3, 300, 68),
+    ([300] + [1] * 30, 0, 96, 64),
+    ([16, 17, 15, 31, 1, 0, 32, 33, 2, 0, 0, 0], 5, 1000, 260),
+    ([0] * 5, 7, 128, 4),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("biased", [False, True], ids=["", "biased"])
+@pytest.mark.parametrize("case", FEW, ids=lambda c: f"{len(c[0])}x{sum(c[0])}x{c[2]}x{c[3]}")
+def test_products_of_few_rows_a_group(lib, case, biased, dtype):
+    from bux_amd import grouped_int8 as g8
+    sizes, past, k, n = case
+    m = sum(sizes) + past
+    announce("int8 products of few rows", case, biased, dtype)
+    a, ac = _random_int8(k, rows=m, k=k)
+    b, bc = _random_int8(n, len(sizes), rows=n, k=k)
+    bias = _normal(3, len(sizes), n, dtype=dtype) if biased else None
+    a.scales[sum(sizes):] = float("nan")  # past the groups
+    if sizes[0] > 1:
+        a.scales[1], ac[1] = float("inf"), 0
+        a.values[:, 1] = 0
+    sz = torch.tensor(sizes, dtype=torch.int32).cuda()
+    buf = torch.full((m * n + 512 * n,), 7.0, dtype=dtype, device="cuda")
+    for height in (m, m + 40):
+        y = g8.rows(a, b, sz, dtype, height, bias=bias)
+        want = _product(ac, a.scales.cpu(), bc, b.scales.cpu(), sizes, height, dtype,
+                        None if bias is None else bias.cpu())
+        if sizes[0] > 1:
+            assert torch.isnan(y[1]).all()
+            y[1], want[1] = 0, 0
+        assert torch.equal(y.cpu(), want), (height, (y.cpu() != want).nonzero()[:5])
+    from bux_amd import grouped_mxfp8
+    tiles = grouped_mxfp8.tiles_of(sz, m, m)
+    _lib.check(lib.bux_int8_grouped_rows_listed(
+        a.values.data_ptr(), a.scales.data_ptr(), b.values.data_ptr(), b.scales.data_ptr(),
+        tiles.buffer.data_ptr(), tiles.buffer.numel(), len(sizes), m, n, -(-k // 128) * 128, m,
+        0 if dtype == BF16 else 1, None if bias is None else bias.data_ptr(),
+        buf[256 * n:].data_ptr(), None))
+    assert (buf[:256 * n] == 7).all() and (buf[256 * n + m * n:] == 7).all()
+
+
+def test_both_kernels_give_the_same_bits(lib):
+    """One product by either kernel: its rows in two groups, and those groups beside many empty
+    ones (which kernel a call takes goes by its rows a group)."""
+    from bux_amd import grouped_int8 as g8
+    direct = lib.bux_int8_direct
+    direct.argtypes, direct.restype = [ctypes.c_int64, ctypes.c_int32], ctypes.c_int
+    m, n, k = 150, 196, 700
+    assert not direct(m, 2) and direct(m, 40)
+    assert [direct(160, 10), direct(161, 10)] == [1, 0]
+    a, _ = _random_int8(1, rows=m, k=k)
+    b, _ = _random_int8(2, 40, rows=n, k=k)
+    two = g8.Int8(b.values[:2].contiguous(), b.scales[:2].contiguous())
+    sizes = torch.zeros(40, dtype=torch.int32).cuda()
+    sizes[:2] = torch.tensor([100, 50])
+    for dtype in (BF16, F32):
+        assert torch.equal(g8.rows(a, b, sizes, dtype), g8.rows(a, two, sizes[:2].contiguous(), dtype))
 
 
 def test_the_largest_sums(lib):
