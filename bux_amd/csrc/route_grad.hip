@@ -13,7 +13,7 @@
 //   dx   = dz_in + G kernel^T,  d_kernel = x^T G,  d_bias = sum over the tokens of G
 //
 // (moe.py:249-270's transpose: the forward's roundings to bfloat16 pass the gradient as they
-// are.) Four kernels: grads_kernel (a wave a token) writes G, in two bfloat16 parts, hi and
+// are.) Four kernels: grads_kernel writes G, in two bfloat16 parts, hi and
 // the rest lo: G to 2^-17 at the rate of two bfloat16 MFMAs, where one part alone would put an
 // error of a bfloat16 step's half (2^-9) into every product, as large as the outputs' rounding.
 // dx_kernel multiplies it by the router's kernel, whose rows lie along n; kernel_grad_kernel
@@ -34,7 +34,7 @@ namespace {
 constexpr int THREADS = 256;  // 4 waves
 constexpr int MAX_LOGITS = 1024;
 constexpr int MAX_PICKS = 16;
-constexpr int MAX_GRADS_BLOCKS = 512;
+constexpr int MAX_GRADS_BLOCKS = 1024;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -43,7 +43,7 @@ typedef __attribute__((address_space(3))) v4s lds_v4s;
 
 struct Params {
   const uint16_t* x;
-  const uint16_t* kernel;  // (d, npad) where n is no multiple of 32: the padded copy
+  const uint16_t* kernel;  // (d, n)
   const int32_t* idx;
   const float* logits;
   const uint16_t* d_weights;
@@ -55,8 +55,9 @@ struct Params {
   int32_t n, npad, scored, k, router;
   float logit_scale, factor;
   bool normalize;
-  uint16_t* hi;  // G's parts [t, npad]
+  uint16_t* hi;  // G's parts, in blocks (at_block)
   uint16_t* lo;
+  uint16_t* blocks;  // the kernel, in blocks
   float* bias_partials;    // [grads blocks, npad], or NULL
   float* kernel_partials;  // [slices, d, npad]
   int32_t grads_blocks, slices;
@@ -66,14 +67,26 @@ struct Params {
   float* d_bias;
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
+// G and the router's kernel lie in blocks of 32 rows by 8 columns, a block's 32 x 16 bytes in one
+// run and a row of blocks' one after another, padded with zeros to npad columns: a wave's load of
+// an MFMA operand (lane l row l % 32, columns 8 (l / 32) .. + 7 of 16) is one run of 1 KiB. (From
+// rows, 32 runs of 32 bytes: dx_kernel 66 us for 16384 tokens of 2048, 128 logits.) The element
+// (r, c), c a multiple of 4:
+__device__ __forceinline__ int64_t at_block(int64_t r, int32_t c, int32_t npad) {
+  return ((r >> 5) * (npad >> 3) + (c >> 3)) * 256 + (r & 31) * 8 + (c & 7);
+}
+
+// Over the L lanes of a token.
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+  for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o);
   return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  for (int o = 1; o < L; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
   return v;
 }
 
@@ -92,24 +105,58 @@ __device__ __forceinline__ float slope_of(int router, float z, float s) {
   return s == 0.0f ? 0.0f : sigmoid / (2.0f * s);
 }
 
-// A wave a token, lane l the logits l, l + 64, ... (Q of them).
-template <int Q>
+// Columns i .. i + 3 of a row of n, `fill` past it.
+__device__ __forceinline__ void load4(const float* row, int i, int n, float fill, float* v) {
+  struct __attribute__((packed, aligned(4))) Four {
+    float at[4];
+  };
+  if (i + 4 <= n) {
+    const Four f = *reinterpret_cast<const Four*>(row + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = f.at[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = i + j < n ? row[i + j] : fill;
+  }
+}
+
+// L lanes a token, lane l the logits 4 l + 4 L c .. + 3 for c < Q / 4: a wave's tokens share its
+// chain of sums (a wave a token: 24.6 us for 16384 tokens of 128 logits).
+template <int L, int Q>
 __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
-  __shared__ float sums[THREADS / 64][Q * 64];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (static_cast<int32_t>(blockIdx.x) >= p.grads_blocks) {  // the kernel into blocks, 4 columns a thread
+    const int64_t i = (static_cast<int64_t>(blockIdx.x - p.grads_blocks) * THREADS + threadIdx.x) * 4;
+    const int64_t r = i / p.npad;
+    if (r >= p.d) return;
+    const int32_t c = static_cast<int32_t>(i - r * p.npad);
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = c + j < p.n ? p.kernel[r * p.n + c + j] : 0;
+    *reinterpret_cast<uint2*>(p.blocks + at_block(r, c, p.npad)) =
+        make_uint2(v[0] | (v[1] << 16), v[2] | (v[3] << 16));
+    return;
+  }
+  static_assert(L >= MAX_PICKS && Q % 4 == 0, "a lane a pick, whole fours of logits");
+  constexpr int TOKENS = THREADS / L;
+  __shared__ float sums[TOKENS][L * Q];
+  const int lane = threadIdx.x % L, sub = threadIdx.x / L;
+  const int first = (threadIdx.x & 63) - lane;  // the token's first lane of its wave
   const int n = p.n, scored = p.scored, k = p.k;
+  auto column = [&](int q) { return (q / 4) * 4 * L + 4 * lane + q % 4; };
   float bias[Q];
 #pragma unroll
   for (int q = 0; q < Q; ++q) bias[q] = 0.0f;
-  for (int64_t tok = static_cast<int64_t>(blockIdx.x) * 4 + wave; tok < p.t;
-       tok += static_cast<int64_t>(gridDim.x) * 4) {
+  // to whole blocks of 32 tokens: those past the last are zeros (their x counts as 0, but a NaN
+  // beside it would not)
+  const int64_t whole = (p.t + 31) / 32 * 32;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * TOKENS; base < whole;
+       base += static_cast<int64_t>(p.grads_blocks) * TOKENS) {
+    const bool live = base + sub < p.t;
+    const int64_t tok = live ? base + sub : p.t - 1;
     const float* row = p.logits + tok * n;
     float z[Q], s[Q], ds[Q];
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int i = lane + 64 * q;
-      z[q] = i < n ? row[i] : -INFINITY;
-    }
+    for (int q = 0; q < Q; q += 4) load4(row, column(q), n, -INFINITY, z + q);
     // the picks, one a lane: those outside the scored experts count for nothing
     int32_t id = -1;
     float zp = 0.0f, g = 0.0f;
@@ -124,102 +171,114 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
       float m = z[0];
 #pragma unroll
       for (int q = 1; q < Q; ++q) m = fmaxf(m, z[q]);
-      m = wave_max(m);
+      m = lanes_max<L>(m);
       float sum = 0.0f;
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         s[q] = expf(z[q] - m);
         sum += s[q];
       }
-      const float all = wave_sum(sum);
+      const float all = lanes_sum<L>(sum);
 #pragma unroll
       for (int q = 0; q < Q; ++q) s[q] /= all;
       w = expf(zp - m) / all;
     } else {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) s[q] = lane + 64 * q < n ? score_of(p.router, z[q]) : 0.0f;
+      for (int q = 0; q < Q; ++q) s[q] = column(q) < n ? score_of(p.router, z[q]) : 0.0f;
       w = score_of(p.router, zp);
     }
     if (!ok) w = g = 0.0f;
     float sink[Q];  // the sinks' gradients
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const int i = lane + 64 * q;
+      const int i = column(q);
       sink[q] = p.d_sinks && i >= scored && i < n
                     ? bf16_to_f32(p.d_sinks[tok * (n - scored) + i - scored]) * p.factor : 0.0f;
     }
     float inv = 1.0f, shift = 0.0f;  // ds = (g - shift) inv
     if (p.normalize) {
       float total = w, dot = g * w;
+      if (n > scored) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int i = lane + 64 * q;
-        if (i >= scored && i < n) {
-          total += s[q];
-          dot += sink[q] * s[q];
-        }
+        for (int q = 0; q < Q; ++q)
+          if (column(q) >= scored && column(q) < n) {
+            total += s[q];
+            dot += sink[q] * s[q];
+          }
       }
-      total = wave_sum(total);
-      dot = wave_sum(dot);
+      total = lanes_sum<L>(total);
+      dot = lanes_sum<L>(dot);
       inv = total == 0.0f ? 0.0f : 1.0f / total;
       shift = total == 0.0f ? 0.0f : dot / total;
     }
     const float dp = ok ? (g - shift) * inv : 0.0f;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int i = lane + 64 * q;
-      ds[q] = i >= scored && i < n ? (sink[q] - shift) * inv : 0.0f;
-      if (p.d_scores && i < scored) ds[q] += p.d_scores[tok * scored + i];
+    for (int q = 0; q < Q; ++q)
+      ds[q] = column(q) >= scored && column(q) < n ? (sink[q] - shift) * inv : 0.0f;
+    if (p.d_scores) {
+#pragma unroll
+      for (int q = 0; q < Q; q += 4) {
+        float v[4];
+        load4(p.d_scores + tok * scored, column(q), scored, 0.0f, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ds[q + j] += v[j];
+      }
     }
     for (int j = 0; j < k; ++j) {
-      const int32_t at = __builtin_amdgcn_readlane(id, j);
-      const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(dp), j));
+      const int32_t at = __shfl(id, first + j);
+      const float v = __shfl(dp, first + j);
 #pragma unroll
-      for (int q = 0; q < Q; ++q)
-        if (lane + 64 * q == at) ds[q] += v;
+      for (int q = 0; q < Q; ++q) ds[q] += column(q) == at ? v : 0.0f;
     }
     float inner = 0.0f;
     if (p.router == BUX_ROUTER_SOFTMAX) {
 #pragma unroll
       for (int q = 0; q < Q; ++q) inner += ds[q] * s[q];
-      inner = wave_sum(inner);
+      inner = lanes_sum<L>(inner);
     }
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const int i = lane + 64 * q;
-      float dl = 0.0f;
-      if (i < n) {
-        dl = p.router == BUX_ROUTER_SOFTMAX ? s[q] * (ds[q] - inner)
-                                            : ds[q] * slope_of(p.router, z[q], s[q]);
-        if (p.d_logits) dl += p.d_logits[tok * n + i];
-        dl *= p.logit_scale;
+      const float slope = p.router == BUX_ROUTER_SOFTMAX ? s[q] : slope_of(p.router, z[q], s[q]);
+      ds[q] = column(q) < n ? (ds[q] - inner) * slope : 0.0f;
+    }
+    if (p.d_logits) {
+#pragma unroll
+      for (int q = 0; q < Q; q += 4) {
+        float v[4];
+        load4(p.d_logits + tok * n, column(q), n, 0.0f, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ds[q + j] += v[j];
       }
-      bias[q] += dl;
-      if (i < p.npad) {
-        const uint16_t h = f32_to_bf16(dl);
-        p.hi[tok * p.npad + i] = h;
-        p.lo[tok * p.npad + i] = f32_to_bf16(dl - bf16_to_f32(h));
+    }
+#pragma unroll
+    for (int q = 0; q < Q; q += 4) {
+      uint16_t h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float dl = live ? ds[q + j] * p.logit_scale : 0.0f;
+        bias[q + j] += dl;
+        h[j] = f32_to_bf16(dl);
+        l[j] = f32_to_bf16(dl - bf16_to_f32(h[j]));
+      }
+      if (column(q) < p.npad) {
+        const int64_t at = at_block(base + sub, column(q), p.npad);
+        *reinterpret_cast<uint2*>(p.hi + at) =
+            make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
+        *reinterpret_cast<uint2*>(p.lo + at) =
+            make_uint2(l[0] | (static_cast<uint32_t>(l[1]) << 16), l[2] | (static_cast<uint32_t>(l[3]) << 16));
       }
     }
   }
   if (p.bias_partials == nullptr) return;
 #pragma unroll
-  for (int q = 0; q < Q; ++q) sums[wave][lane + 64 * q] = bias[q];
+  for (int q = 0; q < Q; ++q) sums[sub][column(q)] = bias[q];
   __syncthreads();
-  for (int i = threadIdx.x; i < p.npad; i += THREADS)
-    p.bias_partials[static_cast<int64_t>(blockIdx.x) * p.npad + i] =
-        (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
-}
-
-// The router's kernel (d, n) with its rows padded by zeros to npad.
-__global__ __launch_bounds__(THREADS) void pad_kernel(const uint16_t* __restrict__ kernel,
-                                                      int64_t d, int32_t n, int32_t npad,
-                                                      uint16_t* __restrict__ out) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
-  if (i >= d * npad) return;
-  const int64_t r = i / npad;
-  const int32_t c = static_cast<int32_t>(i - r * npad);
-  out[i] = c < n ? kernel[r * n + c] : 0;
+  for (int i = threadIdx.x; i < p.npad; i += THREADS) {
+    float s = sums[0][i];
+#pragma unroll
+    for (int j = 1; j < TOKENS; ++j) s += sums[j][i];
+    p.bias_partials[static_cast<int64_t>(blockIdx.x) * p.npad + i] = s;
+  }
 }
 
 __device__ __forceinline__ bf16x8 load8(const uint16_t* p) {
@@ -227,11 +286,13 @@ __device__ __forceinline__ bf16x8 load8(const uint16_t* p) {
 }
 
 // dx: a wave 32 RB tokens by 128 columns, K = npad in 16s, the operands from L2 straight to
-// registers. MFMA with the kernel's rows first: lane l holds token l % 32, runs of 4 columns
-// 8 g + 4 (l / 32) of each block. The results pass LDS (32 tokens at a time) so that 16 lanes
-// store 256 bytes of a row, with dz added in float32 before the one rounding.
+// registers, a step ahead. MFMA with the kernel's rows first: lane l holds token l % 32, runs of 4
+// columns 8 g + 4 (l / 32) of each block. The results pass LDS (32 tokens by 64 columns at a
+// time) so that 8 lanes store 128 bytes of a row, with dz added in float32 before the one
+// rounding; dz's loads go out ahead of what they wait beside: the first 32 tokens' before the
+// products, the next 32's before the first are stored.
 constexpr int COLS = 128;
-constexpr int DX_PITCH = COLS + 4;  // floats: rows 16 bytes past a multiple of the banks
+constexpr int DX_PITCH = COLS / 2 + 4;  // floats: rows 16 bytes past a multiple of the banks
 template <int RB>
 __global__ __launch_bounds__(THREADS) void dx_kernel(Params p, uint32_t columns) {
   __shared__ __align__(16) float out[THREADS / 64][32 * DX_PITCH];
@@ -240,127 +301,181 @@ __global__ __launch_bounds__(THREADS) void dx_kernel(Params p, uint32_t columns)
   const int64_t t0 = static_cast<int64_t>(blockIdx.x / columns) * (32 * RB);
   const int64_t c0 = (static_cast<int64_t>(blockIdx.x % columns) * 4 + wave) * COLS;
   if (c0 >= p.d) return;  // no barrier follows
+  // blocks past the last: the last one's, not stored
+  const int64_t t_last = (p.t - 1) >> 5, c_last = (p.d - 1) >> 5;
+  const int64_t stride = static_cast<int64_t>(p.npad) * 32;  // elements of a row of blocks
   const uint16_t* ah[RB];
   const uint16_t* al[RB];
   const uint16_t* b[4];
 #pragma unroll
-  for (int i = 0; i < RB; ++i) {  // tokens and columns past the last: the last one's, not stored
-    const int64_t tok = t0 + 32 * i + r < p.t ? t0 + 32 * i + r : p.t - 1;
-    ah[i] = p.hi + tok * p.npad + 8 * h;
-    al[i] = p.lo + tok * p.npad + 8 * h;
+  for (int i = 0; i < RB; ++i) {
+    const int64_t at = ((t0 >> 5) + i < t_last ? (t0 >> 5) + i : t_last) * stride;
+    ah[i] = p.hi + at;
+    al[i] = p.lo + at;
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t col = c0 + 32 * j + r < p.d ? c0 + 32 * j + r : p.d - 1;
-    b[j] = p.kernel + col * p.npad + 8 * h;
-  }
+  for (int j = 0; j < 4; ++j)
+    b[j] = p.blocks + ((c0 >> 5) + j < c_last ? (c0 >> 5) + j : c_last) * stride;
+  // this lane's 8 columns of 8 rows of each 32 x 64
+  const int srow = lane >> 3, scol = 8 * (lane & 7);
+  uint4 add[2][4];
+  auto load_dz = [&](int i) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int64_t tok = t0 + 32 * i + it * 8 + srow, col = c0 + 64 * half + scol;
+        add[half][it] = make_uint4(0, 0, 0, 0);
+        if (tok < p.t && col < p.d)
+          add[half][it] = *reinterpret_cast<const uint4*>(p.dz + tok * p.d + col);
+      }
+  };
+  if (p.dz) load_dz(0);
   v16f acc[RB][4];
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = v16f{};
-#pragma unroll 2
-  for (int32_t e = 0; e < p.npad; e += 16) {
+  struct Step {
     bf16x8 hi[RB], lo[RB], w[4];
+  };
+  auto load = [&](Step& s, int32_t e) {
+    const int at = e * 32 + lane * 8;  // two blocks of 8 columns
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
-      hi[i] = load8(ah[i] + e);
-      lo[i] = load8(al[i] + e);
+      s.hi[i] = load8(ah[i] + at);
+      s.lo[i] = load8(al[i] + at);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = load8(b[j] + e);
+    for (int j = 0; j < 4; ++j) s.w[j] = load8(b[j] + at);
+  };
+  auto multiply = [&](const Step& s) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], hi[i], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], lo[i], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(s.w[j], s.hi[i], acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(s.w[j], s.lo[i], acc[i][j], 0, 0, 0);
       }
+  };
+  Step one, two;
+  load(one, 0);
+  for (int32_t e = 0; e < p.npad; e += 32) {  // npad is a multiple of 32
+    load(two, e + 16);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(one);
+    __builtin_amdgcn_sched_barrier(0);
+    if (e + 32 < p.npad) load(one, e + 32);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(two);
+    __builtin_amdgcn_sched_barrier(0);
   }
   float* mine = out[wave];
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
+    uint4 now[2][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<float4*>(mine + r * DX_PITCH + 32 * j + 8 * g + 4 * h) =
-            make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
-                        acc[i][j][4 * g + 3]);
-    // the wave's own region: its LDS operations run in order
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
-    const int64_t col = c0 + 8 * (lane & 15);
+      for (int it = 0; it < 4; ++it) now[half][it] = add[half][it];
+    if (p.dz && i + 1 < RB) load_dz(i + 1);
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int row = it * 4 + (lane >> 4);
-      const int64_t tok = t0 + 32 * i + row;
-      float v[8];
-      Elem<float>::load8(mine + row * DX_PITCH + 8 * (lane & 15), v);
-      if (tok >= p.t || col >= p.d) continue;
-      if (p.dz) {
-        float add[8];
-        Elem<uint16_t>::load8(p.dz + tok * p.d + col, add);
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += add[e];
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const v16f& a = acc[i][2 * half + j];
+          *reinterpret_cast<float4*>(mine + r * DX_PITCH + 32 * j + 8 * g + 4 * h) =
+              make_float4(a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]);
+        }
+      // the wave's own region: its LDS operations run in order
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
+      const int64_t col = c0 + 64 * half + scol;
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int64_t tok = t0 + 32 * i + it * 8 + srow;
+        float v[8];
+        Elem<float>::load8(mine + (it * 8 + srow) * DX_PITCH + scol, v);
+        if (p.dz) {
+          const uint32_t w[4] = {now[half][it].x, now[half][it].y, now[half][it].z, now[half][it].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[2 * e] += __uint_as_float(w[e] << 16);
+            v[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+          }
+        }
+        if (tok < p.t && col < p.d)
+          *reinterpret_cast<uint4*>(p.dx + tok * p.d + col) =
+              make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                         pack_bf16x2(v[6], v[7]));
       }
-      Elem<uint16_t>::store8(p.dx + tok * p.d + col, v);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // d_kernel's partial sums: a workgroup 128 of d by 128 logits over a slice of the tokens, 32 a
-// step, in two LDS stages filled through registers. x and G lie token-major, the contracted
-// axis slow: a stage holds 32 tokens' 256 bytes, 16-byte chunk c of token k at place
-// c ^ 4 (k % 4), and ds_read_b64_tr_b16 transposes on the way out (within each 16 lanes, lane
-// j's 16-bit element e is element j % 4 of the 8 bytes that lane 4 e + j / 4 read).
+// step, in a ring of LDS stages that direct loads fill RING - 1 steps ahead. A stage holds the
+// step's operands as they lie in memory, x's tokens of 256 bytes (16-byte chunk c of token k at
+// place c ^ 4 (k % 4)) and G's blocks, 16 of 32 tokens by one chunk (token k of chunk c at place k
+// ^ 4 (c % 4)): a load is runs of 256 bytes or one of 1 KiB, and the 16 lanes of a read hit
+// every bank once. ds_read_b64_tr_b16 transposes on the way out (within each 16 lanes, lane j's
+// 16-bit element e is element j % 4 of the 8 bytes that lane 4 e + j / 4 read).
+// Columns past d or npad read what follows them in memory, into sums that are not stored;
+// tokens past the last read 0.
 constexpr int STEP = 32;
+constexpr int RING = 3;
+constexpr int KLOADS = 6;  // direct loads a wave issues a step: 2 of each operand
 struct KStage {
   uint16_t x[STEP * COLS], hi[STEP * COLS], lo[STEP * COLS];
 };
 
-__device__ __forceinline__ bf16x8 read_tr(uint32_t at) {
+// 8 tokens of a lane's column: 4 and the 4 after them.
+__device__ __forceinline__ bf16x8 read_tr(uint32_t at, uint32_t at4) {
   const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s*>(at));
-  const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s*>(at + 4 * 256));
+  const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s*>(at4));
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 __global__ __launch_bounds__(THREADS) void kernel_grad_kernel(Params p) {
-  __shared__ __align__(16) KStage st[2];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t j0 = static_cast<int64_t>(blockIdx.x) * COLS;
   const int32_t e0 = blockIdx.y * COLS;
   const int64_t lo_t = blockIdx.z * p.slice;
   const int64_t hi_t = lo_t + p.slice < p.t ? lo_t + p.slice : p.t;
   const int steps = static_cast<int>((hi_t - lo_t + STEP - 1) / STEP);
-  // this thread's two chunks of each operand's stage: tokens row and row + 16
-  const int row = threadIdx.x >> 4, chunk = threadIdx.x & 15;
-  const bool x_in = j0 + 8 * chunk < p.d, g_in = e0 + 8 * chunk < p.npad;
-  uint4 xs[2], hs[2], ls[2];
-  auto load = [&](int s) {
+  const uint32_t lds0 = lds_at(smem);
+  // a wave's load i of x: tokens 8 w + 4 i .. + 3 of the step, lane l token l / 16, the chunk that
+  // belongs in place l % 16; of G's parts: chunks 4 w + 2 i and + 1, lane l the token that belongs
+  // in place l % 32 of chunk 4 w + 2 i + l / 32
+  const int row = 8 * wave + (lane >> 4);
+  const int chunk = (lane & 15) ^ (4 * ((lane >> 4) & 3));
+  const int x_row = static_cast<int>(p.d) * 2, g_tokens = p.npad * 64;  // bytes of 32 tokens of G
+  const int x_off = row * x_row + 16 * chunk;
+  int g_off[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = 4 * wave + 2 * i + (lane >> 5);
+    g_off[i] = c * 512 + ((lane & 31) ^ (4 * (c & 3))) * 16;
+  }
+  auto issue = [&](int s) {
+    const int64_t tok = lo_t + static_cast<int64_t>(s) * STEP;
+    // an operand's part of a stage is 8 KiB, a wave's share of it 2
+    const uint32_t at = lds0 + (s % RING) * sizeof(KStage) + wave * 2048;
+    const i32x4 xr = resource(p.x + tok * p.d + j0, ((p.t - tok) * p.d - j0) * 2);
+    // the 32 tokens' blocks from e0 on
+    const int64_t g = tok * p.npad + static_cast<int64_t>(e0) * 32;
+    const i32x4 hr = resource(p.hi + g, g_tokens - e0 * 64);
+    const i32x4 lr = resource(p.lo + g, g_tokens - e0 * 64);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t tok = lo_t + static_cast<int64_t>(s) * STEP + row + 16 * i;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      xs[i] = hs[i] = ls[i] = zero;
-      if (tok < hi_t) {
-        if (x_in) xs[i] = *reinterpret_cast<const uint4*>(p.x + tok * p.d + j0 + 8 * chunk);
-        if (g_in) {
-          hs[i] = *reinterpret_cast<const uint4*>(p.hi + tok * p.npad + e0 + 8 * chunk);
-          ls[i] = *reinterpret_cast<const uint4*>(p.lo + tok * p.npad + e0 + 8 * chunk);
-        }
-      }
-    }
-  };
-  auto put = [&](int b) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int k = row + 16 * i, at = k * COLS + 8 * (chunk ^ (4 * (k & 3)));
-      *reinterpret_cast<uint4*>(st[b].x + at) = xs[i];
-      *reinterpret_cast<uint4*>(st[b].hi + at) = hs[i];
-      *reinterpret_cast<uint4*>(st[b].lo + at) = ls[i];
+      load_lds16_uniform(xr, at + offsetof(KStage, x) + i * 1024, x_off, i * 4 * x_row);
+      load_lds16_uniform(hr, at + offsetof(KStage, hi) + i * 1024, g_off[i], 0);
+      load_lds16_uniform(lr, at + offsetof(KStage, lo) + i * 1024, g_off[i], 0);
     }
   };
   // wave (a, b) of 2 x 2: 64 of d from 64 a, 64 logits from 64 b; block q of 32 columns
@@ -370,35 +485,41 @@ __global__ __launch_bounds__(THREADS) void kernel_grad_kernel(Params p) {
     return (8 * (lane >> 5) + kq) * 256 + 16 * (4 * (block ^ kq) + (col >> 3)) +
            8 * ((col >> 2) & 1);
   };
+  auto block_offset = [&](int block) {
+    const int c = 4 * block + (col >> 3), k = 8 * (lane >> 5) + kq;
+    return c * 512 + (k ^ (4 * (c & 3))) * 16 + 8 * ((col >> 2) & 1);
+  };
   uint32_t xat[2], gat[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     xat[q] = offset(2 * (wave >> 1) + q);
-    gat[q] = offset(2 * (wave & 1) + q);
+    gat[q] = block_offset(2 * (wave & 1) + q);
   }
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(&st[0]));
   v16f acc[2][2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc[i][j] = v16f{};
-  if (steps > 0) {
-    load(0);
-    put(0);
-  }
+  for (int s = 0; s < RING - 1 && s < steps; ++s) issue(s);
   for (int s = 0; s < steps; ++s) {
-    __syncthreads();
-    if (s + 1 < steps) load(s + 1);
-    const uint32_t at = lds0 + (s & 1) * sizeof(KStage);
+    // this step's loads are in once only those of the steps after it are out
+    if (s + 1 < steps && RING > 2) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // ... in every wave; and every wave has read the stage that the next loads take
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + RING - 1 < steps) issue(s + RING - 1);
+    const uint32_t at = lds0 + (s % RING) * sizeof(KStage);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const uint32_t k16 = half * 16 * 256;
+      // 16 tokens on: 4 KiB of x, 256 bytes of G; 4 tokens on: 1 KiB, and place ^ 4
+      const uint32_t xh = at + offsetof(KStage, x) + half * 4096, gh = at + half * 256;
       bf16x8 xv[2], hv[2], lv[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        xv[q] = read_tr(at + offsetof(KStage, x) + k16 + xat[q]);
-        hv[q] = read_tr(at + offsetof(KStage, hi) + k16 + gat[q]);
-        lv[q] = read_tr(at + offsetof(KStage, lo) + k16 + gat[q]);
+        xv[q] = read_tr(xh + xat[q], xh + xat[q] + 1024);
+        const uint32_t hi = gh + offsetof(KStage, hi), lo = gh + offsetof(KStage, lo);
+        hv[q] = read_tr(hi + gat[q], hi + (gat[q] ^ 64));
+        lv[q] = read_tr(lo + gat[q], lo + (gat[q] ^ 64));
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -408,7 +529,6 @@ __global__ __launch_bounds__(THREADS) void kernel_grad_kernel(Params p) {
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lv[j], xv[i], acc[i][j], 0, 0, 0);
         }
     }
-    if (s + 1 < steps) put((s + 1) & 1);
   }
   float* base = p.kernel_partials + static_cast<int64_t>(blockIdx.z) * p.d * p.npad;
 #pragma unroll
@@ -428,16 +548,16 @@ __global__ __launch_bounds__(THREADS) void kernel_grad_kernel(Params p) {
   }
 }
 
-// d_kernel: the slices' sums in order, 4 logits a thread; d_bias: a block each 64 logits after
-// those, its waves every 4th partial, then the waves' in order.
+// d_kernel: the slices' sums in order, 4 logits a thread; d_bias: a block each 16 logits after
+// those, its 16 threads a logit every 16th partial, then their sums in order.
 __global__ __launch_bounds__(THREADS) void reduce_kernel(Params p, int64_t kernel_blocks) {
-  __shared__ float part[THREADS / 64][64];
+  __shared__ float part[16][16];
   const int64_t size = p.d * p.npad;
   if (static_cast<int64_t>(blockIdx.x) < kernel_blocks) {
     const int64_t i = (static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x) * 4;
     if (i >= size) return;
     float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll 4
+#pragma unroll 8
     for (int32_t s = 0; s < p.slices; ++s) {
       const float4 a = *reinterpret_cast<const float4*>(p.kernel_partials + s * size + i);
       v.x += a.x;
@@ -449,30 +569,29 @@ __global__ __launch_bounds__(THREADS) void reduce_kernel(Params p, int64_t kerne
     const int32_t e = static_cast<int32_t>(i - j * p.npad);
     uint16_t* out = p.d_kernel + j * p.n + e;
     const float f[4] = {v.x, v.y, v.z, v.w};
-    if (p.n % 4 == 0 && e < p.n) {
-      *reinterpret_cast<uint2*>(out) = make_uint2(
-          f32_to_bf16(f[0]) | (static_cast<uint32_t>(f32_to_bf16(f[1])) << 16),
-          f32_to_bf16(f[2]) | (static_cast<uint32_t>(f32_to_bf16(f[3])) << 16));
-    } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (e + q < p.n) out[q] = f32_to_bf16(f[q]);
-    }
+    for (int q = 0; q < 4; ++q)
+      if (e + q < p.n) out[q] = f32_to_bf16(f[q]);
     return;
   }
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int32_t e = static_cast<int32_t>(blockIdx.x - kernel_blocks) * 64 + lane;
+  const int row = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const int32_t e = static_cast<int32_t>(blockIdx.x - kernel_blocks) * 16 + lane;
   float s = 0.0f;
   if (e < p.n) {
-#pragma unroll 4
-    for (int32_t b = wave; b < p.grads_blocks; b += 4)
+#pragma unroll 8
+    for (int32_t b = row; b < p.grads_blocks; b += 16)
       s += p.bias_partials[static_cast<int64_t>(b) * p.npad + e];
   }
-  part[wave][lane] = s;
+  part[row][lane] = s;
   __syncthreads();
-  if (wave == 0 && e < p.n)
-    p.d_bias[e] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+  if (row != 0 || e >= p.n) return;
+#pragma unroll
+  for (int r = 1; r < 16; ++r) s += part[r][lane];
+  p.d_bias[e] = s;
 }
+
+// The lanes grads_kernel gives a token.
+int lanes_of(int32_t npad) { return npad <= 128 ? 16 : npad <= 256 ? 32 : 64; }
 
 int32_t padded(int32_t n) { return static_cast<int32_t>(ceil_div(n, 32) * 32); }
 
@@ -485,8 +604,8 @@ struct Plan {
 Plan plan_of(int64_t t, int64_t d, int32_t n) {
   Plan w{};
   w.npad = padded(n);
-  w.grads_blocks = static_cast<int32_t>(
-      ceil_div(t, 4) < MAX_GRADS_BLOCKS ? ceil_div(t, 4) : MAX_GRADS_BLOCKS);
+  const int64_t blocks = ceil_div(ceil_div(t, 32) * 32, THREADS / lanes_of(w.npad));
+  w.grads_blocks = static_cast<int32_t>(blocks < MAX_GRADS_BLOCKS ? blocks : MAX_GRADS_BLOCKS);
   // as many workgroups as two a CU, slices of 256 tokens at least
   const int64_t tiles = ceil_div(d, COLS) * ceil_div(w.npad, COLS);
   const int64_t most = 512 / tiles > 1 ? 512 / tiles : 1;
@@ -495,10 +614,10 @@ Plan plan_of(int64_t t, int64_t d, int32_t n) {
   w.slice = ceil_div(ceil_div(t > 0 ? t : 1, slices), STEP) * STEP;
   w.slices = static_cast<int32_t>(ceil_div(t, w.slice));
   auto whole = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
-  const size_t part = whole(static_cast<size_t>(t) * w.npad * sizeof(uint16_t));
+  const size_t part = static_cast<size_t>(ceil_div(t, 32) * 32) * w.npad * sizeof(uint16_t);
   w.parts = 0;
   w.kernel = 2 * part;
-  w.bias = w.kernel + (n % 32 == 0 ? 0 : whole(static_cast<size_t>(d) * w.npad * sizeof(uint16_t)));
+  w.bias = w.kernel + static_cast<size_t>(ceil_div(d, 32) * 32) * w.npad * sizeof(uint16_t);
   w.partials = w.bias + whole(static_cast<size_t>(w.grads_blocks) * w.npad * sizeof(float));
   w.bytes = w.partials + static_cast<size_t>(w.slices) * d * w.npad * sizeof(float);
   return w;
@@ -523,9 +642,9 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
                                   size_t workspace_bytes, void* stream) {
   using namespace bux;
   clear_error();
-  BUX_CHECK(t >= 0 && t < (1LL << 31) && d > 0 && d % 16 == 0 && d < (1LL << 31),
-            "bux_route_backward: t=%lld d=%lld (d a positive multiple of 16)", (long long)t,
-            (long long)d);
+  BUX_CHECK(t >= 0 && t < (1LL << 31) && d > 0 && d % 16 == 0 && d <= (1LL << 24),
+            "bux_route_backward: t=%lld d=%lld (d a positive multiple of 16, up to 2^24)",
+            (long long)t, (long long)d);
   BUX_CHECK(n_logits >= 1 && n_logits <= MAX_LOGITS,
             "bux_route_backward: n_logits=%d outside [1, %d]", n_logits, MAX_LOGITS);
   BUX_CHECK(scored >= 1 && scored <= n_logits, "bux_route_backward: scored=%d outside [1, %d]",
@@ -538,6 +657,9 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
   BUX_CHECK(d_sinks == nullptr || n_logits > scored, "bux_route_backward: d_sinks without sinks");
   BUX_CHECK(kernel && d_kernel, "bux_route_backward: NULL kernel or d_kernel");
   BUX_CHECK(t == 0 || (x && idx && logits && d_weights && dx), "bux_route_backward: NULL buffer");
+  auto aligned = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
+  BUX_CHECK(aligned(x) && aligned(dz) && aligned(dx) && aligned(workspace),
+            "bux_route_backward: x, dz, dx and the workspace are 16-byte aligned");
   const Plan w = plan_of(t, d, n_logits);
   // a launch holds fewer than 2^32 threads
   BUX_CHECK(ceil_div(t, 32) * ceil_div(d, 4 * COLS) < (1LL << 24) && d * w.npad < (1LL << 32),
@@ -574,6 +696,7 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
   p.normalize = normalize != 0;
   p.hi = reinterpret_cast<uint16_t*>(ws + w.parts);
   p.lo = reinterpret_cast<uint16_t*>(ws + w.parts + w.kernel / 2);
+  p.blocks = reinterpret_cast<uint16_t*>(ws + w.kernel);
   p.bias_partials = d_bias ? reinterpret_cast<float*>(ws + w.bias) : nullptr;
   p.kernel_partials = reinterpret_cast<float*>(ws + w.partials);
   p.grads_blocks = t > 0 ? w.grads_blocks : 0;
@@ -583,23 +706,18 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
   p.d_kernel = d_kernel;
   p.d_bias = d_bias;
   if (t > 0) {
-    auto grads = [&](auto q) {
-      hipLaunchKernelGGL((grads_kernel<decltype(q)::value>), dim3(w.grads_blocks), dim3(THREADS), 0,
-                         s, p);
+    auto grads = [&](auto lanes, auto q) {
+      hipLaunchKernelGGL((grads_kernel<decltype(lanes)::value, decltype(q)::value>),
+                         dim3(static_cast<unsigned>(w.grads_blocks + ceil_div(d * w.npad, 4 * THREADS))),
+                         dim3(THREADS), 0, s, p);
     };
-    if (p.npad <= 64) grads(std::integral_constant<int, 1>{});
-    else if (p.npad <= 128) grads(std::integral_constant<int, 2>{});
-    else if (p.npad <= 256) grads(std::integral_constant<int, 4>{});
-    else if (p.npad <= 512) grads(std::integral_constant<int, 8>{});
-    else grads(std::integral_constant<int, 16>{});
+    using std::integral_constant;
+    if (p.npad <= 64) grads(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    else if (p.npad <= 128) grads(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    else if (p.npad <= 256) grads(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if (p.npad <= 512) grads(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+    else grads(integral_constant<int, 64>{}, integral_constant<int, 16>{});
     if (int rc = launched("route grads_kernel")) return rc;
-    if (n_logits % 32 != 0) {
-      uint16_t* pad = reinterpret_cast<uint16_t*>(ws + w.kernel);
-      hipLaunchKernelGGL(pad_kernel, dim3(static_cast<unsigned>(ceil_div(d * w.npad, THREADS))),
-                         dim3(THREADS), 0, s, kernel, d, n_logits, w.npad, pad);
-      if (int rc = launched("route pad_kernel")) return rc;
-      p.kernel = pad;
-    }
     const uint32_t columns = static_cast<uint32_t>(ceil_div(d, 4 * COLS));
     auto input = [&](auto rb) {
       constexpr int RB = decltype(rb)::value;
@@ -610,15 +728,20 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
     if (ceil_div(t, 64) * columns >= 256) input(std::integral_constant<int, 2>{});
     else input(std::integral_constant<int, 1>{});
     if (int rc = launched("route dx_kernel")) return rc;
+    constexpr size_t RING_BYTES = RING * sizeof(KStage);
+    if (hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel_grad_kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(RING_BYTES)))
+      return fail(BUX_E_LAUNCH, "route kernel_grad_kernel: %s", hipGetErrorString(err));
     hipLaunchKernelGGL(kernel_grad_kernel,
                        dim3(static_cast<unsigned>(ceil_div(d, COLS)),
                             static_cast<unsigned>(ceil_div(w.npad, COLS)),
                             static_cast<unsigned>(w.slices)),
-                       dim3(THREADS), 0, s, p);
+                       dim3(THREADS), RING_BYTES, s, p);
     if (int rc = launched("route kernel_grad_kernel")) return rc;
   }
   const int64_t kernel_blocks = ceil_div(d * w.npad, 4 * THREADS);
-  const int64_t bias_blocks = d_bias ? ceil_div(n_logits, 64) : 0;
+  const int64_t bias_blocks = d_bias ? ceil_div(n_logits, 16) : 0;
   hipLaunchKernelGGL(reduce_kernel, dim3(static_cast<unsigned>(kernel_blocks + bias_blocks)),
                      dim3(THREADS), 0, s, p, kernel_blocks);
   return launched("route reduce_kernel");

@@ -140,6 +140,8 @@ def route_backward(x: torch.Tensor, kernel: torch.Tensor, idx: torch.Tensor, log
     t = x.numel() // d if d else 0
     dev = x.device
     with on_device(x):
+        # the kernels load 16 bytes at whole 16s
+        x, dz = (v if v is None or v.data_ptr() % 16 == 0 else v.clone() for v in (x, dz))
         dx = torch.empty_like(x)
         d_kernel = torch.empty_like(kernel)
         d_bias = torch.empty(n, dtype=torch.float32, device=dev)

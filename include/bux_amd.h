@@ -734,7 +734,7 @@ int bux_route(const uint16_t* x, const uint16_t* kernel, const float* bias, int6
  * before the one rounding. dx, d_kernel bfloat16; d_bias float32, NULL to skip. The forward's
  * roundings to bfloat16 pass gradients as they are; the choice bias has none. float32 sums, in
  * a fixed order; G enters its products in two bfloat16 parts (2^-17 of each). The limits of
- * bux_route, without groups. workspace: bux_route_backward_workspace_size(t, d, n_logits)
+ * bux_route, without groups; x, dz, dx and the workspace 16-byte aligned. workspace: bux_route_backward_workspace_size(t, d, n_logits)
  * bytes: G, and d_kernel's partial sums. */
 size_t bux_route_backward_workspace_size(int64_t t, int64_t d, int32_t n_logits);
 int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int64_t t, int64_t d,

@@ -84,6 +84,7 @@ def test_the_routers_backward_rejects_bad_arguments(lib):
                       ({"router": 3}, "router=3"), ({"k": 0}, "k=0"), ({"k": 17}, "k=17"),
                       ({"scored": 1, "k": 2}, "k=2"), ({"scored": 32}, "d_sinks"),
                       ({"kernel": None}, "NULL"), ({"d_kernel": None}, "NULL"), ({"x": None}, "NULL"),
+                      ({"x": ctypes.c_void_p(18)}, "aligned"), ({"ws": ctypes.c_void_p(24)}, "aligned"),
                       ({"t": 1 << 30, "d": 4096}, "launch")):
         assert call(**bad) == 1 and word in _msg(lib), (bad, _msg(lib))
     need = lib.bux_route_backward_workspace_size(8, 64, 32)

@@ -290,6 +290,33 @@ def test_in_a_graph(lib):
         assert torch.equal(got.bias, want.bias)
 
 
+def test_tokens_at_any_element(lib):
+    """Tokens and their gradient that begin at an odd element (a slice's): copied, not misread."""
+    v = _inputs(40, 48, 24, 24, 3, seed=15, dz=True)
+    want = _run(v, 24, "softmax", True, 1.0, 1.0)
+    for key in ("x", "dz", "kernel"):
+        buf = torch.zeros(v[key].numel() + 3, dtype=BF16, device="cuda")
+        buf[3:].copy_(v[key].view(-1))
+        v[key] = buf[3:].view(v[key].shape)
+    got = _run(v, 24, "softmax", True, 1.0, 1.0)
+    assert torch.equal(got.x, want.x) and torch.equal(got.kernel, want.kernel)
+
+
+def test_a_workspace_of_nan(lib):
+    """What the workspace holds on entry reaches no output (its padding rows among it)."""
+    t, d, n = 37, 48, 20
+    v = _inputs(t, d, n, n, 3, seed=16)
+    want = _run(v, n, "softmax", True, 1.0, 1.0)
+    need = lib.bux_route_backward_workspace_size(t, d, n)
+    ws = torch.full((need // 2 + 1,), float("nan"), dtype=BF16, device="cuda")
+    dx, dk = torch.empty_like(v["x"]), torch.empty_like(v["kernel"])
+    p = (lambda x: x.data_ptr())
+    _lib.check(lib.bux_route_backward(
+        p(v["x"]), p(v["kernel"]), t, d, n, 1.0, 0, n, p(v["idx"]), 3, 1, 1.0, p(v["logits"]),
+        p(v["d_weights"]), None, None, None, None, p(dx), p(dk), None, p(ws), need, None))
+    assert torch.equal(dx, want.x) and torch.equal(dk, want.kernel)
+
+
 def test_refusals(lib):
     from bux_amd import router as r
     v = _inputs(8, 32, 16, 14, 2, seed=14)
