@@ -90,19 +90,18 @@ __device__ __forceinline__ float lanes_max(float v) {
   return v;
 }
 
-__device__ __forceinline__ float softplus(float v) {
-  return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v)));
-}
-// A logit's score off the softmax.
-__device__ __forceinline__ float score_of(int router, float z) {
-  return router == BUX_ROUTER_SIGMOID ? 1.0f / (1.0f + expf(-z)) : sqrtf(softplus(z));
-}
-// ... and its derivative, in forms that do not cancel for large |z|.
-__device__ __forceinline__ float slope_of(int router, float z, float s) {
-  const float e = expf(-fabsf(z)), p = 1.0f + e;
-  if (router == BUX_ROUTER_SIGMOID) return e / (p * p);
-  const float sigmoid = (z >= 0.0f ? 1.0f : e) / p;
-  return s == 0.0f ? 0.0f : sigmoid / (2.0f * s);
+// A logit's score off the softmax and its derivative, in forms that do not cancel for large |z|:
+// with e = exp(-|z|) and p = 1 / (1 + e), sigmoid(z) is p or e p, its derivative e p^2.
+__device__ __forceinline__ void score_of(int router, float z, float* s, float* slope) {
+  const float e = expf(-fabsf(z)), p = __builtin_amdgcn_rcpf(1.0f + e);
+  const float sigmoid = z >= 0.0f ? p : e * p;
+  if (router == BUX_ROUTER_SIGMOID) {
+    *s = sigmoid;
+    *slope = e * p * p;
+  } else {
+    *s = sqrtf(fmaxf(z, 0.0f) + log1pf(e));
+    *slope = *s == 0.0f ? 0.0f : sigmoid / (2.0f * *s);
+  }
 }
 
 // Columns i .. i + 3 of a row of n, `fill` past it.
@@ -120,8 +119,10 @@ __device__ __forceinline__ void load4(const float* row, int i, int n, float fill
   }
 }
 
-// L lanes a token, lane l the logits 4 l + 4 L c .. + 3 for c < Q / 4: a wave's tokens share its
-// chain of sums (a wave a token: 24.6 us for 16384 tokens of 128 logits).
+// L lanes a token, lane l the logits 4 l + 4 L c .. + 3 for c < Q / 4, so that a wave's tokens
+// share its chain of sums (a wave a token: 24.6 us for 16384 tokens of 128 logits). Bound by
+// VALU work then: each logit's count among the picks, and the sum of their gradients, pass
+// LDS, where the first of equal picks puts them (compared with every logit instead, 11 us).
 template <int L, int Q>
 __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
   if (static_cast<int32_t>(blockIdx.x) >= p.grads_blocks) {  // the kernel into blocks, 4 columns a thread
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
   }
   static_assert(L >= MAX_PICKS && Q % 4 == 0, "a lane a pick, whole fours of logits");
   constexpr int TOKENS = THREADS / L;
-  __shared__ float sums[TOKENS][L * Q];
+  __shared__ __align__(16) float counts[TOKENS][L * Q], grads[TOKENS][L * Q];
   const int lane = threadIdx.x % L, sub = threadIdx.x / L;
   const int first = (threadIdx.x & 63) - lane;  // the token's first lane of its wave
   const int n = p.n, scored = p.scored, k = p.k;
@@ -159,14 +160,57 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
     for (int q = 0; q < Q; q += 4) load4(row, column(q), n, -INFINITY, z + q);
     // the picks, one a lane: those outside the scored experts count for nothing
     int32_t id = -1;
-    float zp = 0.0f, g = 0.0f;
+    float g = 0.0f;
     if (lane < k) {
       id = p.idx[tok * k + lane];
       g = bf16_to_f32(p.d_weights[tok * k + lane]) * p.factor;
+      if (id >= scored || id < 0) id = -1 - lane;  // no other pick's
     }
-    const bool ok = id >= 0 && id < scored;
-    if (ok) zp = row[id];
-    float w;
+    // the picks' counts and gradients by logit: of equal picks the first's lane puts all
+    float count[Q], grad[Q];
+#pragma unroll
+    for (int q = 0; q < Q; q += 4) {
+      *reinterpret_cast<float4*>(&counts[sub][column(q)]) = make_float4(0, 0, 0, 0);
+      *reinterpret_cast<float4*>(&grads[sub][column(q)]) = make_float4(0, 0, 0, 0);
+    }
+    float times = 0.0f, sum_g = 0.0f;
+    int before = k;
+    for (int j = 0; j < k; ++j) {
+      const int32_t other = __shfl(id, first + j);
+      const float v = __shfl(g, first + j);
+      if (other == id) {
+        times += 1.0f;
+        sum_g += v;
+        before = j < before ? j : before;
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's own region
+    __builtin_amdgcn_wave_barrier();
+    if (lane < k && before == lane && id >= 0) {
+      counts[sub][id] = times;
+      grads[sub][id] = sum_g;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int q = 0; q < Q; q += 4) {
+      const float4 c = *reinterpret_cast<const float4*>(&counts[sub][column(q)]);
+      const float4 v = *reinterpret_cast<const float4*>(&grads[sub][column(q)]);
+      count[q] = c.x; count[q + 1] = c.y; count[q + 2] = c.z; count[q + 3] = c.w;
+      grad[q] = v.x; grad[q + 1] = v.y; grad[q + 2] = v.z; grad[q + 3] = v.w;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    if (n > scored) {  // a sink counts once
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int i = column(q);
+        if (i < scored || i >= n) continue;
+        count[q] = 1.0f;
+        if (p.d_sinks) grad[q] = bf16_to_f32(p.d_sinks[tok * (n - scored) + i - scored]) * p.factor;
+      }
+    }
+    float slope[Q];
     if (p.router == BUX_ROUTER_SOFTMAX) {
       float m = z[0];
 #pragma unroll
@@ -178,43 +222,31 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
         s[q] = expf(z[q] - m);
         sum += s[q];
       }
-      const float all = lanes_sum<L>(sum);
+      const float inv = 1.0f / lanes_sum<L>(sum);
 #pragma unroll
-      for (int q = 0; q < Q; ++q) s[q] /= all;
-      w = expf(zp - m) / all;
+      for (int q = 0; q < Q; ++q) slope[q] = s[q] *= inv;
     } else {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) s[q] = column(q) < n ? score_of(p.router, z[q]) : 0.0f;
-      w = score_of(p.router, zp);
+      for (int q = 0; q < Q; ++q) {
+        score_of(p.router, z[q], &s[q], &slope[q]);
+        if (column(q) >= n) s[q] = slope[q] = 0.0f;
+      }
     }
-    if (!ok) w = g = 0.0f;
-    float sink[Q];  // the sinks' gradients
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int i = column(q);
-      sink[q] = p.d_sinks && i >= scored && i < n
-                    ? bf16_to_f32(p.d_sinks[tok * (n - scored) + i - scored]) * p.factor : 0.0f;
-    }
-    float inv = 1.0f, shift = 0.0f;  // ds = (g - shift) inv
+    float inv = 1.0f, shift = 0.0f;  // a pick's ds = (g - shift) inv
     if (p.normalize) {
-      float total = w, dot = g * w;
-      if (n > scored) {
+      float total = 0.0f, dot = 0.0f;
 #pragma unroll
-        for (int q = 0; q < Q; ++q)
-          if (column(q) >= scored && column(q) < n) {
-            total += s[q];
-            dot += sink[q] * s[q];
-          }
+      for (int q = 0; q < Q; ++q) {
+        total += count[q] * s[q];
+        dot += grad[q] * s[q];
       }
       total = lanes_sum<L>(total);
       dot = lanes_sum<L>(dot);
       inv = total == 0.0f ? 0.0f : 1.0f / total;
-      shift = total == 0.0f ? 0.0f : dot / total;
+      shift = dot * inv;
     }
-    const float dp = ok ? (g - shift) * inv : 0.0f;
 #pragma unroll
-    for (int q = 0; q < Q; ++q)
-      ds[q] = column(q) >= scored && column(q) < n ? (sink[q] - shift) * inv : 0.0f;
+    for (int q = 0; q < Q; ++q) ds[q] = (grad[q] - count[q] * shift) * inv;
     if (p.d_scores) {
 #pragma unroll
       for (int q = 0; q < Q; q += 4) {
@@ -224,12 +256,6 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
         for (int j = 0; j < 4; ++j) ds[q + j] += v[j];
       }
     }
-    for (int j = 0; j < k; ++j) {
-      const int32_t at = __shfl(id, first + j);
-      const float v = __shfl(dp, first + j);
-#pragma unroll
-      for (int q = 0; q < Q; ++q) ds[q] += column(q) == at ? v : 0.0f;
-    }
     float inner = 0.0f;
     if (p.router == BUX_ROUTER_SOFTMAX) {
 #pragma unroll
@@ -237,10 +263,7 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
       inner = lanes_sum<L>(inner);
     }
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const float slope = p.router == BUX_ROUTER_SOFTMAX ? s[q] : slope_of(p.router, z[q], s[q]);
-      ds[q] = column(q) < n ? (ds[q] - inner) * slope : 0.0f;
-    }
+    for (int q = 0; q < Q; ++q) ds[q] = (ds[q] - inner) * slope[q];
     if (p.d_logits) {
 #pragma unroll
       for (int q = 0; q < Q; q += 4) {
@@ -252,31 +275,32 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
     }
 #pragma unroll
     for (int q = 0; q < Q; q += 4) {
-      uint16_t h[4], l[4];
+      float d[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float dl = live ? ds[q + j] * p.logit_scale : 0.0f;
-        bias[q + j] += dl;
-        h[j] = f32_to_bf16(dl);
-        l[j] = f32_to_bf16(dl - bf16_to_f32(h[j]));
+        d[j] = live && column(q + j) < n ? ds[q + j] * p.logit_scale : 0.0f;
+        bias[q + j] += d[j];
       }
       if (column(q) < p.npad) {
         const int64_t at = at_block(base + sub, column(q), p.npad);
-        *reinterpret_cast<uint2*>(p.hi + at) =
-            make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
+        const uint32_t h0 = pack_bf16x2(d[0], d[1]), h1 = pack_bf16x2(d[2], d[3]);
+        *reinterpret_cast<uint2*>(p.hi + at) = make_uint2(h0, h1);
         *reinterpret_cast<uint2*>(p.lo + at) =
-            make_uint2(l[0] | (static_cast<uint32_t>(l[1]) << 16), l[2] | (static_cast<uint32_t>(l[3]) << 16));
+            make_uint2(pack_bf16x2(d[0] - __uint_as_float(h0 << 16),
+                                   d[1] - __uint_as_float(h0 & 0xffff0000u)),
+                       pack_bf16x2(d[2] - __uint_as_float(h1 << 16),
+                                   d[3] - __uint_as_float(h1 & 0xffff0000u)));
       }
     }
   }
   if (p.bias_partials == nullptr) return;
 #pragma unroll
-  for (int q = 0; q < Q; ++q) sums[sub][column(q)] = bias[q];
+  for (int q = 0; q < Q; ++q) counts[sub][column(q)] = bias[q];
   __syncthreads();
   for (int i = threadIdx.x; i < p.npad; i += THREADS) {
-    float s = sums[0][i];
+    float s = counts[0][i];
 #pragma unroll
-    for (int j = 1; j < TOKENS; ++j) s += sums[j][i];
+    for (int j = 1; j < TOKENS; ++j) s += counts[j][i];
     p.bias_partials[static_cast<int64_t>(blockIdx.x) * p.npad + i] = s;
   }
 }
@@ -725,7 +749,10 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
                          dim3(static_cast<unsigned>(columns * ceil_div(t, 32 * RB))), dim3(THREADS),
                          0, s, p, columns);
     };
-    if (ceil_div(t, 64) * columns >= 256) input(std::integral_constant<int, 2>{});
+    // 32 tokens a wave where its products are few, with three waves a SIMD to hide their loads; 64
+    // where the kernel's loads for them count (16384 tokens, 2048 columns, 128 logits: 36.7 us and
+    // 43.0; 8192, 7168, 256: 102 and 85) and there are workgroups to fill the chip
+    if (w.npad > 128 && ceil_div(t, 64) * columns >= 256) input(std::integral_constant<int, 2>{});
     else input(std::integral_constant<int, 1>{});
     if (int rc = launched("route dx_kernel")) return rc;
     constexpr size_t RING_BYTES = RING * sizeof(KStage);
