@@ -317,13 +317,14 @@ __device__ __forceinline__ bf16x8 load8(const uint16_t* p) {
 // products, the next 32's before the first are stored.
 constexpr int COLS = 128;
 constexpr int DX_PITCH = COLS / 2 + 4;  // floats: rows 16 bytes past a multiple of the banks
+constexpr size_t DX_BYTES = (THREADS / 64) * 32 * DX_PITCH * sizeof(float);
 template <int RB>
-__global__ __launch_bounds__(THREADS) void dx_kernel(Params p, uint32_t columns) {
-  __shared__ __align__(16) float out[THREADS / 64][32 * DX_PITCH];
+__device__ __forceinline__ void dx_tile(const Params& p, uint32_t block, uint32_t columns,
+                                        uint8_t* smem) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 31, h = lane >> 5;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x / columns) * (32 * RB);
-  const int64_t c0 = (static_cast<int64_t>(blockIdx.x % columns) * 4 + wave) * COLS;
+  const int64_t t0 = static_cast<int64_t>(block / columns) * (32 * RB);
+  const int64_t c0 = (static_cast<int64_t>(block % columns) * 4 + wave) * COLS;
   if (c0 >= p.d) return;  // no barrier follows
   // blocks past the last: the last one's, not stored
   const int64_t t_last = (p.t - 1) >> 5, c_last = (p.d - 1) >> 5;
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(THREADS) void dx_kernel(Params p, uint32_t columns)
     multiply(two);
     __builtin_amdgcn_sched_barrier(0);
   }
-  float* mine = out[wave];
+  float* mine = reinterpret_cast<float*>(smem) + wave * 32 * DX_PITCH;
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
     uint4 now[2][4];
@@ -451,8 +452,7 @@ __global__ __launch_bounds__(THREADS) void dx_kernel(Params p, uint32_t columns)
 // Columns past d or npad read what follows them in memory, into sums that are not stored;
 // tokens past the last read 0.
 constexpr int STEP = 32;
-constexpr int RING = 3;
-constexpr int KLOADS = 6;  // direct loads a wave issues a step: 2 of each operand
+constexpr int RING = 2;
 struct KStage {
   uint16_t x[STEP * COLS], hi[STEP * COLS], lo[STEP * COLS];
 };
@@ -464,12 +464,16 @@ __device__ __forceinline__ bf16x8 read_tr(uint32_t at, uint32_t at4) {
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-__global__ __launch_bounds__(THREADS) void kernel_grad_kernel(Params p) {
-  extern __shared__ __align__(16) uint8_t smem[];
+constexpr size_t RING_BYTES = RING * sizeof(KStage);
+
+__device__ __forceinline__ void kernel_grad_tile(const Params& p, uint32_t block, uint8_t* smem) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t j0 = static_cast<int64_t>(blockIdx.x) * COLS;
-  const int32_t e0 = blockIdx.y * COLS;
-  const int64_t lo_t = blockIdx.z * p.slice;
+  // the logits' tiles of one slice and columns beside each other, then the columns'
+  const uint32_t e_tiles = (p.npad + COLS - 1) / COLS, j_tiles = (p.d + COLS - 1) / COLS;
+  const int32_t e0 = block % e_tiles * COLS;
+  const int64_t j0 = static_cast<int64_t>(block / e_tiles % j_tiles) * COLS;
+  const int64_t slice = block / e_tiles / j_tiles;
+  const int64_t lo_t = slice * p.slice;
   const int64_t hi_t = lo_t + p.slice < p.t ? lo_t + p.slice : p.t;
   const int steps = static_cast<int>((hi_t - lo_t + STEP - 1) / STEP);
   const uint32_t lds0 = lds_at(smem);
@@ -526,9 +530,8 @@ __global__ __launch_bounds__(THREADS) void kernel_grad_kernel(Params p) {
     for (int j = 0; j < 2; ++j) acc[i][j] = v16f{};
   for (int s = 0; s < RING - 1 && s < steps; ++s) issue(s);
   for (int s = 0; s < steps; ++s) {
-    // this step's loads are in once only those of the steps after it are out
-    if (s + 1 < steps && RING > 2) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // this step's loads are in (the next's go out after the barrier)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // ... in every wave; and every wave has read the stage that the next loads take
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (s + RING - 1 < steps) issue(s + RING - 1);
@@ -554,7 +557,7 @@ __global__ __launch_bounds__(THREADS) void kernel_grad_kernel(Params p) {
         }
     }
   }
-  float* base = p.kernel_partials + static_cast<int64_t>(blockIdx.z) * p.d * p.npad;
+  float* base = p.kernel_partials + slice * p.d * p.npad;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int64_t j = j0 + 64 * (wave >> 1) + 32 * i + (lane & 31);
@@ -570,6 +573,16 @@ __global__ __launch_bounds__(THREADS) void kernel_grad_kernel(Params p) {
                           acc[i][q][4 * g + 3]);
       }
   }
+}
+
+// Both products in one launch, so that either's loads fill the other's waits: the kernel's
+// gradient's workgroups first, which take longer.
+template <int RB>
+__global__ __launch_bounds__(THREADS) void products_kernel(Params p, uint32_t kernel_blocks,
+                                                           uint32_t columns) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  if (blockIdx.x < kernel_blocks) kernel_grad_tile(p, blockIdx.x, smem);
+  else dx_tile<RB>(p, blockIdx.x - kernel_blocks, columns, smem);
 }
 
 // d_kernel: the slices' sums in order, 4 logits a thread; d_bias: a block each 16 logits after
@@ -743,29 +756,22 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
     else grads(integral_constant<int, 64>{}, integral_constant<int, 16>{});
     if (int rc = launched("route grads_kernel")) return rc;
     const uint32_t columns = static_cast<uint32_t>(ceil_div(d, 4 * COLS));
-    auto input = [&](auto rb) {
+    const uint32_t tiles =
+        static_cast<uint32_t>(ceil_div(d, COLS) * ceil_div(w.npad, COLS) * w.slices);
+    constexpr size_t LDS = RING_BYTES > DX_BYTES ? RING_BYTES : DX_BYTES;
+    auto products = [&](auto rb) {
       constexpr int RB = decltype(rb)::value;
-      hipLaunchKernelGGL((dx_kernel<RB>),
-                         dim3(static_cast<unsigned>(columns * ceil_div(t, 32 * RB))), dim3(THREADS),
-                         0, s, p, columns);
+      hipLaunchKernelGGL((products_kernel<RB>),
+                         dim3(static_cast<unsigned>(tiles + columns * ceil_div(t, 32 * RB))),
+                         dim3(THREADS), LDS, s, p, tiles, columns);
     };
+    static_assert(LDS <= 64 * 1024, "a launch's LDS without an attribute");
     // 32 tokens a wave where its products are few, with three waves a SIMD to hide their loads; 64
     // where the kernel's loads for them count (16384 tokens, 2048 columns, 128 logits: 36.7 us and
     // 43.0; 8192, 7168, 256: 102 and 85) and there are workgroups to fill the chip
-    if (w.npad > 128 && ceil_div(t, 64) * columns >= 256) input(std::integral_constant<int, 2>{});
-    else input(std::integral_constant<int, 1>{});
-    if (int rc = launched("route dx_kernel")) return rc;
-    constexpr size_t RING_BYTES = RING * sizeof(KStage);
-    if (hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel_grad_kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(RING_BYTES)))
-      return fail(BUX_E_LAUNCH, "route kernel_grad_kernel: %s", hipGetErrorString(err));
-    hipLaunchKernelGGL(kernel_grad_kernel,
-                       dim3(static_cast<unsigned>(ceil_div(d, COLS)),
-                            static_cast<unsigned>(ceil_div(w.npad, COLS)),
-                            static_cast<unsigned>(w.slices)),
-                       dim3(THREADS), RING_BYTES, s, p);
-    if (int rc = launched("route kernel_grad_kernel")) return rc;
+    if (w.npad > 128 && ceil_div(t, 64) * columns >= 256) products(integral_constant<int, 2>{});
+    else products(integral_constant<int, 1>{});
+    if (int rc = launched("route products_kernel")) return rc;
   }
   const int64_t kernel_blocks = ceil_div(d * w.npad, 4 * THREADS);
   const int64_t bias_blocks = d_bias ? ceil_div(n_logits, 16) : 0;
