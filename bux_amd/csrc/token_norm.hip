@@ -190,10 +190,13 @@ __global__ __launch_bounds__(threads_of<W>()) void forward_kernel(
 }
 
 // The backward's workgroups over m rows of W waves of C chunks: as many as the chip holds at
-// once by their registers (4, 3 or 2 waves a SIMD), or a turn each where there are fewer rows.
+// once by their registers (4, 3 or 2 waves a SIMD; of 8 waves two a CU or one, so two), or a turn
+// each where there are fewer rows. (16384 bfloat16 rows of 7168: 384 workgroups of 8 waves 200
+// us, 512 161; the next row's loads out ahead of this one's sums 189.)
 constexpr int64_t MAX_BLOCKS = 1024;
 int64_t backward_blocks(int64_t m, int w, int c) {
-  const int64_t most = (c == 1 ? 4096 : c == 2 ? 3072 : 2048) / (w > 4 ? w : 4);
+  const int64_t waves = c == 1 || (c == 2 && w > 4) ? 4096 : c == 2 ? 3072 : 2048;
+  const int64_t most = waves / (w > 4 ? w : 4);
   const int64_t want = ceil_div(m, w > 4 ? 1 : 4 / w);
   return want < most ? want : most;
 }
