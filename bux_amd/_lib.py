@@ -146,8 +146,11 @@ SIGNATURES = {
     "bux_glu_backward_quantize_f32": (
         _int, [_p, _p, _p, _p, _i64, _i64, _ffn, _i64, _p, _p, _p, _p, _p, _p, _p,
                _size, _p]),
-    "bux_int8_quantize": (_int, [_p, _p, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p]),
-    "bux_int8_quantize_f32": (_int, [_p, _p, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p]),
+    "bux_int8_quantize_workspace_size": (_size, [_i64, _i64, _i64]),
+    "bux_int8_quantize": (
+        _int, [_p, _p, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _size, _p]),
+    "bux_int8_quantize_f32": (
+        _int, [_p, _p, _i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _size, _p]),
     "bux_int8_glu": (_int, [_p, _p, _p, _i64, _i64, _ffn, _i64, _p, _p, _p]),
     "bux_int8_glu_f32": (_int, [_p, _p, _p, _i64, _i64, _ffn, _i64, _p, _p, _p]),
     "bux_int8_quantize_columns": (_int, [_p, _i64, _i64, _i64, _p, _p, _p]),

@@ -5,9 +5,10 @@
 // The schedule is the MXFP8 GEMMs' (tiles.h, grouped_mx.hip): a tile list, a persistent grid,
 // 256 x 256 outputs a workgroup in 4 waves, direct loads into a ring of 4 LDS stages; operands
 // in the same tiled layout, codes [K / 64][rows][64]. A step is 64 of K, 32 MFMAs a wave: an
-// 8-bit integer MFMA has the rate of an MXFP8 one. Both operands' scales are a float a row, and
-// go to LDS beside each step's codes as the MXFP8 scale words do (2 of a wave's 10 loads a
-// step), so that the epilogue finds its tile's in the last step's stage.
+// 8-bit integer MFMA has the rate of an MXFP8 one. Both operands' scales are a float a row: a
+// tile's go to LDS once, with its first step's codes, to one of two places that tiles take in
+// turn, where the epilogue finds them. (A load of each beside every step's codes instead: 131072
+// rows of K 2048, N 1536 510 us and 506, 8192 tokens of gpt-oss-120b's up product 860 and 842.)
 //
 // MFMA lane layout (32 x 32 x 32): lane l holds row l % 32 of either operand, its half l / 32
 // the 16 bytes of K 16 (l / 32) .. + 15; accumulators as the float MFMAs'.
@@ -23,7 +24,7 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
 constexpr int BK = 64;  // bytes of K a step
-constexpr int LOADS_A_STEP = 10;
+constexpr int LOADS_A_STEP = 8;
 constexpr int64_t MAX_K = 131072;
 
 struct Operand {
@@ -33,20 +34,26 @@ struct Operand {
   int32_t rows;
 };
 
-// One K step's codes of 256 rows of A and B, and the rows' scales past the bytes that the
-// epilogue stages outputs in.
+// One K step's codes of 256 rows of A and B, and to the bytes that the epilogue stages outputs in.
 struct Stage {
   uint8_t a[BM * BK];
   uint8_t b[BN * BK];
   uint8_t gap[STAGING - BM * BK - BN * BK];
-  float as[BM];
-  float bs[BN];
+};
+struct Scales {
+  float a[BM];
+  float b[BN];
   float added[BN];  // the columns' biases, written by the epilogue
 };
 struct Lds {
   Stage st[STAGES];
+  Scales tile[2];
 };
 static_assert(sizeof(Lds) <= 160 * 1024, "the stages fit a CU's LDS");
+
+// Which of the two places a tile's scales take rides above its first row's bits.
+constexpr int32_t PLACE_BIT = 1 << 30;
+constexpr int32_t ROW_MASK = PLACE_BIT - 1;
 
 // Where a 64-byte LDS row's 16-byte chunk c sits: c ^ swizzle(row), so that 16 lanes that read
 // one chunk of 16 consecutive rows hit every bank once.
@@ -57,9 +64,11 @@ struct Loads {
   i32x4 rv, rs;
   int32_t voff, soff;    // this lane's
   int32_t chunk_stride;  // a K chunk's bytes: rows x 64
+  int32_t place;         // A's: of the tile's scales
 };
 
-__device__ __forceinline__ Loads loads_for(const Operand& op, int32_t row0) {
+__device__ __forceinline__ Loads loads_for(const Operand& op, int32_t placed_row) {
+  const int32_t row0 = placed_row & ROW_MASK;
   const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
   Loads ld;
   ld.values = op.values;
@@ -69,6 +78,7 @@ __device__ __forceinline__ Loads loads_for(const Operand& op, int32_t row0) {
   ld.voff = (row0 + r) * 64 + 16 * ((l & 3) ^ swizzle(r));
   ld.soff = (row0 + w * 64 + l) * 4;
   ld.chunk_stride = op.rows * 64;
+  ld.place = placed_row >> 30;
   return ld;
 }
 
@@ -84,31 +94,28 @@ __device__ __forceinline__ i32x4 chunk_at(const Loads& l, int32_t c, int32_t& so
   }
 }
 
-// Direct load Q (0 .. 9) of K step ks: Q < 8 a 16-row slice of A's (even Q) or B's (odd Q) rows
-// of this wave, 8 and 9 its rows' scales. In a half tile (H) waves 2 and 3, whose rows of A do
-// not exist, load their scales again in their place, so that every wave issues 10.
+// Direct load Q (0 .. 7) of K step ks: a 16-row slice of A's (even Q) or B's (odd Q) rows of this
+// wave. In a half tile (H) waves 2 and 3, whose rows of A do not exist, load their rows' scales
+// again in their place, so that every wave issues 8.
+__device__ __forceinline__ uint32_t scales_at(uint32_t lds0, int32_t place) {
+  return lds0 + static_cast<uint32_t>(offsetof(Lds, tile) + place * sizeof(Scales));
+}
 template <int Q, bool H, bool W>
 __device__ __forceinline__ void issue_one(const Loads& la, const Loads& lb, int32_t ks,
                                           uint32_t lds0, int st) {
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t at = lds0 + static_cast<uint32_t>(st * sizeof(Stage));
-  if (Q < 8) {
-    constexpr int i = Q >> 1;
-    const uint32_t slice = w * 4096 + i * 1024;
-    int32_t so;
-    if ((Q & 1) == 0 && H && w >= 2) {
-      load_lds4(la.rs, at + offsetof(Stage, as) + w * 256, la.soff, 0);
-    } else if ((Q & 1) == 0) {
-      const i32x4 r = chunk_at<W>(la, ks, so);
-      load_lds16(r, at + offsetof(Stage, a) + slice, la.voff, so + i * 1024);
-    } else {
-      const i32x4 r = chunk_at<W>(lb, ks, so);
-      load_lds16(r, at + offsetof(Stage, b) + slice, lb.voff, so + i * 1024);
-    }
-  } else if (Q == 8) {
-    load_lds4(la.rs, at + offsetof(Stage, as) + w * 256, la.soff, 0);
+  constexpr int i = Q >> 1;
+  const uint32_t slice = w * 4096 + i * 1024;
+  int32_t so;
+  if ((Q & 1) == 0 && H && w >= 2) {
+    load_lds4(la.rs, scales_at(lds0, la.place) + offsetof(Scales, a) + w * 256, la.soff, 0);
+  } else if ((Q & 1) == 0) {
+    const i32x4 r = chunk_at<W>(la, ks, so);
+    load_lds16(r, at + offsetof(Stage, a) + slice, la.voff, so + i * 1024);
   } else {
-    load_lds4(lb.rs, at + offsetof(Stage, bs) + w * 256, lb.soff, 0);
+    const i32x4 r = chunk_at<W>(lb, ks, so);
+    load_lds16(r, at + offsetof(Stage, b) + slice, lb.voff, so + i * 1024);
   }
 }
 template <int Q, bool H, bool W>
@@ -175,15 +182,7 @@ __device__ __forceinline__ void step_of(const Frag& cur, Frag& nxt, const Loads&
         case 4: issue_one<4, H, W>(la, lb, ks_load, lds0, st_load); break;
         case 5: issue_one<5, H, W>(la, lb, ks_load, lds0, st_load); break;
         case 6: issue_one<6, H, W>(la, lb, ks_load, lds0, st_load); break;
-        case 7:
-          issue_one<7, H, W>(la, lb, ks_load, lds0, st_load);
-          if (H) {
-            issue_one<8, H, W>(la, lb, ks_load, lds0, st_load);
-            issue_one<9, H, W>(la, lb, ks_load, lds0, st_load);
-          }
-          break;
-        case 8: issue_one<8, H, W>(la, lb, ks_load, lds0, st_load); break;
-        case 9: issue_one<9, H, W>(la, lb, ks_load, lds0, st_load); break;
+        case 7: issue_one<7, H, W>(la, lb, ks_load, lds0, st_load); break;
         default: break;
       }
     }
@@ -216,13 +215,21 @@ struct Int8 {
   }
   __device__ static __forceinline__ void issue(const Loads& la, const Loads& lb, int32_t ks,
                                                uint32_t lds0, int st, bool half) {
+    // A tile's scales go ahead of its first step's codes (never in a step: those load from step 4
+    // on). The waits count 8 loads a step: these two among later ones make them stricter.
+    if (ks == 0) {
+      const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      const uint32_t at = scales_at(lds0, la.place) + w * 256;
+      load_lds4(la.rs, at + offsetof(Scales, a), la.soff, 0);
+      load_lds4(lb.rs, at + offsetof(Scales, b), lb.soff, 0);
+    }
     if (half) issue_from<0, true, W>(la, lb, ks, lds0, st);
     else issue_from<0, false, W>(la, lb, ks, lds0, st);
   }
   __device__ static __forceinline__ void wait_loads(int32_t steps) {
-    if (steps >= 3) asm volatile("s_waitcnt vmcnt(30)" ::: "memory");
-    else if (steps == 2) asm volatile("s_waitcnt vmcnt(20)" ::: "memory");
-    else if (steps == 1) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    if (steps >= 3) asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
+    else if (steps == 2) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    else if (steps == 1) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   template <bool H>
@@ -280,11 +287,24 @@ struct Scaled {
   }
 };
 
+// The rows GEMM's tiles, each with the place of its scales in turn.
+struct PlacedTiles : RowsTiles<false, true> {
+  mutable int32_t place = 0;
+  __device__ explicit PlacedTiles(const RowsTiles<false, true>& list) : RowsTiles<false, true>(list) {}
+  __device__ bool job(int32_t id, Job& j) const {
+    if (!RowsTiles<false, true>::job(id, j)) return false;
+    j.a_row0 |= place;
+    place ^= PLACE_BIT;
+    return true;
+  }
+};
+
 template <typename T, bool BIASED>
 struct Out {
   T* out;
   int32_t ld;
   const T* bias;  // (groups, ld)
+  Scales* tiles;  // the two places
   __device__ __forceinline__ void store(const v16f acc[4][4], const Job& j, Stage& stage) const {
     // The thread's place, computed here: hoisted out of the tiles' loop, what depends on it
     // alone would be held through every K loop, and went to scratch memory.
@@ -293,22 +313,23 @@ struct Out {
     const int lane = thread & 63, wave = thread >> 6;
     const int row0 = (j.half ? 0 : (wave >> 1) * 128) + (lane & 31);
     const int col0 = (j.half ? wave * 64 : (wave & 1) * 128) + 4 * (lane >> 5);
+    Scales& scales = tiles[j.a_row0 >> 30];
     if (j.n == 0) {  // rows past the groups: no step ran, so the scales are 0 here
-      stage.bs[thread] = 0.0f;
+      scales.b[thread] = 0.0f;
       barrier_lds();
     }
     if constexpr (BIASED) {
       const T* const row = bias + static_cast<int64_t>(j.group) * ld + j.b_row0;
       const int c = thread;
-      stage.added[c] = j.n > 0 && c < j.cols ? Elem<T>::value(row[c]) : 0.0f;
+      scales.added[c] = j.n > 0 && c < j.cols ? Elem<T>::value(row[c]) : 0.0f;
       barrier_lds();
     }
     Scaled<BIASED> from;
     from.acc = acc;
-    from.col = stage.bs + col0;
-    from.added = stage.added + col0;
+    from.col = scales.b + col0;
+    from.added = scales.added + col0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) from.row[i] = j.n > 0 ? stage.as[row0 + 32 * i] : 0.0f;
+    for (int i = 0; i < 4; ++i) from.row[i] = j.n > 0 ? scales.a[row0 + 32 * i] : 0.0f;
     store_plain(from, out, ld, j, stage);
   }
 };
@@ -321,9 +342,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
   extern __shared__ __align__(16) uint8_t smem[];
   if (!list_fits(starts, groups, A.rows, height)) return;
   Lds& lds = *reinterpret_cast<Lds*>(smem);
-  const RowsTiles<false, true> list{tiles, groups, n, height, col_tiles, A.k / BK, A.k};
+  const PlacedTiles list(RowsTiles<false, true>{tiles, groups, n, height, col_tiles, A.k / BK, A.k});
   const int32_t count = starts[groups + 1] * col_tiles;
-  run_tiles<Int8<W>>(list, count, A, B, lds, Out<T, BIASED>{y, n, bias});
+  run_tiles<Int8<W>>(list, count, A, B, lds, Out<T, BIASED>{y, n, bias, lds.tile});
 }
 
 // The loads' 32-bit offsets hold a K chunk's rows (a tile's reads past them included), and the

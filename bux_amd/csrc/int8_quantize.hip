@@ -190,8 +190,8 @@ struct Units {
 };
 
 // A wave a row of the copy's `height`: rows from `rows` or *filled on are 0. C: the row's parts
-// a lane keeps, or 0 to read them twice.
-template <typename T, int C, typename Source>
+// a lane keeps, or 0 to read them twice. PLAIN: the codes row after row, not tiled.
+template <typename T, int C, bool PLAIN, typename Source>
 __global__ __launch_bounds__(THREADS) void rows_kernel(Source from, int64_t rows, int64_t height,
                                                        const int32_t* __restrict__ filled,
                                                        int64_t cols, int64_t k,
@@ -202,9 +202,10 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(Source from, int64_t rows
                     __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (i >= height) return;
   const int64_t live = filled && *filled < rows ? *filled : rows;
-  uint8_t* const out = values + i * 64;
+  uint8_t* const out = values + i * (PLAIN ? k : 64);
   auto put = [&](int64_t c, uint2 codes) {
-    if (c < k) *reinterpret_cast<uint2*>(out + (c >> 6) * (height * 64) + (c & 63)) = codes;
+    const int64_t at = PLAIN ? c : (c >> 6) * (height * 64) + (c & 63);
+    if (c < k) *reinterpret_cast<uint2*>(out + at) = codes;
   };
   if (i >= live) {
     for (int64_t c = 8 * lane; c < k; c += 512) put(c, make_uint2(0, 0));
@@ -238,15 +239,64 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(Source from, int64_t rows
   }
 }
 
-template <typename T, int C, typename Source>
+template <typename T, int C, bool PLAIN = false, typename Source>
 int launch_rows(const char* kernel, const Source& from, int64_t rows, int64_t height,
                 const int32_t* filled, int64_t cols, uint8_t* values, float* scales,
                 hipStream_t s) {
   const int64_t k = ceil_div(cols, 128) * 128;
-  hipLaunchKernelGGL((rows_kernel<T, C, Source>),
+  hipLaunchKernelGGL((rows_kernel<T, C, PLAIN, Source>),
                      dim3(static_cast<unsigned>(ceil_div(height, THREADS / 64))), dim3(THREADS), 0,
                      s, from, rows, height, filled, cols, k, values, scales);
   return launched(kernel);
+}
+
+// Rows by index from tokens quantized once (codes (sources, k) row after row, and their scales).
+// A workgroup moves 128 codes of 256 rows: loads of 64-byte runs, two a token's line, stores of 1
+// KiB in one run. The workgroups go through all rows for one 128 of K after another, an XCD (a
+// workgroup's id modulo 8) a contiguous share, so that those 128 bytes of every token stay in
+// its L2 for all of the token's rows.
+constexpr int GATHERED = 256;
+typedef uint32_t Word4 __attribute__((ext_vector_type(4)));
+__global__ __launch_bounds__(THREADS) void gather_kernel(
+    const uint8_t* __restrict__ codes, const float* __restrict__ from_scales,
+    const int32_t* __restrict__ index, int32_t index_div, int64_t sources, int64_t rows,
+    int64_t height, const int32_t* __restrict__ filled, int64_t k, int64_t row_blocks,
+    int64_t share, uint8_t* __restrict__ values, float* __restrict__ scales) {
+  const int64_t item = (blockIdx.x % 8) * share + blockIdx.x / 8;
+  const int64_t pair = item / row_blocks;
+  if (pair >= k / 128) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, piece = 16 * (lane & 3);
+  const int64_t live = filled && *filled < rows ? *filled : rows;
+  const int64_t i0 = item % row_blocks * GATHERED + wave * 64 + (lane >> 2);
+  constexpr int U = 4;  // of 16 rows
+  int64_t token[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = i0 + 16 * u;
+    const int32_t pick = i < live ? index[i] : -1;
+    token[u] = pick < 0 ? -1 : pick / index_div;
+    if (token[u] >= sources) token[u] = -1;
+  }
+  uint4 v[U][2];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      v[u][h] = make_uint4(0, 0, 0, 0);
+      if (token[u] >= 0)
+        v[u][h] = *reinterpret_cast<const uint4*>(codes + token[u] * k + pair * 128 + 64 * h + piece);
+    }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = i0 + 16 * u;
+    if (i >= height) continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      __builtin_nontemporal_store(
+          __builtin_bit_cast(Word4, v[u][h]),
+          reinterpret_cast<Word4*>(values + (2 * pair + h) * (height * 64) + i * 64 + piece));
+    if (pair == 0 && piece == 0) scales[i] = token[u] >= 0 ? from_scales[token[u]] : 0.0f;
+  }
 }
 
 // --- the kernels' columns ------------------------------------------------------------------
@@ -309,27 +359,62 @@ int check_copy(const char* name, int64_t rows, int64_t cols, int64_t height) {
   return BUX_OK;
 }
 
+// The bytes of the tokens' own codes and scales, or 0 where rows are quantized one by one: few
+// codes, whose second launch costs more than it saves, or not twice as many rows as tokens.
+// us, each row quantized from its token and each token once (bfloat16; float32):
+//   4096 tokens of 2048, 4 rows each   21  19;   30  23      1024 of 7168, 4   19  22;   49  31
+//   16384 of 2048, 2                   38  39;   55  51      1024 of 7168, 8   34  27;   88  36
+//   16384 of 2048, 8                  137  71;  192  83      16384 of 7168, 8 590 240; 1261 421
+//   16384 of 512, 4                    28  21;   45  24      4096 of 512, 8    16  16;   25  15
+size_t gather_workspace(int64_t sources, int64_t rows, int64_t cols) {
+  if (rows < 2 * sources || rows * cols < (1LL << 25)) return 0;
+  return static_cast<size_t>(sources) * (ceil_div(cols, 128) * 128 + sizeof(float));
+}
+
 template <typename T>
 int quantize(const char* name, const T* x, const int32_t* index, int32_t index_div,
              int64_t sources, int64_t rows, int64_t cols, int64_t height, const int32_t* filled,
-             uint8_t* values, float* scales, void* stream) {
+             uint8_t* values, float* scales, void* workspace, size_t workspace_bytes,
+             void* stream) {
   if (int rc = check_copy(name, rows, cols, height)) return rc;
   BUX_CHECK(index == nullptr || (index_div >= 1 && sources >= 0), "%s: index_div=%d sources=%lld",
             name, index_div, (long long)sources);
   if (height == 0) return BUX_OK;
   BUX_CHECK(values && scales && (rows == 0 || x || (index && sources == 0)), "%s: NULL buffer",
             name);
+  hipStream_t s = as_stream(stream);
+  const size_t need = index ? gather_workspace(sources, rows, cols) : 0;
+  const bool gathered = need > 0;
+  if (gathered && (workspace == nullptr || workspace_bytes < need))
+    return fail(BUX_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes,
+                need);
+  const int64_t k = ceil_div(cols, 128) * 128;
+  uint8_t* const codes = static_cast<uint8_t*>(workspace);
+  float* const own = reinterpret_cast<float*>(codes + (gathered ? sources * k : 0));
   auto go = [&](auto c, auto vector) {
-    const Rows<T, decltype(vector)::value> from{x, index, index_div, sources, cols};
-    return launch_rows<T, decltype(c)::value>("int8 rows_kernel", from, rows, height, filled, cols,
-                                              values, scales, as_stream(stream));
+    constexpr int C = decltype(c)::value;
+    const Rows<T, decltype(vector)::value> from{x, gathered ? nullptr : index, index_div, sources,
+                                                cols};
+    if (gathered)  // every token, row after row
+      return launch_rows<T, C, true>("int8 rows_kernel", from, sources, sources, nullptr, cols,
+                                     codes, own, s);
+    return launch_rows<T, C>("int8 rows_kernel", from, rows, height, filled, cols, values, scales,
+                             s);
   };
-  if (cols % 8 != 0) return go(std::integral_constant<int, 0>{}, std::false_type{});
-  if (cols <= 1024) return go(std::integral_constant<int, 2>{}, std::true_type{});
-  if (cols <= 2048) return go(std::integral_constant<int, 4>{}, std::true_type{});
-  if (cols <= 4096) return go(std::integral_constant<int, 8>{}, std::true_type{});
-  if (cols <= 8192) return go(std::integral_constant<int, 16>{}, std::true_type{});
-  return go(std::integral_constant<int, 0>{}, std::true_type{});
+  auto quantized = [&] {
+    if (cols % 8 != 0) return go(std::integral_constant<int, 0>{}, std::false_type{});
+    if (cols <= 1024) return go(std::integral_constant<int, 2>{}, std::true_type{});
+    if (cols <= 2048) return go(std::integral_constant<int, 4>{}, std::true_type{});
+    if (cols <= 4096) return go(std::integral_constant<int, 8>{}, std::true_type{});
+    if (cols <= 8192) return go(std::integral_constant<int, 16>{}, std::true_type{});
+    return go(std::integral_constant<int, 0>{}, std::true_type{});
+  };
+  if (int rc = quantized(); rc != BUX_OK || !gathered) return rc;
+  const int64_t row_blocks = ceil_div(height, GATHERED), share = ceil_div(row_blocks * (k / 128), 8);
+  hipLaunchKernelGGL(gather_kernel, dim3(static_cast<unsigned>(8 * share)), dim3(THREADS), 0, s,
+                     codes, own, index, index_div, sources, rows, height, filled, k, row_blocks,
+                     share, values, scales);
+  return launched("int8 gather_kernel");
 }
 
 template <typename T>
@@ -371,21 +456,26 @@ int quantize_columns(const char* name, const T* w, int64_t groups, int64_t k, in
 }  // namespace
 }  // namespace bux
 
+extern "C" size_t bux_int8_quantize_workspace_size(int64_t sources, int64_t rows, int64_t cols) {
+  return sources < 0 || rows < 0 || cols <= 0 ? 0 : bux::gather_workspace(sources, rows, cols);
+}
 extern "C" int bux_int8_quantize(const uint16_t* x, const int32_t* index, int32_t index_div,
                                  int64_t sources, int64_t rows, int64_t cols, int64_t height,
                                  const int32_t* filled, uint8_t* values, float* scales,
-                                 void* stream) {
+                                 void* workspace,
+    size_t workspace_bytes, void* stream) {
   bux::clear_error();
   return bux::quantize("bux_int8_quantize", x, index, index_div, sources, rows, cols, height,
-                       filled, values, scales, stream);
+                       filled, values, scales, workspace, workspace_bytes, stream);
 }
 extern "C" int bux_int8_quantize_f32(const float* x, const int32_t* index, int32_t index_div,
                                      int64_t sources, int64_t rows, int64_t cols, int64_t height,
                                      const int32_t* filled, uint8_t* values, float* scales,
-                                     void* stream) {
+                                     void* workspace,
+    size_t workspace_bytes, void* stream) {
   bux::clear_error();
   return bux::quantize("bux_int8_quantize_f32", x, index, index_div, sources, rows, cols, height,
-                       filled, values, scales, stream);
+                       filled, values, scales, workspace, workspace_bytes, stream);
 }
 extern "C" int bux_int8_glu(const uint16_t* projected, const uint16_t* weights,
                             const int32_t* filled, int64_t m, int64_t f, const bux_ffn* ffn,

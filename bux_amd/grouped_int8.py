@@ -11,7 +11,7 @@ import torch
 
 from bux_amd import _lib
 from bux_amd.grouped_mxfp8 import K_ALIGN, TileList, tiles_of, whole
-from bux_amd.kernels import lib, on_device, ptr, require, stream
+from bux_amd.kernels import lib, on_device, ptr, require, stream, workspace
 
 MAX_K = 131072  # 127^2 K stays within 32 bits
 
@@ -58,8 +58,10 @@ def quantized(x: torch.Tensor, filled: torch.Tensor | None = None,
                                device=x.device),
                    torch.empty(height, dtype=torch.float32, device=x.device))
         quantize = lib().bux_int8_quantize_f32 if f32 else lib().bux_int8_quantize
+        need = 0 if index is None else lib().bux_int8_quantize_workspace_size(sources, rows, cols)
+        ws = workspace(need, x.device) if need else None
         _lib.check(quantize(ptr(x), ptr(index), index_div, sources, rows, cols, height, ptr(filled),
-                            ptr(out.values), ptr(out.scales), stream()))
+                            ptr(out.values), ptr(out.scales), ptr(ws), need, stream()))
     return out
 
 

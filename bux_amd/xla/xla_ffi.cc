@@ -699,21 +699,23 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxNormBackward, NormBackward,
 // index, filled and bias may be empty.
 
 static ffi::Error Int8Quantize(hipStream_t s, In x, In index, In filled, int64_t index_div,
-                               int64_t rows, Out values, Out scales) {
+                               int64_t rows, Out values, Out scales, Out ws) {
   const int64_t height = dim(values, 1), cols = dim(x, 1), sources = dim(x, 0);
   const int32_t div = static_cast<int32_t>(index_div);
   if (f32(x))
     return status(bux_int8_quantize_f32(at<const float>(x), at<const int32_t>(index), div, sources,
                                         rows, cols, height, at<const int32_t>(filled),
-                                        at<uint8_t>(values), at<float>(scales), s));
+                                        at<uint8_t>(values), at<float>(scales), at<void>(ws),
+                                        ws->size_bytes(), s));
   return status(bux_int8_quantize(at<const uint16_t>(x), at<const int32_t>(index), div, sources,
                                   rows, cols, height, at<const int32_t>(filled),
-                                  at<uint8_t>(values), at<float>(scales), s));
+                                  at<uint8_t>(values), at<float>(scales), at<void>(ws),
+                                  ws->size_bytes(), s));
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8Quantize, Int8Quantize,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
                                   .Attr<int64_t>("index_div").Attr<int64_t>("rows").Ret<In>()
-                                  .Ret<In>());
+                                  .Ret<In>().Ret<In>());
 
 // projected [m, f, p] (p = 2 gated, 1 plain), weights [m].
 static ffi::Error Int8Glu(hipStream_t s, In projected, In weights, In filled, BUX_FFN_PARAMS,

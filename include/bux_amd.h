@@ -655,7 +655,8 @@ int bux_mx_grouped_dglu(const uint8_t* a_values, const uint8_t* a_scales, const 
  *
  * bux_int8_quantize: rows of x, as bux_mx_quantize takes them (index, index_div, sources, filled
  *   likewise; height any, >= rows): values [K/64][height][64], scales [height]; rows from `rows`
- *   or *filled on are 0. Any cols.
+ *   or *filled on are 0. Any cols. workspace: with an index, bux_int8_quantize_workspace_size(
+ *   sources, rows, cols) bytes (0, then NULL, for few rows; else each token's own codes).
  * bux_int8_glu: rows of the activation of projected and the weights, as bux_glu_forward computes
  *   and rounds them (bux_glu_forward, then bux_int8_quantize, bit for bit), in one pass. f a
  *   multiple of 4.
@@ -667,12 +668,15 @@ int bux_mx_grouped_dglu(const uint8_t* a_values, const uint8_t* a_scales, const 
  *   NULL; rows from sum(sizes) to height 0. The list (bux_mx_grouped_tiles, or
  *   bux_moe_permute_layer's) is checked as there. n a multiple of 4, m and n up to 33,554,176.
  */
+size_t bux_int8_quantize_workspace_size(int64_t sources, int64_t rows, int64_t cols);
 int bux_int8_quantize(const uint16_t* x, const int32_t* index, int32_t index_div, int64_t sources,
                       int64_t rows, int64_t cols, int64_t height, const int32_t* filled,
-                      uint8_t* values, float* scales, void* stream);
+                      uint8_t* values, float* scales, void* workspace, size_t workspace_bytes,
+                      void* stream);
 int bux_int8_quantize_f32(const float* x, const int32_t* index, int32_t index_div, int64_t sources,
                           int64_t rows, int64_t cols, int64_t height, const int32_t* filled,
-                          uint8_t* values, float* scales, void* stream);
+                          uint8_t* values, float* scales, void* workspace,
+                          size_t workspace_bytes, void* stream);
 int bux_int8_glu(const uint16_t* projected, const uint16_t* weights, const int32_t* filled,
                  int64_t m, int64_t f, const bux_ffn* ffn, int64_t height, uint8_t* values,
                  float* scales, void* stream);

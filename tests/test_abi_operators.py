@@ -99,8 +99,9 @@ def test_the_int8_quantizers_reject_bad_arguments(lib, twin):
     glu = getattr(lib, "bux_int8_glu" + twin)
     columns = getattr(lib, "bux_int8_quantize_columns" + twin)
 
-    def rows(rows=8, cols=64, height=8, index=None, div=1, sources=8, x=P, values=P):
-        return quantize(x, index, div, sources, rows, cols, height, None, values, P, None)
+    def rows(rows=8, cols=64, height=8, index=None, div=1, sources=8, x=P, values=P, ws=None,
+             nbytes=0):
+        return quantize(x, index, div, sources, rows, cols, height, None, values, P, ws, nbytes, None)
 
     for bad, word in (({"rows": -1}, "rows=-1"), ({"height": 7}, "height=7"),
                       ({"height": 1 << 26}, "height"), ({"cols": 0}, "cols=0"),
@@ -109,6 +110,12 @@ def test_the_int8_quantizers_reject_bad_arguments(lib, twin):
                       ({"values": None}, "NULL")):
         assert rows(**bad) == 1 and word in _msg(lib), (bad, _msg(lib))
     assert rows(rows=0, height=0, x=None, values=None) == 0
+    # many rows of few tokens take room for the tokens' own codes
+    size = lib.bux_int8_quantize_workspace_size
+    assert size(8, 8, 64) == 0 and size(16384, 131072, 2048) >= 16384 * 2052
+    big = {"rows": 131072, "height": 131072, "cols": 2048, "sources": 16384, "index": P, "div": 8}
+    assert rows(**big) == 2 and "workspace" in _msg(lib)
+    assert rows(ws=P, nbytes=size(16384, 131072, 2048) - 1, **big) == 2 and "workspace" in _msg(lib)
 
     def units(m=8, f=64, height=8, act=0, projected=P):
         ffn = _lib.FfnStruct(act, 1, 0, 0.0, 0, 0.0, 0.0)

@@ -138,6 +138,35 @@ def test_rows_by_index(lib, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("cols", [1003, 3968])
+def test_many_rows_by_index(lib, cols, dtype):
+    """Enough rows of few enough tokens that each token is quantized once: the same codes, for
+    any index (repeated, unordered, outside the tokens), any `filled`."""
+    from bux_amd import grouped_int8 as g8
+    tokens, div = 900, 3
+    rows = -(-2**25 // cols) + 77
+    announce("int8 many rows", cols, dtype)
+    assert lib.bux_int8_quantize_workspace_size(tokens, rows, cols) > 0
+    x = _normal(8, tokens, cols, dtype=dtype)
+    x[5], x[6, 1] = 0, float("nan")
+    g = torch.Generator().manual_seed(9)
+    index = torch.randint(-40, tokens * div + 40, (rows,), generator=g, dtype=torch.int32)
+    index[:4] = torch.tensor([2**31 - 1, -2**31, tokens * div - 1, tokens * div])
+    index = index.cuda()
+    filled = torch.tensor([rows - 1000], dtype=torch.int32).cuda()
+    got = g8.quantized(x, filled, index, div, rows + 300)
+    one = g8.quantized(x)
+    token = torch.div(index, div, rounding_mode="floor").long()
+    live = (index >= 0) & (token < tokens) & (torch.arange(rows, device="cuda") < rows - 1000)
+    token = torch.where(live, token, 0)
+    values = torch.where(live[None, :, None], one.values[:, token], 0)
+    assert torch.equal(got.values[:, :rows], values) and (got.values[:, rows:] == 0).all()
+    scales = torch.where(live, one.scales[token], 0.0)
+    assert torch.equal(got.scales[:rows].view(torch.int32), scales.view(torch.int32))
+    assert (got.scales[rows:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("g,k,n", [(1, 1, 1), (2, 64, 64), (3, 100, 70), (2, 300, 129), (1, 1000, 4)])
 def test_kernels_columns(lib, g, k, n, dtype):
     from bux_amd import grouped_int8 as g8
