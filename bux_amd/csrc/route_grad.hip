@@ -232,8 +232,10 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
         if (column(q) >= n) s[q] = slope[q] = 0.0f;
       }
     }
-    float inv = 1.0f, shift = 0.0f;  // a pick's ds = (g - shift) inv
     if (p.normalize) {
+      // a pick's ds = (g T - D) / T^2, each product rounded, so that a single pick's, whose weight
+      // is constant, is 0
+#pragma clang fp contract(off)
       float total = 0.0f, dot = 0.0f;
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
@@ -242,11 +244,13 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
       }
       total = lanes_sum<L>(total);
       dot = lanes_sum<L>(dot);
-      inv = total == 0.0f ? 0.0f : 1.0f / total;
-      shift = dot * inv;
-    }
+      const float inv = total >= __FLT_MIN__ ? 1.0f / total : 0.0f;  // (1 / total may be infinite)
 #pragma unroll
-    for (int q = 0; q < Q; ++q) ds[q] = (grad[q] - count[q] * shift) * inv;
+      for (int q = 0; q < Q; ++q) ds[q] = (grad[q] * total - count[q] * dot) * inv * inv;
+    } else {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) ds[q] = grad[q];
+    }
     if (p.d_scores) {
 #pragma unroll
       for (int q = 0; q < Q; q += 4) {

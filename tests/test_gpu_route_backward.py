@@ -180,6 +180,24 @@ def test_scores_that_underflow_have_no_gradient(lib):
         assert (got.x[1] == 0).all() and (got.bias[3:6] == 0).all()
 
 
+@pytest.mark.parametrize("router", ["softmax", "sigmoid", "sqrtsoftplus"])
+def test_a_normalized_single_pick_is_constant(lib, router):
+    """Its weight is 1 whatever the logits, so its gradient is 0 and no rounding's remainder."""
+    v = _inputs(70, 64, 40, 40, 1, seed=8, dz=True)
+    got = _run(v, 40, router, True, 2.5, 1.0)
+    assert torch.equal(got.x, v["dz"])
+    assert (got.kernel == 0).all() and (got.bias == 0).all()
+
+
+@pytest.mark.parametrize("offset", [-80.0, -86.0, -95.0])
+def test_picks_of_tiny_scores(lib, offset):
+    """Normalized sigmoids about the smallest normal number: finite gradients."""
+    v = _inputs(20, 32, 24, 24, 4, seed=9, offset=offset, scores=True)
+    got = _run(v, 24, "sigmoid", True, 1.0, 1.0)
+    for g in (got.x, got.kernel, got.bias):
+        assert torch.isfinite(g).all()
+
+
 def test_picks_made_twice_and_outside(lib):
     """A pick made twice counts twice in the sum; one outside the scored experts not at all."""
     v = _inputs(6, 64, 20, 18, 3, seed=7)
