@@ -12,8 +12,9 @@
 // codes of 0, so that its products are NaN.
 //
 // The codes are in the GEMM's tiled layout, [K / 64][rows][64] with K padded to whole 128s.
-// Bound by HBM: a wave takes a row, in registers where it has at most 512 C columns (else read
-// twice, the second time from L2); a workgroup's 4 rows write 256 bytes of each K chunk in one run.
+// Bound by HBM: a wave takes a row (narrow rows: 16 lanes each), in registers where it has at most
+// 8192 columns (else read twice, the second time from L2); a workgroup's rows lie in one run of
+// each K chunk.
 
 #include <type_traits>
 
@@ -46,9 +47,11 @@ __device__ __forceinline__ uint32_t top_of(const Part<float>& p) {
   }
   return m;
 }
-__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+// Over a row's L lanes.
+template <int L>
+__device__ __forceinline__ uint32_t row_top(uint32_t v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
+  for (int o = L / 2; o >= 1; o >>= 1) {
     const uint32_t u = __shfl_xor(v, o);
     v = u > v ? u : v;
   }
@@ -108,8 +111,45 @@ struct Coder {
 // --- rows ------------------------------------------------------------------------------
 
 // Where a row's values come from: x[row], or x[index[row] / index_div] (a row of 0 where that
-// lies outside x's `sources` rows). VECTOR: 16-byte loads (columns a multiple of 8).
-template <typename T, bool VECTOR>
+// lies outside x's `sources` rows).
+enum class Load {
+  WHOLE,  // columns a multiple of 8: a part a load (two of float32), at an element's alignment
+  TAIL,   // 8 columns at least: the row's last part from its last 8 columns, moved into place (an
+          // element at a time: 19276 bfloat16 rows of 990 39 us, so 13)
+  NARROW  // fewer: an element at a time
+};
+
+// The part's values from place n (0 .. 7) on, zeros after them: 4, 2 and 1 places where n has
+// those bits (a runtime index would put the part in scratch memory).
+template <typename T>
+__device__ __forceinline__ Part<T> from_place(const Part<T>& p, int n) {
+  constexpr int WORDS = sizeof(Part<T>) / 4;
+  typedef uint32_t Words __attribute__((ext_vector_type(WORDS)));
+  Words w = __builtin_bit_cast(Words, p);
+  auto move = [&](int by, bool wanted) {
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) {
+      const uint32_t from = j + by < WORDS ? w[j + by] : 0u;
+      w[j] = wanted ? from : w[j];
+    }
+  };
+  if constexpr (sizeof(T) == 2) {
+    move(2, n & 4);
+    move(1, n & 2);
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) {
+      const uint32_t next = j + 1 < WORDS ? w[j + 1] : 0u;
+      w[j] = n & 1 ? (w[j] >> 16) | (next << 16) : w[j];
+    }
+  } else {
+    move(4, n & 4);
+    move(2, n & 2);
+    move(1, n & 1);
+  }
+  return __builtin_bit_cast(Part<T>, w);
+}
+
+template <typename T, Load LOAD>
 struct Rows {
   const T* x;
   const int32_t* index;
@@ -127,11 +167,13 @@ struct Rows {
   __device__ __forceinline__ Part<T> load(const Row& r, int64_t c) const {
     Part<T> p{};
     if (r.at == nullptr || c >= cols) return p;
-    if constexpr (VECTOR) {
+    if constexpr (LOAD != Load::NARROW) {
       struct __attribute__((packed, aligned(sizeof(T)))) Any {
         Part<T> p;
       };
-      p = reinterpret_cast<const Any*>(r.at + c)->p;
+      const int64_t at = LOAD == Load::TAIL && c + 8 > cols ? cols - 8 : c;
+      p = reinterpret_cast<const Any*>(r.at + at)->p;
+      if (LOAD == Load::TAIL && at < c) p = from_place(p, static_cast<int>(c - at));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -189,17 +231,19 @@ struct Units {
   }
 };
 
-// A wave a row of the copy's `height`: rows from `rows` or *filled on are 0. C: the row's parts
+// L lanes a row of the copy's `height`: rows from `rows` or *filled on are 0. C: the row's parts
 // a lane keeps, or 0 to read them twice. PLAIN: the codes row after row, not tiled.
-template <typename T, int C, bool PLAIN, typename Source>
+template <typename T, int L, int C, bool PLAIN, typename Source>
 __global__ __launch_bounds__(THREADS) void rows_kernel(Source from, int64_t rows, int64_t height,
                                                        const int32_t* __restrict__ filled,
                                                        int64_t cols, int64_t k,
                                                        uint8_t* __restrict__ values,
                                                        float* __restrict__ scales) {
-  const int lane = threadIdx.x & 63;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * (THREADS / 64) +
-                    __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int TURN = 8 * L;  // columns
+  const int lane = threadIdx.x % L;
+  int sub = threadIdx.x / L;
+  if constexpr (L == 64) sub = __builtin_amdgcn_readfirstlane(sub);
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * (THREADS / L) + sub;
   if (i >= height) return;
   const int64_t live = filled && *filled < rows ? *filled : rows;
   uint8_t* const out = values + i * (PLAIN ? k : 64);
@@ -208,7 +252,7 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(Source from, int64_t rows
     if (c < k) *reinterpret_cast<uint2*>(out + at) = codes;
   };
   if (i >= live) {
-    for (int64_t c = 8 * lane; c < k; c += 512) put(c, make_uint2(0, 0));
+    for (int64_t c = 8 * lane; c < k; c += TURN) put(c, make_uint2(0, 0));
     if (lane == 0) scales[i] = 0.0f;
     return;
   }
@@ -216,38 +260,53 @@ __global__ __launch_bounds__(THREADS) void rows_kernel(Source from, int64_t rows
   if constexpr (C > 0) {
     Part<T> p[C];
 #pragma unroll
-    for (int j = 0; j < C; ++j) p[j] = from.load(row, 512 * j + 8 * lane);
+    for (int j = 0; j < C; ++j) p[j] = from.load(row, TURN * j + 8 * lane);
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const uint32_t t = top_of(p[j]);
       top = t > top ? t : top;
     }
-    const Coder<T> coder(wave_top(top));
+    const Coder<T> coder(row_top<L>(top));
 #pragma unroll
-    for (int j = 0; j < C; ++j) put(512 * j + 8 * lane, coder.codes(p[j]));
+    for (int j = 0; j < C; ++j) put(TURN * j + 8 * lane, coder.codes(p[j]));
     if (lane == 0) scales[i] = coder.scale;
   } else {
     uint32_t top = 0;
-    for (int64_t c = 8 * lane; c < cols; c += 512) {
+    for (int64_t c = 8 * lane; c < cols; c += TURN) {
       const uint32_t t = top_of(from.load(row, c));
       top = t > top ? t : top;
     }
-    const Coder<T> coder(wave_top(top));
-    for (int64_t c = 8 * lane; c < k; c += 512) put(c, coder.codes(from.load(row, c)));
+    const Coder<T> coder(row_top<L>(top));
+    for (int64_t c = 8 * lane; c < k; c += TURN) put(c, coder.codes(from.load(row, c)));
     if (lane == 0) scales[i] = coder.scale;
   }
 }
 
-template <typename T, int C, bool PLAIN = false, typename Source>
+template <typename T, int L, int C, bool PLAIN = false, typename Source>
 int launch_rows(const char* kernel, const Source& from, int64_t rows, int64_t height,
                 const int32_t* filled, int64_t cols, uint8_t* values, float* scales,
                 hipStream_t s) {
   const int64_t k = ceil_div(cols, 128) * 128;
-  hipLaunchKernelGGL((rows_kernel<T, C, PLAIN, Source>),
-                     dim3(static_cast<unsigned>(ceil_div(height, THREADS / 64))), dim3(THREADS), 0,
+  hipLaunchKernelGGL((rows_kernel<T, L, C, PLAIN, Source>),
+                     dim3(static_cast<unsigned>(ceil_div(height, THREADS / L))), dim3(THREADS), 0,
                      s, from, rows, height, filled, cols, k, values, scales);
   return launched(kernel);
+}
+
+// Calls f(L, C) for rows of `cols` columns: narrow ones 4 a wave, whose chains of loads and
+// exchanges overlap (99320 rows of 134 bfloat16 columns: a wave each 40 us, so 15; from 1024
+// columns on 16 lanes are slower, 19276 float32 rows of 1024 26 us and 19).
+template <typename F>
+int with_lanes(int64_t cols, F&& f) {
+  using std::integral_constant;
+  if (cols <= 256) return f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  if (cols <= 512) return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+  if (cols <= 1024) return f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  if (cols <= 2048) return f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  if (cols <= 4096) return f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+  if (cols <= 8192) return f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+  return f(integral_constant<int, 64>{}, integral_constant<int, 0>{});
 }
 
 // Rows by index from tokens quantized once (codes (sources, k) row after row, and their scales).
@@ -391,23 +450,25 @@ int quantize(const char* name, const T* x, const int32_t* index, int32_t index_d
   const int64_t k = ceil_div(cols, 128) * 128;
   uint8_t* const codes = static_cast<uint8_t*>(workspace);
   float* const own = reinterpret_cast<float*>(codes + (gathered ? sources * k : 0));
-  auto go = [&](auto c, auto vector) {
-    constexpr int C = decltype(c)::value;
-    const Rows<T, decltype(vector)::value> from{x, gathered ? nullptr : index, index_div, sources,
-                                                cols};
+  auto go = [&](auto lanes, auto c, auto load) {
+    constexpr int L = decltype(lanes)::value, C = decltype(c)::value;
+    const Rows<T, decltype(load)::value> from{x, gathered ? nullptr : index, index_div, sources,
+                                              cols};
     if (gathered)  // every token, row after row
-      return launch_rows<T, C, true>("int8 rows_kernel", from, sources, sources, nullptr, cols,
-                                     codes, own, s);
-    return launch_rows<T, C>("int8 rows_kernel", from, rows, height, filled, cols, values, scales,
-                             s);
+      return launch_rows<T, L, C, true>("int8 rows_kernel", from, sources, sources, nullptr, cols,
+                                        codes, own, s);
+    return launch_rows<T, L, C>("int8 rows_kernel", from, rows, height, filled, cols, values,
+                                scales, s);
   };
   auto quantized = [&] {
-    if (cols % 8 != 0) return go(std::integral_constant<int, 0>{}, std::false_type{});
-    if (cols <= 1024) return go(std::integral_constant<int, 2>{}, std::true_type{});
-    if (cols <= 2048) return go(std::integral_constant<int, 4>{}, std::true_type{});
-    if (cols <= 4096) return go(std::integral_constant<int, 8>{}, std::true_type{});
-    if (cols <= 8192) return go(std::integral_constant<int, 16>{}, std::true_type{});
-    return go(std::integral_constant<int, 0>{}, std::true_type{});
+    using std::integral_constant;
+    if (cols < 8)
+      return go(integral_constant<int, 16>{}, integral_constant<int, 0>{},
+                integral_constant<Load, Load::NARROW>{});
+    return with_lanes(cols, [&](auto lanes, auto c) {
+      return cols % 8 == 0 ? go(lanes, c, integral_constant<Load, Load::WHOLE>{})
+                           : go(lanes, c, integral_constant<Load, Load::TAIL>{});
+    });
   };
   if (int rc = quantized(); rc != BUX_OK || !gathered) return rc;
   const int64_t row_blocks = ceil_div(height, GATHERED), share = ceil_div(row_blocks * (k / 128), 8);
@@ -430,8 +491,8 @@ int quantize_units(const char* name, const T* projected, const T* weights, const
   return with_kind(act, [&](auto kind) {
     const Units<decltype(kind), T> from{projected, weights, f, act};
     auto go = [&](auto c) {
-      return launch_rows<T, decltype(c)::value>("int8 units rows_kernel", from, m, height, filled,
-                                                f, values, scales, as_stream(stream));
+      return launch_rows<T, 64, decltype(c)::value>("int8 units rows_kernel", from, m, height,
+                                                    filled, f, values, scales, as_stream(stream));
     };
     if (f <= 1024) return go(std::integral_constant<int, 2>{});
     if (f <= 4096) return go(std::integral_constant<int, 8>{});
@@ -462,8 +523,7 @@ extern "C" size_t bux_int8_quantize_workspace_size(int64_t sources, int64_t rows
 extern "C" int bux_int8_quantize(const uint16_t* x, const int32_t* index, int32_t index_div,
                                  int64_t sources, int64_t rows, int64_t cols, int64_t height,
                                  const int32_t* filled, uint8_t* values, float* scales,
-                                 void* workspace,
-    size_t workspace_bytes, void* stream) {
+                                 void* workspace, size_t workspace_bytes, void* stream) {
   bux::clear_error();
   return bux::quantize("bux_int8_quantize", x, index, index_div, sources, rows, cols, height,
                        filled, values, scales, workspace, workspace_bytes, stream);
@@ -471,8 +531,7 @@ extern "C" int bux_int8_quantize(const uint16_t* x, const int32_t* index, int32_
 extern "C" int bux_int8_quantize_f32(const float* x, const int32_t* index, int32_t index_div,
                                      int64_t sources, int64_t rows, int64_t cols, int64_t height,
                                      const int32_t* filled, uint8_t* values, float* scales,
-                                     void* workspace,
-    size_t workspace_bytes, void* stream) {
+                                     void* workspace, size_t workspace_bytes, void* stream) {
   bux::clear_error();
   return bux::quantize("bux_int8_quantize_f32", x, index, index_div, sources, rows, cols, height,
                        filled, values, scales, workspace, workspace_bytes, stream);

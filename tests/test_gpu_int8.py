@@ -68,6 +68,24 @@ def test_rows(lib, rows, cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("cols", [*range(8, 17), *range(249, 259), *range(505, 515), 1017, 4099])
+def test_rows_of_every_last_part(lib, cols, dtype):
+    """Rows whose last 8 columns are cut short anywhere, at any element of a buffer with NaN on
+    either side; the largest value in the row's first or last column."""
+    from bux_amd import grouped_int8 as g8
+    announce("int8 last part", cols, dtype)
+    rows = 21
+    for shift in (0, 1, 3, 8):
+        buffer = torch.full((rows * cols + 16,), float("nan"), dtype=dtype, device="cuda")
+        x = buffer[shift:shift + rows * cols].view(rows, cols)
+        x.copy_(_normal(cols, rows, cols, dtype=dtype))
+        x[::2, -1], x[1::2, 0] = 9.0, -9.0
+        codes, scales = _untiled(g8.quantized(x), cols)
+        want, ws = _codes(x)
+        assert np.array_equal(codes, want) and np.array_equal(scales, ws)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 def test_every_bfloat16_under_many_scales(lib, dtype):
     """Rows of every finite bfloat16 up to the row's largest, over largest values of all kinds of
     mantissas and from the smallest subnormal to the largest: ties and near ties among them."""
