@@ -39,4 +39,8 @@ extern "C" const char* bux_last_error(void) { return bux::last_error; }
 // 0.3.2: float32 twins of the compute format's GEMMs (bux_bf16_grouped_rows_f32,
 // bux_bf16_grouped_contract_f32) and of the activation (bux_glu_forward_f32,
 // bux_glu_backward_f32): a float32 layer runs any pass outside MXFP8.
-extern "C" int bux_version(void) { return 302; }
+// 0.4.0: the tokens' norm (bux_norm_forward, bux_norm_backward and their float32 twins), the
+// router's backward (bux_route_backward), the experts' products in 8-bit integers
+// (bux_int8_quantize, bux_int8_glu, bux_int8_quantize_columns and their float32 twins,
+// bux_int8_grouped_rows_listed).
+extern "C" int bux_version(void) { return 400; }

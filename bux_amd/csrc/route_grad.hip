@@ -13,14 +13,18 @@
 //   dx   = dz_in + G kernel^T,  d_kernel = x^T G,  d_bias = sum over the tokens of G
 //
 // (moe.py:249-270's transpose: the forward's roundings to bfloat16 pass the gradient as they
-// are.) Four kernels: grads_kernel writes G, in two bfloat16 parts, hi and
-// the rest lo: G to 2^-17 at the rate of two bfloat16 MFMAs, where one part alone would put an
-// error of a bfloat16 step's half (2^-9) into every product, as large as the outputs' rounding.
-// dx_kernel multiplies it by the router's kernel, whose rows lie along n; kernel_grad_kernel
-// contracts slices of the tokens, transposing on the way out of LDS; reduce_kernel adds the
+// are.) Three kernels: grads_kernel writes G, in two bfloat16 parts, hi and the rest lo: G to
+// 2^-17 at the rate of two bfloat16 MFMAs, where one part alone would put an error of a bfloat16
+// step's half (2^-9) into every product, as large as the outputs' rounding. products_kernel
+// multiplies it by the router's kernel, whose rows lie along n (dx_tile), and contracts slices of
+// the tokens with it, transposing on the way out of LDS (kernel_grad_tile). reduce_kernel adds the
 // slices, and d_bias's partial sums, in a fixed order.
 //
-// Bound by HBM at a router's sizes: x read once, dx written once (and dz read); n is small.
+// What bounds it: HBM for few logits (x read once, dx written once, dz read; G stays in L2), the
+// MFMAs of G's two parts for many. us of the three: 500 tokens of 2048, 128 logits 5.5, 9.6, 3.9
+// (a launch's latency each); 16384 with dz 8.9, 54, 6.5, where a copy of its 212 MB takes 41; 8192
+// of 7168, 256 logits 14, 126 to 143, 8, whose 120 GFLOP take 98
+// at a large matrix product's rate.
 
 #include <math.h>
 
@@ -70,7 +74,7 @@ struct Params {
 // G and the router's kernel lie in blocks of 32 rows by 8 columns, a block's 32 x 16 bytes in one
 // run and a row of blocks' one after another, padded with zeros to npad columns: a wave's load of
 // an MFMA operand (lane l row l % 32, columns 8 (l / 32) .. + 7 of 16) is one run of 1 KiB. (From
-// rows, 32 runs of 32 bytes: dx_kernel 66 us for 16384 tokens of 2048, 128 logits.) The element
+// rows, 32 runs of 32 bytes: dx alone 68 us for 16384 tokens of 2048, 128 logits, so 43.) The element
 // (r, c), c a multiple of 4:
 __device__ __forceinline__ int64_t at_block(int64_t r, int32_t c, int32_t npad) {
   return ((r >> 5) * (npad >> 3) + (c >> 3)) * 256 + (r & 31) * 8 + (c & 7);
