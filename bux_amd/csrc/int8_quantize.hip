@@ -25,6 +25,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int64_t MAX_K = 131072;  // 127^2 K stays below 2^31
+constexpr int64_t MAX_HEIGHT = (1LL << 26) - 4;
 
 template <typename T>
 struct Part {
@@ -410,9 +411,10 @@ __global__ __launch_bounds__(THREADS) void columns_kernel(const T* __restrict__ 
 }
 
 int check_copy(const char* name, int64_t rows, int64_t cols, int64_t height) {
-  BUX_CHECK(rows >= 0 && height >= rows && height < (1LL << 26),
-            "%s: bad shape rows=%lld height=%lld (at least the rows, below 2^26)", name,
-            (long long)rows, (long long)height);
+  // a launch holds fewer than 2^32 threads, a row's 64 of them
+  BUX_CHECK(rows >= 0 && height >= rows && height <= MAX_HEIGHT,
+            "%s: bad shape rows=%lld height=%lld (at least the rows, up to %lld)", name,
+            (long long)rows, (long long)height, (long long)MAX_HEIGHT);
   BUX_CHECK(cols > 0 && cols <= MAX_K, "%s: cols=%lld outside [1, %lld]", name, (long long)cols,
             (long long)MAX_K);
   return BUX_OK;
@@ -448,6 +450,12 @@ int quantize(const char* name, const T* x, const int32_t* index, int32_t index_d
     return fail(BUX_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes,
                 need);
   const int64_t k = ceil_div(cols, 128) * 128;
+  const int64_t row_blocks = ceil_div(height, GATHERED), share = ceil_div(row_blocks * (k / 128), 8);
+  BUX_CHECK(!gathered || 8 * share * THREADS < (1LL << 32),
+            "%s: height=%lld rows of cols=%lld are more than a launch holds", name,
+            (long long)height, (long long)cols);
+  BUX_CHECK(!gathered || reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+            "%s: the workspace is 16-byte aligned", name);
   uint8_t* const codes = static_cast<uint8_t*>(workspace);
   float* const own = reinterpret_cast<float*>(codes + (gathered ? sources * k : 0));
   auto go = [&](auto lanes, auto c, auto load) {
@@ -471,7 +479,6 @@ int quantize(const char* name, const T* x, const int32_t* index, int32_t index_d
     });
   };
   if (int rc = quantized(); rc != BUX_OK || !gathered) return rc;
-  const int64_t row_blocks = ceil_div(height, GATHERED), share = ceil_div(row_blocks * (k / 128), 8);
   hipLaunchKernelGGL(gather_kernel, dim3(static_cast<unsigned>(8 * share)), dim3(THREADS), 0, s,
                      codes, own, index, index_div, sources, rows, height, filled, k, row_blocks,
                      share, values, scales);

@@ -894,28 +894,30 @@ def experts_int8(
                          f"kernels {quantized.up_shape}")
     if weights.numel() != m:
         raise ValueError(f"experts_int8: {weights.numel()} weights for {m} picks")
-    weights, = _cast(dt, weights)
-    up_bias, down_bias, norm_scale, norm_bias = _cast(dt, up_bias, down_bias, norm_scale, norm_bias)
-    height = grouped_mxfp8.whole(m)
-    with span("permute"):
-        s, row_weights, tiles = sort_for_layer(idx, e, weights, height)
-    with span("quantize x"):
-        x = grouped_int8.quantized(z, s.filled, s.order, k, height)
-    with span("up fprop"):
-        projected = grouped_int8.rows(
-            x, quantized.up, s.sizes, dt, height=m, tiles=tiles,
-            bias=None if up_bias is None else up_bias.reshape(e, f * p))
-    act_weights = row_weights if norm is None else torch.ones_like(row_weights)
-    with span("activation + quantize h"):
-        h = weighted_units_int8(ffn, projected.view(m, f, p), act_weights, s.filled, height)
-    with span("down fprop"):
-        y = grouped_int8.rows(h, quantized.down, s.sizes, dt, height=m, tiles=tiles)
-    if norm is not None:
-        with span("expert norm"):
-            y = expert_norm_forward(y, s.offsets, norm, norm_scale, norm_bias, row_weights,
-                                    None if down_bias is None else down_bias.reshape(e, d))
-    with span("combine"):
-        if down_bias is None or norm is not None:
-            return sum_by_token(y, s.inverse.view(t, k))
-        return sum_by_token_biased(y, s.inverse.view(t, k), down_bias.reshape(e, d), s.offsets,
-                                   row_weights)
+    require(z, idx)
+    with on_device(z):
+        weights, = _cast(dt, weights)
+        up_bias, down_bias, norm_scale, norm_bias = _cast(dt, up_bias, down_bias, norm_scale, norm_bias)
+        height = grouped_mxfp8.whole(m)
+        with span("permute"):
+            s, row_weights, tiles = sort_for_layer(idx, e, weights, height)
+        with span("quantize x"):
+            x = grouped_int8.quantized(z, s.filled, s.order, k, height)
+        with span("up fprop"):
+            projected = grouped_int8.rows(
+                x, quantized.up, s.sizes, dt, height=m, tiles=tiles,
+                bias=None if up_bias is None else up_bias.reshape(e, f * p))
+        act_weights = row_weights if norm is None else torch.ones_like(row_weights)
+        with span("activation + quantize h"):
+            h = weighted_units_int8(ffn, projected.view(m, f, p), act_weights, s.filled, height)
+        with span("down fprop"):
+            y = grouped_int8.rows(h, quantized.down, s.sizes, dt, height=m, tiles=tiles)
+        if norm is not None:
+            with span("expert norm"):
+                y = expert_norm_forward(y, s.offsets, norm, norm_scale, norm_bias, row_weights,
+                                        None if down_bias is None else down_bias.reshape(e, d))
+        with span("combine"):
+            if down_bias is None or norm is not None:
+                return sum_by_token(y, s.inverse.view(t, k))
+            return sum_by_token_biased(y, s.inverse.view(t, k), down_bias.reshape(e, d), s.offsets,
+                                       row_weights)

@@ -654,9 +654,10 @@ int bux_mx_grouped_dglu(const uint8_t* a_values, const uint8_t* a_scales, const 
  * columns); scales float32 [rows]. Columns up to 131072.
  *
  * bux_int8_quantize: rows of x, as bux_mx_quantize takes them (index, index_div, sources, filled
- *   likewise; height any, >= rows): values [K/64][height][64], scales [height]; rows from `rows`
+ *   likewise; height any from rows on, up to 67,108,860): values [K/64][height][64], scales [height]; rows from `rows`
  *   or *filled on are 0. Any cols. workspace: with an index, bux_int8_quantize_workspace_size(
- *   sources, rows, cols) bytes (0, then NULL, for few rows; else each token's own codes).
+ *   sources, rows, cols) bytes, 16-byte aligned (0, then NULL, for few rows; else each
+ *   token's own codes).
  * bux_int8_glu: rows of the activation of projected and the weights, as bux_glu_forward computes
  *   and rounds them (bux_glu_forward, then bux_int8_quantize, bit for bit), in one pass. f a
  *   multiple of 4.

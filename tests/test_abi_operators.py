@@ -104,7 +104,8 @@ def test_the_int8_quantizers_reject_bad_arguments(lib, twin):
         return quantize(x, index, div, sources, rows, cols, height, None, values, P, ws, nbytes, None)
 
     for bad, word in (({"rows": -1}, "rows=-1"), ({"height": 7}, "height=7"),
-                      ({"height": 1 << 26}, "height"), ({"cols": 0}, "cols=0"),
+                      ({"height": 1 << 26}, "height"), ({"height": (1 << 26) - 3}, "height"),
+                      ({"cols": 0}, "cols=0"),
                       ({"cols": 131073}, "cols=131073"), ({"index": P, "div": 0}, "index_div=0"),
                       ({"index": P, "sources": -1}, "sources=-1"), ({"x": None}, "NULL"),
                       ({"values": None}, "NULL")):
@@ -116,6 +117,11 @@ def test_the_int8_quantizers_reject_bad_arguments(lib, twin):
     big = {"rows": 131072, "height": 131072, "cols": 2048, "sources": 16384, "index": P, "div": 8}
     assert rows(**big) == 2 and "workspace" in _msg(lib)
     assert rows(ws=P, nbytes=size(16384, 131072, 2048) - 1, **big) == 2 and "workspace" in _msg(lib)
+
+    odd = ctypes.c_void_p(24)
+    assert rows(ws=odd, nbytes=1 << 30, **big) == 1 and "aligned" in _msg(lib)
+    wide = {"rows": 1 << 25, "height": 1 << 25, "cols": 131072, "sources": 1 << 20, "index": P}
+    assert rows(ws=P, nbytes=1 << 40, **wide) == 1 and "launch" in _msg(lib)
 
     def units(m=8, f=64, height=8, act=0, projected=P):
         ffn = _lib.FfnStruct(act, 1, 0, 0.0, 0, 0.0, 0.0)
