@@ -17,8 +17,8 @@
 // 2^-17 at the rate of two bfloat16 MFMAs, where one part alone would put an error of a bfloat16
 // step's half (2^-9) into every product, as large as the outputs' rounding. products_kernel
 // multiplies it by the router's kernel, whose rows lie along n (dx_tile), and contracts slices of
-// the tokens with it, transposing on the way out of LDS (kernel_grad_tile). reduce_kernel adds the
-// slices, and d_bias's partial sums, in a fixed order.
+// the tokens with it, transposing on the way out of LDS (kernel_grad_tile), and adds d_bias's partial
+// sums. reduce_kernel adds the slices, where there are several. All in a fixed order.
 //
 // What bounds it: HBM for few logits (x read once, dx written once, dz read; G stays in L2), the
 // MFMAs of G's two parts for many. us of the three: 500 tokens of 2048, 128 logits 5.5, 9.6, 3.9
@@ -474,6 +474,20 @@ __device__ __forceinline__ bf16x8 read_tr(uint32_t at, uint32_t at4) {
 
 constexpr size_t RING_BYTES = RING * sizeof(KStage);
 
+// Four logits of row j of d_kernel.
+__device__ __forceinline__ void store_kernel(const Params& p, int64_t j, int32_t e, float4 v) {
+  uint16_t* const out = p.d_kernel + j * p.n + e;
+  if ((p.n & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+    if (e < p.n)
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    return;
+  }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (e + q < p.n) out[q] = f32_to_bf16(f[q]);
+}
+
 __device__ __forceinline__ void kernel_grad_tile(const Params& p, uint32_t block, uint8_t* smem) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   // the logits' tiles of one slice and columns beside each other, then the columns'
@@ -566,6 +580,7 @@ __device__ __forceinline__ void kernel_grad_tile(const Params& p, uint32_t block
     }
   }
   float* base = p.kernel_partials + slice * p.d * p.npad;
+  const bool last = p.slices == 1;  // nothing to add: the gradient itself
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int64_t j = j0 + 64 * (wave >> 1) + 32 * i + (lane & 31);
@@ -575,52 +590,18 @@ __device__ __forceinline__ void kernel_grad_tile(const Params& p, uint32_t block
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int32_t e = e0 + 64 * (wave & 1) + 32 * q + 8 * g + 4 * (lane >> 5);
-        if (e < p.npad)
-          *reinterpret_cast<float4*>(base + j * p.npad + e) =
-              make_float4(acc[i][q][4 * g], acc[i][q][4 * g + 1], acc[i][q][4 * g + 2],
-                          acc[i][q][4 * g + 3]);
+        const float4 v = make_float4(acc[i][q][4 * g], acc[i][q][4 * g + 1], acc[i][q][4 * g + 2],
+                                     acc[i][q][4 * g + 3]);
+        if (last) store_kernel(p, j, e, v);
+        else if (e < p.npad) *reinterpret_cast<float4*>(base + j * p.npad + e) = v;
       }
   }
 }
 
-// Both products in one launch, so that either's loads fill the other's waits: the kernel's
-// gradient's workgroups first, which take longer.
-template <int RB>
-__global__ __launch_bounds__(THREADS) void products_kernel(Params p, uint32_t kernel_blocks,
-                                                           uint32_t columns) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  if (blockIdx.x < kernel_blocks) kernel_grad_tile(p, blockIdx.x, smem);
-  else dx_tile<RB>(p, blockIdx.x - kernel_blocks, columns, smem);
-}
-
-// d_kernel: the slices' sums in order, 4 logits a thread; d_bias: a block each 16 logits after
-// those, its 16 threads a logit every 16th partial, then their sums in order.
-__global__ __launch_bounds__(THREADS) void reduce_kernel(Params p, int64_t kernel_blocks) {
-  __shared__ float part[16][16];
-  const int64_t size = p.d * p.npad;
-  if (static_cast<int64_t>(blockIdx.x) < kernel_blocks) {
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x) * 4;
-    if (i >= size) return;
-    float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-    for (int32_t s = 0; s < p.slices; ++s) {
-      const float4 a = *reinterpret_cast<const float4*>(p.kernel_partials + s * size + i);
-      v.x += a.x;
-      v.y += a.y;
-      v.z += a.z;
-      v.w += a.w;
-    }
-    const int64_t j = i / p.npad;
-    const int32_t e = static_cast<int32_t>(i - j * p.npad);
-    uint16_t* out = p.d_kernel + j * p.n + e;
-    const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (e + q < p.n) out[q] = f32_to_bf16(f[q]);
-    return;
-  }
+// d_bias of 16 logits: 16 threads a logit, every 16th partial each, then their sums in order.
+__device__ __forceinline__ void bias_tile(const Params& p, uint32_t block, float (*part)[16]) {
   const int row = threadIdx.x >> 4, lane = threadIdx.x & 15;
-  const int32_t e = static_cast<int32_t>(blockIdx.x - kernel_blocks) * 16 + lane;
+  const int32_t e = static_cast<int32_t>(block) * 16 + lane;
   float s = 0.0f;
   if (e < p.n) {
 #pragma unroll 8
@@ -633,6 +614,40 @@ __global__ __launch_bounds__(THREADS) void reduce_kernel(Params p, int64_t kerne
 #pragma unroll
   for (int r = 1; r < 16; ++r) s += part[r][lane];
   p.d_bias[e] = s;
+}
+
+// Both products in one launch, so that either's loads fill the other's waits: the kernel's
+// gradient's workgroups first, which take longer; and d_bias's.
+template <int RB>
+__global__ __launch_bounds__(THREADS) void products_kernel(Params p, uint32_t kernel_blocks,
+                                                           uint32_t bias_blocks, uint32_t columns) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint32_t block = blockIdx.x;
+  if (block < kernel_blocks) return kernel_grad_tile(p, block, smem);
+  block -= kernel_blocks;
+  if (block < bias_blocks) return bias_tile(p, block, reinterpret_cast<float(*)[16]>(smem));
+  dx_tile<RB>(p, block - bias_blocks, columns, smem);
+}
+
+// d_kernel: the slices' sums in order, 4 logits a thread; and, with no tokens, d_bias.
+__global__ __launch_bounds__(THREADS) void reduce_kernel(Params p, int64_t kernel_blocks) {
+  __shared__ float part[16][16];
+  const int64_t size = p.d * p.npad;
+  if (static_cast<int64_t>(blockIdx.x) >= kernel_blocks)
+    return bias_tile(p, blockIdx.x - static_cast<uint32_t>(kernel_blocks), part);
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x) * 4;
+  if (i >= size) return;
+  float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+  for (int32_t s = 0; s < p.slices; ++s) {
+    const float4 a = *reinterpret_cast<const float4*>(p.kernel_partials + s * size + i);
+    v.x += a.x;
+    v.y += a.y;
+    v.z += a.z;
+    v.w += a.w;
+  }
+  const int64_t j = i / p.npad;
+  store_kernel(p, j, static_cast<int32_t>(i - j * p.npad), v);
 }
 
 // The lanes grads_kernel gives a token.
@@ -767,12 +782,13 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
     const uint32_t columns = static_cast<uint32_t>(ceil_div(d, 4 * COLS));
     const uint32_t tiles =
         static_cast<uint32_t>(ceil_div(d, COLS) * ceil_div(w.npad, COLS) * w.slices);
+    const uint32_t bias = d_bias ? static_cast<uint32_t>(ceil_div(n_logits, 16)) : 0;
     constexpr size_t LDS = RING_BYTES > DX_BYTES ? RING_BYTES : DX_BYTES;
     auto products = [&](auto rb) {
       constexpr int RB = decltype(rb)::value;
       hipLaunchKernelGGL((products_kernel<RB>),
-                         dim3(static_cast<unsigned>(tiles + columns * ceil_div(t, 32 * RB))),
-                         dim3(THREADS), LDS, s, p, tiles, columns);
+                         dim3(static_cast<unsigned>(tiles + bias + columns * ceil_div(t, 32 * RB))),
+                         dim3(THREADS), LDS, s, p, tiles, bias, columns);
     };
     static_assert(LDS <= 64 * 1024, "a launch's LDS without an attribute");
     // 32 tokens a wave where its products are few, with three waves a SIMD to hide their loads; 64
@@ -780,10 +796,10 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
     // 43.0; 8192, 7168, 256: 102 and 85) and there are workgroups to fill the chip
     if (w.npad > 128 && ceil_div(t, 64) * columns >= 256) products(integral_constant<int, 2>{});
     else products(integral_constant<int, 1>{});
-    if (int rc = launched("route products_kernel")) return rc;
+    if (int rc = launched("route products_kernel"); rc != BUX_OK || w.slices == 1) return rc;
   }
   const int64_t kernel_blocks = ceil_div(d * w.npad, 4 * THREADS);
-  const int64_t bias_blocks = d_bias ? ceil_div(n_logits, 16) : 0;
+  const int64_t bias_blocks = d_bias && t == 0 ? ceil_div(n_logits, 16) : 0;
   hipLaunchKernelGGL(reduce_kernel, dim3(static_cast<unsigned>(kernel_blocks + bias_blocks)),
                      dim3(THREADS), 0, s, p, kernel_blocks);
   return launched("route reduce_kernel");

@@ -200,10 +200,15 @@ __global__ __launch_bounds__(threads_of<W>()) void forward_kernel(
 // 8 waves 200 us, 512 161; the next row's loads to registers ahead of this one's sums 189.)
 constexpr int64_t MAX_BLOCKS = 1024;
 constexpr int64_t SIMDS = 1024;  // 256 CUs of 4
+// One workgroup where it has at most so many turns, whose sums are the gradients themselves: a
+// launch less (4 bfloat16 rows of 512 5.1 us, so 3.0, 4 of 2880, two turns, 6.4 both; eager 15.8
+// and 13.4). At four turns 16 rows of 1027 took 17.1 us and 9.8.
+constexpr int64_t ALONE_TURNS = 2;
 int64_t backward_blocks(int64_t m, int w, int c) {
   const int64_t a_simd = c == 1 || (c == 2 && w > 4) ? 4 : c == 2 ? 3 : 2;
   const int64_t most = a_simd * SIMDS / (w > 4 ? w : 4);
   const int64_t want = ceil_div(m, w > 4 ? 1 : 4 / w);
+  if (want <= ALONE_TURNS) return 1;
   return want < most ? want : most;
 }
 
@@ -262,13 +267,13 @@ struct Ahead {
 };
 
 // BIASED: the bias's gradient too. INPUT: scale_input's. AHEAD: 16-bit rows of whole chunks at
-// 16 bytes' alignment; their operands come through LDS, a row ahead. partials:
-// [1 + BIASED][blocks][d], the gain's first.
+// 16 bytes' alignment; their operands come through LDS, a row ahead. scale_sums, bias_sums:
+// [blocks][d], NULL where the norm has none.
 template <typename T, int W, int C, bool BIASED, bool INPUT, bool TAIL, bool AHEAD>
 __global__ __launch_bounds__(threads_of<W>()) void backward_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const float2* __restrict__ stats,
     const T* __restrict__ d_summed, int64_t m, int d, Settings<T> a, T* __restrict__ dx,
-    float* __restrict__ partials) {
+    float* __restrict__ scale_sums, float* __restrict__ bias_sums) {
   static_assert(!AHEAD || (!TAIL && sizeof(T) == 2), "16-bit rows of whole chunks");
   constexpr int ROWS = threads_of<W>() / (64 * W);
   __shared__ float red[2][2][ROWS][W];
@@ -406,10 +411,9 @@ __global__ __launch_bounds__(threads_of<W>()) void backward_kernel(
     // the next row's loads are in (memory operations end in order; this row's stores may not)
     if constexpr (AHEAD) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C) : "memory");
   }
-  if (partials == nullptr) return;
-  float* at = partials + static_cast<int64_t>(blockIdx.x) * d;
-  if (a.affine) store_sums<W, C, ROWS, TAIL>(dg, sums, d, at);
-  if (BIASED) store_sums<W, C, ROWS, TAIL>(db, sums, d, at + static_cast<int64_t>(gridDim.x) * d);
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * d;
+  if (a.affine) store_sums<W, C, ROWS, TAIL>(dg, sums, d, scale_sums + at);
+  if (BIASED) store_sums<W, C, ROWS, TAIL>(db, sums, d, bias_sums + at);
 }
 
 // d_scale (blockIdx.y 0) and d_bias (1): the workgroups' sums of 64 columns, a wave every
@@ -529,9 +533,9 @@ int backward(const char* name, const T* dy, const T* x, const float* stats, cons
                 need);
   BUX_CHECK(m == 0 || (dy && x && stats && dx), "%s: NULL buffer", name);
   hipStream_t s = as_stream(stream);
+  float* const partials = static_cast<float*>(workspace);
   int64_t blocks = 0;
   if (m > 0) {
-    float* partials = a.affine || a.biased ? static_cast<float*>(workspace) : nullptr;
     with_shape(d, [&](auto w, auto c, auto tail) {
       constexpr int W = decltype(w)::value, C = decltype(c)::value;
       blocks = backward_blocks(m, W, C);
@@ -541,7 +545,8 @@ int backward(const char* name, const T* dy, const T* x, const float* stats, cons
                                             decltype(ahead)::value>),
                            dim3(static_cast<unsigned>(blocks)), dim3(threads_of<W>()), 0, s, dy, x,
                            reinterpret_cast<const float2*>(stats), d_summed, m,
-                           static_cast<int>(d), a, dx, partials);
+                           static_cast<int>(d), a, dx, blocks == 1 ? d_scale : partials,
+                           blocks == 1 ? d_bias : partials + blocks * d);
       };
       auto go = [&](auto biased, auto input) {
         if constexpr (sizeof(T) == 2 && !decltype(tail)::value) {
@@ -557,10 +562,10 @@ int backward(const char* name, const T* dy, const T* x, const float* stats, cons
     });
     if (int rc = launched("token norm backward_kernel")) return rc;
   }
-  if (!a.affine && !a.biased) return BUX_OK;
+  if (blocks == 1 || (!a.affine && !a.biased)) return BUX_OK;
   // with no rows, the sums are 0: a workspace of no partials
   hipLaunchKernelGGL(params_kernel, dim3(static_cast<unsigned>(ceil_div(d, 64)), a.biased ? 2 : 1),
-                     dim3(PARAM_THREADS), 0, s, static_cast<const float*>(workspace), blocks, d,
+                     dim3(PARAM_THREADS), 0, s, static_cast<const float*>(partials), blocks, d,
                      a.affine ? d_scale : nullptr, a.biased ? d_bias : nullptr);
   return launched("token norm params_kernel");
 }
