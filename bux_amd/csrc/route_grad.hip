@@ -616,17 +616,33 @@ __device__ __forceinline__ void bias_tile(const Params& p, uint32_t block, float
   p.d_bias[e] = s;
 }
 
+// Of `count` tiles, workgroup b's: an XCD (a workgroup's id modulo 8) takes a contiguous share, so
+// that the tiles of the same tokens find G in its L2 (16384 tokens of 2048, 128 logits 54.6 us,
+// so 50.6; the kernel's gradient of several tiles of logits loses by it: 8192 of 7168, 256 logits
+// 124 us and 130). in_shares: workgroups for all of them.
+__host__ __device__ __forceinline__ uint32_t in_shares(uint32_t count) { return (count + 7) / 8 * 8; }
+__device__ __forceinline__ uint32_t shared(uint32_t b, uint32_t count) {
+  return b % 8 * ((count + 7) / 8) + b / 8;
+}
+
 // Both products in one launch, so that either's loads fill the other's waits: the kernel's
 // gradient's workgroups first, which take longer; and d_bias's.
 template <int RB>
 __global__ __launch_bounds__(THREADS) void products_kernel(Params p, uint32_t kernel_blocks,
-                                                           uint32_t bias_blocks, uint32_t columns) {
+                                                           uint32_t bias_blocks, uint32_t dx_blocks,
+                                                           uint32_t columns) {
   extern __shared__ __align__(16) uint8_t smem[];
   uint32_t block = blockIdx.x;
-  if (block < kernel_blocks) return kernel_grad_tile(p, block, smem);
-  block -= kernel_blocks;
+  const uint32_t grads = in_shares(kernel_blocks);
+  if (block < grads) {
+    if (p.npad <= COLS) block = shared(block, kernel_blocks);
+    if (block < kernel_blocks) kernel_grad_tile(p, block, smem);
+    return;
+  }
+  block -= grads;
   if (block < bias_blocks) return bias_tile(p, block, reinterpret_cast<float(*)[16]>(smem));
-  dx_tile<RB>(p, block - bias_blocks, columns, smem);
+  block = shared(block - bias_blocks, dx_blocks);
+  if (block < dx_blocks) dx_tile<RB>(p, block, columns, smem);
 }
 
 // d_kernel: the slices' sums in order, 4 logits a thread; and, with no tokens, d_bias.
@@ -786,9 +802,10 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
     constexpr size_t LDS = RING_BYTES > DX_BYTES ? RING_BYTES : DX_BYTES;
     auto products = [&](auto rb) {
       constexpr int RB = decltype(rb)::value;
+      const uint32_t dx_blocks = columns * static_cast<uint32_t>(ceil_div(t, 32 * RB));
       hipLaunchKernelGGL((products_kernel<RB>),
-                         dim3(static_cast<unsigned>(tiles + bias + columns * ceil_div(t, 32 * RB))),
-                         dim3(THREADS), LDS, s, p, tiles, bias, columns);
+                         dim3(in_shares(tiles) + bias + in_shares(dx_blocks)), dim3(THREADS), LDS,
+                         s, p, tiles, bias, dx_blocks, columns);
     };
     static_assert(LDS <= 64 * 1024, "a launch's LDS without an attribute");
     // 32 tokens a wave where its products are few, with three waves a SIMD to hide their loads; 64
