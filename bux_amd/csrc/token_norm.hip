@@ -204,12 +204,19 @@ constexpr int64_t SIMDS = 1024;  // 256 CUs of 4
 // launch less (4 bfloat16 rows of 512 5.1 us, so 3.0, 4 of 2880, two turns, 6.4 both; eager 15.8
 // and 13.4). At four turns 16 rows of 1027 took 17.1 us and 9.8.
 constexpr int64_t ALONE_TURNS = 2;
+// Whole 256s of workgroups of so many turns at least, of 8 waves and of 4: with fewer turns their
+// sums, two rows of float32 each, weigh beside the rows themselves (bfloat16 rows in us: 1000 of
+// 7168 in 512 workgroups 33, in 256 23, 4000 55 and 47; 3001 of 1024 in 751 14.6, in 256 11.9, but
+// 2000 of 2880, two rows a turn, 18.4 in 512 and 19.6 in 256).
+constexpr int64_t SUMS_TURNS_8 = 16, SUMS_TURNS_4 = 3;
 int64_t backward_blocks(int64_t m, int w, int c) {
   const int64_t a_simd = c == 1 || (c == 2 && w > 4) ? 4 : c == 2 ? 3 : 2;
   const int64_t most = a_simd * SIMDS / (w > 4 ? w : 4);
   const int64_t want = ceil_div(m, w > 4 ? 1 : 4 / w);
   if (want <= ALONE_TURNS) return 1;
-  return want < most ? want : most;
+  const int64_t in_turns = ceil_div(want, (w > 4 ? SUMS_TURNS_8 : SUMS_TURNS_4) * 256) * 256;
+  const int64_t enough = in_turns < most ? in_turns : most;
+  return want < enough ? want : enough;
 }
 
 // A lane's sums of its columns' gradients, from the workgroup's waves that hold the same
