@@ -21,10 +21,10 @@
 // sums. reduce_kernel adds the slices, where there are several. All in a fixed order.
 //
 // What bounds it: HBM for few logits (x read once, dx written once, dz read; G stays in L2), the
-// MFMAs of G's two parts for many. us of the three: 500 tokens of 2048, 128 logits 5.5, 9.6, 3.9
-// (a launch's latency each); 16384 with dz 8.9, 54, 6.5, where a copy of its 212 MB takes 41; 8192
-// of 7168, 256 logits 14, 126 to 143, 8, whose 120 GFLOP take 98
-// at a large matrix product's rate.
+// MFMAs of G's two parts for many. us of the three: 500 tokens of 2048, 128 logits 5.5, 9.7, 2.9
+// (a launch's latency each); 16384 with dz 8.4, 50.6, 4.8, where a copy of its 212 MB takes 41;
+// 8192 of 7168, 256 logits 13, 124 to 143 (the card's clock), 5.4, whose 120 GFLOP take 98 at a
+// large matrix product's rate.
 
 #include <math.h>
 

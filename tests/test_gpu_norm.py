@@ -214,6 +214,26 @@ def test_rows_at_any_element_and_nothing_past_the_rows(lib, dtype):
     assert (stats[m] == 7).all() and (params[:, d] == 7).all()
 
 
+@pytest.mark.parametrize("m,d", [(1, 64), (3, 7168), (9, 512), (700, 2880), (1100, 4096), (2100, 1024)])
+def test_the_same_bits_at_any_alignment(lib, m, d):
+    """Aligned rows pass LDS a row ahead, rows an element off load in their turn: the same sums."""
+    from bux_amd import norm as tnorm
+    from bux_amd.moe import ExpertNorm
+    announce("norm alignment", m, d)
+    norm = ExpertNorm("layernorm", bias=True)
+    t = _inputs(m, d, BF16, norm, seed=m)
+    off = {}
+    for k, v in t.items():
+        buffer = torch.zeros(v.numel() + 1, dtype=v.dtype, device="cuda")
+        off[k] = buffer[1:].view(v.shape).copy_(v)
+    got = []
+    for v in (t, off):
+        f = tnorm.normed(v["x"], norm, v["scale"], v["bias"])
+        g = tnorm.normed_backward(v["dy"], v["x"], f.stats, norm, v["scale"], d_summed=v["d_summed"])
+        got.append((f.out, f.stats, *g))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_rows_of_nan_and_infinity_stay_their_own(lib):
     """A row that holds a NaN or an infinity is not a number; the rows beside it, in its own
     workgroup too, are what they are without it."""
