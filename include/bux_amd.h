@@ -654,10 +654,10 @@ int bux_mx_grouped_dglu(const uint8_t* a_values, const uint8_t* a_scales, const 
  * columns); scales float32 [rows]. Columns up to 131072.
  *
  * bux_int8_quantize: rows of x, as bux_mx_quantize takes them (index, index_div, sources, filled
- *   likewise; height any from rows on, up to 67,108,860): values [K/64][height][64], scales [height]; rows from `rows`
- *   or *filled on are 0. Any cols. workspace: with an index, bux_int8_quantize_workspace_size(
- *   sources, rows, cols) bytes, 16-byte aligned (0, then NULL, for few rows; else each
- *   token's own codes).
+ *   likewise; height any from rows on, up to 67,108,860): values [K/64][height][64], scales
+ *   [height]; rows from `rows` or *filled on are 0. Any cols. workspace: with an index,
+ *   bux_int8_quantize_workspace_size(sources, rows, cols) bytes, 16-byte aligned (0, then NULL,
+ *   for few rows; else each token's own codes).
  * bux_int8_glu: rows of the activation of projected and the weights, as bux_glu_forward computes
  *   and rounds them (bux_glu_forward, then bux_int8_quantize, bit for bit), in one pass. f a
  *   multiple of 4.
@@ -739,8 +739,10 @@ int bux_route(const uint16_t* x, const uint16_t* kernel, const float* bias, int6
  * before the one rounding. dx, d_kernel bfloat16; d_bias float32, NULL to skip. The forward's
  * roundings to bfloat16 pass gradients as they are; the choice bias has none. float32 sums, in
  * a fixed order; G enters its products in two bfloat16 parts (2^-17 of each). The limits of
- * bux_route, without groups; x, dz, dx and the workspace 16-byte aligned. workspace: bux_route_backward_workspace_size(t, d, n_logits)
- * bytes: G, and d_kernel's partial sums. */
+ * bux_route, without groups; x, dz, dx and the workspace 16-byte aligned. A normalized single
+ * pick's weight is constant: its gradient is 0, as is that of picks whose scores' sum is below the
+ * smallest normal float32. workspace: bux_route_backward_workspace_size(t, d, n_logits) bytes: G,
+ * and d_kernel's partial sums. */
 size_t bux_route_backward_workspace_size(int64_t t, int64_t d, int32_t n_logits);
 int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int64_t t, int64_t d,
                        int32_t n_logits, float logit_scale, int router, int32_t scored,
