@@ -426,7 +426,8 @@ int check_copy(const char* name, int64_t rows, int64_t cols, int64_t height) {
 //   4096 tokens of 2048, 4 rows each   21  19;   30  23      1024 of 7168, 4   19  22;   49  31
 //   16384 of 2048, 2                   38  39;   55  51      1024 of 7168, 8   34  27;   88  36
 //   16384 of 2048, 8                  137  71;  192  83      16384 of 7168, 8 590 240; 1261 421
-//   16384 of 512, 4                    28  21;   45  24      4096 of 512, 8    16  16;   25  15
+//   16384 of 512, 4                    21  22;   31  23      4096 of 512, 8    12  11;   19  14
+//   12415 of 990, 8                    52  32;   88  37      12415 of 134, 8   15  15;   24  18
 size_t gather_workspace(int64_t sources, int64_t rows, int64_t cols) {
   if (rows < 2 * sources || rows * cols < (1LL << 25)) return 0;
   return static_cast<size_t>(sources) * (ceil_div(cols, 128) * 128 + sizeof(float));
