@@ -13,18 +13,18 @@
 //   dx   = dz_in + G kernel^T,  d_kernel = x^T G,  d_bias = sum over the tokens of G
 //
 // (moe.py:249-270's transpose: the forward's roundings to bfloat16 pass the gradient as they
-// are.) Three kernels: grads_kernel writes G, in two bfloat16 parts, hi and the rest lo: G to
-// 2^-17 at the rate of two bfloat16 MFMAs, where one part alone would put an error of a bfloat16
-// step's half (2^-9) into every product, as large as the outputs' rounding. products_kernel
+// are.) Three kernels: grads_kernel writes G, in three bfloat16 parts of 8 bits of its mantissa
+// each, whose sum is G: its products are float32's, at the rate of three bfloat16 MFMAs (two
+// parts would hold it to 2^-17 alone, which sums that cancel bring to the top). products_kernel
 // multiplies it by the router's kernel, whose rows lie along n (dx_tile), and contracts slices of
 // the tokens with it, transposing on the way out of LDS (kernel_grad_tile), and adds d_bias's partial
 // sums. reduce_kernel adds the slices, where there are several. All in a fixed order.
 //
 // What bounds it: HBM for few logits (x read once, dx written once, dz read; G stays in L2), the
-// MFMAs of G's two parts for many. us of the three: 500 tokens of 2048, 128 logits 5.5, 9.7, 2.9
-// (a launch's latency each); 16384 with dz 8.4, 50.6, 4.8, where a copy of its 212 MB takes 41;
-// 8192 of 7168, 256 logits 13, 124 to 143 (the card's clock), 5.4, whose 120 GFLOP take 98 at a
-// large matrix product's rate.
+// MFMAs of G's three parts for many. us of the three: 500 tokens of 2048, 128 logits 6.1, 11.5, 4.0
+// (a launch's latency each); 16384 with dz 9.4, 62, 5.0, where its 212 MB take 34 at 6.2 TB/s; 8192
+// of 7168, 256 logits 16, 173 to 210 (the card's clock), 5.5, whose 180 GFLOP take 147 at a large
+// matrix product's 1.22 PFLOP/s. With two parts the products took 9.7, 50.6 and 125 to 150.
 
 #include <math.h>
 
@@ -39,6 +39,7 @@ constexpr int THREADS = 256;  // 4 waves
 constexpr int MAX_LOGITS = 1024;
 constexpr int MAX_PICKS = 16;
 constexpr int MAX_GRADS_BLOCKS = 1024;
+constexpr int PARTS = 3;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -59,8 +60,7 @@ struct Params {
   int32_t n, npad, scored, k, router;
   float logit_scale, factor;
   bool normalize;
-  uint16_t* hi;  // G's parts, in blocks (at_block)
-  uint16_t* lo;
+  uint16_t* parts[PARTS];  // G's, in blocks (at_block), the first 8 bits' first
   uint16_t* blocks;  // the kernel, in blocks
   float* bias_partials;    // [grads blocks, npad], or NULL
   float* kernel_partials;  // [slices, d, npad]
@@ -121,6 +121,15 @@ __device__ __forceinline__ void load4(const float* row, int i, int n, float fill
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = i + j < n ? row[i + j] : fill;
   }
+}
+
+// The upper 8 bits of two mantissas as bfloat16 (cut off, so that no part overflows), the rest
+// left in the values, exactly: after three parts 0.
+__device__ __forceinline__ uint32_t next_part(float& a, float& b) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b) & 0xffff0000u;
+  a -= __uint_as_float(x & 0xffff0000u);
+  b -= __uint_as_float(y);
+  return (x >> 16) | y;
 }
 
 // L lanes a token, lane l the logits 4 l + 4 L c .. + 3 for c < Q / 4, so that a wave's tokens
@@ -291,13 +300,10 @@ __global__ __launch_bounds__(THREADS) void grads_kernel(Params p) {
       }
       if (column(q) < p.npad) {
         const int64_t at = at_block(base + sub, column(q), p.npad);
-        const uint32_t h0 = pack_bf16x2(d[0], d[1]), h1 = pack_bf16x2(d[2], d[3]);
-        *reinterpret_cast<uint2*>(p.hi + at) = make_uint2(h0, h1);
-        *reinterpret_cast<uint2*>(p.lo + at) =
-            make_uint2(pack_bf16x2(d[0] - __uint_as_float(h0 << 16),
-                                   d[1] - __uint_as_float(h0 & 0xffff0000u)),
-                       pack_bf16x2(d[2] - __uint_as_float(h1 << 16),
-                                   d[3] - __uint_as_float(h1 & 0xffff0000u)));
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+          *reinterpret_cast<uint2*>(p.parts[part] + at) =
+              make_uint2(next_part(d[0], d[1]), next_part(d[2], d[3]));
       }
     }
   }
@@ -318,7 +324,8 @@ __device__ __forceinline__ bf16x8 load8(const uint16_t* p) {
 }
 
 // dx: a wave 32 RB tokens by 128 columns, K = npad in 16s, the operands from L2 straight to
-// registers, a step ahead. MFMA with the kernel's rows first: lane l holds token l % 32, runs of 4
+// registers: the tokens' a step ahead, the kernel's blocks as the step's last product of each goes
+// out (both a step ahead would leave two waves a SIMD). MFMA with the kernel's rows first: lane l holds token l % 32, runs of 4
 // columns 8 g + 4 (l / 32) of each block. The results pass LDS (32 tokens by 64 columns at a
 // time) so that 8 lanes store 128 bytes of a row, with dz added in float32 before the one
 // rounding; dz's loads go out ahead of what they wait beside: the first 32 tokens' before the
@@ -337,14 +344,13 @@ __device__ __forceinline__ void dx_tile(const Params& p, uint32_t block, uint32_
   // blocks past the last: the last one's, not stored
   const int64_t t_last = (p.t - 1) >> 5, c_last = (p.d - 1) >> 5;
   const int64_t stride = static_cast<int64_t>(p.npad) * 32;  // elements of a row of blocks
-  const uint16_t* ah[RB];
-  const uint16_t* al[RB];
+  const uint16_t* a[RB][PARTS];
   const uint16_t* b[4];
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
     const int64_t at = ((t0 >> 5) + i < t_last ? (t0 >> 5) + i : t_last) * stride;
-    ah[i] = p.hi + at;
-    al[i] = p.lo + at;
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) a[i][part] = p.parts[part] + at;
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -369,39 +375,40 @@ __device__ __forceinline__ void dx_tile(const Params& p, uint32_t block, uint32_
   for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = v16f{};
-  struct Step {
-    bf16x8 hi[RB], lo[RB], w[4];
+  struct Tokens {
+    bf16x8 g[RB][PARTS];
   };
-  auto load = [&](Step& s, int32_t e) {
-    const int at = e * 32 + lane * 8;  // two blocks of 8 columns
+  bf16x8 w[4];
+  auto load = [&](Tokens& s, int32_t e) {
 #pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      s.hi[i] = load8(ah[i] + at);
-      s.lo[i] = load8(al[i] + at);
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) s.g[i][part] = load8(a[i][part] + e * 32 + lane * 8);
+  };
+  auto load_w = [&](int j, int32_t e) { w[j] = load8(b[j] + e * 32 + lane * 8); };  // two blocks of 8
+  // a step: the next one's tokens, then each of the kernel's blocks as its last product is under way
+  auto step = [&](const Tokens& now, Tokens& next, int32_t e, bool more) {
+    if (more) load(next, e + 16);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[j], now.g[i][part], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) load_w(j, e + 16);
+      __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s.w[j] = load8(b[j] + at);
   };
-  auto multiply = [&](const Step& s) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(s.w[j], s.hi[i], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(s.w[j], s.lo[i], acc[i][j], 0, 0, 0);
-      }
-  };
-  Step one, two;
+  Tokens one, two;
   load(one, 0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) load_w(j, 0);
   for (int32_t e = 0; e < p.npad; e += 32) {  // npad is a multiple of 32
-    load(two, e + 16);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(one);
-    __builtin_amdgcn_sched_barrier(0);
-    if (e + 32 < p.npad) load(one, e + 32);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(two);
-    __builtin_amdgcn_sched_barrier(0);
+    step(one, two, e, true);
+    step(two, one, e + 16, e + 32 < p.npad);
   }
   float* mine = reinterpret_cast<float*>(smem) + wave * 32 * DX_PITCH;
 #pragma unroll
@@ -418,9 +425,9 @@ __device__ __forceinline__ void dx_tile(const Params& p, uint32_t block, uint32_
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const v16f& a = acc[i][2 * half + j];
+          const v16f& c = acc[i][2 * half + j];
           *reinterpret_cast<float4*>(mine + r * DX_PITCH + 32 * j + 8 * g + 4 * h) =
-              make_float4(a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]);
+              make_float4(c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]);
         }
       // the wave's own region: its LDS operations run in order
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -450,19 +457,20 @@ __device__ __forceinline__ void dx_tile(const Params& p, uint32_t block, uint32_
   }
 }
 
-// d_kernel's partial sums: a workgroup 128 of d by 128 logits over a slice of the tokens, 32 a
-// step, in a ring of LDS stages that direct loads fill RING - 1 steps ahead. A stage holds the
-// step's operands as they lie in memory, x's tokens of 256 bytes (16-byte chunk c of token k at
-// place c ^ 4 (k % 4)) and G's blocks, 16 of 32 tokens by one chunk (token k of chunk c at place k
-// ^ 4 (c % 4)): a load is runs of 256 bytes or one of 1 KiB, and the 16 lanes of a read hit
-// every bank once. ds_read_b64_tr_b16 transposes on the way out (within each 16 lanes, lane j's
-// 16-bit element e is element j % 4 of the 8 bytes that lane 4 e + j / 4 read).
+// d_kernel's partial sums: a workgroup 128 of d by 128 logits over a slice of the tokens, 16 a
+// step, in a ring of LDS stages that direct loads fill RING - 1 steps ahead (48 KiB, so that three
+// workgroups fit a CU: steps of 32 in two stages of 32 KiB 84 us eager for 16384 tokens of 2048, 128
+// logits, so 79). A stage holds the step's operands as they lie in memory, x's tokens of 256
+// bytes (16-byte chunk c of token k at place c ^ 4 (k % 4)) and G's half blocks, 16 of 16 tokens by
+// one chunk (token k of chunk c at place k ^ 4 (c % 4)): a load is runs of 256 bytes, and the 16
+// lanes of a read hit every bank once. ds_read_b64_tr_b16 transposes on the way out (within each
+// 16 lanes, lane j's 16-bit element e is element j % 4 of the 8 bytes that lane 4 e + j / 4 read).
 // Columns past d or npad read what follows them in memory, into sums that are not stored;
 // tokens past the last read 0.
-constexpr int STEP = 32;
-constexpr int RING = 2;
+constexpr int STEP = 16;
+constexpr int RING = 3;
 struct KStage {
-  uint16_t x[STEP * COLS], hi[STEP * COLS], lo[STEP * COLS];
+  uint16_t x[STEP * COLS], g[PARTS][STEP * COLS];
 };
 
 // 8 tokens of a lane's column: 4 and the 4 after them.
@@ -499,33 +507,26 @@ __device__ __forceinline__ void kernel_grad_tile(const Params& p, uint32_t block
   const int64_t hi_t = lo_t + p.slice < p.t ? lo_t + p.slice : p.t;
   const int steps = static_cast<int>((hi_t - lo_t + STEP - 1) / STEP);
   const uint32_t lds0 = lds_at(smem);
-  // a wave's load i of x: tokens 8 w + 4 i .. + 3 of the step, lane l token l / 16, the chunk that
-  // belongs in place l % 16; of G's parts: chunks 4 w + 2 i and + 1, lane l the token that belongs
-  // in place l % 32 of chunk 4 w + 2 i + l / 32
-  const int row = 8 * wave + (lane >> 4);
+  // a wave's load of x: 4 tokens, lane l the l / 16th's chunk that belongs in place l % 16; of one
+  // of G's parts: 4 chunks, lane l the l / 16th's token that belongs in place l % 16
+  const int row = 4 * wave + (lane >> 4);
   const int chunk = (lane & 15) ^ (4 * ((lane >> 4) & 3));
   const int x_row = static_cast<int>(p.d) * 2, g_tokens = p.npad * 64;  // bytes of 32 tokens of G
   const int x_off = row * x_row + 16 * chunk;
-  int g_off[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int c = 4 * wave + 2 * i + (lane >> 5);
-    g_off[i] = c * 512 + ((lane & 31) ^ (4 * (c & 3))) * 16;
-  }
+  const int g_chunk = 4 * wave + (lane >> 4);
+  const int g_off = g_chunk * 512 + ((lane & 15) ^ (4 * (g_chunk & 3))) * 16;
   auto issue = [&](int s) {
     const int64_t tok = lo_t + static_cast<int64_t>(s) * STEP;
-    // an operand's part of a stage is 8 KiB, a wave's share of it 2
-    const uint32_t at = lds0 + (s % RING) * sizeof(KStage) + wave * 2048;
+    const uint32_t at = lds0 + (s % RING) * sizeof(KStage) + wave * 1024;
     const i32x4 xr = resource(p.x + tok * p.d + j0, ((p.t - tok) * p.d - j0) * 2);
-    // the 32 tokens' blocks from e0 on
-    const int64_t g = tok * p.npad + static_cast<int64_t>(e0) * 32;
-    const i32x4 hr = resource(p.hi + g, g_tokens - e0 * 64);
-    const i32x4 lr = resource(p.lo + g, g_tokens - e0 * 64);
+    load_lds16_uniform(xr, at + offsetof(KStage, x), x_off, 0);
+    // its 32 tokens' blocks from e0 on, and the step's tokens of them
+    const int64_t g = (tok & ~static_cast<int64_t>(31)) * p.npad + static_cast<int64_t>(e0) * 32;
+    const int in_block = static_cast<int>(tok & 31) * 16;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      load_lds16_uniform(xr, at + offsetof(KStage, x) + i * 1024, x_off, i * 4 * x_row);
-      load_lds16_uniform(hr, at + offsetof(KStage, hi) + i * 1024, g_off[i], 0);
-      load_lds16_uniform(lr, at + offsetof(KStage, lo) + i * 1024, g_off[i], 0);
+    for (int part = 0; part < PARTS; ++part) {
+      const i32x4 gr = resource(p.parts[part] + g, g_tokens - e0 * 64);
+      load_lds16_uniform(gr, at + offsetof(KStage, g) + part * sizeof(KStage::g[0]), g_off, in_block);
     }
   };
   // wave (a, b) of 2 x 2: 64 of d from 64 a, 64 logits from 64 b; block q of 32 columns
@@ -537,7 +538,7 @@ __device__ __forceinline__ void kernel_grad_tile(const Params& p, uint32_t block
   };
   auto block_offset = [&](int block) {
     const int c = 4 * block + (col >> 3), k = 8 * (lane >> 5) + kq;
-    return c * 512 + (k ^ (4 * (c & 3))) * 16 + 8 * ((col >> 2) & 1);
+    return c * (16 * STEP) + (k ^ (4 * (c & 3))) * 16 + 8 * ((col >> 2) & 1);
   };
   uint32_t xat[2], gat[2];
 #pragma unroll
@@ -552,32 +553,33 @@ __device__ __forceinline__ void kernel_grad_tile(const Params& p, uint32_t block
     for (int j = 0; j < 2; ++j) acc[i][j] = v16f{};
   for (int s = 0; s < RING - 1 && s < steps; ++s) issue(s);
   for (int s = 0; s < steps; ++s) {
-    // this step's loads are in (the next's go out after the barrier)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // this step's loads are in, those of the RING - 2 after it may not be
+    if (s + RING - 2 < steps)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2) * (1 + PARTS)) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // ... in every wave; and every wave has read the stage that the next loads take
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (s + RING - 1 < steps) issue(s + RING - 1);
     const uint32_t at = lds0 + (s % RING) * sizeof(KStage);
+    bf16x8 xv[2], gv[2][PARTS];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      // 16 tokens on: 4 KiB of x, 256 bytes of G; 4 tokens on: 1 KiB, and place ^ 4
-      const uint32_t xh = at + offsetof(KStage, x) + half * 4096, gh = at + half * 256;
-      bf16x8 xv[2], hv[2], lv[2];
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t x = at + offsetof(KStage, x) + xat[q];
+      xv[q] = read_tr(x, x + 1024);  // 4 tokens on: 1 KiB of x, of G place ^ 4
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        xv[q] = read_tr(xh + xat[q], xh + xat[q] + 1024);
-        const uint32_t hi = gh + offsetof(KStage, hi), lo = gh + offsetof(KStage, lo);
-        hv[q] = read_tr(hi + gat[q], hi + (gat[q] ^ 64));
-        lv[q] = read_tr(lo + gat[q], lo + (gat[q] ^ 64));
+      for (int part = 0; part < PARTS; ++part) {
+        const uint32_t g = at + offsetof(KStage, g) + part * sizeof(KStage::g[0]);
+        gv[q][part] = read_tr(g + gat[q], g + (gat[q] ^ 64));
       }
+    }
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hv[j], xv[i], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lv[j], xv[i], acc[i][j], 0, 0, 0);
-        }
-    }
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gv[j][part], xv[i], acc[i][j], 0, 0, 0);
   }
   float* base = p.kernel_partials + slice * p.d * p.npad;
   const bool last = p.slices == 1;  // nothing to add: the gradient itself
@@ -617,9 +619,9 @@ __device__ __forceinline__ void bias_tile(const Params& p, uint32_t block, float
 }
 
 // Of `count` tiles, workgroup b's: an XCD (a workgroup's id modulo 8) takes a contiguous share, so
-// that the tiles of the same tokens find G in its L2 (16384 tokens of 2048, 128 logits 54.6 us,
-// so 50.6; the kernel's gradient of several tiles of logits loses by it: 8192 of 7168, 256 logits
-// 124 us and 130). in_shares: workgroups for all of them.
+// that the tiles of the same tokens find G in its L2 (16384 tokens of 2048, 128 logits 67.1 us,
+// so 62.0; the kernel's gradient of several tiles of logits loses by it: 8192 of 7168, 256 logits
+// 176 us and 185, the best of 30 each). in_shares: workgroups for all of them.
 __host__ __device__ __forceinline__ uint32_t in_shares(uint32_t count) { return (count + 7) / 8 * 8; }
 __device__ __forceinline__ uint32_t shared(uint32_t b, uint32_t count) {
   return b % 8 * ((count + 7) / 8) + b / 8;
@@ -628,9 +630,8 @@ __device__ __forceinline__ uint32_t shared(uint32_t b, uint32_t count) {
 // Both products in one launch, so that either's loads fill the other's waits: the kernel's
 // gradient's workgroups first, which take longer; and d_bias's.
 template <int RB>
-__global__ __launch_bounds__(THREADS) void products_kernel(Params p, uint32_t kernel_blocks,
-                                                           uint32_t bias_blocks, uint32_t dx_blocks,
-                                                           uint32_t columns) {
+__global__ __launch_bounds__(THREADS, RB == 1 ? 3 : 2) void products_kernel(
+    Params p, uint32_t kernel_blocks, uint32_t bias_blocks, uint32_t dx_blocks, uint32_t columns) {
   extern __shared__ __align__(16) uint8_t smem[];
   uint32_t block = blockIdx.x;
   const uint32_t grads = in_shares(kernel_blocks);
@@ -683,17 +684,18 @@ Plan plan_of(int64_t t, int64_t d, int32_t n) {
   const int64_t blocks = ceil_div(ceil_div(t, 32) * 32, THREADS / lanes_of(w.npad));
   w.grads_blocks = static_cast<int32_t>(blocks < MAX_GRADS_BLOCKS ? blocks : MAX_GRADS_BLOCKS);
   // a workgroup a CU for the kernel's gradient (two measured no faster beside dx's, and their
-  // partial sums' addition 1.6 us slower), slices of 256 tokens at least
+  // partial sums' addition 1.6 us slower), slices of 128 tokens at least (500 tokens of 2048, 128
+  // logits, all three kernels: of 256 20.7 us, of 128 18.0, of 64 19.9)
   const int64_t tiles = ceil_div(d, COLS) * ceil_div(w.npad, COLS);
   const int64_t most = 256 / tiles > 1 ? 256 / tiles : 1;
-  const int64_t by_tokens = ceil_div(t > 0 ? t : 1, 256);
+  const int64_t by_tokens = ceil_div(t > 0 ? t : 1, 128);
   const int64_t slices = most < by_tokens ? most : by_tokens;
   w.slice = ceil_div(ceil_div(t > 0 ? t : 1, slices), STEP) * STEP;
   w.slices = static_cast<int32_t>(ceil_div(t, w.slice));
   auto whole = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
   const size_t part = static_cast<size_t>(ceil_div(t, 32) * 32) * w.npad * sizeof(uint16_t);
   w.parts = 0;
-  w.kernel = 2 * part;
+  w.kernel = PARTS * part;
   w.bias = w.kernel + static_cast<size_t>(ceil_div(d, 32) * 32) * w.npad * sizeof(uint16_t);
   w.partials = w.bias + whole(static_cast<size_t>(w.grads_blocks) * w.npad * sizeof(float));
   w.bytes = w.partials + static_cast<size_t>(w.slices) * d * w.npad * sizeof(float);
@@ -771,8 +773,8 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
   bits &= 0xffff0000u;  // the scaling rounded to bfloat16, as the forward multiplies by it
   __builtin_memcpy(&p.factor, &bits, sizeof(bits));
   p.normalize = normalize != 0;
-  p.hi = reinterpret_cast<uint16_t*>(ws + w.parts);
-  p.lo = reinterpret_cast<uint16_t*>(ws + w.parts + w.kernel / 2);
+  for (int part = 0; part < PARTS; ++part)
+    p.parts[part] = reinterpret_cast<uint16_t*>(ws + w.parts + part * (w.kernel / PARTS));
   p.blocks = reinterpret_cast<uint16_t*>(ws + w.kernel);
   p.bias_partials = d_bias ? reinterpret_cast<float*>(ws + w.bias) : nullptr;
   p.kernel_partials = reinterpret_cast<float*>(ws + w.partials);
@@ -809,8 +811,8 @@ extern "C" int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int
     };
     static_assert(LDS <= 64 * 1024, "a launch's LDS without an attribute");
     // 32 tokens a wave where its products are few, with three waves a SIMD to hide their loads; 64
-    // where the kernel's loads for them count (16384 tokens, 2048 columns, 128 logits: 36.7 us and
-    // 43.0; 8192, 7168, 256: 102 and 85) and there are workgroups to fill the chip
+    // where the kernel's loads for them count (16384 tokens, 2048 columns, 128 logits: 62.0 us and
+    // 65.8; 8192, 7168, 256: 223 and 207) and there are workgroups to fill the chip
     if (w.npad > 128 && ceil_div(t, 64) * columns >= 256) products(integral_constant<int, 2>{});
     else products(integral_constant<int, 1>{});
     if (int rc = launched("route products_kernel"); rc != BUX_OK || w.slices == 1) return rc;

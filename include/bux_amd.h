@@ -737,8 +737,9 @@ int bux_route(const uint16_t* x, const uint16_t* kernel, const float* bias, int6
  * [t, n_logits - scored]; d_scores float32 [t, scored]; d_logits float32 [t, n_logits]; dz
  * bfloat16 [t, d], the gradient that reached the tokens on other ways (NULL for none), added
  * before the one rounding. dx, d_kernel bfloat16; d_bias float32, NULL to skip. The forward's
- * roundings to bfloat16 pass gradients as they are; the choice bias has none. float32 sums, in
- * a fixed order; G enters its products in two bfloat16 parts (2^-17 of each). The limits of
+ * roundings to bfloat16 pass gradients as they are; the choice bias has none. G and its products
+ * are float32 (G in three bfloat16 parts that add up to it), sums float32 in a fixed order; an
+ * infinity among x, kernel or G makes NaN of the outputs that it enters. The limits of
  * bux_route, without groups; x, dz, dx and the workspace 16-byte aligned. A normalized single
  * pick's weight is constant: its gradient is 0, as is that of picks whose scores' sum is below the
  * smallest normal float32. workspace: bux_route_backward_workspace_size(t, d, n_logits) bytes: G,
