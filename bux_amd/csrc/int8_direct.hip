@@ -45,7 +45,7 @@ __device__ __forceinline__ void split_tile(const uint8_t* a, const float* a_scal
   const int lane = threadIdx.x & 63;
   const int quarter = lane >> 4, r16 = lane & 15;
   const int64_t a_chunk = static_cast<int64_t>(a_rows) * 64, b_chunk = static_cast<int64_t>(n) * 64;
-  uint32_t at_a[R], at_b[CB];  // rows past an operand's: its last one's again, not stored
+  uint32_t at_a[R], at_b[CB];  // rows past an operand's: its last one's again (a's count as 0)
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int64_t row = row0 + 16 * i + r16;
@@ -95,13 +95,15 @@ __device__ __forceinline__ void split_tile(const uint8_t* a, const float* a_scal
     if (c + P < hi) multiply(two, c + P);
   }
   // four columns' outputs: the sums times both scales, plus the bias, rounded once
-  auto put = [&](int r, int c, const v4i& sum) {
+  auto put = [&](int r, int c, v4i sum) {
 #pragma clang fp contract(off)
     const int64_t row = row0 + r;
     const int32_t col = col0 + c;
     if (row >= end || col >= n) return;  // n is a multiple of 4
-    // rows past the groups (no chunks): 0
-    const float sa = chunks > 0 ? a_scales[row] : 0.0f;
+    // rows past the groups (no chunks), and those that the sizes put past a's: 0
+    const bool held = chunks > 0 && row < a_rows;
+    const float sa = held ? a_scales[row] : 0.0f;
+    if (!held) sum = v4i{};
     float v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -173,7 +175,10 @@ __global__ __launch_bounds__(64 * S) __attribute__((amdgpu_waves_per_eu(3))) voi
 //   8 of K 4096, N 7168    44  49   44  48    46   47    59   49;  44  48   45  48    49   49;   51  48
 //   16 of K 6400, N 4096   67  72   68  73    83   77    99   82;  58  70   81  81    89   79;   32  60
 //   256 of K 7168, N 4096 968 1184 1116 1301 1452 1448 2066 1501; 956 1110 1194 1292 1527 1476; 810 346
-bool int8_rows_direct(int64_t m, int32_t groups) { return m <= 16 * static_cast<int64_t>(groups); }
+// (Its loads take a's last row for those past it, so there has to be one.)
+bool int8_rows_direct(int64_t m, int32_t groups) {
+  return m > 0 && m <= 16 * static_cast<int64_t>(groups);
+}
 
 int launch_int8_direct(const uint8_t* a_values, const float* a_scales, const uint8_t* b_values,
                        const float* b_scales, const void* list, int64_t slots, int32_t groups,

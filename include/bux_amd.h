@@ -666,8 +666,9 @@ int bux_mx_grouped_dglu(const uint8_t* a_values, const uint8_t* a_scales, const 
  * bux_int8_grouped_rows_listed: bux_mx_grouped_rows_listed for these: y[i][c] = (sum_k a[i][k]
  *   b[g(i)][c][k]) (a_scales[i] b_scales[g(i)][c]) + bias[g(i)][c], the sums exact (32-bit
  *   integers), the rest float32, one rounding to out_dtype; bias [groups, n] of out_dtype, or
- *   NULL; rows from sum(sizes) to height 0. The list (bux_mx_grouped_tiles, or
- *   bux_moe_permute_layer's) is checked as there. n a multiple of 4, m and n up to 33,554,176.
+ *   NULL; rows from sum(sizes) to height 0, a group's rows past m products of 0. The list
+ *   (bux_mx_grouped_tiles, or bux_moe_permute_layer's) is checked as there. n a multiple of 4, m
+ *   and n up to 33,554,176.
  */
 size_t bux_int8_quantize_workspace_size(int64_t sources, int64_t rows, int64_t cols);
 int bux_int8_quantize(const uint16_t* x, const int32_t* index, int32_t index_div, int64_t sources,
