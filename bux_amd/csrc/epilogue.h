@@ -309,5 +309,12 @@ __device__ __forceinline__ void store_plain(const From& from, T* out, int32_t ld
   else store_tile(from, out + j.corner, ld, j.rows, j.cols, stage);
 }
 
+// Whether these stores' 32-bit offsets from a tile's corner hold an output of `rows` rows of n:
+// bytes of bfloat16 in a buffer resource, elements of float32 (half as many bits). Past that, rows
+// of a tile were dropped, and from twice as many on written before the output.
+inline bool stores_fit(int64_t rows, int64_t n) {
+  return 2 * (rows < BM ? rows : BM) * n < (1LL << 31);
+}
+
 }  // namespace
 }  // namespace bux

@@ -359,6 +359,8 @@ template <typename T>
 int launch_rows(const Operand& A, const Operand& B, int32_t groups, int64_t n, int64_t height,
                 const void* list, int64_t slots, const void* bias, void* y, hipStream_t s) {
   const int64_t col_tiles = ceil_div(n, BN);
+  BUX_CHECK(stores_fit(height, n), "bux_int8_grouped_rows_listed: n=%lld columns by height=%lld "
+            "rows: a tile's outputs exceed 2 GiB", (long long)n, (long long)height);
   if (slots * col_tiles >= (1LL << 31))
     return fail(BUX_E_ARGUMENT, "bux_int8_grouped_rows_listed: too many tiles");
   unsigned blocks = 0;

@@ -1204,6 +1204,8 @@ int check_rows(const char* name, const uint8_t* a_values, const uint8_t* a_scale
   BUX_CHECK(n % 4 == 0, "%s: n=%lld is not a multiple of 4", name, (long long)n);
   BUX_CHECK(rows_fit(m) && rows_fit(n), "%s: an operand of %lld rows exceeds %lld", name,
             (long long)(m > n ? m : n), (long long)MAX_ROWS);
+  BUX_CHECK(stores_fit(height, n), "%s: n=%lld columns by height=%lld rows: a tile's outputs "
+            "exceed 2 GiB", name, (long long)n, (long long)height);
   BUX_CHECK(out_dtype == BUX_BF16 || out_dtype == BUX_F32, "%s: out_dtype=%d", name, out_dtype);
   BUX_CHECK(b_values && b_scales && y && (m == 0 || (a_values && a_scales)), "%s: NULL buffer",
             name);
@@ -1221,6 +1223,8 @@ int check_contract(const char* name, const uint8_t* a_values, const uint8_t* a_s
   BUX_CHECK(f % 4 == 0, "%s: f=%lld is not a multiple of 4", name, (long long)f);
   BUX_CHECK(rows_fit(d) && rows_fit(f), "%s: an operand of %lld rows exceeds %lld", name,
             (long long)(d > f ? d : f), (long long)MAX_ROWS);
+  BUX_CHECK(stores_fit(d, f), "%s: f=%lld columns by d=%lld rows: a tile's outputs exceed 2 GiB",
+            name, (long long)f, (long long)d);
   BUX_CHECK(out_dtype == BUX_BF16 || out_dtype == BUX_F32, "%s: out_dtype=%d", name, out_dtype);
   BUX_CHECK(dw && (m == 0 || (a_values && a_scales && b_values && b_scales)), "%s: NULL buffer",
             name);
@@ -1529,6 +1533,8 @@ extern "C" int bux_mx_grouped_glu(const uint8_t* a_values, const uint8_t* a_scal
   BUX_CHECK(narrow(height, k) && narrow(n, k),
             "bux_mx_grouped_glu: an operand of %lld x %lld bytes exceeds 2 GiB",
             (long long)(height > n ? height : n), (long long)k);
+  BUX_CHECK(stores_fit(rows, n), "bux_mx_grouped_glu: n=%lld columns by rows=%lld: a tile's "
+            "outputs exceed 2 GiB", (long long)n, (long long)rows);
   Act act;
   if (int rc = act_of("bux_mx_grouped_glu", ffn, &act)) return rc;
   BUX_CHECK(act.gated && (act.kind == BUX_SWISH || act.kind == BUX_QUICK_GELU || act.kind == BUX_SITU),

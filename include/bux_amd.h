@@ -157,9 +157,10 @@ int bux_mx_quantize_f32(const float* x, const int32_t* index, int32_t index_div,
  *           from sum(sizes) to height are 0. Any height: a's quantized copy may be
  *           padded past the height of y (e.g. to whole tiles) and rows of the groups
  *           past height are not stored. n must be a multiple of 4.
- * Sizes: m, n and height up to 33,554,176 rows (a K chunk's rows x 64 bytes within 2 GiB);
- * an operand's bytes have no cap (past 2 GiB the kernel loads it one K chunk at a time
- * from a 64-bit base).
+ * Sizes: m, n and height up to 33,554,176 rows (a K chunk's rows x 64 bytes within 2 GiB), n
+ * times height (256, if it is more) below 2^30 (a tile's outputs within 2 GiB: n up to 4,194,300
+ * at any height); an operand's bytes have no cap (past 2 GiB the kernel loads it one K chunk at
+ * a time from a 64-bit base).
  */
 enum { BUX_BF16 = 0, BUX_F32 = 1 };
 size_t bux_mx_grouped_rows_workspace_size(int32_t groups, int64_t m, int64_t height);
@@ -253,8 +254,8 @@ int bux_mx_grouped_rows_noalloc(const uint8_t* a_values, const uint8_t* a_scales
  * sizes     device int32 [groups]; sum(sizes) <= m; m a multiple of 128.
  * dw        [groups, d, f], bfloat16 or float32 (out_dtype); 0 for an empty group.
  *           f must be a multiple of 4.
- * Sizes: d and f up to 33,554,176 rows, m below 2^31; an operand's bytes have no cap, as
- * for bux_mx_grouped_rows.
+ * Sizes: d and f up to 33,554,176 rows, f times d (256, if it is more) below 2^30, m below 2^31;
+ * an operand's bytes have no cap, as for bux_mx_grouped_rows.
  */
 size_t bux_mx_grouped_contract_workspace_size(int32_t groups);
 int bux_mx_grouped_contract(const uint8_t* a_values, const uint8_t* a_scales,
@@ -587,7 +588,7 @@ int bux_glu_quantize_f32(const float* projected, const float* weights, const int
  *   height):
  *   a_values/a_scales  x in MXFP8 along its rows, tiled, height rows of k bytes;
  *   b_values/b_scales  each expert's (n, k) up kernels, tiled; n = 2 f, columns in
- *     (up, gate) pairs; f a multiple of 32;
+ *     (up, gate) pairs; f a multiple of 32; n times rows (256, if it is more) below 2^30;
  *   projected  bfloat16 [rows, n] (rows <= height; past sum(sizes): 0);
  *   values/scales  h along its units (K = f rounded up to 128), height rows;
  *   t_values/t_scales  h^T along the rows (K = height, a multiple of 128), f rows;
@@ -668,7 +669,8 @@ int bux_mx_grouped_dglu(const uint8_t* a_values, const uint8_t* a_scales, const 
  *   integers), the rest float32, one rounding to out_dtype; bias [groups, n] of out_dtype, or
  *   NULL; rows from sum(sizes) to height 0, a group's rows past m products of 0. The list
  *   (bux_mx_grouped_tiles, or bux_moe_permute_layer's) is checked as there. n a multiple of 4, m
- *   and n up to 33,554,176.
+ *   and n up to 33,554,176, n times height (256, if it is more) below 2^30 where there are more
+ *   than 16 rows a group.
  */
 size_t bux_int8_quantize_workspace_size(int64_t sources, int64_t rows, int64_t cols);
 int bux_int8_quantize(const uint16_t* x, const int32_t* index, int32_t index_div, int64_t sources,
