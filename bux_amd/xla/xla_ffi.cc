@@ -57,6 +57,28 @@ ffi::Error status(int rc) {
 ffi::Error mismatch(const char* what) {
   return ffi::Error(ffi::ErrorCode::kInvalidArgument, std::string(what));
 }
+// Whether a buffer holds `count` elements of `type`; one that may be absent (an empty buffer) does.
+bool holds(const In& b, ffi::DataType type, int64_t count) {
+  return b.element_type() == type && static_cast<int64_t>(b.element_count()) == count;
+}
+bool absent_or(const In& b, ffi::DataType type, int64_t count) {
+  return b.size_bytes() == 0 || holds(b, type, count);
+}
+bool holds(Out& b, ffi::DataType type, int64_t count) { return holds(*b, type, count); }
+bool absent_or(Out& b, ffi::DataType type, int64_t count) { return absent_or(*b, type, count); }
+// Codes: bytes, whatever XLA calls them.
+bool holds_bytes(const In& b, int64_t count) {
+  return static_cast<int64_t>(b.size_bytes()) == count;
+}
+bool holds_bytes(Out& b, int64_t count) { return holds_bytes(*b, count); }
+bool ranked(const In& b, size_t rank) { return b.dimensions().size() == rank; }
+bool ranked(Out& b, size_t rank) { return ranked(*b, rank); }
+bool layer_type(const In& b) {
+  return b.element_type() == ffi::DataType::BF16 || b.element_type() == ffi::DataType::F32;
+}
+// A row's bytes of 8-bit codes.
+int64_t whole_128(int64_t k) { return (k + 127) / 128 * 128; }
+
 int dtype_of(Out& y) { return y->element_type() == ffi::DataType::F32 ? BUX_F32 : BUX_BF16; }
 bool f32(const In& b) { return b.element_type() == ffi::DataType::F32; }
 
@@ -674,6 +696,15 @@ static ffi::Error token_norm_grad_as(hipStream_t s, In dy, In x, In stats, In d_
 static ffi::Error NormForward(hipStream_t s, In x, In residual, In scale, In bias,
                               BUX_NORM_PARAMS, Out summed, Out out, Out stats) {
   const bux_norm norm = BUX_NORM;
+  if (!ranked(x, 2) || !layer_type(x)) return mismatch("BuxNormForward: x is bfloat16 or float32 [m, d]");
+  const int64_t m = dim(x, 0), d = dim(x, 1);
+  const ffi::DataType type = x.element_type();
+  if (!absent_or(residual, type, m * d) || !absent_or(summed, type, m * d) || !holds(out, type, m * d))
+    return mismatch("BuxNormForward: residual, summed and out have x's shape and dtype");
+  if (!absent_or(scale, type, d) || !absent_or(bias, type, d))
+    return mismatch("BuxNormForward: scale and bias are [d] of x's dtype");
+  if (!absent_or(stats, ffi::DataType::F32, 2 * m))
+    return mismatch("BuxNormForward: stats are float32 [m, 2]");
   return f32(x) ? token_norm_as<float>(s, x, residual, scale, bias, norm, summed, out, stats)
                 : token_norm_as<uint16_t>(s, x, residual, scale, bias, norm, summed, out, stats);
 }
@@ -684,6 +715,16 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxNormForward, NormForward,
 static ffi::Error NormBackward(hipStream_t s, In dy, In x, In stats, In d_summed, In scale,
                                BUX_NORM_PARAMS, Out dx, Out d_scale, Out d_bias, Out ws) {
   const bux_norm norm = BUX_NORM;
+  if (!ranked(x, 2) || !layer_type(x)) return mismatch("BuxNormBackward: x is bfloat16 or float32 [m, d]");
+  const int64_t m = dim(x, 0), d = dim(x, 1);
+  const ffi::DataType type = x.element_type();
+  if (!holds(dy, type, m * d) || !absent_or(d_summed, type, m * d) || !holds(dx, type, m * d))
+    return mismatch("BuxNormBackward: dy, d_summed and dx have x's shape and dtype");
+  if (!absent_or(scale, type, d)) return mismatch("BuxNormBackward: scale is [d] of x's dtype");
+  if (!holds(stats, ffi::DataType::F32, 2 * m))
+    return mismatch("BuxNormBackward: stats are float32 [m, 2]");
+  if (!absent_or(d_scale, ffi::DataType::F32, d) || !absent_or(d_bias, ffi::DataType::F32, d))
+    return mismatch("BuxNormBackward: d_scale and d_bias are float32 [d]");
   return f32(x) ? token_norm_grad_as<float>(s, dy, x, stats, d_summed, scale, norm, dx, d_scale,
                                             d_bias, ws)
                 : token_norm_grad_as<uint16_t>(s, dy, x, stats, d_summed, scale, norm, dx, d_scale,
@@ -700,7 +741,16 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxNormBackward, NormBackward,
 
 static ffi::Error Int8Quantize(hipStream_t s, In x, In index, In filled, int64_t index_div,
                                int64_t rows, Out values, Out scales, Out ws) {
+  if (!ranked(x, 2) || !layer_type(x) || !ranked(values, 3))
+    return mismatch("BuxInt8Quantize: x is bfloat16 or float32 [sources, cols], values [K/64, height, 64]");
   const int64_t height = dim(values, 1), cols = dim(x, 1), sources = dim(x, 0);
+  if (!holds_bytes(values, whole_128(cols) * height) || !holds(scales, ffi::DataType::F32, height))
+    return mismatch("BuxInt8Quantize: values [K/64, height, 64] of cols in whole 128s, scales float32 [height]");
+  if (!absent_or(index, ffi::DataType::S32, static_cast<int64_t>(index.element_count())) ||
+      rows > (index.size_bytes() ? static_cast<int64_t>(index.element_count()) : sources) ||
+      index_div < 1 || index_div > INT32_MAX)
+    return mismatch("BuxInt8Quantize: at most the rows of x, or of an int32 index with its divisor");
+  if (!absent_or(filled, ffi::DataType::S32, 1)) return mismatch("BuxInt8Quantize: filled is an int32");
   const int32_t div = static_cast<int32_t>(index_div);
   if (f32(x))
     return status(bux_int8_quantize_f32(at<const float>(x), at<const int32_t>(index), div, sources,
@@ -721,7 +771,15 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8Quantize, Int8Quantize,
 static ffi::Error Int8Glu(hipStream_t s, In projected, In weights, In filled, BUX_FFN_PARAMS,
                           Out values, Out scales) {
   const bux_ffn ffn = BUX_FFN;
+  if (!ranked(projected, 3) || !layer_type(projected) || dim(projected, 2) != (gated ? 2 : 1) ||
+      !ranked(values, 3))
+    return mismatch("BuxInt8Glu: projected is bfloat16 or float32 [m, f, 2 (gated) or 1], values "
+                    "[K/64, height, 64]");
   const int64_t m = dim(projected, 0), f = dim(projected, 1), height = dim(values, 1);
+  if (!holds(weights, projected.element_type(), m) || !absent_or(filled, ffi::DataType::S32, 1))
+    return mismatch("BuxInt8Glu: weights are [m] of projected's dtype, filled an int32");
+  if (!holds_bytes(values, whole_128(f) * height) || !holds(scales, ffi::DataType::F32, height))
+    return mismatch("BuxInt8Glu: values [K/64, height, 64] of f in whole 128s, scales float32 [height]");
   if (f32(projected))
     return status(bux_int8_glu_f32(at<const float>(projected), at<const float>(weights),
                                    at<const int32_t>(filled), m, f, &ffn, height,
@@ -736,6 +794,11 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8Glu, Int8Glu,
 
 // w [groups, k, n].
 static ffi::Error Int8QuantizeColumns(hipStream_t s, In w, Out values, Out scales) {
+  if (!ranked(w, 3) || !layer_type(w) ||
+      !holds_bytes(values, dim(w, 0) * whole_128(dim(w, 1)) * dim(w, 2)) ||
+      !holds(scales, ffi::DataType::F32, dim(w, 0) * dim(w, 2)))
+    return mismatch("BuxInt8QuantizeColumns: w is bfloat16 or float32 [groups, k, n], values "
+                    "[groups, K/64, n, 64], scales float32 [groups, n]");
   if (f32(w))
     return status(bux_int8_quantize_columns_f32(at<const float>(w), dim(w, 0), dim(w, 1), dim(w, 2),
                                                 at<uint8_t>(values), at<float>(scales), s));
@@ -747,9 +810,18 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8QuantizeColumns, Int8QuantizeColumns,
 
 static ffi::Error Int8GroupedRowsListed(hipStream_t s, In a_values, In a_scales, In b_values,
                                         In b_scales, In list, In bias, Out y) {
-  if (bias.size_bytes() &&
-      (bias.element_type() != y->element_type() ||
-       static_cast<int64_t>(bias.element_count()) != dim(b_scales, 0) * dim(b_scales, 1)))
+  if (!ranked(a_values, 3) || !ranked(b_values, 4) || !ranked(y, 2) || !layer_type(*y) ||
+      dim(a_values, 2) != 64 || dim(b_values, 3) != 64 || dim(b_values, 1) != dim(a_values, 0) ||
+      dim(y, 1) != dim(b_values, 2) ||
+      !holds_bytes(a_values, dim(a_values, 0) * dim(a_values, 1) * 64) ||
+      !holds_bytes(b_values, dim(b_values, 0) * dim(b_values, 1) * dim(b_values, 2) * 64))
+    return mismatch("BuxInt8GroupedRowsListed: codes [K/64, m, 64] times [groups, K/64, n, 64], the "
+                    "product bfloat16 or float32 [height, n]");
+  const int64_t columns = dim(b_values, 0) * dim(b_values, 2);
+  if (!holds(a_scales, ffi::DataType::F32, dim(a_values, 1)) ||
+      !holds(b_scales, ffi::DataType::F32, columns))
+    return mismatch("BuxInt8GroupedRowsListed: scales are float32 [m] and [groups, n]");
+  if (!absent_or(bias, y->element_type(), columns))
     return mismatch("BuxInt8GroupedRowsListed: bias is [groups, n] of the product's dtype");
   return status(bux_int8_grouped_rows_listed(
       at<const uint8_t>(a_values), at<const float>(a_scales), at<const uint8_t>(b_values),
@@ -791,6 +863,20 @@ static ffi::Error RouteBackward(hipStream_t s, In x, In kernel, In idx, In logit
                                 In d_sinks, In d_scores, In d_logits, In dz, float logit_scale,
                                 int64_t router, int64_t scored, int64_t normalize, float scaling,
                                 Out dx, Out d_kernel, Out d_bias, Out ws) {
+  constexpr ffi::DataType BF16 = ffi::DataType::BF16, F32 = ffi::DataType::F32;
+  if (!ranked(x, 2) || !ranked(kernel, 2) || !ranked(idx, 2))
+    return mismatch("BuxRouteBackward: x [t, d], kernel [d, n_logits] and idx [t, k]");
+  const int64_t t = dim(x, 0), d = dim(x, 1), n = dim(kernel, 1), k = dim(idx, 1);
+  if (!holds(x, BF16, t * d) || !holds(kernel, BF16, d * n) || !absent_or(dz, BF16, t * d) ||
+      !holds(dx, BF16, t * d) || !holds(d_kernel, BF16, d * n))
+    return mismatch("BuxRouteBackward: x, dz and dx are bfloat16 [t, d], kernel and d_kernel [d, n_logits]");
+  if (!holds(idx, ffi::DataType::S32, t * k) || !holds(d_weights, BF16, t * k))
+    return mismatch("BuxRouteBackward: idx int32 and d_weights bfloat16 [t, k]");
+  if (scored < 1 || scored > n || !absent_or(d_sinks, BF16, t * (n - scored)) ||
+      !absent_or(d_scores, F32, t * scored))
+    return mismatch("BuxRouteBackward: d_scores float32 [t, scored], d_sinks bfloat16 [t, n_logits - scored]");
+  if (!holds(logits, F32, t * n) || !absent_or(d_logits, F32, t * n) || !absent_or(d_bias, F32, n))
+    return mismatch("BuxRouteBackward: logits and d_logits float32 [t, n_logits], d_bias [n_logits]");
   return status(bux_route_backward(
       at<const uint16_t>(x), at<const uint16_t>(kernel), dim(x, 0), dim(x, 1),
       static_cast<int32_t>(dim(kernel, 1)), logit_scale, static_cast<int>(router),
