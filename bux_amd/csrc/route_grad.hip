@@ -65,7 +65,7 @@ struct Params {
   float* bias_partials;    // [grads blocks, npad], or NULL
   float* kernel_partials;  // [slices, d, npad]
   int32_t grads_blocks, slices;
-  int64_t slice;  // tokens a slice, a multiple of 32
+  int64_t slice;  // tokens a slice, whole steps
   uint16_t* dx;
   uint16_t* d_kernel;
   float* d_bias;
@@ -698,7 +698,9 @@ Plan plan_of(int64_t t, int64_t d, int32_t n) {
   w.kernel = PARTS * part;
   w.bias = w.kernel + static_cast<size_t>(ceil_div(d, 32) * 32) * w.npad * sizeof(uint16_t);
   w.partials = w.bias + whole(static_cast<size_t>(w.grads_blocks) * w.npad * sizeof(float));
-  w.bytes = w.partials + static_cast<size_t>(w.slices) * d * w.npad * sizeof(float);
+  // for as many slices as asked for, though whole steps may fill fewer: so that the size never
+  // falls as t grows
+  w.bytes = w.partials + static_cast<size_t>(slices) * d * w.npad * sizeof(float);
   return w;
 }
 

@@ -746,7 +746,7 @@ int bux_route(const uint16_t* x, const uint16_t* kernel, const float* bias, int6
  * bux_route, without groups; x, dz, dx and the workspace 16-byte aligned. A normalized single
  * pick's weight is constant: its gradient is 0, as is that of picks whose scores' sum is below the
  * smallest normal float32. workspace: bux_route_backward_workspace_size(t, d, n_logits) bytes: G,
- * and d_kernel's partial sums. */
+ * and d_kernel's partial sums; it never falls as t grows. */
 size_t bux_route_backward_workspace_size(int64_t t, int64_t d, int32_t n_logits);
 int bux_route_backward(const uint16_t* x, const uint16_t* kernel, int64_t t, int64_t d,
                        int32_t n_logits, float logit_scale, int router, int32_t scored,
