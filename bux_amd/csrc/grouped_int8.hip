@@ -10,8 +10,9 @@
 // turn, where the epilogue finds them. (A load of each beside every step's codes instead: 131072
 // rows of K 2048, N 1536 510 us and 506, 8192 tokens of gpt-oss-120b's up product 860 and 842.)
 //
-// What bounds it is power: 8192^3 in 536 us, 2050 TOPS, and with codes of 0 in 358. 131072 rows of K
-// 2048, N 1536 in 128 even groups take 453, of K 128 114: the epilogue's share, which no MFMA hides.
+// What bounds it: power on uniform codes (8192^3 in 536 us, 2050 TOPS, and with codes of 0 in 358),
+// and the epilogue, which no MFMA hides: 131072 rows of K 2048, N 1536 in 128 even groups take 453,
+// of K 128 114.
 //
 // MFMA lane layout (32 x 32 x 32): lane l holds row l % 32 of either operand, its half l / 32
 // the 16 bytes of K 16 (l / 32) .. + 15; accumulators as the float MFMAs'.

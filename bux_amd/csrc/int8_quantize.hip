@@ -14,7 +14,8 @@
 // The codes are in the GEMM's tiled layout, [K / 64][rows][64] with K padded to whole 128s.
 // Bound by HBM: a wave takes a row (narrow rows: 16 lanes each), in registers where it has at most
 // 8192 columns (else read twice, the second time from L2); a workgroup's rows lie in one run of
-// each K chunk.
+// each K chunk. The activation of 131072 bfloat16 rows of 768 gated units: 131 us, 3.8 TB/s; of
+// 65536 of 4096 290, 4.6 TB/s; of 4100, past those kept in registers and so computed twice, 430.
 
 #include <type_traits>
 
@@ -362,7 +363,9 @@ __global__ __launch_bounds__(THREADS) void gather_kernel(
 // --- the kernels' columns ------------------------------------------------------------------
 
 // A workgroup 64 columns of a group's (k, n) matrix: each wave every 4th row of it, a lane a
-// column; then 64 rows at a time through LDS, so that a lane writes 16 bytes of a column.
+// column; then 64 rows at a time through LDS, so that a lane writes 16 bytes of a column. Two passes
+// over w, in loads of 2 bytes a lane: 128 bfloat16 kernels of 2048 x 1536 724 us, where their 1.2 GB
+// take 195 at 6.2 TB/s, once as they are loaded.
 constexpr int PITCH = 80;  // bytes of a column's 64 codes in LDS, 16-byte aligned
 template <typename T>
 __global__ __launch_bounds__(THREADS) void columns_kernel(const T* __restrict__ w, int64_t cols,

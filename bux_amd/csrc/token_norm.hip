@@ -22,7 +22,7 @@
 //
 // Forward, 16384 bfloat16 rows of 2048 with their residual: 44.6 us, 6.0 TB/s; one row of 7168 5.1
 // us, its chain of loads and sums. Backward: 8192 bfloat16 rows of 2880 38 us and 16384 of 7168
-// 141 us, 5.0 TB/s (a copy reaches 5.2).
+// 141 us, 5.0 TB/s of the 6.2 that a hand-written copy reaches (the library's 5.1).
 
 #include <type_traits>
 
