@@ -207,7 +207,7 @@ def _plain_product(s):
         if s["product"] is not None:
             dz = dz * _slope(case["activation"], s["product"].float())
         return {"x": (dz @ s["w"].float().T).to(dt), "w": (s["x"].float().T @ dz).to(dt),
-                "bias": dz.sum(0) if s["b"] is not None else None}
+                "bias": dz.sum(0).to(dt) if s["b"] is not None else None}
     y = s["x"].float() @ s["w"].float()
     if s["b"] is not None:
         y = y + s["b"].float()
@@ -253,7 +253,7 @@ def _plain_block(s):
     dp = dp.view(m, f * p)
     out.update(x=(dp @ up.T).to(dt), up=(x.T @ dp).view(d, f, p).to(dt), down=(h.T @ dy).to(dt))
     if s["up_bias"] is not None:
-        out.update(up_bias=dp.sum(0).view(f, p), down_bias=dy.sum(0))
+        out.update(up_bias=dp.sum(0).view(f, p).to(dt), down_bias=dy.sum(0).to(dt))
     return out
 
 
@@ -320,8 +320,8 @@ def work(case):
             return {"bytes": size * (m * k + k * n + m * n * (2 if case["residual"] else 1)
                                      + (n if case["bias"] else 0)), "flops": 2 * m * k * n}
         kept = 0 if case["activation"] == "none" else m * n
-        return {"bytes": size * (2 * m * k + 2 * k * n + m * n + kept)
-                + (4 * n if case["bias"] else 0), "flops": 4 * m * k * n}
+        return {"bytes": size * (2 * m * k + 2 * k * n + m * n + kept
+                                 + (n if case["bias"] else 0)), "flops": 4 * m * k * n}
     if case["kind"] == "block":
         m, d, f, p = case["m"], case["d"], case["f"], 2 if case["gated"] else 1
         weights = (p + 1) * d * f
@@ -329,8 +329,7 @@ def work(case):
         tokens = m * d * (3 if case["residual"] else 2)
         if case["direction"] == "forward":
             return {"bytes": size * (weights + tokens + biases), "flops": 2 * m * weights}
-        return {"bytes": size * (2 * weights + tokens + 2 * m * d + biases) + 4 * biases,
-                "flops": 6 * m * weights}
+        return {"bytes": size * (2 * weights + tokens + 2 * m * d + 2 * biases), "flops": 6 * m * weights}
     d, f, e = case["d"], case["f"], case["experts"]
     values, sums = 3 * e * d * f + d * e, e + 2 * d
     return {"bytes": 2 * (size * values + 4 * sums) + 4, "flops": 3 * (values + sums)}
