@@ -53,6 +53,19 @@ class NormStruct(ctypes.Structure):
 
 _norm = ctypes.POINTER(NormStruct)
 
+class GradientStruct(ctypes.Structure):
+    """``bux_gradient``: a gradient and where its clipped values go."""
+
+    _fields_ = [
+        ("g", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+_gradients = ctypes.POINTER(GradientStruct)
+
 # name -> (restype, argtypes), as include/bux_amd.h declares them.
 SIGNATURES = {
     "bux_last_error": (ctypes.c_char_p, []),
@@ -167,6 +180,22 @@ SIGNATURES = {
     "bux_route_backward": (
         _int, [_p, _p, _i64, _i64, _i32, _f32, _int, _i32, _p, _i32, _int, _f32, _p, _p, _p, _p, _p,
                _p, _p, _p, _p, _p, _size, _p]),
+    "bux_dense_workspace_size": (_size, [_i64, _i64, _i64]),
+    "bux_dense_rows": (
+        _int, [_p, _p, _int, _i64, _i64, _i64, _p, _ffn, _p, _p, _p, _p, _size, _p]),
+    "bux_dense_rows_f32": (
+        _int, [_p, _p, _int, _i64, _i64, _i64, _p, _ffn, _p, _p, _p, _p, _size, _p]),
+    "bux_dense_units_backward": (
+        _int, [_p, _p, _i64, _i64, _i64, _p, _ffn, _p, _p, _size, _p]),
+    "bux_dense_units_backward_f32": (
+        _int, [_p, _p, _i64, _i64, _i64, _p, _ffn, _p, _p, _size, _p]),
+    "bux_dense_contract": (_int, [_p, _p, _i64, _i64, _i64, _p, _p, _size, _p]),
+    "bux_dense_contract_f32": (_int, [_p, _p, _i64, _i64, _i64, _p, _p, _size, _p]),
+    "bux_dense_slope_workspace_size": (_size, [_i64, _i64]),
+    "bux_dense_slope": (_int, [_p, _p, _ffn, _i64, _i64, _p, _p, _p, _size, _p]),
+    "bux_dense_slope_f32": (_int, [_p, _p, _ffn, _i64, _i64, _p, _p, _p, _size, _p]),
+    "bux_clip_workspace_size": (_size, [_i32]),
+    "bux_clip": (_int, [_gradients, _i32, _f32, _p, _p, _size, _p]),
 }
 
 # Constants of include/bux_amd.h.

@@ -43,4 +43,6 @@ extern "C" const char* bux_last_error(void) { return bux::last_error; }
 // router's backward (bux_route_backward), the experts' products in 8-bit integers
 // (bux_int8_quantize, bux_int8_glu, bux_int8_quantize_columns and their float32 twins,
 // bux_int8_grouped_rows_listed).
-extern "C" int bux_version(void) { return 400; }
+// 0.5.0: the dense products (bux_dense_rows, bux_dense_units_backward, bux_dense_contract,
+// bux_dense_slope and their float32 twins), gradients clipped by their norm (bux_clip).
+extern "C" int bux_version(void) { return 500; }

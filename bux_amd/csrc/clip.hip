@@ -1,0 +1,244 @@
+// The global norm of many gradients and their clipping by it.
+//
+//   norm = (sum over every tensor of g^2)^(1/2);  out = g min(1, max_norm / norm)
+//
+// The squares are added in float64: float32's would overflow above 1.8e19 and vanish below
+// 1e-23, and a sum over 10^9 of them would lose its last digits. The tensors are cut into pieces
+// of 8192 elements; a workgroup takes pieces in turn, each lane 8 elements a load at an element's
+// alignment, and leaves one sum. The second kernel's workgroups each add all those sums, in order
+// (16 KiB at most, from L2), so that no atomics decide the order, and then scale their pieces,
+// the last ones first: those are what the first kernel left in the Infinity Cache.
+// Bound by HBM.
+
+#include "common.h"
+
+namespace bux {
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int64_t PIECE = 8192;
+constexpr int ITEMS = 64;       // tensors a launch
+constexpr int64_t GROUPS = 2048;  // workgroups a launch: 8 a CU
+
+struct Item {
+  const void* g;
+  void* out;
+  int64_t n;
+  int64_t first;  // its first piece
+};
+struct Table {
+  Item item[ITEMS];
+  uint64_t f32;  // which are float32
+  int32_t count;
+  int64_t pieces;
+};
+
+// Which item holds piece p: the last whose first is at most p.
+__device__ __forceinline__ int item_of(const Table& t, int64_t p) {
+  int lo = 0, hi = t.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.item[mid].first <= p) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Eight {
+  T at[8];
+};
+
+// f(element index, 8 values) for this lane's groups of 8 of the piece's elements [lo, hi), then
+// g(index, value) for the fewer than 8 left.
+template <typename T, typename F, typename G>
+__device__ __forceinline__ void over(const T* p, int64_t lo, int64_t hi, F&& f, G&& g) {
+  if (hi - lo == PIECE) {
+    Eight<T> e[PIECE / (8 * THREADS)];
+#pragma unroll
+    for (int i = 0; i < PIECE / (8 * THREADS); ++i)
+      e[i] = *reinterpret_cast<const Eight<T>*>(p + lo + 8 * (i * THREADS + threadIdx.x));
+#pragma unroll
+    for (int i = 0; i < PIECE / (8 * THREADS); ++i) f(lo + 8 * (i * THREADS + threadIdx.x), e[i]);
+    return;
+  }
+  for (int64_t at = lo + 8 * threadIdx.x; at < hi; at += 8 * THREADS) {
+    if (at + 8 <= hi) {
+      f(at, *reinterpret_cast<const Eight<T>*>(p + at));
+    } else {
+      for (int64_t i = at; i < hi; ++i) g(i, p[i]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ double squares(const T* p, int64_t lo, int64_t hi) {
+  double s = 0.0;
+  over(p, lo, hi,
+       [&](int64_t, const Eight<T>& e) {
+#pragma unroll
+         for (int j = 0; j < 8; ++j) {
+           const double v = Elem<T>::value(e.at[j]);
+           s = __builtin_fma(v, v, s);
+         }
+       },
+       [&](int64_t, T x) {
+         const double v = Elem<T>::value(x);
+         s = __builtin_fma(v, v, s);
+       });
+  return s;
+}
+
+template <typename T>
+__device__ __forceinline__ void scale(const T* p, T* out, int64_t lo, int64_t hi, float factor) {
+  over(p, lo, hi,
+       [&](int64_t at, const Eight<T>& e) {
+         Eight<T> r;
+#pragma unroll
+         for (int j = 0; j < 8; ++j) r.at[j] = Elem<T>::make(Elem<T>::value(e.at[j]) * factor);
+         *reinterpret_cast<Eight<T>*>(out + at) = r;
+       },
+       [&](int64_t at, T x) { out[at] = Elem<T>::make(Elem<T>::value(x) * factor); });
+}
+
+// The sum over a workgroup, to all of its lanes, in a fixed order.
+__device__ __forceinline__ double group_sum(double v, double* red) {
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) v += __shfl_xor(v, s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double t = red[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) t += red[w];
+  return t;
+}
+
+__global__ __launch_bounds__(THREADS) void squares_kernel(Table t, double* __restrict__ sums) {
+  __shared__ double red[THREADS / 64];
+  double s = 0.0;
+  for (int64_t p = blockIdx.x; p < t.pieces; p += gridDim.x) {
+    const int i = item_of(t, p);
+    const int64_t lo = (p - t.item[i].first) * PIECE;
+    const int64_t hi = lo + PIECE < t.item[i].n ? lo + PIECE : t.item[i].n;
+    if ((t.f32 >> i) & 1) s += squares(static_cast<const float*>(t.item[i].g), lo, hi);
+    else s += squares(static_cast<const uint16_t*>(t.item[i].g), lo, hi);
+  }
+  s = group_sum(s, red);
+  if (threadIdx.x == 0) sums[blockIdx.x] = s;
+}
+
+// The square root of the `count` sums' sum.
+__device__ __forceinline__ double norm_of(const double* sums, int64_t count, double* red) {
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += THREADS) s += sums[i];
+  return sqrt(group_sum(s, red));
+}
+
+__global__ __launch_bounds__(THREADS) void norm_kernel(const double* __restrict__ sums,
+                                                       int64_t count, float* __restrict__ norm) {
+  __shared__ double red[THREADS / 64];
+  const double v = norm_of(sums, count, red);
+  if (threadIdx.x == 0) *norm = static_cast<float>(v);
+}
+
+__global__ __launch_bounds__(THREADS) void scale_kernel(Table t, const double* __restrict__ sums,
+                                                        int64_t count, float max_norm,
+                                                        float* __restrict__ norm) {
+  __shared__ double red[THREADS / 64];
+  const double v = norm_of(sums, count, red);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(v);
+  // a NaN norm makes every gradient NaN
+  const float factor = v <= max_norm ? 1.0f : static_cast<float>(max_norm / v);
+  for (int64_t q = blockIdx.x; q < t.pieces; q += gridDim.x) {
+    const int64_t p = t.pieces - 1 - q;
+    const int i = item_of(t, p);
+    const int64_t lo = (p - t.item[i].first) * PIECE;
+    const int64_t hi = lo + PIECE < t.item[i].n ? lo + PIECE : t.item[i].n;
+    if ((t.f32 >> i) & 1)
+      scale(static_cast<const float*>(t.item[i].g), static_cast<float*>(t.item[i].out), lo, hi,
+            factor);
+    else
+      scale(static_cast<const uint16_t*>(t.item[i].g), static_cast<uint16_t*>(t.item[i].out), lo,
+            hi, factor);
+  }
+}
+
+// The launch's tensors from `at` on (empty ones left out); where the next launch's begin.
+int32_t table_of(const bux_gradient* grads, int32_t count, int32_t at, Table* t) {
+  t->count = 0;
+  t->pieces = 0;
+  t->f32 = 0;
+  for (; at < count && t->count < ITEMS; ++at) {
+    const bux_gradient& g = grads[at];
+    if (g.n == 0) continue;
+    t->item[t->count] = Item{g.g, g.out, g.n, t->pieces};
+    if (g.dtype == BUX_F32) t->f32 |= 1ull << t->count;
+    t->pieces += ceil_div(g.n, PIECE);
+    ++t->count;
+  }
+  return at;
+}
+unsigned groups_of(const Table& t) {
+  return static_cast<unsigned>(t.pieces < GROUPS ? t.pieces : GROUPS);
+}
+
+}  // namespace
+}  // namespace bux
+
+extern "C" size_t bux_clip_workspace_size(int32_t count) {
+  using namespace bux;
+  return count <= 0 ? 0 : static_cast<size_t>(ceil_div(count, ITEMS)) * GROUPS * sizeof(double);
+}
+
+extern "C" int bux_clip(const bux_gradient* grads, int32_t count, float max_norm, float* norm,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace bux;
+  const char* const name = "bux_clip";
+  clear_error();
+  BUX_CHECK(count >= 1 && grads, "%s: %d gradients", name, count);
+  BUX_CHECK(norm, "%s: NULL norm", name);
+  bool clips = false;
+  for (int32_t i = 0; i < count; ++i) {
+    const bux_gradient& g = grads[i];
+    BUX_CHECK(g.n >= 0 && g.n < (1LL << 40), "%s: gradient %d has %lld elements", name, i,
+              (long long)g.n);
+    BUX_CHECK(g.dtype == BUX_BF16 || g.dtype == BUX_F32, "%s: gradient %d: dtype %d", name, i,
+              g.dtype);
+    BUX_CHECK(g.n == 0 || g.g, "%s: gradient %d is NULL", name, i);
+    if (g.n > 0 && g.out) clips = true;
+  }
+  for (int32_t i = 0; i < count; ++i)
+    BUX_CHECK(!clips || grads[i].n == 0 || grads[i].out, "%s: gradient %d has no output", name, i);
+  BUX_CHECK(!clips || max_norm > 0.0f, "%s: max_norm %g", name, max_norm);
+  const size_t need = bux_clip_workspace_size(count);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(BUX_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes,
+                need);
+  BUX_CHECK(reinterpret_cast<uintptr_t>(workspace) % 8 == 0, "%s: unaligned workspace", name);
+  double* const sums = static_cast<double*>(workspace);
+  hipStream_t s = as_stream(stream);
+  Table t;
+  int64_t made = 0;
+  int32_t at = 0;
+  while (at < count) {
+    at = table_of(grads, count, at, &t);
+    if (t.count == 0) break;
+    hipLaunchKernelGGL(squares_kernel, dim3(groups_of(t)), dim3(THREADS), 0, s, t, sums + made);
+    if (int rc = launched("squares_kernel")) return rc;
+    made += groups_of(t);
+  }
+  if (!clips) {
+    hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(THREADS), 0, s, sums, made, norm);
+    return launched("norm_kernel");
+  }
+  float* to = norm;
+  for (at = 0; at < count;) {
+    at = table_of(grads, count, at, &t);
+    if (t.count == 0) break;
+    hipLaunchKernelGGL(scale_kernel, dim3(groups_of(t)), dim3(THREADS), 0, s, t, sums, made,
+                       max_norm, to);
+    if (int rc = launched("scale_kernel")) return rc;
+    to = nullptr;
+  }
+  return BUX_OK;
+}

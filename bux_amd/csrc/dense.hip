@@ -1,0 +1,595 @@
+// Dense matrix products with their epilogues (dense.h), any shape and alignment, in bfloat16
+// (v_mfma_f32_32x32x16_bf16) and float32 (v_mfma_f32_32x32x2_f32), float32 sums:
+//
+//   rows      y = epilogue(x w)     w [k, n], or [n, k] (transposed: x w^T)
+//   contract  dw = x^T dy           x [m, k], dy [m, n]
+//
+// A workgroup of 4 waves makes 128 x 128 of the output, a wave 64 x 64 of it, in steps of 128
+// bytes of K (64 bfloat16, 32 float32). A step's operands come into registers 16 bytes a load at
+// an element's alignment, a step ahead, then into one of two LDS stages of 32 KiB:
+//   K-major (x; w transposed)   128 rows of 128 bytes, 16-byte chunk c of row r at place
+//                               c ^ (r % 8), so that 16 lanes that read one chunk of 16 rows
+//                               take every bank twice at most
+//   MN-major (w; contract's)    K rows of 128 elements, chunk c of K row k at place c ^ 4 (k % 4)
+//                               in bfloat16 (read by ds_read_b64_tr_b16, which transposes) and at
+//                               c ^ 8 ((k / 8) % 2) in float32
+// Rows past an operand's read its last row (no output takes them); K positions past k read 0 in
+// both operands.
+//
+// Few tiles leave CUs idle: K is then split over workgroups, whose sums go to the workspace in
+// float32 and are added in order, with the epilogue, by a second kernel.
+
+#include "dense.h"
+
+namespace bux {
+namespace {
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+constexpr int THREADS = 256;
+constexpr int TILE = 128;
+constexpr int STAGE = 2 * TILE * 128;  // bytes: both operands of a step
+
+template <typename T>
+constexpr int BK = 128 / sizeof(T);
+template <typename T>
+constexpr int PER = 16 / sizeof(T);  // elements of a chunk
+
+// An operand: A(r, k) at p[r ld + k] (K-major) or p[k ld + r], r < rows.
+template <typename T>
+struct Mat {
+  const T* p;
+  int64_t ld, rows;
+};
+
+struct Chunk {
+  uint32_t w[4];
+};
+template <typename T>
+__device__ __forceinline__ Chunk load_chunk(const T* p) {
+  struct __attribute__((packed, aligned(sizeof(T)))) Any {
+    Chunk c;
+  };
+  return reinterpret_cast<const Any*>(p)->c;
+}
+// Its first `count` elements, zeros after them.
+template <typename T>
+__device__ __forceinline__ Chunk load_chunk(const T* p, int64_t count) {
+  if (count >= PER<T>) return load_chunk(p);
+  struct {
+    T at[PER<T>];
+  } e{};
+#pragma unroll
+  for (int j = 0; j < PER<T>; ++j)
+    if (j < count) e.at[j] = p[j];
+  return __builtin_bit_cast(Chunk, e);
+}
+
+// A thread's 4 chunks of an operand's step: K-major chunk i is of row 32 i + tid / 8 at K chunk
+// tid % 8; MN-major of K row (256 i + tid) / (chunks a K row).
+template <typename T, bool KM>
+struct Loader {
+  static constexpr int ROW = KM ? 8 : TILE / PER<T>;  // chunks a row, or a K row
+  const T* at[4];
+  int64_t ld, left;  // MN-major: columns from this lane's on
+  bool whole;        // MN-major: no column of the tile lies past the operand
+  __device__ __forceinline__ Loader(const Mat<T>& a, int64_t row0, int64_t k0) : ld(a.ld) {
+    const int tid = threadIdx.x, c = tid % ROW;
+    whole = KM || row0 + TILE <= a.rows;
+    left = a.rows - row0 - PER<T> * c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = i * (THREADS / ROW) + tid / ROW;
+      if (KM) {
+        const int64_t r = row0 + s;
+        at[i] = a.p + (r < a.rows ? r : a.rows - 1) * ld + k0 + PER<T> * c;
+      } else {
+        at[i] = a.p + (k0 + s) * ld + row0 + PER<T> * c;
+      }
+    }
+  }
+  // The step at K position k (its first), K ending at kend; then on to the next.
+  __device__ __forceinline__ void step(Chunk out[4], int64_t k, int64_t kend) {
+    const int tid = threadIdx.x;
+    if (whole && k + BK<T> <= kend) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[i] = load_chunk(at[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = i * (THREADS / ROW) + tid / ROW;
+        const int64_t count = KM ? kend - k - PER<T> * (tid % ROW) : k + s < kend ? left : 0;
+        out[i] = load_chunk(at[i], count);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i] += KM ? BK<T> : BK<T> * ld;
+  }
+};
+
+template <typename T, bool KM>
+__device__ __forceinline__ void put_step(uint8_t* lds, const Chunk c[4]) {
+  constexpr int ROW = KM ? 8 : TILE / PER<T>;
+  const int tid = threadIdx.x, place = tid % ROW;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = i * (THREADS / ROW) + tid / ROW;
+    const int sw = KM ? (s & 7) : sizeof(T) == 2 ? 4 * (s & 3) : 8 * ((s >> 3) & 1);
+    *reinterpret_cast<Chunk*>(lds + s * (16 * ROW) + 16 * (place ^ sw)) = c[i];
+  }
+}
+
+// bfloat16: the operand of an MFMA over K 16 s .. + 15 of the step, rows base .. base + 31:
+// lane l row base + l % 32, K 8 (l / 32) .. + 7 of those.
+template <bool KM>
+__device__ __forceinline__ v8bf read_bf16(const uint8_t* lds, int base, int s) {
+  const int l = threadIdx.x & 63, h = l >> 5;
+  if constexpr (KM) {
+    const int r = base + (l & 31);
+    return *reinterpret_cast<const v8bf*>(lds + r * 128 + 16 * ((2 * s + h) ^ (r & 7)));
+  } else {
+    const int q = l & 15, kq = q >> 2;
+    const int k = 16 * s + 8 * h + kq, col = base + 16 * ((l >> 4) & 1) + 4 * (q & 3);
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)) + k * 256 +
+                        16 * ((col >> 3) ^ (4 * kq)) + 8 * ((col >> 2) & 1);
+    const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s*>(at));
+    const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s*>(at + 1024));
+    return __builtin_bit_cast(v8bf, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+// float32: 8 of them, for K 16 s + 8 (l / 32) + 0 .. 7.
+template <bool KM>
+__device__ __forceinline__ void read_f32(const uint8_t* lds, int base, int s, float v[8]) {
+  const int l = threadIdx.x & 63, h = l >> 5, r = base + (l & 31);
+  if constexpr (KM) {
+    const int c = 4 * s + 2 * h;
+    const float4 x = *reinterpret_cast<const float4*>(lds + r * 128 + 16 * (c ^ (r & 7)));
+    const float4 y = *reinterpret_cast<const float4*>(lds + r * 128 + 16 * ((c + 1) ^ (r & 7)));
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = 16 * s + 8 * h + j;
+      v[j] = *reinterpret_cast<const float*>(lds + k * 512 + 16 * ((r >> 2) ^ (8 * h)) +
+                                             4 * (r & 3));
+    }
+  }
+}
+
+template <typename T, bool AKM, bool BKM>
+__device__ __forceinline__ void multiply(const uint8_t* a, const uint8_t* b, int wm, int wn,
+                                         f32x16 acc[2][2]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      v8bf x[2], y[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        x[p] = read_bf16<AKM>(a, wm * 64 + p * 32, s);
+        y[p] = read_bf16<BKM>(b, wn * 64 + p * 32, s);
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          acc[p][q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[q], x[p], acc[p][q], 0, 0, 0);
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      float x[2][8], y[2][8];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        read_f32<AKM>(a, wm * 64 + p * 32, s, x[p]);
+        read_f32<BKM>(b, wn * 64 + p * 32, s, y[p]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            acc[p][q] = __builtin_amdgcn_mfma_f32_32x32x2f32(y[q][j], x[p][j], acc[p][q], 0, 0, 0);
+    }
+  }
+}
+
+// Tile `id` of an output of row_tiles x col_tiles: bands of 8 row tiles, a band's columns one
+// after another, so that neighbouring tiles share both operands' rows in an XCD's L2.
+__device__ __forceinline__ void place_of(int64_t id, int64_t row_tiles, int64_t col_tiles,
+                                         int64_t* row, int64_t* col) {
+  const int64_t band = id / (8 * col_tiles), first = 8 * band;
+  const int64_t high = row_tiles - first < 8 ? row_tiles - first : 8;
+  const int64_t rest = id - first * col_tiles;
+  *row = first + rest % high;
+  *col = rest / high;
+}
+
+// C[r][c] = sum over K of A(r, k) B(c, k), K [0, k) in `splits` parts of `part` each: with one
+// part `epi` takes the sums, else `partial` (part i's m rows after those before it).
+template <typename T, bool AKM, bool BKM, typename Epi>
+__global__ __launch_bounds__(THREADS, 2) void tile_kernel(Mat<T> A, Mat<T> B, int64_t m, int64_t n,
+                                                          int64_t k, int64_t part, int64_t splits,
+                                                          Epi epi) {
+  __shared__ __align__(16) uint8_t lds[2 * STAGE];
+  const int64_t row_tiles = (m + TILE - 1) / TILE, col_tiles = (n + TILE - 1) / TILE;
+  const int64_t tiles = row_tiles * col_tiles, count = tiles * splits;
+  // an XCD (workgroup id % 8) takes a contiguous run
+  const int64_t id = (blockIdx.x % 8) * ((count + 7) / 8) + blockIdx.x / 8;
+  if (blockIdx.x / 8 >= (count + 7) / 8 || id >= count) return;
+  const int64_t split = id / tiles;
+  int64_t row, col;
+  place_of(id - split * tiles, row_tiles, col_tiles, &row, &col);
+  row *= TILE;
+  col *= TILE;
+  const int64_t k0 = split * part, kend = k0 + part < k ? k0 + part : k;
+  const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[p][q][j] = 0.0f;
+  Loader<T, AKM> la(A, row, k0);
+  Loader<T, BKM> lb(B, col, k0);
+  Chunk a[4], b[4];
+  if (k0 < kend) {
+    la.step(a, k0, kend);
+    lb.step(b, k0, kend);
+  }
+  int stage = 0;
+  for (int64_t at = k0; at < kend; at += BK<T>) {
+    uint8_t* const s = lds + stage * STAGE;
+    put_step<T, AKM>(s, a);
+    put_step<T, BKM>(s + STAGE / 2, b);
+    // The last step's reads of the other stage are behind this barrier, so the next step's
+    // writes may follow it.
+    __syncthreads();
+    if (at + BK<T> < kend) {
+      la.step(a, at + BK<T>, kend);
+      lb.step(b, at + BK<T>, kend);
+    }
+    multiply<T, AKM, BKM>(s, s + STAGE / 2, wm, wn, acc);
+    stage ^= 1;
+  }
+  __syncthreads();
+  uint8_t* const region = lds + wave * (2 * UNIT_BYTES);
+  put_unit(region, acc[0][0], acc[0][1]);
+  put_unit(region + UNIT_BYTES, acc[1][0], acc[1][1]);
+  wave_done_lds();
+  Epi mine = epi;
+  if constexpr (std::is_same<Epi, Partial>::value) mine.out += split * m * epi.pitch;
+#pragma unroll 1
+  for (int u = 0; u < 2; ++u)
+    store_unit(mine, region + u * UNIT_BYTES, row + wm * 64 + u * 32, col + wn * 64, m, n);
+}
+
+// The sums of the splits' parts, in order, through the epilogue: a thread 8 columns of a row.
+template <typename Epi>
+__global__ __launch_bounds__(THREADS) void join_kernel(const float* __restrict__ parts,
+                                                       int64_t splits, int64_t m, int64_t n,
+                                                       int64_t pitch, Epi epi) {
+  const int64_t per = pitch / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+  if (i >= m * per) return;
+  const int64_t row = i / per, col = 8 * (i - row * per);
+  const typename Epi::In in = epi.load(row, col);
+  float v[8] = {};
+  const float* p = parts + row * pitch + col;
+  for (int64_t s = 0; s < splits; ++s, p += m * pitch) {
+    float w[8];
+    Elem<float>::load8(p, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += w[j];
+  }
+  epi.choose([&](auto kind) { epi.store(kind, row, col, v, in); });
+}
+
+int64_t pitch_of(int64_t n) { return (n + 7) / 8 * 8; }
+
+// How many parts K is split into: enough that the tiles fill the chip's two workgroups a CU, as
+// long as a part has 8 steps.
+int64_t splits_of(int64_t m, int64_t n, int64_t k, int64_t bk) {
+  const int64_t tiles = ceil_div(m, TILE) * ceil_div(n, TILE);
+  const int64_t steps = ceil_div(k, bk);
+  int64_t s = tiles > 0 ? 512 / tiles : 1;
+  if (s > steps / 8) s = steps / 8;
+  return s < 1 ? 1 : s;
+}
+
+template <typename T>
+size_t workspace_for(int64_t m, int64_t n, int64_t k) {
+  const int64_t s = splits_of(m, n, k, BK<T>);
+  return s == 1 ? 0 : static_cast<size_t>(s) * m * pitch_of(n) * sizeof(float);
+}
+
+// m, n, k > 0.
+template <typename T, bool AKM, bool BKM, typename Epi>
+int run(const char* name, const Mat<T>& A, const Mat<T>& B, int64_t m, int64_t n, int64_t k,
+        const Epi& epi, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  const int64_t splits = splits_of(m, n, k, BK<T>), pitch = pitch_of(n);
+  const size_t need = workspace_for<T>(m, n, k);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(BUX_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes,
+                need);
+  BUX_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: unaligned workspace", name);
+  const int64_t tiles = ceil_div(m, TILE) * ceil_div(n, TILE);
+  const int64_t blocks = 8 * ceil_div(tiles * splits, 8);
+  BUX_CHECK(blocks < (1LL << 31), "%s: too many tiles", name);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (splits == 1) {
+    hipLaunchKernelGGL((tile_kernel<T, AKM, BKM, Epi>), grid, dim3(THREADS), 0, s, A, B, m, n, k, k,
+                       splits, epi);
+    return launched("dense tile_kernel");
+  }
+  const int64_t part = ceil_div(ceil_div(k, BK<T>), splits) * BK<T>;
+  float* const parts = static_cast<float*>(workspace);
+  hipLaunchKernelGGL((tile_kernel<T, AKM, BKM, Partial>), grid, dim3(THREADS), 0, s, A, B, m, n, k,
+                     part, splits, Partial{parts, pitch});
+  if (int rc = launched("dense tile_kernel")) return rc;
+  const int64_t threads = m * (pitch / 8);
+  BUX_CHECK(ceil_div(threads, THREADS) < (1LL << 31), "%s: too many rows", name);
+  hipLaunchKernelGGL(join_kernel<Epi>, dim3(static_cast<unsigned>(ceil_div(threads, THREADS))),
+                     dim3(THREADS), 0, s, parts, splits, m, n, pitch, epi);
+  return launched("dense join_kernel");
+}
+
+constexpr int64_t MOST = 1LL << 31;
+
+int check_shape(const char* name, int64_t m, int64_t n, int64_t k) {
+  BUX_CHECK(m >= 0 && n > 0 && k > 0, "%s: bad shape m=%lld n=%lld k=%lld", name, (long long)m,
+            (long long)n, (long long)k);
+  BUX_CHECK(m < MOST && n < MOST && k < MOST, "%s: m=%lld n=%lld k=%lld: each below 2^31", name,
+            (long long)m, (long long)n, (long long)k);
+  return BUX_OK;
+}
+
+// ffn, or no activation where it is NULL.
+int act_or_none(const char* name, const bux_ffn* ffn, Act* act) {
+  if (ffn != nullptr) return act_of(name, ffn, act);
+  *act = Act{NO_ACT, 0, 0, 0.0f, 0, 0.0f, 0.0f};
+  return BUX_OK;
+}
+
+template <typename T>
+int rows(const char* name, const T* x, const T* w, int transposed, int64_t m, int64_t n, int64_t k,
+         const T* bias, const bux_ffn* ffn, const T* residual, T* product, T* out, void* workspace,
+         size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_shape(name, m, n, k)) return rc;
+  Act act;
+  if (int rc = act_or_none(name, ffn, &act)) return rc;
+  BUX_CHECK(!act.gated || (n % 2 == 0 && residual == nullptr),
+            "%s: a gated activation takes an even n (%lld) and no residual", name, (long long)n);
+  if (m == 0) return BUX_OK;
+  BUX_CHECK(x && w && out, "%s: NULL buffer", name);
+  hipStream_t s = as_stream(stream);
+  const Mat<T> A{x, k, m}, B{w, transposed ? k : n, n};
+  auto with = [&](auto epi) {
+    return transposed ? run<T, true, true>(name, A, B, m, n, k, epi, workspace, workspace_bytes, s)
+                      : run<T, true, false>(name, A, B, m, n, k, epi, workspace, workspace_bytes, s);
+  };
+  if (act.gated) return with(Forward<T, true>{act, bias, residual, product, out, n});
+  return with(Forward<T, false>{act, bias, residual, product, out, n});
+}
+
+template <typename T>
+int units_backward(const char* name, const T* dy, const T* down, int64_t m, int64_t f, int64_t d,
+                   const T* product, const bux_ffn* ffn, T* dp, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_shape(name, m, f, d)) return rc;
+  Act act;
+  if (int rc = act_of(name, ffn, &act)) return rc;
+  if (m == 0) return BUX_OK;
+  BUX_CHECK(dy && down && product && dp, "%s: NULL buffer", name);
+  hipStream_t s = as_stream(stream);
+  const Mat<T> A{dy, d, m}, B{down, d, f};
+  if (act.gated)
+    return run<T, true, true>(name, A, B, m, f, d, Backward<T, true>{act, product, dp, f},
+                              workspace, workspace_bytes, s);
+  return run<T, true, true>(name, A, B, m, f, d, Backward<T, false>{act, product, dp, f}, workspace,
+                            workspace_bytes, s);
+}
+
+template <typename T>
+int contract(const char* name, const T* x, const T* dy, int64_t m, int64_t k, int64_t n, T* dw,
+             void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_shape(name, m, n, k)) return rc;
+  BUX_CHECK(dw && (m == 0 || (x && dy)), "%s: NULL buffer", name);
+  const Act none{NO_ACT, 0, 0, 0.0f, 0, 0.0f, 0.0f};
+  const Mat<T> A{x, k, k}, B{dy, n, n};
+  return run<T, false, false>(name, A, B, k, n, m,
+                              Forward<T, false>{none, nullptr, nullptr, nullptr, dw, n}, workspace,
+                              workspace_bytes, as_stream(stream));
+}
+
+// --- the activation's gradient alone, and sums over the rows ---------------------------------
+//
+// dz = dy act'(product) (dy itself without a product) and the column sums of it before its
+// rounding. L lanes (a power of two) take a row's 8 L columns, 256 / L rows a workgroup; its
+// sums over the rows that it takes in turn meet in LDS and, where there are more workgroups
+// along the rows, are added in order by a second kernel.
+
+constexpr int64_t MAX_RUNS = 256;  // workgroups along the rows
+
+int lanes_of(int64_t n) {
+  int l = 1;
+  while (l < 64 && 8 * l < n) l *= 2;
+  return l;
+}
+int64_t runs_of(int64_t m, int64_t n) {
+  const int64_t rows = THREADS / lanes_of(n), strips = ceil_div(n, 8 * lanes_of(n));
+  int64_t r = ceil_div(m, 4 * rows);  // 4 turns a workgroup at least
+  const int64_t most = 2048 / strips > 1 ? 2048 / strips : 1;
+  if (r > most) r = most;
+  if (r > MAX_RUNS) r = MAX_RUNS;
+  return r < 1 ? 1 : r;
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void slope_kernel(const T* __restrict__ dy,
+                                                        const T* __restrict__ product, Act act,
+                                                        int64_t m, int64_t n, int lanes,
+                                                        T* __restrict__ dz, T* __restrict__ sums,
+                                                        float* __restrict__ parts) {
+  __shared__ float red[THREADS][9];
+  const int lane = threadIdx.x % lanes, sub = threadIdx.x / lanes, rows = THREADS / lanes;
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * lanes + lane) * 8, count = n - col;
+  float sum[8] = {};
+  if (count > 0) {
+    of_kind<false>(act.kind, [&](auto kind) {
+      using K = decltype(kind);
+      for (int64_t r = static_cast<int64_t>(blockIdx.y) * rows + sub; r < m;
+           r += static_cast<int64_t>(gridDim.y) * rows) {
+        const Eight<T> g = load_eight(dy + r * n + col, count);
+        float v[8];
+        if constexpr (std::is_same<K, NoAct>::value) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = g.value(j);
+        } else {
+          const Eight<T> z = load_eight(product + r * n + col, count);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float dg, dw;
+            glu_unit_grad<K, sizeof(T) == 4>(act, z.value(j), 0.0f, 1.0f, g.value(j), &v[j], &dg,
+                                             &dw);
+          }
+        }
+        if (dz) store_some<T>(dz + r * n + col, v, count);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += v[j];
+      }
+    });
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) red[threadIdx.x][j] = sum[j];
+  __syncthreads();
+  if (sub != 0 || count <= 0) return;
+  for (int s = 1; s < rows; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] += red[s * lanes + lane][j];
+  if (gridDim.y == 1) {
+    store_some<T>(sums + col, sum, count);
+  } else {
+    float* const p = parts + blockIdx.y * n + col;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) p[j] = sum[j];
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void sums_kernel(const float* __restrict__ parts,
+                                                       int64_t runs, int64_t n,
+                                                       T* __restrict__ sums) {
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+  if (c >= n) return;
+  float v = 0.0f;
+  for (int64_t r = 0; r < runs; ++r) v += parts[r * n + c];
+  sums[c] = Elem<T>::make(v);
+}
+
+template <typename T>
+int slope(const char* name, const T* dy, const T* product, const bux_ffn* ffn, int64_t m, int64_t n,
+          T* dz, T* sums, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_shape(name, m, n, 1)) return rc;
+  Act act;
+  if (int rc = act_or_none(name, ffn, &act)) return rc;
+  BUX_CHECK(!act.gated, "%s: a gated activation", name);
+  BUX_CHECK((ffn == nullptr) == (product == nullptr), "%s: an activation's gradient takes its product",
+            name);
+  BUX_CHECK(dz || sums, "%s: nothing asked for", name);
+  BUX_CHECK(m == 0 || dy, "%s: NULL buffer", name);
+  const int64_t runs = runs_of(m, n);
+  const size_t need = sums && runs > 1 ? static_cast<size_t>(runs) * n * sizeof(float) : 0;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(BUX_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes,
+                need);
+  if (m == 0 && !sums) return BUX_OK;
+  const int lanes = lanes_of(n);
+  hipStream_t s = as_stream(stream);
+  float* const parts = static_cast<float*>(workspace);
+  hipLaunchKernelGGL(slope_kernel<T>, dim3(static_cast<unsigned>(ceil_div(n, 8 * lanes)),
+                                           static_cast<unsigned>(runs)),
+                     dim3(THREADS), 0, s, dy, product, act, m, n, lanes, dz, sums, parts);
+  if (int rc = launched("dense slope_kernel")) return rc;
+  if (!sums || runs == 1) return BUX_OK;
+  hipLaunchKernelGGL(sums_kernel<T>, dim3(static_cast<unsigned>(ceil_div(n, THREADS))),
+                     dim3(THREADS), 0, s, parts, runs, n, sums);
+  return launched("dense sums_kernel");
+}
+
+}  // namespace
+}  // namespace bux
+
+extern "C" size_t bux_dense_workspace_size(int64_t m, int64_t n, int64_t k) {
+  using namespace bux;
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const size_t a = workspace_for<uint16_t>(m, n, k), b = workspace_for<float>(m, n, k);
+  return a > b ? a : b;
+}
+extern "C" size_t bux_dense_slope_workspace_size(int64_t m, int64_t n) {
+  using namespace bux;
+  if (m <= 0 || n <= 0 || runs_of(m, n) == 1) return 0;
+  return static_cast<size_t>(runs_of(m, n)) * n * sizeof(float);
+}
+
+extern "C" int bux_dense_rows(const uint16_t* x, const uint16_t* w, int transposed, int64_t m,
+                              int64_t n, int64_t k, const uint16_t* bias, const bux_ffn* ffn,
+                              const uint16_t* residual, uint16_t* product, uint16_t* out,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  return bux::rows("bux_dense_rows", x, w, transposed, m, n, k, bias, ffn, residual, product, out,
+                   workspace, workspace_bytes, stream);
+}
+extern "C" int bux_dense_rows_f32(const float* x, const float* w, int transposed, int64_t m,
+                                  int64_t n, int64_t k, const float* bias, const bux_ffn* ffn,
+                                  const float* residual, float* product, float* out,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  return bux::rows("bux_dense_rows_f32", x, w, transposed, m, n, k, bias, ffn, residual, product,
+                   out, workspace, workspace_bytes, stream);
+}
+extern "C" int bux_dense_units_backward(const uint16_t* dy, const uint16_t* down, int64_t m,
+                                        int64_t f, int64_t d, const uint16_t* product,
+                                        const bux_ffn* ffn, uint16_t* dp, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  return bux::units_backward("bux_dense_units_backward", dy, down, m, f, d, product, ffn, dp,
+                             workspace, workspace_bytes, stream);
+}
+extern "C" int bux_dense_units_backward_f32(const float* dy, const float* down, int64_t m,
+                                            int64_t f, int64_t d, const float* product,
+                                            const bux_ffn* ffn, float* dp, void* workspace,
+                                            size_t workspace_bytes, void* stream) {
+  return bux::units_backward("bux_dense_units_backward_f32", dy, down, m, f, d, product, ffn, dp,
+                             workspace, workspace_bytes, stream);
+}
+extern "C" int bux_dense_contract(const uint16_t* x, const uint16_t* dy, int64_t m, int64_t k,
+                                  int64_t n, uint16_t* dw, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  return bux::contract("bux_dense_contract", x, dy, m, k, n, dw, workspace, workspace_bytes, stream);
+}
+extern "C" int bux_dense_contract_f32(const float* x, const float* dy, int64_t m, int64_t k,
+                                      int64_t n, float* dw, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  return bux::contract("bux_dense_contract_f32", x, dy, m, k, n, dw, workspace, workspace_bytes,
+                       stream);
+}
+extern "C" int bux_dense_slope(const uint16_t* dy, const uint16_t* product, const bux_ffn* ffn,
+                               int64_t m, int64_t n, uint16_t* dz, uint16_t* sums, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  return bux::slope("bux_dense_slope", dy, product, ffn, m, n, dz, sums, workspace, workspace_bytes,
+                    stream);
+}
+extern "C" int bux_dense_slope_f32(const float* dy, const float* product, const bux_ffn* ffn,
+                                   int64_t m, int64_t n, float* dz, float* sums, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  return bux::slope("bux_dense_slope_f32", dy, product, ffn, m, n, dz, sums, workspace,
+                    workspace_bytes, stream);
+}

@@ -21,6 +21,7 @@
 
 #include <cstdint>
 #include <string>
+#include <vector>
 
 #include "bux_amd.h"
 #include "xla/ffi/api/ffi.h"
@@ -913,5 +914,142 @@ static ffi::Error MxUnpackRows(hipStream_t s, In packed, Out out) {
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxMxUnpackRows, MxUnpackRows,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Ret<In>());
+
+// --- dense products beside the experts ---------------------------------------------------
+// Each picks its float32 twin by x's (dy's) type, which every other operand has.
+
+// x [m, k]; w [k, n], or [n, k] transposed; bias [n], residual [m, n] (out's shape): may be empty.
+// activation -1: none. product [m, n], or empty; out [m, n], or [m, n / 2] of a gated one.
+static ffi::Error DenseRows(hipStream_t s, In x, In w, In bias, In residual, int64_t transposed,
+                            BUX_FFN_PARAMS, Out product, Out out, Out ws) {
+  if (!layer_type(x) || !ranked(x, 2) || !ranked(w, 2) || !ranked(out, 2))
+    return mismatch("BuxDenseRows: x, w and out are bfloat16 or float32 matrices");
+  const int64_t m = dim(x, 0), k = dim(x, 1), n = dim(w, transposed ? 0 : 1);
+  const int64_t wide = activation >= 0 && gated ? n / 2 : n;
+  const ffi::DataType type = x.element_type();
+  if (!holds(w, type, k * n) || dim(w, transposed ? 1 : 0) != k || !absent_or(bias, type, n) ||
+      !absent_or(residual, type, m * n) || !absent_or(product, type, m * n) ||
+      !holds(out, type, m * wide))
+    return mismatch("BuxDenseRows: operands of x's type and of [m, k] times [k, n]");
+  const bux_ffn ffn = BUX_FFN;
+  const bux_ffn* const act = activation < 0 ? nullptr : &ffn;
+  if (f32(x))
+    return status(bux_dense_rows_f32(
+        at<const float>(x), at<const float>(w), static_cast<int>(transposed), m, n, k,
+        at<const float>(bias), act, at<const float>(residual), at<float>(product), at<float>(out),
+        at<void>(ws), ws->size_bytes(), s));
+  return status(bux_dense_rows(
+      at<const uint16_t>(x), at<const uint16_t>(w), static_cast<int>(transposed), m, n, k,
+      at<const uint16_t>(bias), act, at<const uint16_t>(residual), at<uint16_t>(product),
+      at<uint16_t>(out), at<void>(ws), ws->size_bytes(), s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseRows, DenseRows,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
+                                  .Arg<In>().Attr<int64_t>("transposed") BUX_FFN_ATTRS
+                                  .Ret<In>().Ret<In>().Ret<In>());
+
+// dy [m, d], down [f, d], product and dp [m, f, 2] or [m, f].
+static ffi::Error DenseUnitsBackward(hipStream_t s, In dy, In down, In product, BUX_FFN_PARAMS,
+                                     Out dp, Out ws) {
+  if (!layer_type(dy) || !ranked(dy, 2) || !ranked(down, 2))
+    return mismatch("BuxDenseUnitsBackward: dy and down are bfloat16 or float32 matrices");
+  const int64_t m = dim(dy, 0), d = dim(dy, 1), f = dim(down, 0), p = gated ? 2 : 1;
+  const ffi::DataType type = dy.element_type();
+  if (!holds(down, type, f * d) || dim(down, 1) != d || !holds(product, type, m * f * p) ||
+      !holds(dp, type, m * f * p))
+    return mismatch("BuxDenseUnitsBackward: operands of dy's type and of [m, d] times [f, d]");
+  const bux_ffn ffn = BUX_FFN;
+  if (f32(dy))
+    return status(bux_dense_units_backward_f32(at<const float>(dy), at<const float>(down), m, f, d,
+                                               at<const float>(product), &ffn, at<float>(dp),
+                                               at<void>(ws), ws->size_bytes(), s));
+  return status(bux_dense_units_backward(at<const uint16_t>(dy), at<const uint16_t>(down), m, f, d,
+                                         at<const uint16_t>(product), &ffn, at<uint16_t>(dp),
+                                         at<void>(ws), ws->size_bytes(), s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseUnitsBackward, DenseUnitsBackward,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
+                                  BUX_FFN_ATTRS.Ret<In>().Ret<In>());
+
+// x [m, k], dy [m, n], dw [k, n].
+static ffi::Error DenseContract(hipStream_t s, In x, In dy, Out dw, Out ws) {
+  if (!layer_type(x) || !ranked(x, 2) || !ranked(dy, 2) || dim(dy, 0) != dim(x, 0) ||
+      dy.element_type() != x.element_type() ||
+      !holds(dw, x.element_type(), dim(x, 1) * dim(dy, 1)))
+    return mismatch("BuxDenseContract: x [m, k], dy [m, n] and dw [k, n] of one type");
+  if (f32(x))
+    return status(bux_dense_contract_f32(at<const float>(x), at<const float>(dy), dim(x, 0),
+                                         dim(x, 1), dim(dy, 1), at<float>(dw), at<void>(ws),
+                                         ws->size_bytes(), s));
+  return status(bux_dense_contract(at<const uint16_t>(x), at<const uint16_t>(dy), dim(x, 0),
+                                   dim(x, 1), dim(dy, 1), at<uint16_t>(dw), at<void>(ws),
+                                   ws->size_bytes(), s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseContract, DenseContract,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>()
+                                  .Ret<In>().Ret<In>());
+
+// dy [m, n]; product [m, n], or empty with activation -1; dz [m, n] or empty; sums [n] or empty.
+static ffi::Error DenseSlope(hipStream_t s, In dy, In product, BUX_FFN_PARAMS, Out dz, Out sums,
+                             Out ws) {
+  if (!layer_type(dy) || !ranked(dy, 2))
+    return mismatch("BuxDenseSlope: dy is a bfloat16 or float32 matrix");
+  const int64_t m = dim(dy, 0), n = dim(dy, 1);
+  const ffi::DataType type = dy.element_type();
+  if (!absent_or(product, type, m * n) || !absent_or(dz, type, m * n) || !absent_or(sums, type, n))
+    return mismatch("BuxDenseSlope: product, dz and sums of dy's type and size");
+  const bux_ffn ffn = BUX_FFN;
+  const bux_ffn* const act = activation < 0 ? nullptr : &ffn;
+  if (f32(dy))
+    return status(bux_dense_slope_f32(at<const float>(dy), at<const float>(product), act, m, n,
+                                      at<float>(dz), at<float>(sums), at<void>(ws),
+                                      ws->size_bytes(), s));
+  return status(bux_dense_slope(at<const uint16_t>(dy), at<const uint16_t>(product), act, m, n,
+                                at<uint16_t>(dz), at<uint16_t>(sums), at<void>(ws),
+                                ws->size_bytes(), s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseSlope, DenseSlope,
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>() BUX_FFN_ATTRS
+                                  .Ret<In>().Ret<In>().Ret<In>());
+
+// --- gradients clipped by their global norm ------------------------------------------------
+
+// args: the gradients. rets: as many outputs of their types and lengths, each of which may be
+// aliased to its gradient (or none: the norm alone), then the norm (float32, one element), then
+// the workspace.
+static ffi::Error Clip(hipStream_t s, ffi::RemainingArgs grads, float max_norm,
+                       ffi::RemainingRets rets) {
+  const char* const wrong =
+      "BuxClip: gradients of bfloat16 or float32, then as many outputs of their types and lengths "
+      "(or none), the norm (float32) and the workspace";
+  const size_t count = grads.size();
+  const bool clips = rets.size() == count + 2;
+  if (count == 0 || (!clips && rets.size() != 2)) return mismatch(wrong);
+  std::vector<bux_gradient> table;
+  for (size_t i = 0; i < count; ++i) {
+    auto g = grads.get<In>(i);
+    if (!g.has_value() || !layer_type(g.value())) return mismatch(wrong);
+    void* out = nullptr;
+    if (clips) {
+      auto o = rets.get<In>(i);
+      if (!o.has_value() || !holds(o.value(), g.value().element_type(),
+                                   static_cast<int64_t>(g.value().element_count())))
+        return mismatch(wrong);
+      out = at<void>(o.value());
+    }
+    table.push_back(bux_gradient{at<const void>(g.value()), out,
+                                 static_cast<int64_t>(g.value().element_count()),
+                                 f32(g.value()) ? BUX_F32 : BUX_BF16});
+  }
+  auto norm = rets.get<In>(clips ? count : 0), ws = rets.get<In>(clips ? count + 1 : 1);
+  if (!norm.has_value() || !ws.has_value() || !holds(norm.value(), ffi::DataType::F32, 1))
+    return mismatch(wrong);
+  return status(bux_clip(table.data(), static_cast<int32_t>(count), max_norm,
+                         at<float>(norm.value()), at<void>(ws.value()), ws.value()->size_bytes(),
+                         s));
+}
+XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxClip, Clip,
+                              ffi::Ffi::Bind().Ctx<Stream>().RemainingArgs()
+                                  .Attr<float>("max_norm").RemainingRets());
 
 #endif  // __has_include("xla/ffi/api/ffi.h")

@@ -776,6 +776,80 @@ int bux_mx_pack_rows(const uint16_t* x, const int32_t* index, int32_t index_div,
                      int64_t m, int64_t d, uint8_t* packed, void* stream);
 int bux_mx_unpack_rows(const uint8_t* packed, int64_t m, int64_t d, uint16_t* out, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Dense products beside the experts: a layer's projections, its dense feed-forward block
+ * (layers/mlp.py:20-61 of the reference's mlp and gated_mlp) and their backward. bfloat16, and
+ * float32 twins (_f32) whose products and sums are float32's; any shape below 2^31 a side, any
+ * alignment; float32 sums in a fixed order. A workspace of bux_dense_workspace_size(rows of the
+ * output, columns of the sums, the contracted length) bytes, 16-byte aligned (0: none needed).
+ *
+ * bux_dense_rows: z = x w + bias; out = act(z) + residual, each rounded once, from float32.
+ *   x         [m, k].  w: [k, n], or [n, k] with `transposed` (x w^T).
+ *   bias      NULL, or [n].
+ *   ffn       NULL for no activation, else the block's: plain, out [m, n]; or gated, z's columns
+ *             the (up, gate) pairs of n / 2 units, out [m, n / 2] (n even, no residual).
+ *   residual  NULL, or [m, n].
+ *   product   NULL, or [m, n]: z, rounded, for the backward.
+ * bux_dense_units_backward: dp = (dy down^T) d act(product), the down product's gradient to its
+ *   units and the activation's in one kernel. dy [m, d], down [f, d], product and dp [m, f, 2]
+ *   (gated) or [m, f].
+ * bux_dense_contract: dw = x^T dy. x [m, k], dy [m, n], dw [k, n]; 0 for m = 0.
+ *   Its workspace: bux_dense_workspace_size(k, n, m).
+ * bux_dense_slope: dz = dy act'(product) for a plain activation (ffn and product both NULL: dy
+ *   itself), and the sums of dz over its m rows before their rounding. dy, product, dz [m, n];
+ *   sums [n]; dz or sums NULL where not asked for. Its workspace: bux_dense_slope_workspace_size.
+ */
+size_t bux_dense_workspace_size(int64_t m, int64_t n, int64_t k);
+int bux_dense_rows(const uint16_t* x, const uint16_t* w, int transposed, int64_t m, int64_t n,
+                   int64_t k, const uint16_t* bias, const bux_ffn* ffn, const uint16_t* residual,
+                   uint16_t* product, uint16_t* out, void* workspace, size_t workspace_bytes,
+                   void* stream);
+int bux_dense_rows_f32(const float* x, const float* w, int transposed, int64_t m, int64_t n,
+                       int64_t k, const float* bias, const bux_ffn* ffn, const float* residual,
+                       float* product, float* out, void* workspace, size_t workspace_bytes,
+                       void* stream);
+int bux_dense_units_backward(const uint16_t* dy, const uint16_t* down, int64_t m, int64_t f,
+                             int64_t d, const uint16_t* product, const bux_ffn* ffn, uint16_t* dp,
+                             void* workspace, size_t workspace_bytes, void* stream);
+int bux_dense_units_backward_f32(const float* dy, const float* down, int64_t m, int64_t f,
+                                 int64_t d, const float* product, const bux_ffn* ffn, float* dp,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+int bux_dense_contract(const uint16_t* x, const uint16_t* dy, int64_t m, int64_t k, int64_t n,
+                       uint16_t* dw, void* workspace, size_t workspace_bytes, void* stream);
+int bux_dense_contract_f32(const float* x, const float* dy, int64_t m, int64_t k, int64_t n,
+                           float* dw, void* workspace, size_t workspace_bytes, void* stream);
+size_t bux_dense_slope_workspace_size(int64_t m, int64_t n);
+int bux_dense_slope(const uint16_t* dy, const uint16_t* product, const bux_ffn* ffn, int64_t m,
+                    int64_t n, uint16_t* dz, uint16_t* sums, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int bux_dense_slope_f32(const float* dy, const float* product, const bux_ffn* ffn, int64_t m,
+                        int64_t n, float* dz, float* sums, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * The global norm of many gradients, and their clipping by it.
+ *
+ * norm = (sum over all gradients' elements of g^2)^(1/2), added in float64 in a fixed order;
+ * out = g min(1, max_norm / norm), rounded once to g's type. An infinite norm scales by 0 (an
+ * infinity becomes a NaN), a NaN makes every output NaN.
+ *
+ * grads      host array of `count`: each n elements of `dtype` at g, and where they go, out (g
+ *            itself, or elsewhere; NULL in all of them: the norm alone). Read before the call
+ *            returns.
+ * max_norm   above 0 (with outputs).
+ * norm       device float32 [1].
+ * workspace  bux_clip_workspace_size(count) bytes, 8-byte aligned.
+ */
+typedef struct bux_gradient {
+  const void* g;
+  void* out;
+  int64_t n;
+  int32_t dtype; /* BUX_BF16 or BUX_F32 */
+} bux_gradient;
+size_t bux_clip_workspace_size(int32_t count);
+int bux_clip(const bux_gradient* grads, int32_t count, float max_norm, float* norm,
+             void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

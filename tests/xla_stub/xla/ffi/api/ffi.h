@@ -5,6 +5,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <optional>
 #include <string>
 #include <utility>
 #include <vector>
@@ -62,6 +63,45 @@ class Result {
 
 template <typename T>
 struct PlatformStream {};
+
+template <typename T>
+class ErrorOr {
+ public:
+  ErrorOr(T value) : value_(std::move(value)), has_(true) {}
+  ErrorOr() = default;
+  bool has_value() const { return has_; }
+  T& value() { return *value_; }
+
+ private:
+  std::optional<T> value_;
+  bool has_ = false;
+};
+
+// A handler's operands and results past its named ones.
+class RemainingArgs {
+ public:
+  explicit RemainingArgs(std::vector<AnyBuffer> buffers) : buffers_(std::move(buffers)) {}
+  size_t size() const { return buffers_.size(); }
+  template <typename T>
+  ErrorOr<T> get(size_t i) const {
+    return i < buffers_.size() ? ErrorOr<T>(buffers_[i]) : ErrorOr<T>();
+  }
+
+ private:
+  std::vector<AnyBuffer> buffers_;
+};
+class RemainingRets {
+ public:
+  explicit RemainingRets(std::vector<AnyBuffer> buffers) : buffers_(std::move(buffers)) {}
+  size_t size() const { return buffers_.size(); }
+  template <typename T>
+  ErrorOr<Result<T>> get(size_t i) const {
+    return i < buffers_.size() ? ErrorOr<Result<T>>(Result<T>(buffers_[i])) : ErrorOr<Result<T>>();
+  }
+
+ private:
+  std::vector<AnyBuffer> buffers_;
+};
 
 }  // namespace xla::ffi
 
