@@ -15,7 +15,7 @@
 #include "glu.h"
 
 namespace bux {
-namespace {
+namespace dense {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -49,8 +49,17 @@ __device__ __forceinline__ void store_some(T* p, const float* v, int64_t count) 
     T at[N];
   };
   Some s;
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) s.at[j] = Elem<T>::make(v[j]);
+    for (int j = 0; j < N; j += 2) {
+      const uint32_t w = pack_bf16x2(v[j], v[j + 1]);
+      s.at[j] = static_cast<T>(w & 0xffffu);
+      s.at[j + 1] = static_cast<T>(w >> 16);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) s.at[j] = Elem<T>::make(v[j]);
+  }
   if (count >= N) {
     *reinterpret_cast<Some*>(p) = s;
   } else {
@@ -80,6 +89,51 @@ __device__ __forceinline__ void of_kind(int kind, F&& f) {
   }
 }
 
+// --- whole tiles ---------------------------------------------------------------------------
+//
+// A tile that lies inside outputs of whole, aligned 16 bytes moves its values at 32-bit offsets
+// from its corner, without a check a chunk: a lane's own offset (row l / 8, columns 8 (l % 8) of a
+// unit, below) and a scalar one. Stores are non-temporal: another kernel reads them, and they would
+// push the operands out of L2.
+
+typedef uint32_t words4 __attribute__((ext_vector_type(4)));
+typedef uint32_t words2 __attribute__((ext_vector_type(2)));
+constexpr int NON_TEMPORAL = 2;
+
+struct Place {
+  __amdgpu_buffer_rsrc_t rsrc;
+  int32_t lane;   // bytes
+  int32_t pitch;  // bytes a row
+};
+// `columns` elements a chunk of 8 columns of sums (8, 4 of a gated act's units, 16 of its pairs).
+template <int COLUMNS>
+__device__ __forceinline__ Place place_in(const uint16_t* p, int64_t row, int64_t col, int64_t n) {
+  const int lane = threadIdx.x & 63;
+  const int64_t ld = n * COLUMNS / 8;
+  Place r;
+  r.rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(p) + row * ld + col * COLUMNS / 8, 0, 0x7fffffff, 0x00020000);
+  r.pitch = static_cast<int32_t>(ld) * 2;
+  r.lane = (lane >> 3) * r.pitch + (lane & 7) * COLUMNS * 2;
+  return r;
+}
+template <int COLUMNS>
+__device__ __forceinline__ int32_t scalar_in(const Place& p, int row, int col) {
+  return row * p.pitch + col * COLUMNS / 8 * 2;
+}
+__device__ __forceinline__ words4 packed8(const float* v) {
+  return words4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                pack_bf16x2(v[6], v[7])};
+}
+__device__ __forceinline__ float half_of(words4 w, int j) {
+  const uint32_t x = w[j >> 1];
+  return __uint_as_float(j & 1 ? x & 0xffff0000u : x << 16);
+}
+// Whether every row of `columns` bfloat16 from p on begins at 16 bytes.
+__device__ __forceinline__ bool aligned16(const void* p, int64_t columns) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && columns % 8 == 0;
+}
+
 // An epilogue E: In, what a row's 8 columns need beside their sums; load(row, col) of it;
 // choose(f), which calls f with the activation's kind; store(kind, row, col, v, in).
 
@@ -92,6 +146,72 @@ struct Forward {
   T* product;
   T* out;
   int64_t n;  // columns of the sums
+
+  struct Tile {
+    Place out, product, residual;
+    words4 bias[2];  // of a wave's two units of 64 columns
+  };
+  struct Fast {
+    words4 residual;
+  };
+  // Whether tiles inside the output take the path above.
+  __device__ __forceinline__ bool aligned() const {
+    return aligned16(out, GATED ? n / 2 : n) && n % 8 == 0 && n < (1 << 20) &&
+           (product == nullptr || aligned16(product, n)) &&
+           (residual == nullptr || aligned16(residual, n)) &&
+           (bias == nullptr || aligned16(bias, n));
+  }
+  __device__ __forceinline__ Tile tile(int64_t row, int64_t col) const {
+    Tile t;
+    t.out = place_in<GATED ? 4 : 8>(out, row, col, n);
+    t.product = place_in<8>(product, row, col, n);
+    t.residual = place_in<8>(residual, row, col, n);
+    const int c = 8 * (threadIdx.x & 7);
+    if (bias) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        t.bias[u] = *reinterpret_cast<const words4*>(bias + col + 64 * u + c);
+    }
+    return t;
+  }
+  __device__ __forceinline__ Fast fast(const Tile& t, int row, int col) const {
+    Fast f{};
+    if (!GATED && residual)
+      f.residual = __builtin_amdgcn_raw_buffer_load_b128(
+          t.residual.rsrc, t.residual.lane, scalar_in<8>(t.residual, row, col), 0);
+    return f;
+  }
+  template <typename K>
+  __device__ __forceinline__ void store_fast(K, const Tile& t, int row, int col, float v[8],
+                                             const Fast& f) const {
+    if (bias) {
+      const words4 b = col ? t.bias[1] : t.bias[0];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += half_of(b, j);
+    }
+    if (product)
+      __builtin_amdgcn_raw_buffer_store_b128(packed8(v), t.product.rsrc, t.product.lane,
+                                             scalar_in<8>(t.product, row, col), NON_TEMPORAL);
+    if constexpr (GATED) {
+      float h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = glu_unit<K, F32>(act, v[2 * j], v[2 * j + 1], 1.0f);
+      __builtin_amdgcn_raw_buffer_store_b64(
+          words2{pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])}, t.out.rsrc, t.out.lane,
+          scalar_in<4>(t.out, row, col), NON_TEMPORAL);
+    } else {
+      if constexpr (!std::is_same<K, NoAct>::value) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = glu_unit<K, F32>(act, v[j], 0.0f, 1.0f);
+      }
+      if (residual) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += half_of(f.residual, j);
+      }
+      __builtin_amdgcn_raw_buffer_store_b128(packed8(v), t.out.rsrc, t.out.lane,
+                                             scalar_in<8>(t.out, row, col), NON_TEMPORAL);
+    }
+  }
 
   struct In {
     Eight<T> residual;
@@ -146,6 +266,50 @@ struct Backward {
   T* out;            // the same
   int64_t n;         // units
 
+  struct Tile {
+    Place out, product;
+  };
+  struct Fast {
+    words4 p[P];
+  };
+  __device__ __forceinline__ bool aligned() const {
+    return aligned16(out, n) && aligned16(product, n) && n < (1 << 20);
+  }
+  __device__ __forceinline__ Tile tile(int64_t row, int64_t col) const {
+    return Tile{place_in<8 * P>(out, row, col, n), place_in<8 * P>(product, row, col, n)};
+  }
+  __device__ __forceinline__ Fast fast(const Tile& t, int row, int col) const {
+    Fast f;
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      f.p[i] = __builtin_amdgcn_raw_buffer_load_b128(
+          t.product.rsrc, t.product.lane + 16 * i, scalar_in<8 * P>(t.product, row, col), 0);
+    return f;
+  }
+  template <typename K>
+  __device__ __forceinline__ void store_fast(K, const Tile& t, int row, int col, float v[8],
+                                             const Fast& f) const {
+    float d[8 * P];
+    if constexpr (std::is_same<K, NoAct>::value) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float du, dg, dw;
+        const float up = half_of(f.p[j * P / 8], j * P % 8);
+        const float gate = GATED ? half_of(f.p[j * P / 8], j * P % 8 + 1) : 0.0f;
+        glu_unit_grad<K, F32>(act, up, gate, 1.0f, v[j], &du, &dg, &dw);
+        d[j * P] = du;
+        if (GATED) d[j * P + 1] = dg;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      __builtin_amdgcn_raw_buffer_store_b128(packed8(d + 8 * i), t.out.rsrc, t.out.lane + 16 * i,
+                                             scalar_in<8 * P>(t.out, row, col), NON_TEMPORAL);
+  }
+
   struct In {
     Eight<T> p[P];
   };
@@ -188,6 +352,27 @@ struct Backward {
 struct Partial {
   float* out;
   int64_t pitch;
+  struct Tile {
+    Place out;
+  };
+  struct Fast {};
+  __device__ __forceinline__ bool aligned() const { return pitch < (1 << 20); }
+  __device__ __forceinline__ Tile tile(int64_t row, int64_t col) const {
+    // (as pairs of 16 bits)
+    return Tile{place_in<16>(reinterpret_cast<const uint16_t*>(out), row, col, pitch)};
+  }
+  __device__ __forceinline__ Fast fast(const Tile&, int, int) const { return Fast{}; }
+  template <typename K>
+  __device__ __forceinline__ void store_fast(K, const Tile& t, int row, int col, float v[8],
+                                             const Fast&) const {
+    const int32_t at = scalar_in<16>(t.out, row, col);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      __builtin_amdgcn_raw_buffer_store_b128(
+          words4{__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                 __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])},
+          t.out.rsrc, t.out.lane + 16 * i, at, 0);
+  }
   struct In {};
   __device__ __forceinline__ In load(int64_t, int64_t) const { return In{}; }
   template <typename F>
@@ -245,21 +430,47 @@ __device__ __forceinline__ void store_unit(const Epi& epi, const uint8_t* region
                                            int64_t col0, int64_t m, int64_t n) {
   const int lane = threadIdx.x & 63;
   const int64_t row = row0 + (lane >> 3), col = col0 + 8 * (lane & 7);
-  typename Epi::In in[4];
-#pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    in[it] = typename Epi::In{};
-    if (row + 8 * it < m && col < n) in[it] = epi.load(row + 8 * it, col);
-  }
   epi.choose([&](auto kind) {
-#pragma unroll
+#pragma unroll 1
     for (int it = 0; it < 4; ++it) {
+      if (row + 8 * it >= m || col >= n) continue;
+      const typename Epi::In in = epi.load(row + 8 * it, col);
       float v[8];
       get_row(region, it, v);
-      if (row + 8 * it < m && col < n) epi.store(kind, row + 8 * it, col, v, in[it]);
+      epi.store(kind, row + 8 * it, col, v, in);
     }
   });
 }
 
-}  // namespace
+// --- the kernels' operands ------------------------------------------------------------------
+
+// A(r, k) at p[r ld + k] (K-major) or p[k ld + r], r < rows.
+template <typename T>
+struct Mat {
+  const T* p;
+  int64_t ld, rows;
+};
+
+inline int64_t pitch_of(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Tile `id` of an output of row_tiles x col_tiles: bands of 8 row tiles, a band's columns one
+// after another, so that neighbouring tiles share both operands' rows in an XCD's L2.
+__device__ __forceinline__ void place_of(int32_t id, int32_t row_tiles, int32_t col_tiles,
+                                         int32_t* row, int32_t* col) {
+  const int32_t band = id / (8 * col_tiles), first = 8 * band;
+  const int32_t high = row_tiles - first < 8 ? row_tiles - first : 8;
+  const int32_t rest = id - first * col_tiles;
+  *row = first + rest % high;
+  *col = rest / high;
+}
+
+// The large tiles' kernel (dense_tiles.hip): whether it takes the operands, and its launch, K
+// [0, k) in `splits` parts of `units` 64s.
+bool large_takes(const Mat<uint16_t>& A, bool a_km, const Mat<uint16_t>& B, bool b_km, int64_t m,
+                 int64_t n, int64_t k);
+template <bool AKM, bool BKM, typename Epi>
+int launch_large(const Mat<uint16_t>& A, const Mat<uint16_t>& B, int64_t m, int64_t n, int64_t k,
+                 int64_t units, int64_t splits, const Epi& epi, hipStream_t s);
+
+}  // namespace dense
 }  // namespace bux

@@ -22,6 +22,7 @@
 #include "dense.h"
 
 namespace bux {
+using namespace dense;
 namespace {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
@@ -36,13 +37,6 @@ template <typename T>
 constexpr int BK = 128 / sizeof(T);
 template <typename T>
 constexpr int PER = 16 / sizeof(T);  // elements of a chunk
-
-// An operand: A(r, k) at p[r ld + k] (K-major) or p[k ld + r], r < rows.
-template <typename T>
-struct Mat {
-  const T* p;
-  int64_t ld, rows;
-};
 
 struct Chunk {
   uint32_t w[4];
@@ -197,17 +191,6 @@ __device__ __forceinline__ void multiply(const uint8_t* a, const uint8_t* b, int
   }
 }
 
-// Tile `id` of an output of row_tiles x col_tiles: bands of 8 row tiles, a band's columns one
-// after another, so that neighbouring tiles share both operands' rows in an XCD's L2.
-__device__ __forceinline__ void place_of(int64_t id, int64_t row_tiles, int64_t col_tiles,
-                                         int64_t* row, int64_t* col) {
-  const int64_t band = id / (8 * col_tiles), first = 8 * band;
-  const int64_t high = row_tiles - first < 8 ? row_tiles - first : 8;
-  const int64_t rest = id - first * col_tiles;
-  *row = first + rest % high;
-  *col = rest / high;
-}
-
 // C[r][c] = sum over K of A(r, k) B(c, k), K [0, k) in `splits` parts of `part` each: with one
 // part `epi` takes the sums, else `partial` (part i's m rows after those before it).
 template <typename T, bool AKM, bool BKM, typename Epi>
@@ -221,10 +204,11 @@ __global__ __launch_bounds__(THREADS, 2) void tile_kernel(Mat<T> A, Mat<T> B, in
   const int64_t id = (blockIdx.x % 8) * ((count + 7) / 8) + blockIdx.x / 8;
   if (blockIdx.x / 8 >= (count + 7) / 8 || id >= count) return;
   const int64_t split = id / tiles;
-  int64_t row, col;
-  place_of(id - split * tiles, row_tiles, col_tiles, &row, &col);
-  row *= TILE;
-  col *= TILE;
+  int32_t row_tile, col_tile;
+  place_of(static_cast<int32_t>(id - split * tiles), static_cast<int32_t>(row_tiles),
+           static_cast<int32_t>(col_tiles), &row_tile, &col_tile);
+  const int64_t row = static_cast<int64_t>(row_tile) * TILE;
+  const int64_t col = static_cast<int64_t>(col_tile) * TILE;
   const int64_t k0 = split * part, kend = k0 + part < k ? k0 + part : k;
   const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
   f32x16 acc[2][2];
@@ -289,8 +273,6 @@ __global__ __launch_bounds__(THREADS) void join_kernel(const float* __restrict__
   epi.choose([&](auto kind) { epi.store(kind, row, col, v, in); });
 }
 
-int64_t pitch_of(int64_t n) { return (n + 7) / 8 * 8; }
-
 // How many parts K is split into: enough that the tiles fill the chip's two workgroups a CU, as
 // long as a part has 8 steps.
 int64_t splits_of(int64_t m, int64_t n, int64_t k, int64_t bk) {
@@ -317,6 +299,11 @@ int run(const char* name, const Mat<T>& A, const Mat<T>& B, int64_t m, int64_t n
     return fail(BUX_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes,
                 need);
   BUX_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: unaligned workspace", name);
+  if constexpr (sizeof(T) == 2) {
+    if (splits == 1 && ceil_div(m, 256) * ceil_div(n, 256) >= 200 &&
+        large_takes(A, AKM, B, BKM, m, n, k))
+      return launch_large<AKM, BKM>(A, B, m, n, k, ceil_div(k, 64), 1, epi, s);
+  }
   const int64_t tiles = ceil_div(m, TILE) * ceil_div(n, TILE);
   const int64_t blocks = 8 * ceil_div(tiles * splits, 8);
   BUX_CHECK(blocks < (1LL << 31), "%s: too many tiles", name);

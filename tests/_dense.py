@@ -49,7 +49,7 @@ class V:
 
     def holds(self, got, what):
         assert tuple(got.shape) == tuple(self.v.shape), (what, got.shape, self.v.shape)
-        over = (got.to(F64).cpu() - self.v).abs() - self.e
+        over = (got.to(F64).to(self.v.device) - self.v).abs() - self.e
         assert torch.isfinite(got).all() or not torch.isfinite(self.v).all(), what
         worst = over.max().item() if over.numel() else -1.0
         assert worst <= 0, (what, worst, over.argmax().item())
