@@ -472,5 +472,14 @@ template <bool AKM, bool BKM, typename Epi>
 int launch_large(const Mat<uint16_t>& A, const Mat<uint16_t>& B, int64_t m, int64_t n, int64_t k,
                  int64_t units, int64_t splits, const Epi& epi, hipStream_t s);
 
+
+// The few rows' kernel (dense_few.hip): whether it takes the operands (x K-major), the parts that K
+// is split into, and its launch.
+bool few_takes(const Mat<uint16_t>& A, const Mat<uint16_t>& B, int64_t m, int64_t n, int64_t k);
+int64_t few_splits(int64_t n, int64_t k);
+template <bool BKM, typename Epi>
+int launch_few(const Mat<uint16_t>& A, const Mat<uint16_t>& B, int64_t m, int64_t n, int64_t k,
+               int64_t splits, const Epi& epi, hipStream_t s);
+
 }  // namespace dense
 }  // namespace bux

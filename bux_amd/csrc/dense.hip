@@ -283,41 +283,61 @@ int64_t splits_of(int64_t m, int64_t n, int64_t k, int64_t bk) {
   return s < 1 ? 1 : s;
 }
 
+// Which kernel a product runs on, and the parts of K.
+enum class Form { TILE, LARGE, FEW };
+struct Plan {
+  Form form;
+  int64_t splits;
+};
+template <typename T>
+Plan plan_of(const Mat<T>& A, bool a_km, const Mat<T>& B, bool b_km, int64_t m, int64_t n,
+             int64_t k) {
+  if constexpr (sizeof(T) == 2) {
+    if (a_km && few_takes(A, B, m, n, k)) return Plan{Form::FEW, few_splits(n, k)};
+    if (ceil_div(m, 256) * ceil_div(n, 256) >= 200 && large_takes(A, a_km, B, b_km, m, n, k))
+      return Plan{Form::LARGE, 1};
+  }
+  return Plan{Form::TILE, splits_of(m, n, k, BK<T>)};
+}
+
+// What any form may ask for: the operands' alignment decides, which is not known here.
 template <typename T>
 size_t workspace_for(int64_t m, int64_t n, int64_t k) {
-  const int64_t s = splits_of(m, n, k, BK<T>);
+  int64_t s = splits_of(m, n, k, BK<T>);
+  if (sizeof(T) == 2 && m <= 64 && few_splits(n, k) > s) s = few_splits(n, k);
   return s == 1 ? 0 : static_cast<size_t>(s) * m * pitch_of(n) * sizeof(float);
 }
 
-// m, n, k > 0.
+// m, n > 0.
 template <typename T, bool AKM, bool BKM, typename Epi>
 int run(const char* name, const Mat<T>& A, const Mat<T>& B, int64_t m, int64_t n, int64_t k,
         const Epi& epi, void* workspace, size_t workspace_bytes, hipStream_t s) {
-  const int64_t splits = splits_of(m, n, k, BK<T>), pitch = pitch_of(n);
   const size_t need = workspace_for<T>(m, n, k);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(BUX_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes,
                 need);
   BUX_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: unaligned workspace", name);
-  if constexpr (sizeof(T) == 2) {
-    if (splits == 1 && ceil_div(m, 256) * ceil_div(n, 256) >= 200 &&
-        large_takes(A, AKM, B, BKM, m, n, k))
-      return launch_large<AKM, BKM>(A, B, m, n, k, ceil_div(k, 64), 1, epi, s);
-  }
-  const int64_t tiles = ceil_div(m, TILE) * ceil_div(n, TILE);
-  const int64_t blocks = 8 * ceil_div(tiles * splits, 8);
-  BUX_CHECK(blocks < (1LL << 31), "%s: too many tiles", name);
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (splits == 1) {
-    hipLaunchKernelGGL((tile_kernel<T, AKM, BKM, Epi>), grid, dim3(THREADS), 0, s, A, B, m, n, k, k,
-                       splits, epi);
+  const Plan plan = plan_of(A, AKM, B, BKM, m, n, k);
+  const int64_t splits = plan.splits, pitch = pitch_of(n);
+  auto launch = [&](const auto& e) {
+    if constexpr (sizeof(T) == 2) {
+      if constexpr (AKM) {
+        if (plan.form == Form::FEW) return launch_few<BKM>(A, B, m, n, k, splits, e, s);
+      }
+      if (plan.form == Form::LARGE)
+        return launch_large<AKM, BKM>(A, B, m, n, k, ceil_div(ceil_div(k, 64), splits), splits, e, s);
+    }
+    const int64_t blocks = 8 * ceil_div(ceil_div(m, TILE) * ceil_div(n, TILE) * splits, 8);
+    if (blocks >= (1LL << 31)) return fail(BUX_E_ARGUMENT, "%s: too many tiles", name);
+    const int64_t part = ceil_div(ceil_div(k, BK<T>), splits) * BK<T>;
+    hipLaunchKernelGGL((tile_kernel<T, AKM, BKM, std::decay_t<decltype(e)>>),
+                       dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, s, A, B, m, n, k, part,
+                       splits, e);
     return launched("dense tile_kernel");
-  }
-  const int64_t part = ceil_div(ceil_div(k, BK<T>), splits) * BK<T>;
+  };
+  if (splits == 1) return launch(epi);
   float* const parts = static_cast<float*>(workspace);
-  hipLaunchKernelGGL((tile_kernel<T, AKM, BKM, Partial>), grid, dim3(THREADS), 0, s, A, B, m, n, k,
-                     part, splits, Partial{parts, pitch});
-  if (int rc = launched("dense tile_kernel")) return rc;
+  if (int rc = launch(Partial{parts, pitch})) return rc;
   const int64_t threads = m * (pitch / 8);
   BUX_CHECK(ceil_div(threads, THREADS) < (1LL << 31), "%s: too many rows", name);
   hipLaunchKernelGGL(join_kernel<Epi>, dim3(static_cast<unsigned>(ceil_div(threads, THREADS))),
