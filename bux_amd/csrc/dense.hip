@@ -62,17 +62,27 @@ __device__ __forceinline__ Chunk load_chunk(const T* p, int64_t count) {
 }
 
 // A thread's 4 chunks of an operand's step: K-major chunk i is of row 32 i + tid / 8 at K chunk
-// tid % 8; MN-major of K row (256 i + tid) / (chunks a K row).
+// tid % 8; MN-major of K row (256 i + tid) / (chunks a K row). K is `k` long in all.
 template <typename T, bool KM>
 struct Loader {
   static constexpr int ROW = KM ? 8 : TILE / PER<T>;  // chunks a row, or a K row
   const T* at[4];
   int64_t ld, left;  // MN-major: columns from this lane's on
-  bool whole;        // MN-major: no column of the tile lies past the operand
-  __device__ __forceinline__ Loader(const Mat<T>& a, int64_t row0, int64_t k0) : ld(a.ld) {
+  int64_t plain;     // steps that end at or before this K position load without a check
+  __device__ __forceinline__ Loader(const Mat<T>& a, int64_t row0, int64_t k0, int64_t k,
+                                    int64_t kend)
+      : ld(a.ld) {
     const int tid = threadIdx.x, c = tid % ROW;
-    whole = KM || row0 + TILE <= a.rows;
     left = a.rows - row0 - PER<T> * c;
+    plain = kend;
+    if (!KM && row0 + TILE > a.rows) {
+      // The tile reaches past the columns. A chunk that they cut reads on into the next K row (its
+      // columns are no output's), which the last K row does not have; the lanes past them read the
+      // row's last chunk.
+      if (a.rows % PER<T> != 0 && kend == k) plain = k - 1;
+      if (a.rows < PER<T>) plain = k0;
+    }
+    const int64_t col = left > 0 || a.rows < PER<T> ? row0 + PER<T> * c : a.rows - PER<T>;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int s = i * (THREADS / ROW) + tid / ROW;
@@ -80,14 +90,14 @@ struct Loader {
         const int64_t r = row0 + s;
         at[i] = a.p + (r < a.rows ? r : a.rows - 1) * ld + k0 + PER<T> * c;
       } else {
-        at[i] = a.p + (k0 + s) * ld + row0 + PER<T> * c;
+        at[i] = a.p + (k0 + s) * ld + col;
       }
     }
   }
   // The step at K position k (its first), K ending at kend; then on to the next.
   __device__ __forceinline__ void step(Chunk out[4], int64_t k, int64_t kend) {
     const int tid = threadIdx.x;
-    if (whole && k + BK<T> <= kend) {
+    if (k + BK<T> <= plain) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[i] = load_chunk(at[i]);
     } else {
@@ -218,8 +228,8 @@ __global__ __launch_bounds__(THREADS, 2) void tile_kernel(Mat<T> A, Mat<T> B, in
     for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[p][q][j] = 0.0f;
-  Loader<T, AKM> la(A, row, k0);
-  Loader<T, BKM> lb(B, col, k0);
+  Loader<T, AKM> la(A, row, k0, k, kend);
+  Loader<T, BKM> lb(B, col, k0, k, kend);
   Chunk a[4], b[4];
   if (k0 < kend) {
     la.step(a, k0, kend);
@@ -273,51 +283,85 @@ __global__ __launch_bounds__(THREADS) void join_kernel(const float* __restrict__
   epi.choose([&](auto kind) { epi.store(kind, row, col, v, in); });
 }
 
-// How many parts K is split into: enough that the tiles fill the chip's two workgroups a CU, as
-// long as a part has 8 steps.
-int64_t splits_of(int64_t m, int64_t n, int64_t k, int64_t bk) {
-  const int64_t tiles = ceil_div(m, TILE) * ceil_div(n, TILE);
-  const int64_t steps = ceil_div(k, bk);
-  int64_t s = tiles > 0 ? 512 / tiles : 1;
-  if (s > steps / 8) s = steps / 8;
-  return s < 1 ? 1 : s;
-}
-
 // Which kernel a product runs on, and the parts of K.
 enum class Form { TILE, LARGE, FEW };
 struct Plan {
   Form form;
   int64_t splits;
 };
-template <typename T>
-Plan plan_of(const Mat<T>& A, bool a_km, const Mat<T>& B, bool b_km, int64_t m, int64_t n,
-             int64_t k) {
-  if constexpr (sizeof(T) == 2) {
-    if (a_km && few_takes(A, B, m, n, k)) return Plan{Form::FEW, few_splits(n, k)};
-    if (ceil_div(m, 256) * ceil_div(n, 256) >= 200 && large_takes(A, a_km, B, b_km, m, n, k))
-      return Plan{Form::LARGE, 1};
+
+// About how many microseconds `splits` parts of K take, fitted to measured times (201 x 2880 x 5760 up
+// to 8192 x 7168 x 4096, within a quarter): a launch; a 256 x 256 tile's unit of 64 K takes a CU
+// 1.2, a 128 x 128 tile's step 0.73 where it has the CU to itself and 1.15 beside another (float32:
+// its MFMAs, 1.9 a tile); the parts' join is a launch and their sums written and read.
+double cost_of(Form form, bool f32, int64_t m, int64_t n, int64_t k, int64_t splits) {
+  const int64_t side = form == Form::LARGE ? 256 : TILE, bk = f32 ? 32 : 64;
+  const int64_t jobs = ceil_div(m, side) * ceil_div(n, side) * splits;
+  const double steps = static_cast<double>(ceil_div(ceil_div(k, bk), splits));
+  double t = 5;
+  if (form == Form::LARGE) {
+    t += static_cast<double>(ceil_div(jobs, 256)) * (1.2 * steps + 5);
+  } else if (f32) {
+    t += static_cast<double>(ceil_div(jobs, 256)) * (1.9 * steps + 1);
+  } else {
+    const int64_t pairs = jobs / 512, rest = jobs - 512 * pairs;
+    t += static_cast<double>(pairs) * (1.15 * steps + 2);
+    if (rest > 0) t += (rest > 256 ? 1.15 : 0.73) * steps + 2;
   }
-  return Plan{Form::TILE, splits_of(m, n, k, BK<T>)};
+  if (splits > 1) t += 2.5 + static_cast<double>(splits) * m * n * 8e-7;
+  return t;
+}
+// No part has no steps.
+int64_t whole_splits(int64_t steps, int64_t splits) {
+  return ceil_div(steps, ceil_div(steps, splits));
+}
+Plan plan_of(bool f32, bool large, bool few, int64_t m, int64_t n, int64_t k) {
+  if (few) return Plan{Form::FEW, few_splits(n, k)};
+  Plan best{Form::TILE, 1};
+  double least = 1e30;
+  for (const Form form : {Form::TILE, Form::LARGE}) {
+    if (form == Form::LARGE && !large) continue;
+    const int64_t side = form == Form::LARGE ? 256 : TILE;
+    const int64_t tiles = ceil_div(m, side) * ceil_div(n, side);
+    const int64_t steps = ceil_div(k, form == Form::TILE && f32 ? 32 : 64);
+    for (int64_t s = 1; s <= 32 && s <= steps && (s == 1 || s * tiles <= 768); s += s < 4 ? 1 : s / 4) {
+      const int64_t splits = steps > 0 ? whole_splits(steps, s) : 1;
+      const double t = cost_of(form, f32, m, n, k, splits);
+      if (t < least) {
+        least = t;
+        best = Plan{form, splits};
+      }
+    }
+  }
+  return best;
 }
 
-// What any form may ask for: the operands' alignment decides, which is not known here.
-template <typename T>
-size_t workspace_for(int64_t m, int64_t n, int64_t k) {
-  int64_t s = splits_of(m, n, k, BK<T>);
-  if (sizeof(T) == 2 && m <= 64 && few_splits(n, k) > s) s = few_splits(n, k);
-  return s == 1 ? 0 : static_cast<size_t>(s) * m * pitch_of(n) * sizeof(float);
+// What any form may ask for: the operands' alignment decides between them, which is not known here.
+size_t workspace_for(bool f32, int64_t m, int64_t n, int64_t k) {
+  int64_t most = plan_of(f32, false, false, m, n, k).splits;
+  if (!f32) {
+    const int64_t large = plan_of(f32, true, false, m, n, k).splits;
+    if (large > most) most = large;
+    if (m <= 64 && few_splits(n, k) > most) most = few_splits(n, k);
+  }
+  return most == 1 ? 0 : static_cast<size_t>(most) * m * pitch_of(n) * sizeof(float);
 }
 
 // m, n > 0.
 template <typename T, bool AKM, bool BKM, typename Epi>
 int run(const char* name, const Mat<T>& A, const Mat<T>& B, int64_t m, int64_t n, int64_t k,
         const Epi& epi, void* workspace, size_t workspace_bytes, hipStream_t s) {
-  const size_t need = workspace_for<T>(m, n, k);
+  const size_t need = workspace_for(sizeof(T) == 4, m, n, k);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(BUX_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes,
                 need);
   BUX_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: unaligned workspace", name);
-  const Plan plan = plan_of(A, AKM, B, BKM, m, n, k);
+  bool large = false, few = false;
+  if constexpr (sizeof(T) == 2) {
+    large = large_takes(A, AKM, B, BKM, m, n, k);
+    few = AKM && few_takes(A, B, m, n, k);
+  }
+  const Plan plan = plan_of(sizeof(T) == 4, large, few, m, n, k);
   const int64_t splits = plan.splits, pitch = pitch_of(n);
   auto launch = [&](const auto& e) {
     if constexpr (sizeof(T) == 2) {
@@ -452,25 +496,37 @@ __global__ __launch_bounds__(THREADS) void slope_kernel(const T* __restrict__ dy
   if (count > 0) {
     of_kind<false>(act.kind, [&](auto kind) {
       using K = decltype(kind);
-      for (int64_t r = static_cast<int64_t>(blockIdx.y) * rows + sub; r < m;
-           r += static_cast<int64_t>(gridDim.y) * rows) {
-        const Eight<T> g = load_eight(dy + r * n + col, count);
-        float v[8];
-        if constexpr (std::is_same<K, NoAct>::value) {
+      constexpr int TURN = 4;  // rows on their way at once
+      constexpr bool PLAIN = std::is_same<K, NoAct>::value;
+      const int64_t stride = static_cast<int64_t>(gridDim.y) * rows;
+      for (int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows + sub; r0 < m; r0 += TURN * stride) {
+        Eight<T> g[TURN], z[TURN];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = g.value(j);
-        } else {
-          const Eight<T> z = load_eight(product + r * n + col, count);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float dg, dw;
-            glu_unit_grad<K, sizeof(T) == 4>(act, z.value(j), 0.0f, 1.0f, g.value(j), &v[j], &dg,
-                                             &dw);
-          }
+        for (int i = 0; i < TURN; ++i) {
+          const int64_t r = r0 + i * stride;
+          g[i] = load_eight(dy + r * n + col, r < m ? count : 0);
+          if (!PLAIN) z[i] = load_eight(product + r * n + col, r < m ? count : 0);
         }
-        if (dz) store_some<T>(dz + r * n + col, v, count);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] += v[j];
+        for (int i = 0; i < TURN; ++i) {
+          const int64_t r = r0 + i * stride;
+          if (r >= m) break;
+          float v[8];
+          if constexpr (PLAIN) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = g[i].value(j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float dg, dw;
+              glu_unit_grad<K, sizeof(T) == 4>(act, z[i].value(j), 0.0f, 1.0f, g[i].value(j), &v[j],
+                                               &dg, &dw);
+            }
+          }
+          if (dz) store_some<T>(dz + r * n + col, v, count);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[j] += v[j];
+        }
       }
     });
   }
@@ -492,14 +548,24 @@ __global__ __launch_bounds__(THREADS) void slope_kernel(const T* __restrict__ dy
   }
 }
 
+// 64 columns a workgroup: its 4 waves take the runs in turn, and their sums meet in order.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void sums_kernel(const float* __restrict__ parts,
                                                        int64_t runs, int64_t n,
                                                        T* __restrict__ sums) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
-  if (c >= n) return;
+  __shared__ float red[THREADS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
   float v = 0.0f;
-  for (int64_t r = 0; r < runs; ++r) v += parts[r * n + c];
+  if (c < n) {
+#pragma unroll 8
+    for (int64_t r = wave; r < runs; r += THREADS / 64) v += parts[r * n + c];
+  }
+  red[threadIdx.x] = v;
+  __syncthreads();
+  if (wave != 0 || c >= n) return;
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) v += red[64 * w + lane];
   sums[c] = Elem<T>::make(v);
 }
 
@@ -529,7 +595,7 @@ int slope(const char* name, const T* dy, const T* product, const bux_ffn* ffn, i
                      dim3(THREADS), 0, s, dy, product, act, m, n, lanes, dz, sums, parts);
   if (int rc = launched("dense slope_kernel")) return rc;
   if (!sums || runs == 1) return BUX_OK;
-  hipLaunchKernelGGL(sums_kernel<T>, dim3(static_cast<unsigned>(ceil_div(n, THREADS))),
+  hipLaunchKernelGGL(sums_kernel<T>, dim3(static_cast<unsigned>(ceil_div(n, 64))),
                      dim3(THREADS), 0, s, parts, runs, n, sums);
   return launched("dense sums_kernel");
 }
@@ -540,7 +606,7 @@ int slope(const char* name, const T* dy, const T* product, const bux_ffn* ffn, i
 extern "C" size_t bux_dense_workspace_size(int64_t m, int64_t n, int64_t k) {
   using namespace bux;
   if (m <= 0 || n <= 0 || k <= 0) return 0;
-  const size_t a = workspace_for<uint16_t>(m, n, k), b = workspace_for<float>(m, n, k);
+  const size_t a = workspace_for(false, m, n, k), b = workspace_for(true, m, n, k);
   return a > b ? a : b;
 }
 extern "C" size_t bux_dense_slope_workspace_size(int64_t m, int64_t n) {
