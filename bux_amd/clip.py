@@ -4,6 +4,7 @@
 float32 in one list.
 """
 
+import ctypes
 from typing import NamedTuple, Sequence
 
 import torch
@@ -19,17 +20,21 @@ class Clipped(NamedTuple):
     norm: torch.Tensor  # float32 scalar: the global norm before the clipping
 
 
+_DTYPES = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
 def _list(name: str, grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None):
-    table = (_lib.GradientStruct * len(grads))()
-    dtypes = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+    """The gradients as ``bux_gradient``s, which are 4 words each."""
+    words = []
+    device = grads[0].device
     for i, g in enumerate(grads):
-        if g.dtype not in dtypes:
+        dtype = _DTYPES.get(g.dtype)
+        if dtype is None:
             raise TypeError(f"{name}: gradient {i} is bfloat16 or float32, not {g.dtype}")
-        if g.device != grads[0].device:
-            raise ValueError(f"{name}: gradient {i} on {g.device} beside {grads[0].device}")
-        table[i] = _lib.GradientStruct(ptr(g), None if outs is None else ptr(outs[i]), g.numel(),
-                                       dtypes[g.dtype])
-    return table
+        if g.device != device:
+            raise ValueError(f"{name}: gradient {i} on {g.device} beside {device}")
+        words += (g.data_ptr(), 0 if outs is None else outs[i].data_ptr(), g.numel(), dtype)
+    return ctypes.cast((ctypes.c_int64 * len(words))(*words), _lib.gradients)
 
 
 def _run(name: str, grads: Sequence[torch.Tensor], outs, max_norm: float) -> torch.Tensor:

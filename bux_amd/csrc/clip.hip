@@ -4,8 +4,8 @@
 //
 // The squares are added in float64: float32's would overflow above 1.8e19 and vanish below
 // 1e-23, and a sum over 10^9 of them would lose its last digits. The tensors are cut into pieces
-// of 8192 elements; a workgroup takes pieces in turn, each lane 8 elements a load at an element's
-// alignment, and leaves one sum. The second kernel's workgroups each add all those sums, in order
+// of 32 KiB; a workgroup takes pieces in turn, each lane 16 bytes a load at an element's alignment,
+// 8 of them on their way at once, and leaves one sum. The second kernel's workgroups each add all those sums, in order
 // (16 KiB at most, from L2), so that no atomics decide the order, and then scale their pieces,
 // the last ones first: those are what the first kernel left in the Infinity Cache.
 // Bound by HBM.
@@ -16,9 +16,11 @@ namespace bux {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int64_t PIECE = 8192;
-constexpr int ITEMS = 64;       // tensors a launch
-constexpr int64_t GROUPS = 2048;  // workgroups a launch: 8 a CU
+constexpr int64_t PIECE_BYTES = 32768;
+template <typename T>
+constexpr int64_t PIECE = PIECE_BYTES / sizeof(T);
+constexpr int ITEMS = 64;         // tensors a launch
+constexpr int64_t GROUPS = 1024;  // workgroups a launch: 4 a CU
 
 struct Item {
   const void* g;
@@ -26,14 +28,17 @@ struct Item {
   int64_t n;
   int64_t first;  // its first piece
 };
+// N: its items, for lists that hold fewer than ITEMS (a launch copies its arguments).
+template <int N>
 struct Table {
-  Item item[ITEMS];
+  Item item[N];
   uint64_t f32;  // which are float32
   int32_t count;
   int64_t pieces;
 };
 
 // Which item holds piece p: the last whose first is at most p.
+template <typename Table>
 __device__ __forceinline__ int item_of(const Table& t, int64_t p) {
   int lo = 0, hi = t.count;
   while (hi - lo > 1) {
@@ -44,27 +49,30 @@ __device__ __forceinline__ int item_of(const Table& t, int64_t p) {
   return lo;
 }
 
+// 16 bytes at an element's alignment.
 template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Eight {
-  T at[8];
+struct __attribute__((packed, aligned(sizeof(T)))) Chunk {
+  static constexpr int N = 16 / sizeof(T);
+  T at[N];
 };
 
-// f(element index, 8 values) for this lane's groups of 8 of the piece's elements [lo, hi), then
-// g(index, value) for the fewer than 8 left.
+// f(index, chunk) for this lane's chunks of the elements [lo, hi), a piece at most, then g(index,
+// value) for the elements left.
 template <typename T, typename F, typename G>
 __device__ __forceinline__ void over(const T* p, int64_t lo, int64_t hi, F&& f, G&& g) {
-  if (hi - lo == PIECE) {
-    Eight<T> e[PIECE / (8 * THREADS)];
+  constexpr int N = Chunk<T>::N, TURN = N * THREADS, TURNS = PIECE<T> / TURN;
+  if (hi - lo == PIECE<T>) {
+    Chunk<T> e[TURNS];
 #pragma unroll
-    for (int i = 0; i < PIECE / (8 * THREADS); ++i)
-      e[i] = *reinterpret_cast<const Eight<T>*>(p + lo + 8 * (i * THREADS + threadIdx.x));
+    for (int i = 0; i < TURNS; ++i)
+      e[i] = *reinterpret_cast<const Chunk<T>*>(p + lo + N * (i * THREADS + threadIdx.x));
 #pragma unroll
-    for (int i = 0; i < PIECE / (8 * THREADS); ++i) f(lo + 8 * (i * THREADS + threadIdx.x), e[i]);
+    for (int i = 0; i < TURNS; ++i) f(lo + N * (i * THREADS + threadIdx.x), e[i]);
     return;
   }
-  for (int64_t at = lo + 8 * threadIdx.x; at < hi; at += 8 * THREADS) {
-    if (at + 8 <= hi) {
-      f(at, *reinterpret_cast<const Eight<T>*>(p + at));
+  for (int64_t at = lo + N * threadIdx.x; at < hi; at += TURN) {
+    if (at + N <= hi) {
+      f(at, *reinterpret_cast<const Chunk<T>*>(p + at));
     } else {
       for (int64_t i = at; i < hi; ++i) g(i, p[i]);
     }
@@ -72,31 +80,41 @@ __device__ __forceinline__ void over(const T* p, int64_t lo, int64_t hi, F&& f, 
 }
 
 template <typename T>
-__device__ __forceinline__ double squares(const T* p, int64_t lo, int64_t hi) {
+__device__ __forceinline__ double squares(const void* from, int64_t piece, int64_t n) {
+  const T* const p = static_cast<const T*>(from);
+  const int64_t lo = piece * PIECE<T>, hi = lo + PIECE<T> < n ? lo + PIECE<T> : n;
   double s = 0.0;
+  auto add = [&](T x) {
+    const double v = Elem<T>::value(x);
+    s = __builtin_fma(v, v, s);
+  };
   over(p, lo, hi,
-       [&](int64_t, const Eight<T>& e) {
+       [&](int64_t, const Chunk<T>& e) {
 #pragma unroll
-         for (int j = 0; j < 8; ++j) {
-           const double v = Elem<T>::value(e.at[j]);
-           s = __builtin_fma(v, v, s);
-         }
+         for (int j = 0; j < Chunk<T>::N; ++j) add(e.at[j]);
        },
-       [&](int64_t, T x) {
-         const double v = Elem<T>::value(x);
-         s = __builtin_fma(v, v, s);
-       });
+       [&](int64_t, T x) { add(x); });
   return s;
 }
 
+typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+
 template <typename T>
-__device__ __forceinline__ void scale(const T* p, T* out, int64_t lo, int64_t hi, float factor) {
+__device__ __forceinline__ void scale(const void* from, void* to, int64_t piece, int64_t n,
+                                      float factor) {
+  const T* const p = static_cast<const T*>(from);
+  T* const out = static_cast<T*>(to);
+  const int64_t lo = piece * PIECE<T>, hi = lo + PIECE<T> < n ? lo + PIECE<T> : n;
   over(p, lo, hi,
-       [&](int64_t at, const Eight<T>& e) {
-         Eight<T> r;
+       [&](int64_t at, const Chunk<T>& e) {
+         // Stored past the caches: nothing here reads it again, and what the squares left is still
+         // to be read.
+         Chunk<T> r;
 #pragma unroll
-         for (int j = 0; j < 8; ++j) r.at[j] = Elem<T>::make(Elem<T>::value(e.at[j]) * factor);
-         *reinterpret_cast<Eight<T>*>(out + at) = r;
+         for (int j = 0; j < Chunk<T>::N; ++j)
+           r.at[j] = Elem<T>::make(Elem<T>::value(e.at[j]) * factor);
+         __builtin_nontemporal_store(__builtin_bit_cast(Words, r),
+                                     reinterpret_cast<Words*>(out + at));
        },
        [&](int64_t at, T x) { out[at] = Elem<T>::make(Elem<T>::value(x) * factor); });
 }
@@ -113,15 +131,15 @@ __device__ __forceinline__ double group_sum(double v, double* red) {
   return t;
 }
 
+template <typename Table>
 __global__ __launch_bounds__(THREADS) void squares_kernel(Table t, double* __restrict__ sums) {
   __shared__ double red[THREADS / 64];
   double s = 0.0;
   for (int64_t p = blockIdx.x; p < t.pieces; p += gridDim.x) {
     const int i = item_of(t, p);
-    const int64_t lo = (p - t.item[i].first) * PIECE;
-    const int64_t hi = lo + PIECE < t.item[i].n ? lo + PIECE : t.item[i].n;
-    if ((t.f32 >> i) & 1) s += squares(static_cast<const float*>(t.item[i].g), lo, hi);
-    else s += squares(static_cast<const uint16_t*>(t.item[i].g), lo, hi);
+    const Item& it = t.item[i];
+    if ((t.f32 >> i) & 1) s += squares<float>(it.g, p - it.first, it.n);
+    else s += squares<uint16_t>(it.g, p - it.first, it.n);
   }
   s = group_sum(s, red);
   if (threadIdx.x == 0) sums[blockIdx.x] = s;
@@ -141,6 +159,7 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(const double* __restrict_
   if (threadIdx.x == 0) *norm = static_cast<float>(v);
 }
 
+template <typename Table>
 __global__ __launch_bounds__(THREADS) void scale_kernel(Table t, const double* __restrict__ sums,
                                                         int64_t count, float max_norm,
                                                         float* __restrict__ norm) {
@@ -152,34 +171,61 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(Table t, const double* _
   for (int64_t q = blockIdx.x; q < t.pieces; q += gridDim.x) {
     const int64_t p = t.pieces - 1 - q;
     const int i = item_of(t, p);
-    const int64_t lo = (p - t.item[i].first) * PIECE;
-    const int64_t hi = lo + PIECE < t.item[i].n ? lo + PIECE : t.item[i].n;
-    if ((t.f32 >> i) & 1)
-      scale(static_cast<const float*>(t.item[i].g), static_cast<float*>(t.item[i].out), lo, hi,
-            factor);
-    else
-      scale(static_cast<const uint16_t*>(t.item[i].g), static_cast<uint16_t*>(t.item[i].out), lo,
-            hi, factor);
+    const Item& it = t.item[i];
+    if ((t.f32 >> i) & 1) scale<float>(it.g, it.out, p - it.first, it.n, factor);
+    else scale<uint16_t>(it.g, it.out, p - it.first, it.n, factor);
   }
 }
 
 // The launch's tensors from `at` on (empty ones left out); where the next launch's begin.
-int32_t table_of(const bux_gradient* grads, int32_t count, int32_t at, Table* t) {
+template <int N>
+int32_t table_of(const bux_gradient* grads, int32_t count, int32_t at, Table<N>* t) {
   t->count = 0;
   t->pieces = 0;
   t->f32 = 0;
-  for (; at < count && t->count < ITEMS; ++at) {
+  for (; at < count && t->count < N; ++at) {
     const bux_gradient& g = grads[at];
     if (g.n == 0) continue;
     t->item[t->count] = Item{g.g, g.out, g.n, t->pieces};
     if (g.dtype == BUX_F32) t->f32 |= 1ull << t->count;
-    t->pieces += ceil_div(g.n, PIECE);
+    t->pieces += ceil_div(g.n, PIECE_BYTES / (g.dtype == BUX_F32 ? 4 : 2));
     ++t->count;
   }
   return at;
 }
-unsigned groups_of(const Table& t) {
+template <int N>
+unsigned groups_of(const Table<N>& t) {
   return static_cast<unsigned>(t.pieces < GROUPS ? t.pieces : GROUPS);
+}
+
+// N: a launch's tensors.
+template <int N>
+int clip(const bux_gradient* grads, int32_t count, bool clips, float max_norm, float* norm,
+         double* sums, hipStream_t s) {
+  Table<N> t;
+  int64_t made = 0;
+  for (int32_t at = 0; at < count;) {
+    at = table_of(grads, count, at, &t);
+    if (t.count == 0) break;
+    hipLaunchKernelGGL(squares_kernel<Table<N>>, dim3(groups_of(t)), dim3(THREADS), 0, s, t,
+                       sums + made);
+    if (int rc = launched("squares_kernel")) return rc;
+    made += groups_of(t);
+  }
+  if (!clips) {
+    hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(THREADS), 0, s, sums, made, norm);
+    return launched("norm_kernel");
+  }
+  float* to = norm;
+  for (int32_t at = 0; at < count;) {
+    at = table_of(grads, count, at, &t);
+    if (t.count == 0) break;
+    hipLaunchKernelGGL(scale_kernel<Table<N>>, dim3(groups_of(t)), dim3(THREADS), 0, s, t, sums,
+                       made, max_norm, to);
+    if (int rc = launched("scale_kernel")) return rc;
+    to = nullptr;
+  }
+  return BUX_OK;
 }
 
 }  // namespace
@@ -217,28 +263,7 @@ extern "C" int bux_clip(const bux_gradient* grads, int32_t count, float max_norm
   BUX_CHECK(reinterpret_cast<uintptr_t>(workspace) % 8 == 0, "%s: unaligned workspace", name);
   double* const sums = static_cast<double*>(workspace);
   hipStream_t s = as_stream(stream);
-  Table t;
-  int64_t made = 0;
-  int32_t at = 0;
-  while (at < count) {
-    at = table_of(grads, count, at, &t);
-    if (t.count == 0) break;
-    hipLaunchKernelGGL(squares_kernel, dim3(groups_of(t)), dim3(THREADS), 0, s, t, sums + made);
-    if (int rc = launched("squares_kernel")) return rc;
-    made += groups_of(t);
-  }
-  if (!clips) {
-    hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(THREADS), 0, s, sums, made, norm);
-    return launched("norm_kernel");
-  }
-  float* to = norm;
-  for (at = 0; at < count;) {
-    at = table_of(grads, count, at, &t);
-    if (t.count == 0) break;
-    hipLaunchKernelGGL(scale_kernel, dim3(groups_of(t)), dim3(THREADS), 0, s, t, sums, made,
-                       max_norm, to);
-    if (int rc = launched("scale_kernel")) return rc;
-    to = nullptr;
-  }
-  return BUX_OK;
+  // (a list of empty tensors alone has the norm 0 and nothing to scale)
+  return count <= 8 ? clip<8>(grads, count, clips, max_norm, norm, sums, s)
+                    : clip<ITEMS>(grads, count, clips, max_norm, norm, sums, s);
 }

@@ -292,8 +292,8 @@ struct Plan {
 
 // About how many microseconds `splits` parts of K take, fitted to measured times (201 x 2880 x 5760 up
 // to 8192 x 7168 x 4096, within a quarter): a launch; a 256 x 256 tile's unit of 64 K takes a CU
-// 1.2, a 128 x 128 tile's step 0.73 where it has the CU to itself and 1.15 beside another (float32:
-// its MFMAs, 1.9 a tile); the parts' join is a launch and their sums written and read.
+// 1.2, a 128 x 128 tile's step 0.73 where it has the CU to itself and 1.15 beside another (float32: 2.7
+// and 4.1, its MFMAs); the parts' join is a launch and their sums written and read.
 double cost_of(Form form, bool f32, int64_t m, int64_t n, int64_t k, int64_t splits) {
   const int64_t side = form == Form::LARGE ? 256 : TILE, bk = f32 ? 32 : 64;
   const int64_t jobs = ceil_div(m, side) * ceil_div(n, side) * splits;
@@ -301,12 +301,11 @@ double cost_of(Form form, bool f32, int64_t m, int64_t n, int64_t k, int64_t spl
   double t = 5;
   if (form == Form::LARGE) {
     t += static_cast<double>(ceil_div(jobs, 256)) * (1.2 * steps + 5);
-  } else if (f32) {
-    t += static_cast<double>(ceil_div(jobs, 256)) * (1.9 * steps + 1);
   } else {
+    const double alone = f32 ? 2.7 : 0.73, beside = f32 ? 4.1 : 1.15;
     const int64_t pairs = jobs / 512, rest = jobs - 512 * pairs;
-    t += static_cast<double>(pairs) * (1.15 * steps + 2);
-    if (rest > 0) t += (rest > 256 ? 1.15 : 0.73) * steps + 2;
+    t += static_cast<double>(pairs) * (beside * steps + 2);
+    if (rest > 0) t += (rest > 256 ? beside : alone) * steps + 2;
   }
   if (splits > 1) t += 2.5 + static_cast<double>(splits) * m * n * 8e-7;
   return t;
