@@ -70,23 +70,49 @@ __device__ __forceinline__ void store_some(T* p, const float* v, int64_t count) 
 }
 
 struct NoAct {};
-// Calls f(Kind<kind, GATED>{}), or f(NoAct{}) for none: a branch that every lane takes alike.
-template <bool GATED, typename F>
+// An activation's kind, and whether its up branch is neither clipped nor capped: known where it
+// runs, so that the units a lane makes at once have no branches between them.
+template <int KIND, bool GATED, bool BARE>
+struct Choice {
+  using K = Kind<KIND, GATED>;
+  static __device__ __forceinline__ Act of(const Act& act) {
+    Act a = act;
+    if (BARE) a.clamped = a.capped = 0;
+    return a;
+  }
+};
+// Calls f(Choice<kind, GATED, ..>{}), or f(NoAct{}) for none: a branch that every lane takes alike.
+template <bool GATED, bool BARE, typename F>
 __device__ __forceinline__ void of_kind(int kind, F&& f) {
   switch (kind) {
-    case BUX_SWISH: f(Kind<BUX_SWISH, GATED>{}); break;
-    case BUX_QUICK_GELU: f(Kind<BUX_QUICK_GELU, GATED>{}); break;
-    case BUX_RELU: f(Kind<BUX_RELU, GATED>{}); break;
-    case BUX_RELU2: f(Kind<BUX_RELU2, GATED>{}); break;
-    case BUX_GELU: f(Kind<BUX_GELU, GATED>{}); break;
-    case BUX_GELU_TANH: f(Kind<BUX_GELU_TANH, GATED>{}); break;
-    case BUX_SIGMOID: f(Kind<BUX_SIGMOID, GATED>{}); break;
-    case BUX_TANH: f(Kind<BUX_TANH, GATED>{}); break;
-    case BUX_SOFTPLUS: f(Kind<BUX_SOFTPLUS, GATED>{}); break;
-    case BUX_SITU: f(Kind<BUX_SITU, GATED>{}); break;
+    case BUX_SWISH: f(Choice<BUX_SWISH, GATED, BARE>{}); break;
+    case BUX_QUICK_GELU: f(Choice<BUX_QUICK_GELU, GATED, BARE>{}); break;
+    case BUX_RELU: f(Choice<BUX_RELU, GATED, BARE>{}); break;
+    case BUX_RELU2: f(Choice<BUX_RELU2, GATED, BARE>{}); break;
+    case BUX_GELU: f(Choice<BUX_GELU, GATED, BARE>{}); break;
+    case BUX_GELU_TANH: f(Choice<BUX_GELU_TANH, GATED, BARE>{}); break;
+    case BUX_SIGMOID: f(Choice<BUX_SIGMOID, GATED, BARE>{}); break;
+    case BUX_TANH: f(Choice<BUX_TANH, GATED, BARE>{}); break;
+    case BUX_SOFTPLUS: f(Choice<BUX_SOFTPLUS, GATED, BARE>{}); break;
+    case BUX_SITU: f(Choice<BUX_SITU, GATED, BARE>{}); break;
     default:
-      if constexpr (!GATED) f(NoAct{});
+      if constexpr (!GATED && BARE) f(NoAct{});
   }
+}
+template <bool GATED, typename F>
+__device__ __forceinline__ void of_act(const Act& act, F&& f) {
+  if (act.clamped || act.capped) of_kind<GATED, false>(act.kind, f);
+  else of_kind<GATED, true>(act.kind, f);
+}
+template <typename C, bool F32>
+__device__ __forceinline__ float unit_of(const Act& act, float up, float gate) {
+  return glu_unit<typename C::K, F32>(C::of(act), up, gate, 1.0f);
+}
+template <typename C, bool F32>
+__device__ __forceinline__ void unit_grad_of(const Act& act, float up, float gate, float dh,
+                                             float* d_up, float* d_gate) {
+  float dw;
+  glu_unit_grad<typename C::K, F32>(C::of(act), up, gate, 1.0f, dh, d_up, d_gate, &dw);
 }
 
 // --- whole tiles ---------------------------------------------------------------------------
@@ -195,14 +221,14 @@ struct Forward {
     if constexpr (GATED) {
       float h[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) h[j] = glu_unit<K, F32>(act, v[2 * j], v[2 * j + 1], 1.0f);
+      for (int j = 0; j < 4; ++j) h[j] = unit_of<K, F32>(act, v[2 * j], v[2 * j + 1]);
       __builtin_amdgcn_raw_buffer_store_b64(
           words2{pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])}, t.out.rsrc, t.out.lane,
           scalar_in<4>(t.out, row, col), NON_TEMPORAL);
     } else {
       if constexpr (!std::is_same<K, NoAct>::value) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = glu_unit<K, F32>(act, v[j], 0.0f, 1.0f);
+        for (int j = 0; j < 8; ++j) v[j] = unit_of<K, F32>(act, v[j], 0.0f);
       }
       if (residual) {
 #pragma unroll
@@ -223,7 +249,7 @@ struct Forward {
   }
   template <typename F>
   __device__ __forceinline__ void choose(F&& f) const {
-    of_kind<GATED>(act.kind, f);
+    of_act<GATED>(act, f);
   }
   template <typename K>
   __device__ __forceinline__ void store(K, int64_t row, int64_t col, const float v[8],
@@ -241,12 +267,12 @@ struct Forward {
     if constexpr (GATED) {
       float h[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) h[j] = glu_unit<K, F32>(act, z[2 * j], z[2 * j + 1], 1.0f);
+      for (int j = 0; j < 4; ++j) h[j] = unit_of<K, F32>(act, z[2 * j], z[2 * j + 1]);
       store_some<T, 4>(out + row * (n / 2) + col / 2, h, count / 2);
     } else {
       if constexpr (!std::is_same<K, NoAct>::value) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = glu_unit<K, F32>(act, z[j], 0.0f, 1.0f);
+        for (int j = 0; j < 8; ++j) z[j] = unit_of<K, F32>(act, z[j], 0.0f);
       }
       if (residual) {
 #pragma unroll
@@ -296,10 +322,10 @@ struct Backward {
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float du, dg, dw;
+        float du, dg;
         const float up = half_of(f.p[j * P / 8], j * P % 8);
         const float gate = GATED ? half_of(f.p[j * P / 8], j * P % 8 + 1) : 0.0f;
-        glu_unit_grad<K, F32>(act, up, gate, 1.0f, v[j], &du, &dg, &dw);
+        unit_grad_of<K, F32>(act, up, gate, v[j], &du, &dg);
         d[j * P] = du;
         if (GATED) d[j * P + 1] = dg;
       }
@@ -322,7 +348,7 @@ struct Backward {
   }
   template <typename F>
   __device__ __forceinline__ void choose(F&& f) const {
-    of_kind<GATED>(act.kind, f);
+    of_act<GATED>(act, f);
   }
   template <typename K>
   __device__ __forceinline__ void store(K, int64_t row, int64_t col, const float v[8],
@@ -334,10 +360,10 @@ struct Backward {
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float du, dg, dw;
+        float du, dg;
         const float up = in.p[j * P / 8].value(j * P % 8);
         const float gate = GATED ? in.p[j * P / 8].value(j * P % 8 + 1) : 0.0f;
-        glu_unit_grad<K, F32>(act, up, gate, 1.0f, v[j], &du, &dg, &dw);
+        unit_grad_of<K, F32>(act, up, gate, v[j], &du, &dg);
         d[j * P] = du;
         if (GATED) d[j * P + 1] = dg;
       }

@@ -493,7 +493,7 @@ __global__ __launch_bounds__(THREADS) void slope_kernel(const T* __restrict__ dy
   const int64_t col = (static_cast<int64_t>(blockIdx.x) * lanes + lane) * 8, count = n - col;
   float sum[8] = {};
   if (count > 0) {
-    of_kind<false>(act.kind, [&](auto kind) {
+    of_act<false>(act, [&](auto kind) {
       using K = decltype(kind);
       constexpr int TURN = 4;  // rows on their way at once
       constexpr bool PLAIN = std::is_same<K, NoAct>::value;
@@ -517,9 +517,8 @@ __global__ __launch_bounds__(THREADS) void slope_kernel(const T* __restrict__ dy
           } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              float dg, dw;
-              glu_unit_grad<K, sizeof(T) == 4>(act, z[i].value(j), 0.0f, 1.0f, g[i].value(j), &v[j],
-                                               &dg, &dw);
+              float dg;
+              unit_grad_of<K, sizeof(T) == 4>(act, z[i].value(j), 0.0f, g[i].value(j), &v[j], &dg);
             }
           }
           if (dz) store_some<T>(dz + r * n + col, v, count);
