@@ -119,7 +119,10 @@ __device__ __forceinline__ void unit_grad_of(const Act& act, float up, float gat
 //
 // A tile that lies inside outputs of whole, aligned 16 bytes moves its values at 32-bit offsets
 // from its corner, without a check a chunk: a lane's own offset (row l / 8, columns 8 (l % 8) of a
-// unit, below) and a scalar one. Stores are non-temporal: another kernel reads them, and they would
+// unit, below) and a scalar one. Where 8 columns are 32 bytes (HALVES) a lane takes columns 4 (l % 8)
+// of the unit's two halves instead, so that 8 lanes store 128 bytes in a row. (Stores of every other
+// 16 bytes, past the caches, took 184 of the 627 us of the gated block's gradient of 16384 x 8192
+// units.) Stores are non-temporal: another kernel reads them, and they would
 // push the operands out of L2.
 
 typedef uint32_t words4 __attribute__((ext_vector_type(4)));
@@ -131,7 +134,7 @@ struct Place {
   int32_t lane;   // bytes
   int32_t pitch;  // bytes a row
 };
-// `columns` elements a chunk of 8 columns of sums (8, 4 of a gated act's units, 16 of its pairs).
+// `COLUMNS` elements to 8 columns of sums (8, 4 of a gated act's units, 16 of its pairs).
 template <int COLUMNS>
 __device__ __forceinline__ Place place_in(const uint16_t* p, int64_t row, int64_t col, int64_t n) {
   const int lane = threadIdx.x & 63;
@@ -140,9 +143,10 @@ __device__ __forceinline__ Place place_in(const uint16_t* p, int64_t row, int64_
   r.rsrc = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint16_t*>(p) + row * ld + col * COLUMNS / 8, 0, 0x7fffffff, 0x00020000);
   r.pitch = static_cast<int32_t>(ld) * 2;
-  r.lane = (lane >> 3) * r.pitch + (lane & 7) * COLUMNS * 2;
+  r.lane = (lane >> 3) * r.pitch + (lane & 7) * (COLUMNS == 16 ? 16 : COLUMNS * 2);
   return r;
 }
+constexpr int HALF = 128;  // bytes from a lane's first 16 to its second, where COLUMNS is 16
 template <int COLUMNS>
 __device__ __forceinline__ int32_t scalar_in(const Place& p, int row, int col) {
   return row * p.pitch + col * COLUMNS / 8 * 2;
@@ -165,6 +169,7 @@ __device__ __forceinline__ bool aligned16(const void* p, int64_t columns) {
 
 template <typename T, bool GATED>
 struct Forward {
+  static constexpr bool HALVES = false;
   static constexpr bool F32 = sizeof(T) == 4;
   Act act;  // kind NO_ACT: none
   const T* bias;
@@ -287,6 +292,7 @@ template <typename T, bool GATED>
 struct Backward {
   static constexpr bool F32 = sizeof(T) == 4;
   static constexpr int P = GATED ? 2 : 1;
+  static constexpr bool HALVES = GATED;
   Act act;
   const T* product;  // [m, n, P]
   T* out;            // the same
@@ -309,7 +315,7 @@ struct Backward {
 #pragma unroll
     for (int i = 0; i < P; ++i)
       f.p[i] = __builtin_amdgcn_raw_buffer_load_b128(
-          t.product.rsrc, t.product.lane + 16 * i, scalar_in<8 * P>(t.product, row, col), 0);
+          t.product.rsrc, t.product.lane + HALF * i, scalar_in<8 * P>(t.product, row, col), 0);
     return f;
   }
   template <typename K>
@@ -332,7 +338,7 @@ struct Backward {
     }
 #pragma unroll
     for (int i = 0; i < P; ++i)
-      __builtin_amdgcn_raw_buffer_store_b128(packed8(d + 8 * i), t.out.rsrc, t.out.lane + 16 * i,
+      __builtin_amdgcn_raw_buffer_store_b128(packed8(d + 8 * i), t.out.rsrc, t.out.lane + HALF * i,
                                              scalar_in<8 * P>(t.out, row, col), NON_TEMPORAL);
   }
 
@@ -376,6 +382,7 @@ struct Backward {
 
 // The workspace's rows are whole 8s of columns, `pitch`.
 struct Partial {
+  static constexpr bool HALVES = true;
   float* out;
   int64_t pitch;
   struct Tile {
@@ -397,7 +404,7 @@ struct Partial {
       __builtin_amdgcn_raw_buffer_store_b128(
           words4{__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
                  __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])},
-          t.out.rsrc, t.out.lane + 16 * i, at, 0);
+          t.out.rsrc, t.out.lane + HALF * i, at, 0);
   }
   struct In {};
   __device__ __forceinline__ In load(int64_t, int64_t) const { return In{}; }
@@ -441,10 +448,13 @@ __device__ __forceinline__ void put_unit(uint8_t* region, const f32x16& c0, cons
           make_float4(a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]);
   }
 }
+// (HALVES: columns 4 (l % 8) and 32 + 4 (l % 8).)
+template <bool HALVES = false>
 __device__ __forceinline__ void get_row(const uint8_t* region, int it, float v[8]) {
-  const int lane = threadIdx.x & 63, r = (lane >> 3) + 8 * it, c = 2 * (lane & 7);
+  const int lane = threadIdx.x & 63, r = (lane >> 3) + 8 * it;
+  const int c = HALVES ? lane & 7 : 2 * (lane & 7), d = HALVES ? c + 8 : c + 1;
   const float4 x = *reinterpret_cast<const float4*>(region + r * 256 + 16 * (c ^ (r & 15)));
-  const float4 y = *reinterpret_cast<const float4*>(region + r * 256 + 16 * ((c + 1) ^ (r & 15)));
+  const float4 y = *reinterpret_cast<const float4*>(region + r * 256 + 16 * (d ^ (r & 15)));
   v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
   v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
 }

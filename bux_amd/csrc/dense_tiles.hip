@@ -361,8 +361,10 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
     // units 2 p .. 2 p + 4 of pair p
     uint32_t s0 = slot(0), s1 = slot(1), s2 = slot(2), s3 = slot(3), s4 = slot(4);
     Frag cur, nxt;
-    wait_units<2>();
-    barrier_lds();
+    if (ahead == 0) {  // (a later tile's units 0 and 1 landed before the last one's epilogue)
+      wait_units<2>();
+      barrier_lds();
+    }
     {
       const Reader<AKM, BKM, 0> r(ra, rb, s0, s1);
 #pragma unroll
@@ -400,6 +402,9 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
       step<BKM, false, false>(nxt, cur, fb, 0, 0, Reader<AKM, BKM, 0>(ra, rb, s2, s3), acc);
     }
     settled(acc);
+    // The next tile's units 0 and 1 have landed, so that its first step need not wait for the stores
+    // that follow.
+    wait_units<1>();
     // The last pair's slots are free (every wave has read them before the last barrier): 16 KiB of
     // them a wave for the outputs.
     uint8_t* const r0 = lds + (base + 2 * pairs - 2) % SLOTS * SLOT + wave * UNIT_BYTES;
@@ -428,7 +433,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(1, 1)))
         }
         float v[4][8];
 #pragma unroll
-        for (int it = 0; it < 4; ++it) get_row(u & 1 ? r1 : r0, it, v[it]);
+        for (int it = 0; it < 4; ++it) get_row<Epi::HALVES>(u & 1 ? r1 : r0, it, v[it]);
         out.choose([&](auto kind) {
 #pragma unroll
           for (int it = 0; it < 4; ++it) out.store_fast(kind, t, r + 8 * it, c, v[it], now[it]);
