@@ -182,11 +182,11 @@ SIGNATURES = {
                _p, _p, _p, _p, _p, _size, _p]),
     "bux_dense_workspace_size": (_size, [_i64, _i64, _i64]),
     "bux_dense_rows": (
-        _int, [_p, _p, _int, _i64, _i64, _i64, _p, _ffn, _p, _p, _p, _p, _size, _p]),
+        _int, [_p, _p, _int, _i64, _i64, _i64, _p, _ffn, _p, _p, _p, _p, _p, _size, _p]),
     "bux_dense_rows_f32": (
         _int, [_p, _p, _int, _i64, _i64, _i64, _p, _ffn, _p, _p, _p, _p, _size, _p]),
     "bux_dense_units_backward": (
-        _int, [_p, _p, _i64, _i64, _i64, _p, _ffn, _p, _p, _size, _p]),
+        _int, [_p, _p, _i64, _i64, _i64, _p, _p, _ffn, _p, _p, _size, _p]),
     "bux_dense_units_backward_f32": (
         _int, [_p, _p, _i64, _i64, _i64, _p, _ffn, _p, _p, _size, _p]),
     "bux_dense_contract": (_int, [_p, _p, _i64, _i64, _i64, _p, _p, _size, _p]),

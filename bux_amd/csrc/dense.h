@@ -4,6 +4,7 @@
 //   Forward   z = v + bias (kept as `product`, if asked for);  out = act(z) + residual, where a
 //             gated act takes the columns as (up, gate) pairs and gives half as many
 //   Backward  v is the gradient dh of the activation's output: dp = dh d act(product)
+//             (bfloat16: from 24 bits of each value, where its low bytes were kept too)
 //   Partial   v as it is, to a split's own place in the workspace
 //
 // act runs in float32 on the sums themselves, before their rounding: `product` is rounded only
@@ -66,6 +67,53 @@ __device__ __forceinline__ void store_some(T* p, const float* v, int64_t count) 
 #pragma unroll
     for (int j = 0; j < N; ++j)
       if (j < count) p[j] = s.at[j];
+  }
+}
+
+// --- a bfloat16 value's next 8 bits ---------------------------------------------------------
+//
+// z kept as bfloat16 alone would put a rounding of 2^-9 of it into the activation's gradient beside
+// the one that d product takes to be multiplied: of a block's gradients to x and up sqrt 3 rather
+// than sqrt 2 of their outputs' own. A signed byte beside it, the difference of the float32's bits
+// from the bfloat16's in units of 2^8, keeps 16 bits of mantissa, at half the bytes that float32 would
+// add. (A value that rounds to infinity comes back finite; a NaN stays one.)
+
+__device__ __forceinline__ uint32_t low_byte(float z, uint32_t high) {
+  const int32_t off = static_cast<int32_t>(__float_as_uint(z)) - static_cast<int32_t>(high << 16);
+  const int32_t b = (off + 128) >> 8;
+  return static_cast<uint32_t>(b < -128 ? -128 : b > 127 ? 127 : b) & 0xffu;
+}
+// 8 values' low bytes, the first lowest; `high`: their bfloat16s, in pairs.
+__device__ __forceinline__ uint64_t low_bytes(const float v[8], const uint32_t high[4]) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    w[j / 4] |= low_byte(v[j], j & 1 ? high[j / 2] >> 16 : high[j / 2] & 0xffffu) << (8 * (j % 4));
+  return static_cast<uint64_t>(w[1]) << 32 | w[0];
+}
+__device__ __forceinline__ float with_low(float z, uint64_t low, int j) {
+  const uint32_t w = static_cast<uint32_t>(j < 4 ? low : low >> 32);
+  const int32_t b = static_cast<int32_t>(w << (24 - 8 * (j & 3))) >> 24;
+  return __uint_as_float(__float_as_uint(z) + (static_cast<uint32_t>(b) << 8));
+}
+__device__ __forceinline__ uint64_t load_low(const uint8_t* p, int64_t count) {
+  uint64_t v = 0;
+  if (count >= 8) {
+    __builtin_memcpy(&v, p, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) v |= static_cast<uint64_t>(p[j]) << (8 * j);
+  }
+  return v;
+}
+__device__ __forceinline__ void store_low(uint8_t* p, uint64_t v, int64_t count) {
+  if (count >= 8) {
+    __builtin_memcpy(p, &v, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) p[j] = static_cast<uint8_t>(v >> (8 * j));
   }
 }
 
@@ -147,6 +195,18 @@ __device__ __forceinline__ Place place_in(const uint16_t* p, int64_t row, int64_
   return r;
 }
 constexpr int HALF = 128;  // bytes from a lane's first 16 to its second, where COLUMNS is 16
+// As many bytes, one an element, of COLUMNS (8 or 16) elements.
+template <int COLUMNS>
+__device__ __forceinline__ Place bytes_in(const uint8_t* p, int64_t row, int64_t col, int64_t n) {
+  const int lane = threadIdx.x & 63;
+  const int64_t ld = n * COLUMNS / 8;
+  Place r;
+  r.rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(p) + row * ld + col * COLUMNS / 8, 0, 0x7fffffff, 0x00020000);
+  r.pitch = static_cast<int32_t>(ld);
+  r.lane = (lane >> 3) * r.pitch + (lane & 7) * 8;
+  return r;
+}
 template <int COLUMNS>
 __device__ __forceinline__ int32_t scalar_in(const Place& p, int row, int col) {
   return row * p.pitch + col * COLUMNS / 8 * 2;
@@ -175,11 +235,12 @@ struct Forward {
   const T* bias;
   const T* residual;  // (a gated act has none)
   T* product;
+  uint8_t* low;  // product's low bytes (bfloat16)
   T* out;
   int64_t n;  // columns of the sums
 
   struct Tile {
-    Place out, product, residual;
+    Place out, product, low, residual;
     words4 bias[2];  // of a wave's two units of 64 columns
   };
   struct Fast {
@@ -189,6 +250,7 @@ struct Forward {
   __device__ __forceinline__ bool aligned() const {
     return aligned16(out, GATED ? n / 2 : n) && n % 8 == 0 && n < (1 << 20) &&
            (product == nullptr || aligned16(product, n)) &&
+           (low == nullptr || reinterpret_cast<uintptr_t>(low) % 8 == 0) &&
            (residual == nullptr || aligned16(residual, n)) &&
            (bias == nullptr || aligned16(bias, n));
   }
@@ -196,6 +258,7 @@ struct Forward {
     Tile t;
     t.out = place_in<GATED ? 4 : 8>(out, row, col, n);
     t.product = place_in<8>(product, row, col, n);
+    t.low = bytes_in<8>(low, row, col, n);
     t.residual = place_in<8>(residual, row, col, n);
     const int c = 8 * (threadIdx.x & 7);
     if (bias) {
@@ -220,9 +283,17 @@ struct Forward {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += half_of(b, j);
     }
-    if (product)
-      __builtin_amdgcn_raw_buffer_store_b128(packed8(v), t.product.rsrc, t.product.lane,
+    if (product) {
+      const words4 z = packed8(v);
+      __builtin_amdgcn_raw_buffer_store_b128(z, t.product.rsrc, t.product.lane,
                                              scalar_in<8>(t.product, row, col), NON_TEMPORAL);
+      if (low) {
+        const uint32_t high[4] = {z.x, z.y, z.z, z.w};
+        __builtin_amdgcn_raw_buffer_store_b64(
+            __builtin_bit_cast(words2, low_bytes(v, high)), t.low.rsrc, t.low.lane,
+            row * t.low.pitch + col, NON_TEMPORAL);
+      }
+    }
     if constexpr (GATED) {
       float h[4];
 #pragma unroll
@@ -269,6 +340,14 @@ struct Forward {
       for (int j = 0; j < 8; ++j) z[j] += b.value(j);
     }
     if (product) store_some<T>(product + row * n + col, z, count);
+    if constexpr (!F32) {
+      if (low) {
+        uint32_t high[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) high[j] = pack_bf16x2(z[2 * j], z[2 * j + 1]);
+        store_low(low + row * n + col, low_bytes(z, high), count);
+      }
+    }
     if constexpr (GATED) {
       float h[4];
 #pragma unroll
@@ -294,21 +373,25 @@ struct Backward {
   static constexpr int P = GATED ? 2 : 1;
   static constexpr bool HALVES = GATED;
   Act act;
-  const T* product;  // [m, n, P]
-  T* out;            // the same
+  const T* product;    // [m, n, P]
+  const uint8_t* low;  // its low bytes (bfloat16), or NULL
+  T* out;              // product's shape
   int64_t n;         // units
 
   struct Tile {
-    Place out, product;
+    Place out, product, low;
   };
   struct Fast {
     words4 p[P];
+    words2 low[P];
   };
   __device__ __forceinline__ bool aligned() const {
-    return aligned16(out, n) && aligned16(product, n) && n < (1 << 20);
+    return aligned16(out, n) && aligned16(product, n) && n < (1 << 20) &&
+           (low == nullptr || reinterpret_cast<uintptr_t>(low) % 8 == 0);
   }
   __device__ __forceinline__ Tile tile(int64_t row, int64_t col) const {
-    return Tile{place_in<8 * P>(out, row, col, n), place_in<8 * P>(product, row, col, n)};
+    return Tile{place_in<8 * P>(out, row, col, n), place_in<8 * P>(product, row, col, n),
+                bytes_in<8 * P>(low, row, col, n)};
   }
   __device__ __forceinline__ Fast fast(const Tile& t, int row, int col) const {
     Fast f;
@@ -316,6 +399,12 @@ struct Backward {
     for (int i = 0; i < P; ++i)
       f.p[i] = __builtin_amdgcn_raw_buffer_load_b128(
           t.product.rsrc, t.product.lane + HALF * i, scalar_in<8 * P>(t.product, row, col), 0);
+    if (low) {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        f.low[i] = __builtin_amdgcn_raw_buffer_load_b64(t.low.rsrc, t.low.lane + HALF / 2 * i,
+                                                        row * t.low.pitch + col * P, 0);
+    }
     return f;
   }
   template <typename K>
@@ -329,8 +418,13 @@ struct Backward {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float du, dg;
-        const float up = half_of(f.p[j * P / 8], j * P % 8);
-        const float gate = GATED ? half_of(f.p[j * P / 8], j * P % 8 + 1) : 0.0f;
+        float up = half_of(f.p[j * P / 8], j * P % 8);
+        float gate = GATED ? half_of(f.p[j * P / 8], j * P % 8 + 1) : 0.0f;
+        if (low) {
+          const uint64_t b = __builtin_bit_cast(uint64_t, f.low[j * P / 8]);
+          up = with_low(up, b, j * P % 8);
+          if (GATED) gate = with_low(gate, b, j * P % 8 + 1);
+        }
         unit_grad_of<K, F32>(act, up, gate, v[j], &du, &dg);
         d[j * P] = du;
         if (GATED) d[j * P + 1] = dg;
@@ -344,12 +438,18 @@ struct Backward {
 
   struct In {
     Eight<T> p[P];
+    uint64_t low[P];
   };
   __device__ __forceinline__ In load(int64_t row, int64_t col) const {
     In in{};
 #pragma unroll
     for (int i = 0; i < P; ++i)
       in.p[i] = load_eight(product + (row * n + col) * P + 8 * i, (n - col) * P - 8 * i);
+    if (!F32 && low) {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        in.low[i] = load_low(low + (row * n + col) * P + 8 * i, (n - col) * P - 8 * i);
+    }
     return in;
   }
   template <typename F>
@@ -367,8 +467,12 @@ struct Backward {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float du, dg;
-        const float up = in.p[j * P / 8].value(j * P % 8);
-        const float gate = GATED ? in.p[j * P / 8].value(j * P % 8 + 1) : 0.0f;
+        float up = in.p[j * P / 8].value(j * P % 8);
+        float gate = GATED ? in.p[j * P / 8].value(j * P % 8 + 1) : 0.0f;
+        if (!F32 && low) {
+          up = with_low(up, in.low[j * P / 8], j * P % 8);
+          if (GATED) gate = with_low(gate, in.low[j * P / 8], j * P % 8 + 1);
+        }
         unit_grad_of<K, F32>(act, up, gate, v[j], &du, &dg);
         d[j * P] = du;
         if (GATED) d[j * P + 1] = dg;

@@ -407,14 +407,15 @@ int act_or_none(const char* name, const bux_ffn* ffn, Act* act) {
 
 template <typename T>
 int rows(const char* name, const T* x, const T* w, int transposed, int64_t m, int64_t n, int64_t k,
-         const T* bias, const bux_ffn* ffn, const T* residual, T* product, T* out, void* workspace,
-         size_t workspace_bytes, void* stream) {
+         const T* bias, const bux_ffn* ffn, const T* residual, T* product, uint8_t* low, T* out,
+         void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   if (int rc = check_shape(name, m, n, k)) return rc;
   Act act;
   if (int rc = act_or_none(name, ffn, &act)) return rc;
   BUX_CHECK(!act.gated || (n % 2 == 0 && residual == nullptr),
             "%s: a gated activation takes an even n (%lld) and no residual", name, (long long)n);
+  BUX_CHECK(low == nullptr || product != nullptr, "%s: low bytes without the product", name);
   if (m == 0) return BUX_OK;
   BUX_CHECK(x && w && out, "%s: NULL buffer", name);
   hipStream_t s = as_stream(stream);
@@ -423,14 +424,14 @@ int rows(const char* name, const T* x, const T* w, int transposed, int64_t m, in
     return transposed ? run<T, true, true>(name, A, B, m, n, k, epi, workspace, workspace_bytes, s)
                       : run<T, true, false>(name, A, B, m, n, k, epi, workspace, workspace_bytes, s);
   };
-  if (act.gated) return with(Forward<T, true>{act, bias, residual, product, out, n});
-  return with(Forward<T, false>{act, bias, residual, product, out, n});
+  if (act.gated) return with(Forward<T, true>{act, bias, residual, product, low, out, n});
+  return with(Forward<T, false>{act, bias, residual, product, low, out, n});
 }
 
 template <typename T>
 int units_backward(const char* name, const T* dy, const T* down, int64_t m, int64_t f, int64_t d,
-                   const T* product, const bux_ffn* ffn, T* dp, void* workspace,
-                   size_t workspace_bytes, void* stream) {
+                   const T* product, const uint8_t* low, const bux_ffn* ffn, T* dp,
+                   void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   if (int rc = check_shape(name, m, f, d)) return rc;
   Act act;
@@ -440,9 +441,9 @@ int units_backward(const char* name, const T* dy, const T* down, int64_t m, int6
   hipStream_t s = as_stream(stream);
   const Mat<T> A{dy, d, m}, B{down, d, f};
   if (act.gated)
-    return run<T, true, true>(name, A, B, m, f, d, Backward<T, true>{act, product, dp, f},
+    return run<T, true, true>(name, A, B, m, f, d, Backward<T, true>{act, product, low, dp, f},
                               workspace, workspace_bytes, s);
-  return run<T, true, true>(name, A, B, m, f, d, Backward<T, false>{act, product, dp, f}, workspace,
+  return run<T, true, true>(name, A, B, m, f, d, Backward<T, false>{act, product, low, dp, f}, workspace,
                             workspace_bytes, s);
 }
 
@@ -455,7 +456,7 @@ int contract(const char* name, const T* x, const T* dy, int64_t m, int64_t k, in
   const Act none{NO_ACT, 0, 0, 0.0f, 0, 0.0f, 0.0f};
   const Mat<T> A{x, k, k}, B{dy, n, n};
   return run<T, false, false>(name, A, B, k, n, m,
-                              Forward<T, false>{none, nullptr, nullptr, nullptr, dw, n}, workspace,
+                              Forward<T, false>{none, nullptr, nullptr, nullptr, nullptr, dw, n}, workspace,
                               workspace_bytes, as_stream(stream));
 }
 
@@ -615,31 +616,33 @@ extern "C" size_t bux_dense_slope_workspace_size(int64_t m, int64_t n) {
 
 extern "C" int bux_dense_rows(const uint16_t* x, const uint16_t* w, int transposed, int64_t m,
                               int64_t n, int64_t k, const uint16_t* bias, const bux_ffn* ffn,
-                              const uint16_t* residual, uint16_t* product, uint16_t* out,
-                              void* workspace, size_t workspace_bytes, void* stream) {
-  return bux::rows("bux_dense_rows", x, w, transposed, m, n, k, bias, ffn, residual, product, out,
-                   workspace, workspace_bytes, stream);
+                              const uint16_t* residual, uint16_t* product, uint8_t* product_low,
+                              uint16_t* out, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  return bux::rows("bux_dense_rows", x, w, transposed, m, n, k, bias, ffn, residual, product,
+                   product_low, out, workspace, workspace_bytes, stream);
 }
 extern "C" int bux_dense_rows_f32(const float* x, const float* w, int transposed, int64_t m,
                                   int64_t n, int64_t k, const float* bias, const bux_ffn* ffn,
                                   const float* residual, float* product, float* out,
                                   void* workspace, size_t workspace_bytes, void* stream) {
-  return bux::rows("bux_dense_rows_f32", x, w, transposed, m, n, k, bias, ffn, residual, product,
-                   out, workspace, workspace_bytes, stream);
+  return bux::rows<float>("bux_dense_rows_f32", x, w, transposed, m, n, k, bias, ffn, residual,
+                          product, nullptr, out, workspace, workspace_bytes, stream);
 }
 extern "C" int bux_dense_units_backward(const uint16_t* dy, const uint16_t* down, int64_t m,
                                         int64_t f, int64_t d, const uint16_t* product,
-                                        const bux_ffn* ffn, uint16_t* dp, void* workspace,
-                                        size_t workspace_bytes, void* stream) {
-  return bux::units_backward("bux_dense_units_backward", dy, down, m, f, d, product, ffn, dp,
-                             workspace, workspace_bytes, stream);
+                                        const uint8_t* product_low, const bux_ffn* ffn,
+                                        uint16_t* dp, void* workspace, size_t workspace_bytes,
+                                        void* stream) {
+  return bux::units_backward("bux_dense_units_backward", dy, down, m, f, d, product, product_low,
+                             ffn, dp, workspace, workspace_bytes, stream);
 }
 extern "C" int bux_dense_units_backward_f32(const float* dy, const float* down, int64_t m,
                                             int64_t f, int64_t d, const float* product,
                                             const bux_ffn* ffn, float* dp, void* workspace,
                                             size_t workspace_bytes, void* stream) {
-  return bux::units_backward("bux_dense_units_backward_f32", dy, down, m, f, d, product, ffn, dp,
-                             workspace, workspace_bytes, stream);
+  return bux::units_backward<float>("bux_dense_units_backward_f32", dy, down, m, f, d, product,
+                                    nullptr, ffn, dp, workspace, workspace_bytes, stream);
 }
 extern "C" int bux_dense_contract(const uint16_t* x, const uint16_t* dy, int64_t m, int64_t k,
                                   int64_t n, uint16_t* dw, void* workspace, size_t workspace_bytes,

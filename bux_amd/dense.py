@@ -78,13 +78,18 @@ def room(m: int, n: int, k: int, dev: torch.device) -> tuple[torch.Tensor | None
 
 def rows_into(x: torch.Tensor, w: torch.Tensor, transposed: bool, m: int, n: int, k: int,
               bias: torch.Tensor | None, st: _lib.FfnStruct | None,
-              residual: torch.Tensor | None, product: torch.Tensor | None, out: torch.Tensor
-              ) -> None:
+              residual: torch.Tensor | None, product: torch.Tensor | None, out: torch.Tensor,
+              low: torch.Tensor | None = None) -> None:
     """``bux_dense_rows`` of tensors already checked."""
     ws, need = room(m, n, k, x.device)
-    rows = lib().bux_dense_rows_f32 if x.dtype == torch.float32 else lib().bux_dense_rows
-    _lib.check(rows(ptr(x), ptr(w), int(transposed), m, n, k, ptr(bias), _ref(st), ptr(residual),
-                    ptr(product), ptr(out), ptr(ws), need, stream()))
+    if x.dtype == torch.float32:
+        _lib.check(lib().bux_dense_rows_f32(
+            ptr(x), ptr(w), int(transposed), m, n, k, ptr(bias), _ref(st), ptr(residual),
+            ptr(product), ptr(out), ptr(ws), need, stream()))
+    else:
+        _lib.check(lib().bux_dense_rows(
+            ptr(x), ptr(w), int(transposed), m, n, k, ptr(bias), _ref(st), ptr(residual),
+            ptr(product), ptr(low), ptr(out), ptr(ws), need, stream()))
 
 
 def product(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,

@@ -27,6 +27,9 @@ class Saved(NamedTuple):
     x: torch.Tensor  # the rows (..., d)
     projected: torch.Tensor  # x up + up_bias, before the activation (..., f, p)
     h: torch.Tensor  # the units (..., f)
+    # bfloat16: int8, projected's next 8 bits (..., f, p), which keep the activation's gradient
+    # from a second rounding beside its own; None (float32, or left out): from projected alone
+    low: torch.Tensor | None = None
 
 
 class FeedForward(NamedTuple):
@@ -76,23 +79,31 @@ def feed_forward(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, ffn: Ffn
         new = dict(dtype=x.dtype, device=x.device)
         h = torch.empty(*x.shape[:-1], f, **new)
         projected = torch.empty(*x.shape[:-1], f, p, **new) if keep else None
+        low = None
+        if keep and x.dtype == torch.bfloat16:
+            low = torch.empty(*x.shape[:-1], f, p, dtype=torch.int8, device=x.device)
         out = torch.empty(x.shape, **new)
         with span("up + activation"):
-            rows_into(x, up, False, m, f * p, d, up_bias, st, None, projected, h)
+            rows_into(x, up, False, m, f * p, d, up_bias, st, None, projected, h, low)
         with span("down"):
             rows_into(h, down, False, m, d, f, down_bias, None, residual, None, out)
-    return FeedForward(out, Saved(x, projected, h) if keep else None)
+    return FeedForward(out, Saved(x, projected, h, low) if keep else None)
 
 
-def units_backward(dy: torch.Tensor, down: torch.Tensor, projected: torch.Tensor, st: _lib.FfnStruct,
-                   m: int, f: int, d: int) -> torch.Tensor:
+def units_backward(dy: torch.Tensor, down: torch.Tensor, projected: torch.Tensor,
+                   low: torch.Tensor | None, st: _lib.FfnStruct, m: int, f: int, d: int
+                   ) -> torch.Tensor:
     """``bux_dense_units_backward`` of tensors already checked: the gradient to `projected`."""
     dp = torch.empty_like(projected)
     ws, need = room(m, f, d, dy.device)
-    backward = (lib().bux_dense_units_backward_f32 if dy.dtype == torch.float32
-                else lib().bux_dense_units_backward)
-    _lib.check(backward(ptr(dy), ptr(down), m, f, d, ptr(projected), ctypes.byref(st), ptr(dp),
-                        ptr(ws), need, stream()))
+    if dy.dtype == torch.float32:
+        _lib.check(lib().bux_dense_units_backward_f32(
+            ptr(dy), ptr(down), m, f, d, ptr(projected), ctypes.byref(st), ptr(dp), ptr(ws), need,
+            stream()))
+    else:
+        _lib.check(lib().bux_dense_units_backward(
+            ptr(dy), ptr(down), m, f, d, ptr(projected), ptr(low), ctypes.byref(st), ptr(dp),
+            ptr(ws), need, stream()))
     return dp
 
 
@@ -101,18 +112,23 @@ def feed_forward_backward(dy: torch.Tensor, saved: Saved, up: torch.Tensor, down
     """Return the gradients of `feed_forward` given dy (x's shape) and what it kept: to x, up
     (d, f, p), down (f, d) and, with `bias`, the biases; `ffn` as the forward's. The residual's
     gradient is dy. Each is rounded once to x's dtype, from float32 sums."""
-    x, projected, h = saved
-    require(dy, x, projected, h, up, down)
+    x, projected, h, low = saved
+    require(dy, x, projected, h, low, up, down)
     is_f32("feed_forward_backward", x, dy, projected, h, up, down)
     d, f, p = _kernels("feed_forward_backward", up, down)
     m = rows_of("feed_forward_backward", x, d)
     shaped("feed_forward_backward", "dy", dy, *x.shape)
     shaped("feed_forward_backward", "projected", projected, *x.shape[:-1], f, p)
     shaped("feed_forward_backward", "h", h, *x.shape[:-1], f)
+    shaped("feed_forward_backward", "low", low, *projected.shape)
+    if low is not None and (low.dtype != torch.int8 or low.device != x.device
+                            or x.dtype != torch.bfloat16):
+        raise ValueError(f"feed_forward_backward: low is int8 beside bfloat16 rows on {x.device}, "
+                         f"not {low.dtype} beside {x.dtype} on {low.device}")
     st = ffn.struct(gated=p == 2)
     with on_device(x):
         with span("down dgrad + activation backward"):
-            dp = units_backward(dy, down, projected, st, m, f, d)
+            dp = units_backward(dy, down, projected, low, st, m, f, d)
         with span("down wgrad"):
             d_down = weight_grad(h, dy)
         dp = dp.view(*x.shape[:-1], f * p)

@@ -791,7 +791,7 @@ static ffi::Error Int8Glu(hipStream_t s, In projected, In weights, In filled, BU
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8Glu, Int8Glu,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
-                                  BUX_FFN_ATTRS.Ret<In>().Ret<In>());
+                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>());
 
 // w [groups, k, n].
 static ffi::Error Int8QuantizeColumns(hipStream_t s, In w, Out values, Out scales) {
@@ -919,9 +919,10 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxMxUnpackRows, MxUnpackRows,
 // Each picks its float32 twin by x's (dy's) type, which every other operand has.
 
 // x [m, k]; w [k, n], or [n, k] transposed; bias [n], residual [m, n] (out's shape): may be empty.
-// activation -1: none. product [m, n], or empty; out [m, n], or [m, n / 2] of a gated one.
+// activation -1: none. product [m, n], or empty; low: its low bytes (of bfloat16), or empty; out
+// [m, n], or [m, n / 2] of a gated one.
 static ffi::Error DenseRows(hipStream_t s, In x, In w, In bias, In residual, int64_t transposed,
-                            BUX_FFN_PARAMS, Out product, Out out, Out ws) {
+                            BUX_FFN_PARAMS, Out product, Out low, Out out, Out ws) {
   if (!layer_type(x) || !ranked(x, 2) || !ranked(w, 2) || !ranked(out, 2))
     return mismatch("BuxDenseRows: x, w and out are bfloat16 or float32 matrices");
   const int64_t m = dim(x, 0), k = dim(x, 1), n = dim(w, transposed ? 0 : 1);
@@ -929,7 +930,8 @@ static ffi::Error DenseRows(hipStream_t s, In x, In w, In bias, In residual, int
   const ffi::DataType type = x.element_type();
   if (!holds(w, type, k * n) || dim(w, transposed ? 1 : 0) != k || !absent_or(bias, type, n) ||
       !absent_or(residual, type, m * n) || !absent_or(product, type, m * n) ||
-      !holds(out, type, m * wide))
+      !holds(out, type, m * wide) ||
+      (low->size_bytes() != 0 && (f32(x) || !holds_bytes(low, m * n))))
     return mismatch("BuxDenseRows: operands of x's type and of [m, k] times [k, n]");
   const bux_ffn ffn = BUX_FFN;
   const bux_ffn* const act = activation < 0 ? nullptr : &ffn;
@@ -941,22 +943,23 @@ static ffi::Error DenseRows(hipStream_t s, In x, In w, In bias, In residual, int
   return status(bux_dense_rows(
       at<const uint16_t>(x), at<const uint16_t>(w), static_cast<int>(transposed), m, n, k,
       at<const uint16_t>(bias), act, at<const uint16_t>(residual), at<uint16_t>(product),
-      at<uint16_t>(out), at<void>(ws), ws->size_bytes(), s));
+      at<uint8_t>(low), at<uint16_t>(out), at<void>(ws), ws->size_bytes(), s));
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseRows, DenseRows,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
                                   .Arg<In>().Attr<int64_t>("transposed") BUX_FFN_ATTRS
-                                  .Ret<In>().Ret<In>().Ret<In>());
+                                  .Ret<In>().Ret<In>().Ret<In>().Ret<In>());
 
-// dy [m, d], down [f, d], product and dp [m, f, 2] or [m, f].
-static ffi::Error DenseUnitsBackward(hipStream_t s, In dy, In down, In product, BUX_FFN_PARAMS,
-                                     Out dp, Out ws) {
+// dy [m, d], down [f, d], product and dp [m, f, 2] or [m, f]; low: product's low bytes, or empty.
+static ffi::Error DenseUnitsBackward(hipStream_t s, In dy, In down, In product, In low,
+                                     BUX_FFN_PARAMS, Out dp, Out ws) {
   if (!layer_type(dy) || !ranked(dy, 2) || !ranked(down, 2))
     return mismatch("BuxDenseUnitsBackward: dy and down are bfloat16 or float32 matrices");
   const int64_t m = dim(dy, 0), d = dim(dy, 1), f = dim(down, 0), p = gated ? 2 : 1;
   const ffi::DataType type = dy.element_type();
   if (!holds(down, type, f * d) || dim(down, 1) != d || !holds(product, type, m * f * p) ||
-      !holds(dp, type, m * f * p))
+      !holds(dp, type, m * f * p) ||
+      (low.size_bytes() != 0 && (f32(dy) || !holds_bytes(low, m * f * p))))
     return mismatch("BuxDenseUnitsBackward: operands of dy's type and of [m, d] times [f, d]");
   const bux_ffn ffn = BUX_FFN;
   if (f32(dy))
@@ -964,12 +967,12 @@ static ffi::Error DenseUnitsBackward(hipStream_t s, In dy, In down, In product, 
                                                at<const float>(product), &ffn, at<float>(dp),
                                                at<void>(ws), ws->size_bytes(), s));
   return status(bux_dense_units_backward(at<const uint16_t>(dy), at<const uint16_t>(down), m, f, d,
-                                         at<const uint16_t>(product), &ffn, at<uint16_t>(dp),
-                                         at<void>(ws), ws->size_bytes(), s));
+                                         at<const uint16_t>(product), at<const uint8_t>(low), &ffn,
+                                         at<uint16_t>(dp), at<void>(ws), ws->size_bytes(), s));
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseUnitsBackward, DenseUnitsBackward,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
-                                  BUX_FFN_ATTRS.Ret<In>().Ret<In>());
+                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>());
 
 // x [m, k], dy [m, n], dw [k, n].
 static ffi::Error DenseContract(hipStream_t s, In x, In dy, Out dw, Out ws) {

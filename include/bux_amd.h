@@ -790,9 +790,11 @@ int bux_mx_unpack_rows(const uint8_t* packed, int64_t m, int64_t d, uint16_t* ou
  *             the (up, gate) pairs of n / 2 units, out [m, n / 2] (n even, no residual).
  *   residual  NULL, or [m, n].
  *   product   NULL, or [m, n]: z, rounded, for the backward.
+ *   product_low  NULL, or [m, n] signed bytes beside product: the bits of z's float32 less those of
+ *             its bfloat16, in units of 2^8, so that the two hold 16 bits of z's mantissa.
  * bux_dense_units_backward: dp = (dy down^T) d act(product), the down product's gradient to its
- *   units and the activation's in one kernel. dy [m, d], down [f, d], product and dp [m, f, 2]
- *   (gated) or [m, f].
+ *   units and the activation's in one kernel. dy [m, d], down [f, d], product (and
+ *   product_low, or NULL) and dp [m, f, 2] (gated) or [m, f].
  * bux_dense_contract: dw = x^T dy. x [m, k], dy [m, n], dw [k, n]; 0 for m = 0.
  *   Its workspace: bux_dense_workspace_size(k, n, m).
  * bux_dense_slope: dz = dy act'(product) for a plain activation (ffn and product both NULL: dy
@@ -802,15 +804,16 @@ int bux_mx_unpack_rows(const uint8_t* packed, int64_t m, int64_t d, uint16_t* ou
 size_t bux_dense_workspace_size(int64_t m, int64_t n, int64_t k);
 int bux_dense_rows(const uint16_t* x, const uint16_t* w, int transposed, int64_t m, int64_t n,
                    int64_t k, const uint16_t* bias, const bux_ffn* ffn, const uint16_t* residual,
-                   uint16_t* product, uint16_t* out, void* workspace, size_t workspace_bytes,
-                   void* stream);
+                   uint16_t* product, uint8_t* product_low, uint16_t* out, void* workspace,
+                   size_t workspace_bytes, void* stream);
 int bux_dense_rows_f32(const float* x, const float* w, int transposed, int64_t m, int64_t n,
                        int64_t k, const float* bias, const bux_ffn* ffn, const float* residual,
                        float* product, float* out, void* workspace, size_t workspace_bytes,
                        void* stream);
 int bux_dense_units_backward(const uint16_t* dy, const uint16_t* down, int64_t m, int64_t f,
-                             int64_t d, const uint16_t* product, const bux_ffn* ffn, uint16_t* dp,
-                             void* workspace, size_t workspace_bytes, void* stream);
+                             int64_t d, const uint16_t* product, const uint8_t* product_low,
+                             const bux_ffn* ffn, uint16_t* dp, void* workspace,
+                             size_t workspace_bytes, void* stream);
 int bux_dense_units_backward_f32(const float* dy, const float* down, int64_t m, int64_t f,
                                  int64_t d, const float* product, const bux_ffn* ffn, float* dp,
                                  void* workspace, size_t workspace_bytes, void* stream);

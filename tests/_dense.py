@@ -144,5 +144,14 @@ def units(ffn, z, gated, dtype):
     return times(a, uo), times(a, du), times(times(uo, s), below)
 
 
+def kept(saved):
+    """The projections that the backward works from: bfloat16 with their next 8 bits, where kept."""
+    if saved.low is None:
+        return saved.projected.to(F64)
+    bits = (saved.projected.contiguous().view(torch.int16).to(torch.int32) << 16) + (
+        saved.low.to(torch.int32) << 8)
+    return bits.view(torch.float32).to(F64)
+
+
 def randn(g, *shape, scale=1.0):
     return scale * torch.randn(*shape, generator=g, dtype=F64)

@@ -25,10 +25,12 @@ def _ffn(activation=0, gated=1, clamped=0, limit=0.0, capped=0, cap=0.0):
 
 @pytest.mark.parametrize("twin", ["", "_f32"])
 def test_rows(lib, twin):
-    def rows(x=P, w=P, m=4, n=64, k=64, ffn=None, residual=None, out=P, ws=None, nbytes=0):
+    def rows(x=P, w=P, m=4, n=64, k=64, ffn=None, residual=None, out=P, ws=None, nbytes=0,
+             low=None):
         st = None if ffn is None else ctypes.byref(ffn)
-        return getattr(lib, "bux_dense_rows" + twin)(x, w, 0, m, n, k, None, st, residual, None, out,
-                                                     ws, nbytes, None)
+        kept = (None,) if twin else (None, low)  # product, and bfloat16's low bytes
+        return getattr(lib, "bux_dense_rows" + twin)(x, w, 0, m, n, k, None, st, residual, *kept,
+                                                     out, ws, nbytes, None)
 
     for shape in (dict(m=-1), dict(n=0), dict(k=0), dict(n=-8)):
         assert rows(**shape) == 1 and "bad shape" in _msg(lib)
@@ -47,6 +49,8 @@ def test_rows(lib, twin):
     assert rows(k=65536, ws=P, nbytes=8) == 2 and "workspace of 8 bytes" in _msg(lib)
     assert rows(k=65536) == 2
     assert rows(k=65536, ws=ctypes.c_void_p(8), nbytes=need) == 1 and "unaligned" in _msg(lib)
+    if not twin:
+        assert rows(low=P) == 1 and "low bytes" in _msg(lib)
     assert rows(m=0, x=None) == 0  # nothing to do
 
 
@@ -54,7 +58,8 @@ def test_rows(lib, twin):
 def test_units_backward(lib, twin):
     def backward(dy=P, m=4, f=64, d=64, ffn=_ffn(), nbytes=0, dp=P):
         st = None if ffn is None else ctypes.byref(ffn)
-        return getattr(lib, "bux_dense_units_backward" + twin)(dy, P, m, f, d, P, st, dp, None,
+        kept = (P,) if twin else (P, None)
+        return getattr(lib, "bux_dense_units_backward" + twin)(dy, P, m, f, d, *kept, st, dp, None,
                                                                nbytes, None)
 
     assert backward(f=0) == 1 and "bad shape" in _msg(lib)

@@ -6,7 +6,7 @@ tiles a workgroup. Against the formulas in float64, on the GPU, within bounds co
 import pytest
 import torch
 
-from _dense import BF16, F64, V, act, times, units
+from _dense import BF16, F64, V, act, kept, times, units
 from _util import announce
 
 pytestmark = pytest.mark.gpu
@@ -75,11 +75,12 @@ def test_block(lib, shape, gated):
     z = _v(x) @ V(up.to(F64).view(d, f * p)) + V(ub.to(F64).view(-1))
     z = V(z.v.view(m, f, p), z.e.view(m, f, p))
     z.rounded(BF16).holds(r.saved.projected, "projected")
+    V(z.v, z.e + 2.0 ** -15 * (z.v.abs() + z.e)).holds(kept(r.saved), "24 bits")
     units(ffn, z, gated, BF16)[0].rounded(BF16).holds(r.saved.h, "h")
     (_v(r.saved.h) @ _v(down)).rounded(BF16).holds(r.out, "out")
     got = mlp.feed_forward_backward(dy, r.saved, up, down, ffn)
     dh = _v(dy) @ _v(down).t()
-    _, du, dg = units(ffn, _v(r.saved.projected), gated, BF16)
+    _, du, dg = units(ffn, _v(kept(r.saved)), gated, BF16)
     parts = [times(dh, s) for s in (du, dg)[:p]]
     dp = V(torch.stack([q.v for q in parts], -1).view(m, f * p),
            torch.stack([q.e for q in parts], -1).view(m, f * p)).rounded(BF16)

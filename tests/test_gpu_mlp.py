@@ -5,7 +5,7 @@ forward kept."""
 import pytest
 import torch
 
-from _dense import BF16, F32, F64, V, randn, times, units
+from _dense import BF16, F32, F64, V, kept, randn, times, units
 from _util import announce
 
 pytestmark = pytest.mark.gpu
@@ -54,6 +54,9 @@ def test_forward_and_backward(lib, shape, p, dtype):
             z = z + V(_v(ub).v.view(-1))
         zp = V(z.v.view(m, f, p), z.e.view(m, f, p))
         zp.rounded(dtype).holds(r.saved.projected, "projected")
+        assert (r.saved.low is None) == (dtype == F32)
+        if dtype == BF16:  # in units of 2^8 of a 23-bit mantissa, one more where a byte ends
+            V(zp.v, zp.e + 2.0 ** -15 * (zp.v.abs() + zp.e)).holds(kept(r.saved), "24 bits")
         h = units(ffn, zp, p == 2, dtype)[0].rounded(dtype)
         h.holds(r.saved.h, "h")
         y = _v(r.saved.h) @ _v(t["down"])
@@ -67,7 +70,7 @@ def test_forward_and_backward(lib, shape, p, dtype):
 
         got = mlp.feed_forward_backward(t["dy"], r.saved, t["up"], t["down"], ffn, bias=biased)
         dh = _v(t["dy"]) @ _v(t["down"]).t()
-        _, du, dg = units(ffn, _v(r.saved.projected), p == 2, dtype)
+        _, du, dg = units(ffn, _v(kept(r.saved)), p == 2, dtype)
         parts = [times(dh, s) for s in (du, dg)[:p]]
         dp = V(torch.stack([q.v for q in parts], -1).view(m, f * p),
                torch.stack([q.e for q in parts], -1).view(m, f * p)).rounded(dtype)
@@ -82,6 +85,52 @@ def test_forward_and_backward(lib, shape, p, dtype):
             _v(t["dy"]).sum0().rounded(dtype).holds(got.down_bias, "ddown_bias")
         else:
             assert got.up_bias is None and got.down_bias is None
+
+
+@pytest.mark.parametrize("m", [5, 200])
+def test_backward_from_the_bfloat16_projections_alone(lib, m):
+    from bux_amd import mlp
+    from bux_amd.moe import Ffn
+
+    g = torch.Generator().manual_seed(m)
+    d, f = 136, 72
+    t = _make(g, BF16, m, d, f, 2)
+    r = mlp.feed_forward(t["x"], t["up"], t["down"])
+    alone = r.saved._replace(low=None)
+    announce("mlp without low bytes", m)
+    got = mlp.feed_forward_backward(t["dy"], alone, t["up"], t["down"])
+    dh = _v(t["dy"]) @ _v(t["down"]).t()
+    _, du, dg = units(Ffn(), _v(kept(alone)), True, BF16)
+    parts = [times(dh, s) for s in (du, dg)]
+    dp = V(torch.stack([q.v for q in parts], -1).view(m, f * 2),
+           torch.stack([q.e for q in parts], -1).view(m, f * 2)).rounded(BF16)
+    (dp @ V(_v(t["up"]).v.view(d, f * 2)).t()).rounded(BF16).holds(got.x, "dx")
+
+
+def test_projections_at_the_ends_of_their_type(lib):
+    """Values that round to infinity, infinities, NaN, zeros and the smallest, through the kept 24
+    bits: h is act(u) of a plain relu block with one input a unit, dp its gradient."""
+    from bux_amd import mlp
+    from bux_amd.moe import Ffn
+
+    vals = [3.3e38, -3.3e38, float("inf"), float("-inf"), float("nan"), 0.0, -0.0, 1e-38, 1.0, -1.0,
+            2.0 ** -126, 255.5]
+    up = torch.tensor(vals, dtype=BF16, device="cuda").view(1, -1, 1).contiguous()
+    f = len(vals)
+    x = torch.tensor([[1.0], [1.00390625 * 1.0]], dtype=BF16, device="cuda")
+    down = torch.ones(f, 1, dtype=BF16, device="cuda")
+    announce("mlp ends of bfloat16")
+    r = mlp.feed_forward(x, up, down, Ffn("relu"))
+    v = up.view(-1).double()
+    want = kept(r.saved)[0, :, 0]
+    assert torch.equal(want.isnan(), v.isnan())
+    assert torch.equal(want[~v.isnan()], v[~v.isnan()])
+    got = mlp.feed_forward_backward(torch.ones_like(x), r.saved, up, down, Ffn("relu"))
+    # d up = x^T dp with dp = 1 where the projection is above 0, 0 where it is not
+    sums = x.double().sum().item()
+    for j, val in enumerate(vals):
+        if val == val:
+            assert abs(got.up.view(-1)[j].item() - (sums if val > 0 else 0.0)) <= 2.0 ** -8 * sums
 
 
 def test_gradients_against_differences(lib):
@@ -213,3 +262,7 @@ def test_refusals(lib):
         mlp.feed_forward_backward(x, r.saved._replace(projected=r.saved.h), up, down)
     with pytest.raises(ValueError, match="h is"):
         mlp.feed_forward_backward(x, r.saved._replace(h=x), up, down)
+    with pytest.raises(ValueError, match="low is"):
+        mlp.feed_forward_backward(x, r.saved._replace(low=r.saved.low[..., 0].contiguous()), up, down)
+    with pytest.raises(ValueError, match="low is int8"):
+        mlp.feed_forward_backward(x, r.saved._replace(low=r.saved.low.float()), up, down)

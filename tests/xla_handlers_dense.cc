@@ -10,14 +10,14 @@ static int calls = 0;
 extern "C" {
 const char* bux_last_error() { return ""; }
 int bux_dense_rows(const uint16_t*, const uint16_t*, int, int64_t, int64_t, int64_t, const uint16_t*,
-                   const bux_ffn*, const uint16_t*, uint16_t*, uint16_t*, void*, size_t,
+                   const bux_ffn*, const uint16_t*, uint16_t*, uint8_t*, uint16_t*, void*, size_t,
                    void*) { return ++calls, 0; }
 int bux_dense_rows_f32(const float*, const float*, int, int64_t, int64_t, int64_t, const float*,
                        const bux_ffn*, const float*, float*, float*, void*, size_t,
                        void*) { return ++calls, 0; }
 int bux_dense_units_backward(const uint16_t*, const uint16_t*, int64_t, int64_t, int64_t,
-                             const uint16_t*, const bux_ffn*, uint16_t*, void*, size_t,
-                             void*) { return ++calls, 0; }
+                             const uint16_t*, const uint8_t*, const bux_ffn*, uint16_t*, void*,
+                             size_t, void*) { return ++calls, 0; }
 int bux_dense_units_backward_f32(const float*, const float*, int64_t, int64_t, int64_t, const float*,
                                  const bux_ffn*, float*, void*, size_t, void*) { return ++calls, 0; }
 int bux_dense_contract(const uint16_t*, const uint16_t*, int64_t, int64_t, int64_t, uint16_t*, void*,
@@ -49,13 +49,14 @@ static void line(const char* what, bool taken, const ffi::Error& e) {
 
 struct Rows {
   DataType t = BF;
-  std::vector<int64_t> x{6, 32}, w{32, 20}, bias{20}, residual{6, 20}, product{6, 20}, out{6, 20};
+  std::vector<int64_t> x{6, 32}, w{32, 20}, bias{20}, residual{6, 20}, product{6, 20}, low{0}, out{6, 20};
   DataType wt = BF;
   int64_t transposed = 0, activation = 0, gated = 0;
   void call(bool taken) const {
     line("rows", taken,
          DenseRows(nullptr, buffer(t, x), buffer(wt, w), buffer(t, bias), buffer(t, residual),
                    transposed, activation, gated, 0, 0.0f, 0, 0.0f, 0.0f, result(t, product),
+                   result(U, low),
                    result(t, out), result(U, {64})));
   }
 };
@@ -73,6 +74,8 @@ int main() {
   f.call(true);
   with(&Rows::residual, Dims{0}).call(true);
   with(&Rows::bias, Dims{0}).call(true);
+  with(&Rows::low, Dims{6, 20}).call(true);
+  with(&Rows::low, Dims{6, 19}).call(false);
   with(&Rows::activation, int64_t{-1}).call(true);
   Rows g;
   g.gated = 1, g.residual = {0}, g.out = {6, 10};
@@ -89,13 +92,18 @@ int main() {
   with(&Rows::x, Dims{192}).call(false);
   with(&Rows::gated, int64_t{1}).call(false);  // out of half the columns
 
-  auto units = [](bool taken, DataType t, Dims dy, Dims down, Dims product, Dims dp, int64_t gated) {
+  auto units = [](bool taken, DataType t, Dims dy, Dims down, Dims product, Dims dp, int64_t gated,
+                  Dims low = {0}) {
     line("units backward", taken,
-         DenseUnitsBackward(nullptr, buffer(t, dy), buffer(t, down), buffer(t, product), 0, gated, 0,
+         DenseUnitsBackward(nullptr, buffer(t, dy), buffer(t, down), buffer(t, product), buffer(U, low), 0,
+                            gated, 0,
                             0.0f, 0, 0.0f, 0.0f, result(t, dp), result(U, {64})));
   };
   units(true, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1);
   units(true, F, {6, 32}, {10, 32}, {6, 10}, {6, 10}, 0);
+  units(true, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1, {6, 10, 2});
+  units(false, F, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1, {6, 10, 2});
+  units(false, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1, {6, 10});
   units(false, BF, {6, 32}, {10, 31}, {6, 10, 2}, {6, 10, 2}, 1);
   units(false, BF, {6, 32}, {10, 32}, {6, 10}, {6, 10, 2}, 1);
   units(false, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10}, 1);
