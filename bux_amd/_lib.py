@@ -186,13 +186,13 @@ SIGNATURES = {
     "bux_dense_rows_f32": (
         _int, [_p, _p, _int, _i64, _i64, _i64, _p, _ffn, _p, _p, _p, _p, _size, _p]),
     "bux_dense_units_backward": (
-        _int, [_p, _p, _i64, _i64, _i64, _p, _p, _ffn, _p, _p, _size, _p]),
+        _int, [_p, _p, _i64, _i64, _i64, _p, _p, _ffn, _p, _p, _p, _size, _p]),
     "bux_dense_units_backward_f32": (
         _int, [_p, _p, _i64, _i64, _i64, _p, _ffn, _p, _p, _size, _p]),
     "bux_dense_contract": (_int, [_p, _p, _i64, _i64, _i64, _p, _p, _size, _p]),
     "bux_dense_contract_f32": (_int, [_p, _p, _i64, _i64, _i64, _p, _p, _size, _p]),
     "bux_dense_slope_workspace_size": (_size, [_i64, _i64]),
-    "bux_dense_slope": (_int, [_p, _p, _ffn, _i64, _i64, _p, _p, _p, _size, _p]),
+    "bux_dense_slope": (_int, [_p, _p, _p, _ffn, _i64, _i64, _p, _p, _p, _size, _p]),
     "bux_dense_slope_f32": (_int, [_p, _p, _ffn, _i64, _i64, _p, _p, _p, _size, _p]),
     "bux_clip_workspace_size": (_size, [_i32]),
     "bux_clip": (_int, [gradients, _i32, _f32, _p, _p, _size, _p]),

@@ -376,10 +376,11 @@ struct Backward {
   const T* product;    // [m, n, P]
   const uint8_t* low;  // its low bytes (bfloat16), or NULL
   T* out;              // product's shape
+  uint8_t* out_low;    // its low bytes (bfloat16), or NULL: what the biases' sums take
   int64_t n;         // units
 
   struct Tile {
-    Place out, product, low;
+    Place out, product, low, out_low;
   };
   struct Fast {
     words4 p[P];
@@ -387,11 +388,12 @@ struct Backward {
   };
   __device__ __forceinline__ bool aligned() const {
     return aligned16(out, n) && aligned16(product, n) && n < (1 << 20) &&
-           (low == nullptr || reinterpret_cast<uintptr_t>(low) % 8 == 0);
+           (low == nullptr || reinterpret_cast<uintptr_t>(low) % 8 == 0) &&
+           (out_low == nullptr || reinterpret_cast<uintptr_t>(out_low) % 8 == 0);
   }
   __device__ __forceinline__ Tile tile(int64_t row, int64_t col) const {
     return Tile{place_in<8 * P>(out, row, col, n), place_in<8 * P>(product, row, col, n),
-                bytes_in<8 * P>(low, row, col, n)};
+                bytes_in<8 * P>(low, row, col, n), bytes_in<8 * P>(out_low, row, col, n)};
   }
   __device__ __forceinline__ Fast fast(const Tile& t, int row, int col) const {
     Fast f;
@@ -431,9 +433,17 @@ struct Backward {
       }
     }
 #pragma unroll
-    for (int i = 0; i < P; ++i)
-      __builtin_amdgcn_raw_buffer_store_b128(packed8(d + 8 * i), t.out.rsrc, t.out.lane + HALF * i,
+    for (int i = 0; i < P; ++i) {
+      const words4 w = packed8(d + 8 * i);
+      __builtin_amdgcn_raw_buffer_store_b128(w, t.out.rsrc, t.out.lane + HALF * i,
                                              scalar_in<8 * P>(t.out, row, col), NON_TEMPORAL);
+      if (out_low) {
+        const uint32_t high[4] = {w.x, w.y, w.z, w.w};
+        __builtin_amdgcn_raw_buffer_store_b64(
+            __builtin_bit_cast(words2, low_bytes(d + 8 * i, high)), t.out_low.rsrc,
+            t.out_low.lane + HALF / 2 * i, row * t.out_low.pitch + col * P, NON_TEMPORAL);
+      }
+    }
   }
 
   struct In {
@@ -479,8 +489,19 @@ struct Backward {
       }
     }
 #pragma unroll
-    for (int i = 0; i < P; ++i)
-      store_some<T>(out + (row * n + col) * P + 8 * i, d + 8 * i, (n - col) * P - 8 * i);
+    for (int i = 0; i < P; ++i) {
+      const int64_t at = (row * n + col) * P + 8 * i, count = (n - col) * P - 8 * i;
+      store_some<T>(out + at, d + 8 * i, count);
+      if constexpr (!F32) {
+        if (out_low) {
+          uint32_t high[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            high[j] = pack_bf16x2(d[8 * i + 2 * j], d[8 * i + 2 * j + 1]);
+          store_low(out_low + at, low_bytes(d + 8 * i, high), count);
+        }
+      }
+    }
   }
 };
 

@@ -431,7 +431,7 @@ int rows(const char* name, const T* x, const T* w, int transposed, int64_t m, in
 template <typename T>
 int units_backward(const char* name, const T* dy, const T* down, int64_t m, int64_t f, int64_t d,
                    const T* product, const uint8_t* low, const bux_ffn* ffn, T* dp,
-                   void* workspace, size_t workspace_bytes, void* stream) {
+                   uint8_t* dp_low, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   if (int rc = check_shape(name, m, f, d)) return rc;
   Act act;
@@ -441,9 +441,9 @@ int units_backward(const char* name, const T* dy, const T* down, int64_t m, int6
   hipStream_t s = as_stream(stream);
   const Mat<T> A{dy, d, m}, B{down, d, f};
   if (act.gated)
-    return run<T, true, true>(name, A, B, m, f, d, Backward<T, true>{act, product, low, dp, f},
+    return run<T, true, true>(name, A, B, m, f, d, Backward<T, true>{act, product, low, dp, dp_low, f},
                               workspace, workspace_bytes, s);
-  return run<T, true, true>(name, A, B, m, f, d, Backward<T, false>{act, product, low, dp, f}, workspace,
+  return run<T, true, true>(name, A, B, m, f, d, Backward<T, false>{act, product, low, dp, dp_low, f}, workspace,
                             workspace_bytes, s);
 }
 
@@ -485,6 +485,7 @@ int64_t runs_of(int64_t m, int64_t n) {
 
 template <typename T>
 __global__ __launch_bounds__(THREADS) void slope_kernel(const T* __restrict__ dy,
+                                                        const uint8_t* __restrict__ dy_low,
                                                         const T* __restrict__ product, Act act,
                                                         int64_t m, int64_t n, int lanes,
                                                         T* __restrict__ dz, T* __restrict__ sums,
@@ -501,10 +502,12 @@ __global__ __launch_bounds__(THREADS) void slope_kernel(const T* __restrict__ dy
       const int64_t stride = static_cast<int64_t>(gridDim.y) * rows;
       for (int64_t r0 = static_cast<int64_t>(blockIdx.y) * rows + sub; r0 < m; r0 += TURN * stride) {
         Eight<T> g[TURN], z[TURN];
+        uint64_t low[TURN];
 #pragma unroll
         for (int i = 0; i < TURN; ++i) {
           const int64_t r = r0 + i * stride;
           g[i] = load_eight(dy + r * n + col, r < m ? count : 0);
+          if (PLAIN && sizeof(T) == 2 && dy_low) low[i] = load_low(dy_low + r * n + col, r < m ? count : 0);
           if (!PLAIN) z[i] = load_eight(product + r * n + col, r < m ? count : 0);
         }
 #pragma unroll
@@ -515,6 +518,10 @@ __global__ __launch_bounds__(THREADS) void slope_kernel(const T* __restrict__ dy
           if constexpr (PLAIN) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = g[i].value(j);
+            if (sizeof(T) == 2 && dy_low) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = with_low(v[j], low[i], j);
+            }
           } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -569,7 +576,7 @@ __global__ __launch_bounds__(THREADS) void sums_kernel(const float* __restrict__
 }
 
 template <typename T>
-int slope(const char* name, const T* dy, const T* product, const bux_ffn* ffn, int64_t m, int64_t n,
+int slope(const char* name, const T* dy, const uint8_t* dy_low, const T* product, const bux_ffn* ffn, int64_t m, int64_t n,
           T* dz, T* sums, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   if (int rc = check_shape(name, m, n, 1)) return rc;
@@ -579,6 +586,8 @@ int slope(const char* name, const T* dy, const T* product, const bux_ffn* ffn, i
   BUX_CHECK((ffn == nullptr) == (product == nullptr), "%s: an activation's gradient takes its product",
             name);
   BUX_CHECK(dz || sums, "%s: nothing asked for", name);
+  BUX_CHECK(dy_low == nullptr || (ffn == nullptr && dz == nullptr),
+            "%s: low bytes are for dy's own sums", name);
   BUX_CHECK(m == 0 || dy, "%s: NULL buffer", name);
   const int64_t runs = runs_of(m, n);
   const size_t need = sums && runs > 1 ? static_cast<size_t>(runs) * n * sizeof(float) : 0;
@@ -591,7 +600,7 @@ int slope(const char* name, const T* dy, const T* product, const bux_ffn* ffn, i
   float* const parts = static_cast<float*>(workspace);
   hipLaunchKernelGGL(slope_kernel<T>, dim3(static_cast<unsigned>(ceil_div(n, 8 * lanes)),
                                            static_cast<unsigned>(runs)),
-                     dim3(THREADS), 0, s, dy, product, act, m, n, lanes, dz, sums, parts);
+                     dim3(THREADS), 0, s, dy, dy_low, product, act, m, n, lanes, dz, sums, parts);
   if (int rc = launched("dense slope_kernel")) return rc;
   if (!sums || runs == 1) return BUX_OK;
   hipLaunchKernelGGL(sums_kernel<T>, dim3(static_cast<unsigned>(ceil_div(n, 64))),
@@ -632,17 +641,17 @@ extern "C" int bux_dense_rows_f32(const float* x, const float* w, int transposed
 extern "C" int bux_dense_units_backward(const uint16_t* dy, const uint16_t* down, int64_t m,
                                         int64_t f, int64_t d, const uint16_t* product,
                                         const uint8_t* product_low, const bux_ffn* ffn,
-                                        uint16_t* dp, void* workspace, size_t workspace_bytes,
-                                        void* stream) {
+                                        uint16_t* dp, uint8_t* dp_low, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
   return bux::units_backward("bux_dense_units_backward", dy, down, m, f, d, product, product_low,
-                             ffn, dp, workspace, workspace_bytes, stream);
+                             ffn, dp, dp_low, workspace, workspace_bytes, stream);
 }
 extern "C" int bux_dense_units_backward_f32(const float* dy, const float* down, int64_t m,
                                             int64_t f, int64_t d, const float* product,
                                             const bux_ffn* ffn, float* dp, void* workspace,
                                             size_t workspace_bytes, void* stream) {
   return bux::units_backward<float>("bux_dense_units_backward_f32", dy, down, m, f, d, product,
-                                    nullptr, ffn, dp, workspace, workspace_bytes, stream);
+                                    nullptr, ffn, dp, nullptr, workspace, workspace_bytes, stream);
 }
 extern "C" int bux_dense_contract(const uint16_t* x, const uint16_t* dy, int64_t m, int64_t k,
                                   int64_t n, uint16_t* dw, void* workspace, size_t workspace_bytes,
@@ -655,15 +664,16 @@ extern "C" int bux_dense_contract_f32(const float* x, const float* dy, int64_t m
   return bux::contract("bux_dense_contract_f32", x, dy, m, k, n, dw, workspace, workspace_bytes,
                        stream);
 }
-extern "C" int bux_dense_slope(const uint16_t* dy, const uint16_t* product, const bux_ffn* ffn,
-                               int64_t m, int64_t n, uint16_t* dz, uint16_t* sums, void* workspace,
-                               size_t workspace_bytes, void* stream) {
-  return bux::slope("bux_dense_slope", dy, product, ffn, m, n, dz, sums, workspace, workspace_bytes,
+extern "C" int bux_dense_slope(const uint16_t* dy, const uint8_t* dy_low, const uint16_t* product,
+                               const bux_ffn* ffn, int64_t m, int64_t n, uint16_t* dz,
+                               uint16_t* sums, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  return bux::slope("bux_dense_slope", dy, dy_low, product, ffn, m, n, dz, sums, workspace, workspace_bytes,
                     stream);
 }
 extern "C" int bux_dense_slope_f32(const float* dy, const float* product, const bux_ffn* ffn,
                                    int64_t m, int64_t n, float* dz, float* sums, void* workspace,
                                    size_t workspace_bytes, void* stream) {
-  return bux::slope("bux_dense_slope_f32", dy, product, ffn, m, n, dz, sums, workspace,
+  return bux::slope<float>("bux_dense_slope_f32", dy, nullptr, product, ffn, m, n, dz, sums, workspace,
                     workspace_bytes, stream);
 }

@@ -135,19 +135,23 @@ def weight_grad(x: torch.Tensor, dy: torch.Tensor) -> torch.Tensor:
 
 
 def slope(dy: torch.Tensor, m: int, n: int, product: torch.Tensor | None = None,
-          st: _lib.FfnStruct | None = None, sums: bool = False
+          st: _lib.FfnStruct | None = None, sums: bool = False, low: torch.Tensor | None = None
           ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
-    """``bux_dense_slope`` of dy (m, n), already checked: dy times the activation's derivative at
-    `product` (None without one), and with `sums` that gradient's sums over the rows."""
+    """``bux_dense_slope`` of dy (m, n) (its sums with its low bytes, `low`), already checked: dy
+    times the activation's derivative at `product` (None without one), and with `sums` that
+    gradient's sums over the rows."""
     dz = torch.empty_like(dy) if product is not None else None
     out = torch.empty(n, dtype=dy.dtype, device=dy.device) if sums else None
     if dz is None and out is None:
         return None, None
     need = lib().bux_dense_slope_workspace_size(m, n) if sums else 0
     ws = workspace(need, dy.device) if need else None
-    grad = lib().bux_dense_slope_f32 if dy.dtype == torch.float32 else lib().bux_dense_slope
-    _lib.check(grad(ptr(dy), ptr(product), _ref(st), m, n, ptr(dz), ptr(out), ptr(ws), need,
-                    stream()))
+    if dy.dtype == torch.float32:
+        _lib.check(lib().bux_dense_slope_f32(ptr(dy), ptr(product), _ref(st), m, n, ptr(dz),
+                                             ptr(out), ptr(ws), need, stream()))
+    else:
+        _lib.check(lib().bux_dense_slope(ptr(dy), ptr(low), ptr(product), _ref(st), m, n, ptr(dz),
+                                         ptr(out), ptr(ws), need, stream()))
     return dz, out
 
 

@@ -91,10 +91,14 @@ def feed_forward(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, ffn: Ffn
 
 
 def units_backward(dy: torch.Tensor, down: torch.Tensor, projected: torch.Tensor,
-                   low: torch.Tensor | None, st: _lib.FfnStruct, m: int, f: int, d: int
-                   ) -> torch.Tensor:
-    """``bux_dense_units_backward`` of tensors already checked: the gradient to `projected`."""
+                   low: torch.Tensor | None, st: _lib.FfnStruct, m: int, f: int, d: int,
+                   sums: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``bux_dense_units_backward`` of tensors already checked: the gradient to `projected`, and with
+    `sums` (bfloat16) its low bytes, which its sums over the rows take."""
     dp = torch.empty_like(projected)
+    dp_low = None
+    if sums and dy.dtype == torch.bfloat16:
+        dp_low = torch.empty(dp.shape, dtype=torch.int8, device=dp.device)
     ws, need = room(m, f, d, dy.device)
     if dy.dtype == torch.float32:
         _lib.check(lib().bux_dense_units_backward_f32(
@@ -103,8 +107,8 @@ def units_backward(dy: torch.Tensor, down: torch.Tensor, projected: torch.Tensor
     else:
         _lib.check(lib().bux_dense_units_backward(
             ptr(dy), ptr(down), m, f, d, ptr(projected), ptr(low), ctypes.byref(st), ptr(dp),
-            ptr(ws), need, stream()))
-    return dp
+            ptr(dp_low), ptr(ws), need, stream()))
+    return dp, dp_low
 
 
 def feed_forward_backward(dy: torch.Tensor, saved: Saved, up: torch.Tensor, down: torch.Tensor,
@@ -128,7 +132,7 @@ def feed_forward_backward(dy: torch.Tensor, saved: Saved, up: torch.Tensor, down
     st = ffn.struct(gated=p == 2)
     with on_device(x):
         with span("down dgrad + activation backward"):
-            dp = units_backward(dy, down, projected, low, st, m, f, d)
+            dp, dp_low = units_backward(dy, down, projected, low, st, m, f, d, bias)
         with span("down wgrad"):
             d_down = weight_grad(h, dy)
         dp = dp.view(*x.shape[:-1], f * p)
@@ -140,6 +144,6 @@ def feed_forward_backward(dy: torch.Tensor, saved: Saved, up: torch.Tensor, down
         d_up_bias = d_down_bias = None
         if bias:
             with span("bias grads"):
-                d_up_bias = slope(dp, m, f * p, sums=True)[1].view(f, p)
+                d_up_bias = slope(dp, m, f * p, sums=True, low=dp_low)[1].view(f, p)
                 d_down_bias = slope(dy, m, d, sums=True)[1]
     return FeedForwardGrads(dx, d_up, d_down, d_up_bias, d_down_bias)

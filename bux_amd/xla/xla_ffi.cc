@@ -389,7 +389,7 @@ static ffi::Error GluBackward(hipStream_t s, In projected, In weights, In dh, In
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxGluBackward, GluBackward,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
-                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>());
+                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>().Ret<In>());
 
 // h may be an empty result (not kept); f from the row copy's K is not exact, so it is an
 // attribute, as are m and height.
@@ -791,7 +791,7 @@ static ffi::Error Int8Glu(hipStream_t s, In projected, In weights, In filled, BU
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8Glu, Int8Glu,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
-                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>());
+                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>().Ret<In>());
 
 // w [groups, k, n].
 static ffi::Error Int8QuantizeColumns(hipStream_t s, In w, Out values, Out scales) {
@@ -950,16 +950,18 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseRows, DenseRows,
                                   .Arg<In>().Attr<int64_t>("transposed") BUX_FFN_ATTRS
                                   .Ret<In>().Ret<In>().Ret<In>().Ret<In>());
 
-// dy [m, d], down [f, d], product and dp [m, f, 2] or [m, f]; low: product's low bytes, or empty.
+// dy [m, d], down [f, d], product and dp [m, f, 2] or [m, f]; low and dp_low: product's and dp's
+// low bytes, or empty.
 static ffi::Error DenseUnitsBackward(hipStream_t s, In dy, In down, In product, In low,
-                                     BUX_FFN_PARAMS, Out dp, Out ws) {
+                                     BUX_FFN_PARAMS, Out dp, Out dp_low, Out ws) {
   if (!layer_type(dy) || !ranked(dy, 2) || !ranked(down, 2))
     return mismatch("BuxDenseUnitsBackward: dy and down are bfloat16 or float32 matrices");
   const int64_t m = dim(dy, 0), d = dim(dy, 1), f = dim(down, 0), p = gated ? 2 : 1;
   const ffi::DataType type = dy.element_type();
   if (!holds(down, type, f * d) || dim(down, 1) != d || !holds(product, type, m * f * p) ||
       !holds(dp, type, m * f * p) ||
-      (low.size_bytes() != 0 && (f32(dy) || !holds_bytes(low, m * f * p))))
+      (low.size_bytes() != 0 && (f32(dy) || !holds_bytes(low, m * f * p))) ||
+      (dp_low->size_bytes() != 0 && (f32(dy) || !holds_bytes(dp_low, m * f * p))))
     return mismatch("BuxDenseUnitsBackward: operands of dy's type and of [m, d] times [f, d]");
   const bux_ffn ffn = BUX_FFN;
   if (f32(dy))
@@ -968,11 +970,11 @@ static ffi::Error DenseUnitsBackward(hipStream_t s, In dy, In down, In product, 
                                                at<void>(ws), ws->size_bytes(), s));
   return status(bux_dense_units_backward(at<const uint16_t>(dy), at<const uint16_t>(down), m, f, d,
                                          at<const uint16_t>(product), at<const uint8_t>(low), &ffn,
-                                         at<uint16_t>(dp), at<void>(ws), ws->size_bytes(), s));
+                                         at<uint16_t>(dp), at<uint8_t>(dp_low), at<void>(ws), ws->size_bytes(), s));
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseUnitsBackward, DenseUnitsBackward,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
-                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>());
+                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>().Ret<In>());
 
 // x [m, k], dy [m, n], dw [k, n].
 static ffi::Error DenseContract(hipStream_t s, In x, In dy, Out dw, Out ws) {
@@ -992,28 +994,29 @@ XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseContract, DenseContract,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>()
                                   .Ret<In>().Ret<In>());
 
-// dy [m, n]; product [m, n], or empty with activation -1; dz [m, n] or empty; sums [n] or empty.
-static ffi::Error DenseSlope(hipStream_t s, In dy, In product, BUX_FFN_PARAMS, Out dz, Out sums,
-                             Out ws) {
+// dy [m, n]; low: its low bytes, or empty; product [m, n], or empty with activation -1; dz [m, n] or empty; sums [n] or empty.
+static ffi::Error DenseSlope(hipStream_t s, In dy, In low, In product, BUX_FFN_PARAMS, Out dz,
+                             Out sums, Out ws) {
   if (!layer_type(dy) || !ranked(dy, 2))
     return mismatch("BuxDenseSlope: dy is a bfloat16 or float32 matrix");
   const int64_t m = dim(dy, 0), n = dim(dy, 1);
   const ffi::DataType type = dy.element_type();
-  if (!absent_or(product, type, m * n) || !absent_or(dz, type, m * n) || !absent_or(sums, type, n))
-    return mismatch("BuxDenseSlope: product, dz and sums of dy's type and size");
+  if (!absent_or(product, type, m * n) || !absent_or(dz, type, m * n) || !absent_or(sums, type, n) ||
+      (low.size_bytes() != 0 && (f32(dy) || !holds_bytes(low, m * n))))
+    return mismatch("BuxDenseSlope: low bytes, product, dz and sums of dy's type and size");
   const bux_ffn ffn = BUX_FFN;
   const bux_ffn* const act = activation < 0 ? nullptr : &ffn;
   if (f32(dy))
     return status(bux_dense_slope_f32(at<const float>(dy), at<const float>(product), act, m, n,
                                       at<float>(dz), at<float>(sums), at<void>(ws),
                                       ws->size_bytes(), s));
-  return status(bux_dense_slope(at<const uint16_t>(dy), at<const uint16_t>(product), act, m, n,
-                                at<uint16_t>(dz), at<uint16_t>(sums), at<void>(ws),
-                                ws->size_bytes(), s));
+  return status(bux_dense_slope(at<const uint16_t>(dy), at<const uint8_t>(low),
+                                at<const uint16_t>(product), act, m, n, at<uint16_t>(dz),
+                                at<uint16_t>(sums), at<void>(ws), ws->size_bytes(), s));
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxDenseSlope, DenseSlope,
-                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>() BUX_FFN_ATTRS
-                                  .Ret<In>().Ret<In>().Ret<In>());
+                              ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
+                                  BUX_FFN_ATTRS.Ret<In>().Ret<In>().Ret<In>());
 
 // --- gradients clipped by their global norm ------------------------------------------------
 

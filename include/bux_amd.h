@@ -794,12 +794,13 @@ int bux_mx_unpack_rows(const uint8_t* packed, int64_t m, int64_t d, uint16_t* ou
  *             its bfloat16, in units of 2^8, so that the two hold 16 bits of z's mantissa.
  * bux_dense_units_backward: dp = (dy down^T) d act(product), the down product's gradient to its
  *   units and the activation's in one kernel. dy [m, d], down [f, d], product (and
- *   product_low, or NULL) and dp [m, f, 2] (gated) or [m, f].
+ *   product_low, or NULL) and dp [m, f, 2] (gated) or [m, f]; dp_low NULL, or dp's low bytes, for
+ *   sums over its rows.
  * bux_dense_contract: dw = x^T dy. x [m, k], dy [m, n], dw [k, n]; 0 for m = 0.
  *   Its workspace: bux_dense_workspace_size(k, n, m).
  * bux_dense_slope: dz = dy act'(product) for a plain activation (ffn and product both NULL: dy
  *   itself), and the sums of dz over its m rows before their rounding. dy, product, dz [m, n];
- *   sums [n]; dz or sums NULL where not asked for. Its workspace: bux_dense_slope_workspace_size.
+ *   sums [n]; dz or sums NULL where not asked for. dy_low: NULL, or dy's low bytes, for its sums. Its workspace: bux_dense_slope_workspace_size.
  */
 size_t bux_dense_workspace_size(int64_t m, int64_t n, int64_t k);
 int bux_dense_rows(const uint16_t* x, const uint16_t* w, int transposed, int64_t m, int64_t n,
@@ -812,7 +813,7 @@ int bux_dense_rows_f32(const float* x, const float* w, int transposed, int64_t m
                        void* stream);
 int bux_dense_units_backward(const uint16_t* dy, const uint16_t* down, int64_t m, int64_t f,
                              int64_t d, const uint16_t* product, const uint8_t* product_low,
-                             const bux_ffn* ffn, uint16_t* dp, void* workspace,
+                             const bux_ffn* ffn, uint16_t* dp, uint8_t* dp_low, void* workspace,
                              size_t workspace_bytes, void* stream);
 int bux_dense_units_backward_f32(const float* dy, const float* down, int64_t m, int64_t f,
                                  int64_t d, const float* product, const bux_ffn* ffn, float* dp,
@@ -822,9 +823,9 @@ int bux_dense_contract(const uint16_t* x, const uint16_t* dy, int64_t m, int64_t
 int bux_dense_contract_f32(const float* x, const float* dy, int64_t m, int64_t k, int64_t n,
                            float* dw, void* workspace, size_t workspace_bytes, void* stream);
 size_t bux_dense_slope_workspace_size(int64_t m, int64_t n);
-int bux_dense_slope(const uint16_t* dy, const uint16_t* product, const bux_ffn* ffn, int64_t m,
-                    int64_t n, uint16_t* dz, uint16_t* sums, void* workspace,
-                    size_t workspace_bytes, void* stream);
+int bux_dense_slope(const uint16_t* dy, const uint8_t* dy_low, const uint16_t* product,
+                    const bux_ffn* ffn, int64_t m, int64_t n, uint16_t* dz, uint16_t* sums,
+                    void* workspace, size_t workspace_bytes, void* stream);
 int bux_dense_slope_f32(const float* dy, const float* product, const bux_ffn* ffn, int64_t m,
                         int64_t n, float* dz, float* sums, void* workspace, size_t workspace_bytes,
                         void* stream);

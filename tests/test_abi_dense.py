@@ -58,8 +58,8 @@ def test_rows(lib, twin):
 def test_units_backward(lib, twin):
     def backward(dy=P, m=4, f=64, d=64, ffn=_ffn(), nbytes=0, dp=P):
         st = None if ffn is None else ctypes.byref(ffn)
-        kept = (P,) if twin else (P, None)
-        return getattr(lib, "bux_dense_units_backward" + twin)(dy, P, m, f, d, *kept, st, dp, None,
+        kept, out = ((P,), (dp,)) if twin else ((P, None), (dp, None))  # and the low bytes
+        return getattr(lib, "bux_dense_units_backward" + twin)(dy, P, m, f, d, *kept, st, *out, None,
                                                                nbytes, None)
 
     assert backward(f=0) == 1 and "bad shape" in _msg(lib)
@@ -84,9 +84,10 @@ def test_contract(lib, twin):
 
 @pytest.mark.parametrize("twin", ["", "_f32"])
 def test_slope(lib, twin):
-    def slope(dy=P, product=P, ffn=_ffn(gated=0), m=4, n=64, dz=P, sums=None):
+    def slope(dy=P, product=P, ffn=_ffn(gated=0), m=4, n=64, dz=P, sums=None, low=None):
         st = None if ffn is None else ctypes.byref(ffn)
-        return getattr(lib, "bux_dense_slope" + twin)(dy, product, st, m, n, dz, sums, None, 0, None)
+        given = (dy, product) if twin else (dy, low, product)
+        return getattr(lib, "bux_dense_slope" + twin)(*given, st, m, n, dz, sums, None, 0, None)
 
     assert slope(n=0) == 1 and "bad shape" in _msg(lib)
     assert slope(ffn=_ffn()) == 1 and "gated" in _msg(lib)
@@ -94,6 +95,9 @@ def test_slope(lib, twin):
     assert slope(ffn=None) == 1 and "product" in _msg(lib)
     assert slope(dz=None) == 1 and "nothing" in _msg(lib)
     assert slope(dy=None) == 1 and "NULL" in _msg(lib)
+    if not twin:
+        assert slope(low=P) == 1 and "low bytes" in _msg(lib)
+        assert slope(low=P, ffn=None, product=None) == 1 and "low bytes" in _msg(lib)
     assert slope(m=1 << 20, sums=P) == 2 and "workspace" in _msg(lib)
 
 

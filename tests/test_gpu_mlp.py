@@ -72,15 +72,18 @@ def test_forward_and_backward(lib, shape, p, dtype):
         dh = _v(t["dy"]) @ _v(t["down"]).t()
         _, du, dg = units(ffn, _v(kept(r.saved)), p == 2, dtype)
         parts = [times(dh, s) for s in (du, dg)[:p]]
-        dp = V(torch.stack([q.v for q in parts], -1).view(m, f * p),
-               torch.stack([q.e for q in parts], -1).view(m, f * p)).rounded(dtype)
+        exact = V(torch.stack([q.v for q in parts], -1).view(m, f * p),
+                  torch.stack([q.e for q in parts], -1).view(m, f * p))
+        dp = exact.rounded(dtype)
         up = V(_v(t["up"]).v.view(d, f * p))
         (dp @ up.t()).rounded(dtype).holds(got.x, "dx")
         dup = (_v(t["x"]).t() @ dp).rounded(dtype)
         V(dup.v.view(d, f, p), dup.e.view(d, f, p)).holds(got.up, "dup")
         (_v(r.saved.h).t() @ _v(t["dy"])).rounded(dtype).holds(got.down, "ddown")
         if biased:
-            s = dp.sum0().rounded(dtype)
+            # its 24 bits (of bfloat16), not the 16 that the products take
+            low = 2.0 ** -15 * (exact.v.abs() + exact.e) if dtype == BF16 else 0.0
+            s = V(exact.v, exact.e + low).sum0().rounded(dtype)
             V(s.v.view(f, p), s.e.view(f, p)).holds(got.up_bias, "dup_bias")
             _v(t["dy"]).sum0().rounded(dtype).holds(got.down_bias, "ddown_bias")
         else:

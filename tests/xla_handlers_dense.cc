@@ -16,15 +16,15 @@ int bux_dense_rows_f32(const float*, const float*, int, int64_t, int64_t, int64_
                        const bux_ffn*, const float*, float*, float*, void*, size_t,
                        void*) { return ++calls, 0; }
 int bux_dense_units_backward(const uint16_t*, const uint16_t*, int64_t, int64_t, int64_t,
-                             const uint16_t*, const uint8_t*, const bux_ffn*, uint16_t*, void*,
-                             size_t, void*) { return ++calls, 0; }
+                             const uint16_t*, const uint8_t*, const bux_ffn*, uint16_t*, uint8_t*,
+                             void*, size_t, void*) { return ++calls, 0; }
 int bux_dense_units_backward_f32(const float*, const float*, int64_t, int64_t, int64_t, const float*,
                                  const bux_ffn*, float*, void*, size_t, void*) { return ++calls, 0; }
 int bux_dense_contract(const uint16_t*, const uint16_t*, int64_t, int64_t, int64_t, uint16_t*, void*,
                        size_t, void*) { return ++calls, 0; }
 int bux_dense_contract_f32(const float*, const float*, int64_t, int64_t, int64_t, float*, void*,
                            size_t, void*) { return ++calls, 0; }
-int bux_dense_slope(const uint16_t*, const uint16_t*, const bux_ffn*, int64_t, int64_t, uint16_t*,
+int bux_dense_slope(const uint16_t*, const uint8_t*, const uint16_t*, const bux_ffn*, int64_t, int64_t, uint16_t*,
                     uint16_t*, void*, size_t, void*) { return ++calls, 0; }
 int bux_dense_slope_f32(const float*, const float*, const bux_ffn*, int64_t, int64_t, float*, float*,
                         void*, size_t, void*) { return ++calls, 0; }
@@ -93,17 +93,20 @@ int main() {
   with(&Rows::gated, int64_t{1}).call(false);  // out of half the columns
 
   auto units = [](bool taken, DataType t, Dims dy, Dims down, Dims product, Dims dp, int64_t gated,
-                  Dims low = {0}) {
+                  Dims low = {0}, Dims dp_low = {0}) {
     line("units backward", taken,
          DenseUnitsBackward(nullptr, buffer(t, dy), buffer(t, down), buffer(t, product), buffer(U, low), 0,
                             gated, 0,
-                            0.0f, 0, 0.0f, 0.0f, result(t, dp), result(U, {64})));
+                            0.0f, 0, 0.0f, 0.0f, result(t, dp), result(U, dp_low),
+                            result(U, {64})));
   };
   units(true, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1);
   units(true, F, {6, 32}, {10, 32}, {6, 10}, {6, 10}, 0);
   units(true, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1, {6, 10, 2});
   units(false, F, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1, {6, 10, 2});
   units(false, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1, {6, 10});
+  units(true, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1, {0}, {6, 10, 2});
+  units(false, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10, 2}, 1, {0}, {5, 10, 2});
   units(false, BF, {6, 32}, {10, 31}, {6, 10, 2}, {6, 10, 2}, 1);
   units(false, BF, {6, 32}, {10, 32}, {6, 10}, {6, 10, 2}, 1);
   units(false, BF, {6, 32}, {10, 32}, {6, 10, 2}, {6, 10}, 1);
@@ -118,13 +121,17 @@ int main() {
   contract(false, BF, BF, {6, 32}, {5, 10}, {32, 10});
   contract(false, BF, BF, {6, 32}, {6, 10}, {32, 11});
 
-  auto slope = [](bool taken, DataType t, Dims product, int64_t activation, Dims dz, Dims sums) {
+  auto slope = [](bool taken, DataType t, Dims product, int64_t activation, Dims dz, Dims sums,
+                  Dims low = {0}) {
     line("slope", taken,
-         DenseSlope(nullptr, buffer(t, {6, 20}), buffer(t, product), activation, 0, 0, 0.0f, 0, 0.0f,
+         DenseSlope(nullptr, buffer(t, {6, 20}), buffer(U, low), buffer(t, product), activation, 0, 0, 0.0f, 0, 0.0f,
                     0.0f, result(t, dz), result(t, sums), result(U, {64})));
   };
   slope(true, BF, {6, 20}, 0, {6, 20}, {20});
   slope(true, F, {0}, -1, {0}, {20});
+  slope(true, BF, {0}, -1, {0}, {20}, {6, 20});
+  slope(false, BF, {0}, -1, {0}, {20}, {6, 21});
+  slope(false, F, {0}, -1, {0}, {20}, {6, 20});
   slope(false, BF, {6, 19}, 0, {6, 20}, {20});
   slope(false, BF, {6, 20}, 0, {6, 21}, {20});
   slope(false, BF, {6, 20}, 0, {6, 20}, {6});
