@@ -66,9 +66,10 @@ def clipped(grads: Sequence[torch.Tensor], max_norm: float, in_place: bool = Fal
     if not max_norm > 0:
         raise ValueError(f"clipped: max_norm {max_norm} is not above 0")
     require(*grads)
-    if in_place and len({g.data_ptr() for g in grads if g.numel()}) != sum(
-            1 for g in grads if g.numel()):
-        raise ValueError("clipped: the same memory twice in one list, in place")
+    if in_place:
+        spans = sorted((g.data_ptr(), g.numel() * g.element_size()) for g in grads if g.numel())
+        if any(a + size > b for (a, size), (b, _) in zip(spans, spans[1:])):
+            raise ValueError("clipped: the same memory twice in one list, in place")
     with on_device(grads[0]):
         outs = list(grads) if in_place else [torch.empty_like(g) for g in grads]
         return Clipped(outs, _run("clipped", grads, outs, float(max_norm)))

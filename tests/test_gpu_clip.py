@@ -112,6 +112,10 @@ def test_a_tensor_twice(lib):
     assert torch.equal(r.grads[0], r.grads[1]) and torch.allclose(r.grads[0], x / 2)
     with pytest.raises(ValueError, match="twice"):
         clip.clipped([x, x], 15.0, in_place=True)
+    with pytest.raises(ValueError, match="twice"):  # a part of another's memory
+        clip.clipped([x[40:], x[10:41], x[:10]], 15.0, in_place=True)
+    apart = clip.clipped([x[25:], x[:25]], 3.0, in_place=True)
+    assert torch.equal(torch.cat([apart.grads[1], apart.grads[0]]), x)
 
 
 def test_captured(lib):

@@ -13,7 +13,11 @@ pytestmark = pytest.mark.gpu
 # long K (K in parts), no rows, whole tiles
 SHAPES = [(1, 1, 1), (1, 7, 9), (3, 64, 8), (1, 2048, 256), (17, 300, 33), (33, 129, 130),
           (128, 64, 128), (129, 65, 257), (64, 4100, 72), (200, 1443, 1027), (300, 512, 264),
-          (0, 64, 32), (256, 256, 512), (513, 96, 520), (16, 7168, 96), (5, 96, 2880)]
+          (0, 64, 32), (256, 256, 512), (513, 96, 520), (16, 7168, 96), (5, 96, 2880),
+          # few rows: one to four blocks of 16, K in parts and whole, cut steps, columns of no whole
+          # 64s, enough columns for one part
+          (16, 520, 264), (20, 1032, 264), (40, 2048, 1000), (48, 1000, 4104), (64, 4096, 136),
+          (64, 72, 12296), (65, 512, 64)]
 
 
 def _make(g, dtype, m, k, n, transposed=False):

@@ -13,7 +13,9 @@ pytestmark = pytest.mark.gpu
 
 # m, k, n
 SHAPES = [(4352, 8, 4608), (4100, 64, 4104), (3400, 72, 4104), (4352, 128, 4608), (4096, 192, 4096),
-          (4097, 200, 3928), (5000, 320, 2824), (260, 456, 51208), (33000, 136, 520)]
+          (4097, 200, 3928), (5000, 320, 2824), (260, 456, 51208), (33000, 136, 520),
+          # K in parts, whole and cut
+          (1024, 4096, 4096), (1000, 4104, 4000), (520, 7168, 4096)]
 
 
 def _randn(g, *shape, scale=1.0):
@@ -46,7 +48,8 @@ def test_product(lib, shape, transposed):
 
 
 @pytest.mark.parametrize("shape", [(8, 4352, 4608), (72, 4104, 3400), (200, 3928, 4104),
-                                   (456, 260, 51208), (1001, 4096, 4096)], ids=str)
+                                   (456, 260, 51208), (1001, 4096, 4096), (4096, 1024, 4096),
+                                   (8200, 2048, 1032)], ids=str)
 def test_weight_grad(lib, shape):
     from bux_amd import dense
 
@@ -58,7 +61,8 @@ def test_weight_grad(lib, shape):
 
 
 @pytest.mark.parametrize("gated", [True, False], ids=["gated", "plain"])
-@pytest.mark.parametrize("shape", [(4100, 136, 4104), (8200, 64, 1928), (3000, 264, 5000)], ids=str)
+@pytest.mark.parametrize("shape", [(4100, 136, 4104), (8200, 64, 1928), (3000, 264, 5000),
+                                   (1024, 4096, 2048)], ids=str)
 def test_block(lib, shape, gated):
     from bux_amd import mlp
     from bux_amd.moe import Ffn
