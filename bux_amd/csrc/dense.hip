@@ -6,7 +6,7 @@
 //
 // A workgroup of 4 waves makes 128 x 128 of the output, a wave 64 x 64 of it, in steps of 128
 // bytes of K (64 bfloat16, 32 float32). A step's operands come into registers 16 bytes a load at
-// an element's alignment, a step ahead, then into one of two LDS stages of 32 KiB:
+// an element's alignment, two steps ahead, then into one of two LDS stages of 32 KiB:
 //   K-major (x; w transposed)   128 rows of 128 bytes, 16-byte chunk c of row r at place
 //                               c ^ (r % 8), so that 16 lanes that read one chunk of 16 rows
 //                               take every bank twice at most
@@ -230,25 +230,30 @@ __global__ __launch_bounds__(THREADS, 2) void tile_kernel(Mat<T> A, Mat<T> B, in
       for (int j = 0; j < 16; ++j) acc[p][q][j] = 0.0f;
   Loader<T, AKM> la(A, row, k0, k, kend);
   Loader<T, BKM> lb(B, col, k0, k, kend);
-  Chunk a[4], b[4];
-  if (k0 < kend) {
-    la.step(a, k0, kend);
-    lb.step(b, k0, kend);
-  }
-  int stage = 0;
-  for (int64_t at = k0; at < kend; at += BK<T>) {
-    uint8_t* const s = lds + stage * STAGE;
-    put_step<T, AKM>(s, a);
-    put_step<T, BKM>(s + STAGE / 2, b);
+  // Two steps' operands are on their way while a third is multiplied.
+  struct Step {
+    Chunk a[4], b[4];
+  };
+  auto load = [&](Step& o, int64_t at) {
+    if (at >= kend) return;
+    la.step(o.a, at, kend);
+    lb.step(o.b, at, kend);
+  };
+  auto turn = [&](Step& o, int64_t at, uint8_t* s) {
+    put_step<T, AKM>(s, o.a);
+    put_step<T, BKM>(s + STAGE / 2, o.b);
     // The last step's reads of the other stage are behind this barrier, so the next step's
     // writes may follow it.
     __syncthreads();
-    if (at + BK<T> < kend) {
-      la.step(a, at + BK<T>, kend);
-      lb.step(b, at + BK<T>, kend);
-    }
+    load(o, at + 2 * BK<T>);
     multiply<T, AKM, BKM>(s, s + STAGE / 2, wm, wn, acc);
-    stage ^= 1;
+  };
+  Step even, odd;
+  load(even, k0);
+  load(odd, k0 + BK<T>);
+  for (int64_t at = k0; at < kend; at += 2 * BK<T>) {
+    turn(even, at, lds);
+    if (at + BK<T> < kend) turn(odd, at + BK<T>, lds + STAGE);
   }
   __syncthreads();
   uint8_t* const region = lds + wave * (2 * UNIT_BYTES);
