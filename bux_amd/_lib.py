@@ -63,9 +63,6 @@ class GradientStruct(ctypes.Structure):
         ("dtype", ctypes.c_int32),
     ]
 
-
-gradients = ctypes.POINTER(GradientStruct)
-
 # name -> (restype, argtypes), as include/bux_amd.h declares them.
 SIGNATURES = {
     "bux_last_error": (ctypes.c_char_p, []),
@@ -195,7 +192,7 @@ SIGNATURES = {
     "bux_dense_slope": (_int, [_p, _p, _p, _ffn, _i64, _i64, _p, _p, _p, _size, _p]),
     "bux_dense_slope_f32": (_int, [_p, _p, _ffn, _i64, _i64, _p, _p, _p, _size, _p]),
     "bux_clip_workspace_size": (_size, [_i32]),
-    "bux_clip": (_int, [gradients, _i32, _f32, _p, _p, _size, _p]),
+    "bux_clip": (_int, [_p, _i32, _f32, _p, _p, _size, _p]),
 }
 
 # Constants of include/bux_amd.h.

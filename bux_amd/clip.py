@@ -26,15 +26,15 @@ _DTYPES = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 def _list(name: str, grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None):
     """The gradients as ``bux_gradient``s, which are 4 words each."""
     words = []
-    device = grads[0].device
-    for i, g in enumerate(grads):
+    device = grads[0].get_device()
+    for g, out in zip(grads, outs or grads):
         dtype = _DTYPES.get(g.dtype)
         if dtype is None:
-            raise TypeError(f"{name}: gradient {i} is bfloat16 or float32, not {g.dtype}")
-        if g.device != device:
-            raise ValueError(f"{name}: gradient {i} on {g.device} beside {device}")
-        words += (g.data_ptr(), 0 if outs is None else outs[i].data_ptr(), g.numel(), dtype)
-    return ctypes.cast((ctypes.c_int64 * len(words))(*words), _lib.gradients)
+            raise TypeError(f"{name}: gradients are bfloat16 or float32, not {g.dtype}")
+        if g.get_device() != device:
+            raise ValueError(f"{name}: a gradient on {g.device} beside {grads[0].device}")
+        words += (g.data_ptr(), 0 if outs is None else out.data_ptr(), g.numel(), dtype)
+    return (ctypes.c_int64 * len(words))(*words)
 
 
 def _run(name: str, grads: Sequence[torch.Tensor], outs, max_norm: float) -> torch.Tensor:

@@ -295,42 +295,37 @@ struct Plan {
   int64_t splits;
 };
 
-// About how many microseconds `splits` parts of K take, fitted to measured times (201 x 2880 x 5760 up
-// to 8192 x 7168 x 4096, within a quarter): a launch; a 256 x 256 tile's unit of 64 K takes a CU
-// 1.2, a 128 x 128 tile's step 0.73 where it has the CU to itself and 1.15 beside another (float32: 2.7
-// and 4.1, its MFMAs); the parts' join is a launch and their sums written and read.
-double cost_of(Form form, bool f32, int64_t m, int64_t n, int64_t k, int64_t splits) {
-  const int64_t side = form == Form::LARGE ? 256 : TILE, bk = f32 ? 32 : 64;
-  const int64_t jobs = ceil_div(m, side) * ceil_div(n, side) * splits;
-  const double steps = static_cast<double>(ceil_div(ceil_div(k, bk), splits));
-  double t = 5;
-  if (form == Form::LARGE) {
-    t += static_cast<double>(ceil_div(jobs, 256)) * (1.2 * steps + 5);
-  } else {
-    const double alone = f32 ? 2.7 : 0.73, beside = f32 ? 4.1 : 1.15;
-    const int64_t pairs = jobs / 512, rest = jobs - 512 * pairs;
-    t += static_cast<double>(pairs) * (beside * steps + 2);
-    if (rest > 0) t += (rest > 256 ? beside : alone) * steps + 2;
-  }
-  if (splits > 1) t += 2.5 + static_cast<double>(splits) * m * n * 8e-7;
-  return t;
-}
-// No part has no steps.
-int64_t whole_splits(int64_t steps, int64_t splits) {
-  return ceil_div(steps, ceil_div(steps, splits));
-}
-Plan plan_of(bool f32, bool large, bool few, int64_t m, int64_t n, int64_t k) {
-  if (few) return Plan{Form::FEW, few_splits(n, k)};
+// The tiles and the parts of K that take the fewest microseconds by a fit to measured times (300 x
+// 512 x 512 up to 8192 x 7168 x 4096, within a quarter): a launch; a 256 x 256 tile's unit of 64 K
+// takes a CU 1.2, a 128 x 128 tile's step 0.7 where it has the CU to itself and 1.15 beside another
+// (float32: 2.7 and 4.1, its MFMAs); the parts' join is a launch and their sums written and read.
+// (1024 x 4096 x 4096: large tiles in 4 parts 48.2 us, 128s 53.4; 2048^3: 128s 30.7, large ones 36.6 at
+// best; 201 x 2880 x 5760: 128s in 4 parts 25.4, in one 36.7.)
+Plan cheapest(bool f32, bool large, int64_t m, int64_t n, int64_t k) {
   Plan best{Form::TILE, 1};
   double least = 1e30;
   for (const Form form : {Form::TILE, Form::LARGE}) {
     if (form == Form::LARGE && !large) continue;
-    const int64_t side = form == Form::LARGE ? 256 : TILE;
+    const bool big = form == Form::LARGE;
+    const int64_t side = big ? 256 : TILE;
     const int64_t tiles = ceil_div(m, side) * ceil_div(n, side);
-    const int64_t steps = ceil_div(k, form == Form::TILE && f32 ? 32 : 64);
-    for (int64_t s = 1; s <= 32 && s <= steps && (s == 1 || s * tiles <= 768); s += s < 4 ? 1 : s / 4) {
-      const int64_t splits = steps > 0 ? whole_splits(steps, s) : 1;
-      const double t = cost_of(form, f32, m, n, k, splits);
+    const int64_t steps = ceil_div(k, !big && f32 ? 32 : 64);
+    const double alone = f32 ? 2.7 : 0.7, beside = f32 ? 4.1 : 1.15;
+    for (int64_t s = 1; s <= 32 && s <= (steps > 1 ? steps : 1) && (s == 1 || s * tiles <= 768);
+         s += s < 4 ? 1 : s / 4) {
+      // no part has no steps
+      const int64_t each = ceil_div(steps, s), splits = s == 1 ? 1 : ceil_div(steps, each);
+      const int64_t jobs = tiles * splits;
+      const double part = static_cast<double>(each);
+      double t = 5;
+      if (big) {
+        t += static_cast<double>((jobs + 255) >> 8) * (1.2 * part + 5);
+      } else {
+        const int64_t rest = jobs & 511;
+        t += static_cast<double>(jobs >> 9) * (beside * part + 2);
+        if (rest > 0) t += (rest > 256 ? beside : alone) * part + 2;
+      }
+      if (splits > 1) t += 2.5 + static_cast<double>(splits * m) * n * 8e-7;
       if (t < least) {
         least = t;
         best = Plan{form, splits};
@@ -338,6 +333,20 @@ Plan plan_of(bool f32, bool large, bool few, int64_t m, int64_t n, int64_t k) {
     }
   }
   return best;
+}
+// ... kept for the shapes that this thread asked for last: a call asks several times.
+Plan plan_of(bool f32, bool large, bool few, int64_t m, int64_t n, int64_t k) {
+  if (few) return Plan{Form::FEW, few_splits(n, k)};
+  struct Entry {
+    int64_t m, n, k;
+    Plan plan;
+  };
+  static thread_local Entry kept[64] = {};
+  const uint64_t at = (static_cast<uint64_t>(m) * 31 + static_cast<uint64_t>(n) * 7 +
+                       static_cast<uint64_t>(k)) % 16;
+  Entry& e = kept[at * 4 + (f32 ? 2 : 0) + (large ? 1 : 0)];
+  if (e.m != m || e.n != n || e.k != k) e = Entry{m, n, k, cheapest(f32, large, m, n, k)};
+  return e.plan;
 }
 
 // What any form may ask for: the operands' alignment decides between them, which is not known here.

@@ -76,14 +76,14 @@ __global__ __launch_bounds__(THREADS) void few_kernel(const uint16_t* __restrict
 #pragma unroll
     for (int j = 0; j < BLOCKS_N; ++j) {
       if constexpr (BKM)
-        load_lds16_uniform(rb, at + j * 1024, vb + 16 * in_row, s * (STEP * 2) + j * 16 * k * 2);
+        load_lds16(rb, at + j * 1024, vb + 16 * in_row, s * (STEP * 2) + j * 16 * k * 2);
       else  // rows 8 j ..: their k / 8 is j's
-        load_lds16_uniform(rb, at + j * 1024, vb + 16 * (in_row ^ (4 * (j & 1))),
+        load_lds16(rb, at + j * 1024, vb + 16 * (in_row ^ (4 * (j & 1))),
                            (s * STEP + 8 * j) * n * 2);
     }
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
-      load_lds16_uniform(ra, at + (BLOCKS_N + b) * 1024, va, s * (STEP * 2) + b * 16 * k * 2);
+      load_lds16(ra, at + (BLOCKS_N + b) * 1024, va, s * (STEP * 2) + b * 16 * k * 2);
   };
 
   const int g = lane >> 4, r = lane & 15;
