@@ -1,5 +1,5 @@
 """The dense feed-forward block on MI355X, gated or plain, and its backward: a model's ``mlp``
-and ``gated_mlp`` layers (src/bux/architecture/layers/mlp.py:20-61), a shared expert beside the
+and ``gated_mlp`` layers (src/bux/architecture/layers/mlp.py:20-35), a shared expert beside the
 routed ones, with the activation settings of `moe.Ffn`.
 
 The up and gate projections, the activation and their product are one kernel (the up product's

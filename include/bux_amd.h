@@ -778,7 +778,7 @@ int bux_mx_unpack_rows(const uint8_t* packed, int64_t m, int64_t d, uint16_t* ou
 
 /* ---------------------------------------------------------------------------------
  * Dense products beside the experts: a layer's projections, its dense feed-forward block
- * (layers/mlp.py:20-61 of the reference's mlp and gated_mlp) and their backward. bfloat16, and
+ * (layers/mlp.py:20-35 of the reference's mlp and gated_mlp) and their backward. bfloat16, and
  * float32 twins (_f32) whose products and sums are float32's; any shape below 2^31 a side, any
  * alignment; float32 sums in a fixed order. A workspace of bux_dense_workspace_size(rows of the
  * output, columns of the sums, the contracted length) bytes, 16-byte aligned (0: none needed).
