@@ -4,8 +4,8 @@
 //   rows      y = epilogue(x w)     w [k, n], or [n, k] (transposed: x w^T)
 //   contract  dw = x^T dy           x [m, k], dy [m, n]
 //
-// A workgroup of 4 waves makes 128 x 128 of the output, a wave 64 x 64 of it, in steps of 128
-// bytes of K (64 bfloat16, 32 float32). A step's operands come into registers 16 bytes a load at
+// A workgroup of 4 waves makes 128 x 128 of the output, a wave 64 x 64 of it (in float32 also 128 x
+// 64, which leave less of a narrow or an odd output to nothing), in steps of 128 bytes of K (64 bfloat16, 32 float32). A step's operands come into registers 16 bytes a load at
 // an element's alignment, two steps ahead, then into one of two LDS stages of 32 KiB:
 //   K-major (x; w transposed)   128 rows of 128 bytes, 16-byte chunk c of row r at place
 //                               c ^ (r % 8), so that 16 lanes that read one chunk of 16 rows
@@ -31,7 +31,6 @@ typedef __attribute__((address_space(3))) v4s lds_v4s;
 
 constexpr int THREADS = 256;
 constexpr int TILE = 128;
-constexpr int STAGE = 2 * TILE * 128;  // bytes: both operands of a step
 
 template <typename T>
 constexpr int BK = 128 / sizeof(T);
@@ -61,12 +60,13 @@ __device__ __forceinline__ Chunk load_chunk(const T* p, int64_t count) {
   return __builtin_bit_cast(Chunk, e);
 }
 
-// A thread's 4 chunks of an operand's step: K-major chunk i is of row 32 i + tid / 8 at K chunk
+// A thread's chunks of an operand's step, SIDE rows of it: K-major chunk i is of row 32 i + tid / 8 at K chunk
 // tid % 8; MN-major of K row (256 i + tid) / (chunks a K row). K is `k` long in all.
-template <typename T, bool KM>
+template <typename T, bool KM, int SIDE>
 struct Loader {
-  static constexpr int ROW = KM ? 8 : TILE / PER<T>;  // chunks a row, or a K row
-  const T* at[4];
+  static constexpr int ROW = KM ? 8 : SIDE / PER<T>;  // chunks a row, or a K row
+  static constexpr int N = SIDE / 32;                 // chunks a thread
+  const T* at[N];
   int64_t ld, left;  // MN-major: columns from this lane's on
   int64_t plain;     // steps that end at or before this K position load without a check
   __device__ __forceinline__ Loader(const Mat<T>& a, int64_t row0, int64_t k0, int64_t k,
@@ -75,7 +75,7 @@ struct Loader {
     const int tid = threadIdx.x, c = tid % ROW;
     left = a.rows - row0 - PER<T> * c;
     plain = kend;
-    if (!KM && row0 + TILE > a.rows) {
+    if (!KM && row0 + SIDE > a.rows) {
       // The tile reaches past the columns. A chunk that they cut reads on into the next K row (its
       // columns are no output's), which the last K row does not have; the lanes past them read the
       // row's last chunk.
@@ -84,7 +84,7 @@ struct Loader {
     }
     const int64_t col = left > 0 || a.rows < PER<T> ? row0 + PER<T> * c : a.rows - PER<T>;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
       const int s = i * (THREADS / ROW) + tid / ROW;
       if (KM) {
         const int64_t r = row0 + s;
@@ -95,30 +95,30 @@ struct Loader {
     }
   }
   // The step at K position k (its first), K ending at kend; then on to the next.
-  __device__ __forceinline__ void step(Chunk out[4], int64_t k, int64_t kend) {
+  __device__ __forceinline__ void step(Chunk out[N], int64_t k, int64_t kend) {
     const int tid = threadIdx.x;
     if (k + BK<T> <= plain) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) out[i] = load_chunk(at[i]);
+      for (int i = 0; i < N; ++i) out[i] = load_chunk(at[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < N; ++i) {
         const int s = i * (THREADS / ROW) + tid / ROW;
         const int64_t count = KM ? kend - k - PER<T> * (tid % ROW) : k + s < kend ? left : 0;
         out[i] = load_chunk(at[i], count);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) at[i] += KM ? BK<T> : BK<T> * ld;
+    for (int i = 0; i < N; ++i) at[i] += KM ? BK<T> : BK<T> * ld;
   }
 };
 
-template <typename T, bool KM>
-__device__ __forceinline__ void put_step(uint8_t* lds, const Chunk c[4]) {
-  constexpr int ROW = KM ? 8 : TILE / PER<T>;
+template <typename T, bool KM, int SIDE>
+__device__ __forceinline__ void put_step(uint8_t* lds, const Chunk c[SIDE / 32]) {
+  constexpr int ROW = KM ? 8 : SIDE / PER<T>;
   const int tid = threadIdx.x, place = tid % ROW;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < SIDE / 32; ++i) {
     const int s = i * (THREADS / ROW) + tid / ROW;
     const int sw = KM ? (s & 7) : sizeof(T) == 2 ? 4 * (s & 3) : 8 * ((s >> 3) & 1);
     *reinterpret_cast<Chunk*>(lds + s * (16 * ROW) + 16 * (place ^ sw)) = c[i];
@@ -144,7 +144,7 @@ __device__ __forceinline__ v8bf read_bf16(const uint8_t* lds, int base, int s) {
   }
 }
 // float32: 8 of them, for K 16 s + 8 (l / 32) + 0 .. 7.
-template <bool KM>
+template <bool KM, int SIDE>
 __device__ __forceinline__ void read_f32(const uint8_t* lds, int base, int s, float v[8]) {
   const int l = threadIdx.x & 63, h = l >> 5, r = base + (l & 31);
   if constexpr (KM) {
@@ -157,58 +157,60 @@ __device__ __forceinline__ void read_f32(const uint8_t* lds, int base, int s, fl
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int k = 16 * s + 8 * h + j;
-      v[j] = *reinterpret_cast<const float*>(lds + k * 512 + 16 * ((r >> 2) ^ (8 * h)) +
+      v[j] = *reinterpret_cast<const float*>(lds + k * (4 * SIDE) + 16 * ((r >> 2) ^ (8 * h)) +
                                              4 * (r & 3));
     }
   }
 }
 
-template <typename T, bool AKM, bool BKM>
-__device__ __forceinline__ void multiply(const uint8_t* a, const uint8_t* b, int wm, int wn,
-                                         f32x16 acc[2][2]) {
+// A wave's part of a step: P x Q blocks of 32 x 32 from row and col on.
+template <typename T, bool AKM, bool BKM, int P, int Q, int SIDE_N>
+__device__ __forceinline__ void multiply(const uint8_t* a, const uint8_t* b, int row, int col,
+                                         f32x16 acc[P][Q]) {
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      v8bf x[2], y[2];
+      v8bf x[P], y[Q];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        x[p] = read_bf16<AKM>(a, wm * 64 + p * 32, s);
-        y[p] = read_bf16<BKM>(b, wn * 64 + p * 32, s);
-      }
+      for (int p = 0; p < P; ++p) x[p] = read_bf16<AKM>(a, row + p * 32, s);
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+      for (int q = 0; q < Q; ++q) y[q] = read_bf16<BKM>(b, col + q * 32, s);
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
           acc[p][q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[q], x[p], acc[p][q], 0, 0, 0);
     }
   } else {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      float x[2][8], y[2][8];
+      float x[P][8], y[Q][8];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        read_f32<AKM>(a, wm * 64 + p * 32, s, x[p]);
-        read_f32<BKM>(b, wn * 64 + p * 32, s, y[p]);
-      }
+      for (int p = 0; p < P; ++p) read_f32<AKM, TILE>(a, row + p * 32, s, x[p]);
+#pragma unroll
+      for (int q = 0; q < Q; ++q) read_f32<BKM, SIDE_N>(b, col + q * 32, s, y[q]);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
+        for (int p = 0; p < P; ++p)
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
+          for (int q = 0; q < Q; ++q)
             acc[p][q] = __builtin_amdgcn_mfma_f32_32x32x2f32(y[q][j], x[p][j], acc[p][q], 0, 0, 0);
     }
   }
 }
 
 // C[r][c] = sum over K of A(r, k) B(c, k), K [0, k) in `splits` parts of `part` each: with one
-// part `epi` takes the sums, else `partial` (part i's m rows after those before it).
-template <typename T, bool AKM, bool BKM, typename Epi>
-__global__ __launch_bounds__(THREADS, 2) void tile_kernel(Mat<T> A, Mat<T> B, int64_t m, int64_t n,
-                                                          int64_t k, int64_t part, int64_t splits,
-                                                          Epi epi) {
+// part `epi` takes the sums, else `partial` (part i's m rows after those before it). Tiles of 128
+// rows and SIDE_N columns, 128 (a wave 64 x 64) or 64 (a wave 32 x 64).
+template <typename T, bool AKM, bool BKM, int SIDE_N, typename Epi>
+__global__ __launch_bounds__(THREADS, SIDE_N == 64 ? 3 : 2) void tile_kernel(
+    Mat<T> A, Mat<T> B, int64_t m, int64_t n, int64_t k, int64_t part, int64_t splits, Epi epi) {
+  constexpr int P = SIDE_N / 64, Q = 2;
+  constexpr int A_BYTES = TILE * 128, STAGE = A_BYTES + SIDE_N * 128;
+  static_assert(2 * STAGE >= 4 * P * UNIT_BYTES, "the outputs' units fit");
   __shared__ __align__(16) uint8_t lds[2 * STAGE];
-  const int64_t row_tiles = (m + TILE - 1) / TILE, col_tiles = (n + TILE - 1) / TILE;
+  const int64_t row_tiles = (m + TILE - 1) / TILE, col_tiles = (n + SIDE_N - 1) / SIDE_N;
   const int64_t tiles = row_tiles * col_tiles, count = tiles * splits;
   // an XCD (workgroup id % 8) takes a contiguous run
   const int64_t id = (blockIdx.x % 8) * ((count + 7) / 8) + blockIdx.x / 8;
@@ -218,21 +220,22 @@ __global__ __launch_bounds__(THREADS, 2) void tile_kernel(Mat<T> A, Mat<T> B, in
   place_of(static_cast<int32_t>(id - split * tiles), static_cast<int32_t>(row_tiles),
            static_cast<int32_t>(col_tiles), &row_tile, &col_tile);
   const int64_t row = static_cast<int64_t>(row_tile) * TILE;
-  const int64_t col = static_cast<int64_t>(col_tile) * TILE;
+  const int64_t col = static_cast<int64_t>(col_tile) * SIDE_N;
   const int64_t k0 = split * part, kend = k0 + part < k ? k0 + part : k;
-  const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  f32x16 acc[2][2];
+  const int wave = threadIdx.x >> 6;
+  const int wrow = P == 2 ? 64 * (wave >> 1) : 32 * wave, wcol = P == 2 ? 64 * (wave & 1) : 0;
+  f32x16 acc[P][Q];
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
+  for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+    for (int q = 0; q < Q; ++q)
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[p][q][j] = 0.0f;
-  Loader<T, AKM> la(A, row, k0, k, kend);
-  Loader<T, BKM> lb(B, col, k0, k, kend);
+  Loader<T, AKM, TILE> la(A, row, k0, k, kend);
+  Loader<T, BKM, SIDE_N> lb(B, col, k0, k, kend);
   // Two steps' operands are on their way while a third is multiplied.
   struct Step {
-    Chunk a[4], b[4];
+    Chunk a[TILE / 32], b[SIDE_N / 32];
   };
   auto load = [&](Step& o, int64_t at) {
     if (at >= kend) return;
@@ -240,13 +243,13 @@ __global__ __launch_bounds__(THREADS, 2) void tile_kernel(Mat<T> A, Mat<T> B, in
     lb.step(o.b, at, kend);
   };
   auto turn = [&](Step& o, int64_t at, uint8_t* s) {
-    put_step<T, AKM>(s, o.a);
-    put_step<T, BKM>(s + STAGE / 2, o.b);
+    put_step<T, AKM, TILE>(s, o.a);
+    put_step<T, BKM, SIDE_N>(s + A_BYTES, o.b);
     // The last step's reads of the other stage are behind this barrier, so the next step's
     // writes may follow it.
     __syncthreads();
     load(o, at + 2 * BK<T>);
-    multiply<T, AKM, BKM>(s, s + STAGE / 2, wm, wn, acc);
+    multiply<T, AKM, BKM, P, Q, SIDE_N>(s, s + A_BYTES, wrow, wcol, acc);
   };
   Step even, odd;
   load(even, k0);
@@ -256,15 +259,15 @@ __global__ __launch_bounds__(THREADS, 2) void tile_kernel(Mat<T> A, Mat<T> B, in
     if (at + BK<T> < kend) turn(odd, at + BK<T>, lds + STAGE);
   }
   __syncthreads();
-  uint8_t* const region = lds + wave * (2 * UNIT_BYTES);
-  put_unit(region, acc[0][0], acc[0][1]);
-  put_unit(region + UNIT_BYTES, acc[1][0], acc[1][1]);
+  uint8_t* const region = lds + wave * (P * UNIT_BYTES);
+#pragma unroll
+  for (int p = 0; p < P; ++p) put_unit(region + p * UNIT_BYTES, acc[p][0], acc[p][1]);
   wave_done_lds();
   Epi mine = epi;
   if constexpr (std::is_same<Epi, Partial>::value) mine.out += split * m * epi.pitch;
 #pragma unroll 1
-  for (int u = 0; u < 2; ++u)
-    store_unit(mine, region + u * UNIT_BYTES, row + wm * 64 + u * 32, col + wn * 64, m, n);
+  for (int u = 0; u < P; ++u)
+    store_unit(mine, region + u * UNIT_BYTES, row + wrow + u * 32, col + wcol, m, n);
 }
 
 // The sums of the splits' parts, in order, through the epilogue: a thread 8 columns of a row.
@@ -289,7 +292,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(const float* __restrict__
 }
 
 // Which kernel a product runs on, and the parts of K.
-enum class Form { TILE, LARGE, FEW };
+enum class Form { TILE, NARROW, LARGE, FEW };
 struct Plan {
   Form form;
   int64_t splits;
@@ -298,17 +301,21 @@ struct Plan {
 // The tiles and the parts of K that take the fewest microseconds by a fit to measured times (300 x
 // 512 x 512 up to 8192 x 7168 x 4096, within a quarter): a launch; a 256 x 256 tile's unit of 64 K
 // takes a CU 1.2, a 128 x 128 tile's step 0.7 where it has the CU to itself and 1.15 beside another
-// (float32: 2.7 and 4.1, its MFMAs); the parts' join is a launch and their sums written and read.
+// (float32: 2.7 and 4.1, its MFMAs), a float32 128 x 64 tile's step 1.2, or 1.15 for each on the CU; the
+// parts' join is a launch and their sums written and read.
 // (1024 x 4096 x 4096: large tiles in 4 parts 48.2 us, 128s 53.4; 2048^3: 128s 30.7, large ones 36.6 at
-// best; 201 x 2880 x 5760: 128s in 4 parts 25.4, in one 36.7.)
+// best; 201 x 2880 x 5760: 128s in 4 parts 25.4, in one 36.7. float32: 128 x 64 takes 300 x 512 x 512 in
+// 12.5 us, 128 x 128 at best 14.9, 3000 x 2000 x 700 83 and 94; 1001 x 1027 x 1443 47 and 46, 1 x 4096 x
+// 4096 43 and 42.)
 Plan cheapest(bool f32, bool large, int64_t m, int64_t n, int64_t k) {
   Plan best{Form::TILE, 1};
   double least = 1e30;
-  for (const Form form : {Form::TILE, Form::LARGE}) {
+  for (const Form form : {Form::TILE, Form::NARROW, Form::LARGE}) {
     if (form == Form::LARGE && !large) continue;
-    const bool big = form == Form::LARGE;
-    const int64_t side = big ? 256 : TILE;
-    const int64_t tiles = ceil_div(m, side) * ceil_div(n, side);
+    if (form == Form::NARROW && !f32) continue;
+    const bool big = form == Form::LARGE, narrow = form == Form::NARROW;
+    const int64_t tiles =
+        ceil_div(m, big ? 256 : TILE) * ceil_div(n, big ? 256 : narrow ? TILE / 2 : TILE);
     const int64_t steps = ceil_div(k, !big && f32 ? 32 : 64);
     const double alone = f32 ? 2.7 : 0.7, beside = f32 ? 4.1 : 1.15;
     for (int64_t s = 1; s <= 32 && s <= (steps > 1 ? steps : 1) && (s == 1 || s * tiles <= 768);
@@ -320,6 +327,9 @@ Plan cheapest(bool f32, bool large, int64_t m, int64_t n, int64_t k) {
       double t = 5;
       if (big) {
         t += static_cast<double>((jobs + 255) >> 8) * (1.2 * part + 5);
+      } else if (narrow) {
+        const int64_t on = (jobs + 255) >> 8;  // a CU's
+        t += on == 1 ? 1.2 * part + 2 : 1.15 * static_cast<double>(on) * part + 2 * ((on + 2) / 3);
       } else {
         const int64_t rest = jobs & 511;
         t += static_cast<double>(jobs >> 9) * (beside * part + 2);
@@ -384,13 +394,20 @@ int run(const char* name, const Mat<T>& A, const Mat<T>& B, int64_t m, int64_t n
       if (plan.form == Form::LARGE)
         return launch_large<AKM, BKM>(A, B, m, n, k, ceil_div(ceil_div(k, 64), splits), splits, e, s);
     }
-    const int64_t blocks = 8 * ceil_div(ceil_div(m, TILE) * ceil_div(n, TILE) * splits, 8);
-    if (blocks >= (1LL << 31)) return fail(BUX_E_ARGUMENT, "%s: too many tiles", name);
-    const int64_t part = ceil_div(ceil_div(k, BK<T>), splits) * BK<T>;
-    hipLaunchKernelGGL((tile_kernel<T, AKM, BKM, std::decay_t<decltype(e)>>),
-                       dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, s, A, B, m, n, k, part,
-                       splits, e);
-    return launched("dense tile_kernel");
+    auto tiles = [&](auto side) {
+      constexpr int SIDE_N = decltype(side)::value;
+      const int64_t blocks = 8 * ceil_div(ceil_div(m, TILE) * ceil_div(n, SIDE_N) * splits, 8);
+      if (blocks >= (1LL << 31)) return fail(BUX_E_ARGUMENT, "%s: too many tiles", name);
+      const int64_t part = ceil_div(ceil_div(k, BK<T>), splits) * BK<T>;
+      hipLaunchKernelGGL((tile_kernel<T, AKM, BKM, SIDE_N, std::decay_t<decltype(e)>>),
+                         dim3(static_cast<unsigned>(blocks)), dim3(THREADS), 0, s, A, B, m, n, k,
+                         part, splits, e);
+      return launched("dense tile_kernel");
+    };
+    if constexpr (sizeof(T) == 4) {
+      if (plan.form == Form::NARROW) return tiles(std::integral_constant<int, TILE / 2>{});
+    }
+    return tiles(std::integral_constant<int, TILE>{});
   };
   if (splits == 1) return launch(epi);
   float* const parts = static_cast<float*>(workspace);
