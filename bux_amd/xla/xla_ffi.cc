@@ -389,7 +389,7 @@ static ffi::Error GluBackward(hipStream_t s, In projected, In weights, In dh, In
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxGluBackward, GluBackward,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
-                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>().Ret<In>());
+                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>());
 
 // h may be an empty result (not kept); f from the row copy's K is not exact, so it is an
 // attribute, as are m and height.
@@ -791,7 +791,7 @@ static ffi::Error Int8Glu(hipStream_t s, In projected, In weights, In filled, BU
 }
 XLA_FFI_DEFINE_HANDLER_SYMBOL(BuxInt8Glu, Int8Glu,
                               ffi::Ffi::Bind().Ctx<Stream>().Arg<In>().Arg<In>().Arg<In>()
-                                  .Arg<In>() BUX_FFN_ATTRS.Ret<In>().Ret<In>().Ret<In>());
+                                  BUX_FFN_ATTRS.Ret<In>().Ret<In>());
 
 // w [groups, k, n].
 static ffi::Error Int8QuantizeColumns(hipStream_t s, In w, Out values, Out scales) {
