@@ -614,9 +614,10 @@ int slope(const char* name, const T* dy, const uint8_t* dy_low, const T* product
   Act act;
   if (int rc = act_or_none(name, ffn, &act)) return rc;
   BUX_CHECK(!act.gated, "%s: a gated activation", name);
-  BUX_CHECK((ffn == nullptr) == (product == nullptr), "%s: an activation's gradient takes its product",
-            name);
-  BUX_CHECK(dz || sums, "%s: nothing asked for", name);
+  // (of no rows dy, product and dz are empty: their addresses may be NULL)
+  BUX_CHECK(m == 0 || (ffn == nullptr) == (product == nullptr),
+            "%s: an activation's gradient takes its product", name);
+  BUX_CHECK(m == 0 || dz || sums, "%s: nothing asked for", name);
   BUX_CHECK(dy_low == nullptr || (ffn == nullptr && dz == nullptr),
             "%s: low bytes are for dy's own sums", name);
   BUX_CHECK(m == 0 || dy, "%s: NULL buffer", name);

@@ -800,7 +800,9 @@ int bux_mx_unpack_rows(const uint8_t* packed, int64_t m, int64_t d, uint16_t* ou
  *   Its workspace: bux_dense_workspace_size(k, n, m).
  * bux_dense_slope: dz = dy act'(product) for a plain activation (ffn and product both NULL: dy
  *   itself), and the sums of dz over its m rows before their rounding. dy, product, dz [m, n];
- *   sums [n]; dz or sums NULL where not asked for. dy_low: NULL, or dy's low bytes, for its sums. Its workspace: bux_dense_slope_workspace_size.
+ *   sums [n]; dz or sums NULL where not asked for. dy_low: NULL, or dy's low bytes, for its sums.
+ *   Of no rows (m = 0) dy, product and dz may be NULL, and sums are 0. Its workspace:
+ *   bux_dense_slope_workspace_size.
  */
 size_t bux_dense_workspace_size(int64_t m, int64_t n, int64_t k);
 int bux_dense_rows(const uint16_t* x, const uint16_t* w, int transposed, int64_t m, int64_t n,
