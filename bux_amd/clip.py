@@ -57,10 +57,12 @@ def global_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
 
 
 def clipped(grads: Sequence[torch.Tensor], max_norm: float, in_place: bool = False) -> Clipped:
-    """Return the gradients times ``min(1, max_norm / norm)``, each rounded once to its dtype, and
-    their `global_norm`; with `in_place` in the gradients' own memory. A norm that is infinite
-    scales by 0, one that is NaN makes every gradient NaN. The same tensor twice in one list
-    counts twice (in place it is refused)."""
+    """Return the gradients times ``min(1, max_norm / norm)`` and their `global_norm`; with
+    `in_place` in the gradients' own memory. The factor and the products are float64's, rounded
+    once to float32 and from there to bfloat16; the factor is of the float64 norm, also where
+    the norm returned overflows float32. An infinite gradient scales by 0 (and becomes a NaN), a NaN
+    makes every gradient NaN; with an infinite `max_norm` they stay as they are. The same tensor
+    twice in one list counts twice (in place it is refused)."""
     if not grads:
         raise ValueError("clipped: no gradients")
     if not max_norm > 0:

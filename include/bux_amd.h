@@ -836,8 +836,11 @@ int bux_dense_slope_f32(const float* dy, const float* product, const bux_ffn* ff
  * The global norm of many gradients, and their clipping by it.
  *
  * norm = (sum over all gradients' elements of g^2)^(1/2), added in float64 in a fixed order;
- * out = g min(1, max_norm / norm), rounded once to g's type. An infinite norm scales by 0 (an
- * infinity becomes a NaN), a NaN makes every output NaN.
+ * out = g min(1, max_norm / norm), the factor and the product in float64, rounded once to float32
+ * and from there to bfloat16. The factor is of the float64 norm: a norm of finite gradients past
+ * float32 is returned as infinity and scales as it is. An infinite gradient scales by 0 (itself
+ * becomes a NaN), a NaN makes every output NaN; an infinite max_norm scales by 1 unless the norm is
+ * a NaN.
  *
  * grads      host array of `count`: each n elements of `dtype` at g, and where they go, out (g
  *            itself, or elsewhere; NULL in all of them: the norm alone). Read before the call
