@@ -72,11 +72,12 @@ __device__ __forceinline__ void store_some(T* p, const float* v, int64_t count) 
 
 // --- a bfloat16 value's next 8 bits ---------------------------------------------------------
 //
-// z kept as bfloat16 alone would put a rounding of 2^-9 of it into the activation's gradient beside
-// the one that d product takes to be multiplied: of a block's gradients to x and up sqrt 3 rather
-// than sqrt 2 of their outputs' own. A signed byte beside it, the difference of the float32's bits
-// from the bfloat16's in units of 2^8, keeps 16 bits of mantissa, at half the bytes that float32 would
-// add. (A value that rounds to infinity comes back finite; a NaN stays one.)
+// z kept as bfloat16 alone would put a rounding of up to 2^-8 of it into the activation's gradient
+// beside the one that d product takes to be multiplied: of a block's gradients to x and up sqrt 3
+// rather than sqrt 2 of their outputs' own. A signed byte beside it, the difference of the float32's
+// bits from the bfloat16's in units of 2^8, keeps 16 bits of mantissa, at half the bytes that float32
+// would add. (A value that bfloat16 rounds to infinity comes back finite, but for the 128 next to
+// float32's infinity; a NaN stays one.)
 
 __device__ __forceinline__ uint32_t low_byte(float z, uint32_t high) {
   const int32_t off = static_cast<int32_t>(__float_as_uint(z)) - static_cast<int32_t>(high << 16);

@@ -1,7 +1,8 @@
 """A dense matrix product on MI355X with its bias, activation and residual in the epilogue, and
 its backward: the projections around a layer's experts.
 
-float32 sums with one rounding of each output, bfloat16 or float32 throughout. `mlp` makes the
+float32 sums with one rounding of each output, bfloat16 or float32 throughout; in the backward
+with an activation the gradient before the products is rounded too. `mlp` makes the
 dense feed-forward block of them; the experts' own products are `grouped`, `grouped_mxfp8` and
 `grouped_int8`.
 """
@@ -160,7 +161,10 @@ def product_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
                      transposed: bool = False, bias: bool = False) -> ProductGrads:
     """Return the gradients of `product` to x, w and, with `bias`, its bias, given dy (..., n):
     with an activation, `product` is what the forward kept. The residual's gradient is dy. Each
-    is rounded once to x's dtype, from float32 sums."""
+    is rounded to x's dtype from float32 sums. With an activation in bfloat16, dz = dy act'(product)
+    is rounded to bfloat16 too before its products with w and x, as the MFMAs take it (a bfloat16
+    step of 2^-8 at most in each term), not before the bias's sums; and act' is taken at the kept
+    `product`, itself rounded."""
     require(dy, x, w, product)
     is_f32("product_backward", x, dy, w, product)
     k, n = _sides("product_backward", w, transposed)

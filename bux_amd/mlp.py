@@ -5,8 +5,8 @@ routed ones, with the activation settings of `moe.Ffn`.
 The up and gate projections, the activation and their product are one kernel (the up product's
 epilogue); the down product adds its bias and the residual in its own. In the backward the down
 product's gradient to the units goes through the activation's in its epilogue. bfloat16 or
-float32: float32 sums and activation, one rounding of each output and of the units between the
-products.
+float32: float32 sums and activation, one rounding of each output, of the units and of the
+projections' gradient between the products.
 """
 
 import ctypes
@@ -64,9 +64,10 @@ def feed_forward(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, ffn: Ffn
     """Return ``h down + down_bias + residual`` with ``h = act(gate) (up + offset)`` of ``x up +
     up_bias`` for the rows x (..., d): up (d, f, 2), [..., 0] up and [..., 1] gate, or (d, f, 1)
     for a plain block, ``h = act(up)``; down (f, d); up_bias (f, p), down_bias (d,), residual x's
-    shape. All in x's dtype, bfloat16 or float32. With `keep` it keeps what
-    `feed_forward_backward` takes; without, as for serving, the projections are never in
-    memory."""
+    shape. All in x's dtype, bfloat16 or float32; h is rounded to it before its product with down.
+    With `keep` it keeps what `feed_forward_backward` takes (bfloat16: 3 bytes a projection, 2 of
+    `projected` and 1 of `low`, and 2 a unit); without, as for serving, the projections are never
+    in memory."""
     require(x, up, down, up_bias, down_bias, residual)
     is_f32("feed_forward", x, up, down, up_bias, down_bias, residual)
     d, f, p = _kernels("feed_forward", up, down)
@@ -115,7 +116,9 @@ def feed_forward_backward(dy: torch.Tensor, saved: Saved, up: torch.Tensor, down
                           ffn: Ffn = Ffn(), bias: bool = False) -> FeedForwardGrads:
     """Return the gradients of `feed_forward` given dy (x's shape) and what it kept: to x, up
     (d, f, p), down (f, d) and, with `bias`, the biases; `ffn` as the forward's. The residual's
-    gradient is dy. Each is rounded once to x's dtype, from float32 sums."""
+    gradient is dy. Each is rounded to x's dtype from float32 sums; so is d projected before its
+    products with up and x, as the MFMAs take it (bfloat16: 2^-8 at most of each term), but not
+    before up_bias's sums, which take 24 bits of it."""
     x, projected, h, low = saved
     require(dy, x, projected, h, low, up, down)
     is_f32("feed_forward_backward", x, dy, projected, h, up, down)

@@ -781,7 +781,8 @@ int bux_mx_unpack_rows(const uint8_t* packed, int64_t m, int64_t d, uint16_t* ou
  * (layers/mlp.py:20-35 of the reference's mlp and gated_mlp) and their backward. bfloat16, and
  * float32 twins (_f32) whose products and sums are float32's; any shape below 2^31 a side, any
  * alignment; float32 sums in a fixed order. A workspace of bux_dense_workspace_size(rows of the
- * output, columns of the sums, the contracted length) bytes, 16-byte aligned (0: none needed).
+ * output, columns of the sums, the contracted length) bytes, 16-byte aligned (0: none needed): as
+ * much as either type may ask for.
  *
  * bux_dense_rows: z = x w + bias; out = act(z) + residual, each rounded once, from float32.
  *   x         [m, k].  w: [k, n], or [n, k] with `transposed` (x w^T).
